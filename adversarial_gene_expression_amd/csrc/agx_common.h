@@ -106,6 +106,7 @@ int ff_hx(void *stream, const float *hrows, int ldh, int HL, float *X, int ldx, 
 // true if the heuristic launches the TN product dW[M,N] (K rows) on a kernel that has the fused
 // epilogue, without split-K (then fused and unfused runs sum in the same order: bit-identical)
 bool gemm_can_fuse_opt(int M, int N, int K, int64_t ws_floats);
+int fill_zero(void *stream, float *p, int64_t n);   // elementwise.hip
 int colstats_scratch_init();   // corr.hip: address of the static scratch of agx_colstats_noalloc on the current device
 // Loss-log snapshot done by the last small-gradient launch of a captured iteration: n floats from
 // src to the address stored at *dst_slot (left there by iter_stage; NULL address: no copy).

@@ -1224,7 +1224,7 @@ int record_iteration(agx_cgan *h, hipStream_t st, const agx_iter_args_t *a, int 
       AGX_TRY(agx::ff_stage(st, h->gp + gm0.w_off[Lg0], gm0.ldw[Lg0], h->gp + gm0.b_off[Lg0], gm0.dims[Lg0], G, h->ncov, h->he,
                             h->Xbuf[0] - (size_t)h->HD * h->ldx, h->ldx, h->hxp));
       if (h->hxp > h->hx)
-        AGX_HIP(hipMemsetAsync(h->D[1] - (size_t)(h->HD - h->hx) * h->ldh[1], 0, (size_t)(h->hxp - h->hx) * h->ldh[1] * sizeof(float), st));
+        AGX_TRY(agx::fill_zero(st, h->D[1] - (size_t)(h->HD - h->hx) * h->ldh[1], (int64_t)(h->hxp - h->hx) * h->ldh[1]));
     } else
     AGX_TRY(gen_layers(h, st, S * B, h->F, h->ldsx, fold0 ? &du : nullptr, B));
     // real rows were staged into buffer 0 rows [0,B) (agx_cgan_iter_stage) and stay there for all

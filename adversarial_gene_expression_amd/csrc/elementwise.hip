@@ -1378,6 +1378,20 @@ extern "C" int agx_wgan_loss(void *stream, const float *out, int32_t n0, int32_t
   return AGX_OK;
 }
 
+// floats [0, n) <- 0 by a kernel: a captured graph records no memset node
+namespace {
+__global__ __launch_bounds__(256) void fill_zero_kernel(float *p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0.f;
+}
+}  // namespace
+int agx::fill_zero(void *stream, float *p, int64_t n) {
+  if (n <= 0) return AGX_OK;
+  hipLaunchKernelGGL(fill_zero_kernel, dim3((unsigned)agx::cdiv64(n, 256)), dim3(256), 0, agx::as_stream(stream), p, n);
+  AGX_LAUNCH_CHECK();
+  return AGX_OK;
+}
+
 extern "C" int agx_colsum(void *stream, const float *A, int32_t lda, int32_t r0, int32_t r1,
                           int32_t H, float *out, int32_t accumulate) {
   AGX_CHECK_ARG(A && out && lda >= H && r0 >= 0 && r1 >= r0, "agx_colsum: bad argument");
