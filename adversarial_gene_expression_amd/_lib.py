@@ -167,6 +167,57 @@ class SmallGrads(C.Structure):
     ]
 
 
+AGX_F32, AGX_BF16 = 0, 1
+
+
+class NormDesc(C.Structure):
+    _fields_ = [
+        ('x', C.c_void_p), ('dy', C.c_void_p), ('u', C.c_void_p),
+        ('y', C.c_void_p), ('dx', C.c_void_p), ('ddy', C.c_void_p),
+        ('gamma', C.c_void_p), ('beta', C.c_void_p),
+        ('mean', C.c_void_p), ('rstd', C.c_void_p),
+        ('dgamma', C.c_void_p), ('dbeta', C.c_void_p),
+        ('ws', C.c_void_p), ('ws_floats', C.c_int64),
+        ('ldx', C.c_int64), ('lddy', C.c_int64), ('ldu', C.c_int64), ('ldy', C.c_int64), ('lddx', C.c_int64),
+        ('ldddy', C.c_int64),
+        ('rows', C.c_int64), ('width', C.c_int64),
+        ('eps', C.c_float), ('slope', C.c_float),
+        ('dtype', C.c_int32), ('act', C.c_int32),
+        ('accumulate_dx', C.c_int32), ('accumulate_params', C.c_int32),
+    ]
+
+
+AGX_MAX_ORTH, AGX_ORTH_MAX_SIDE, AGX_ORTH_MAX_STEPS = 16, 4096, 16
+
+
+class OrthDesc(C.Structure):
+    _fields_ = [
+        ('x', C.c_void_p), ('out', C.c_void_p), ('ldx', C.c_int64), ('ldo', C.c_int64),
+        ('rows', C.c_int32), ('cols', C.c_int32), ('dtype', C.c_int32), ('reserved', C.c_int32),
+    ]
+
+
+class OrthOpts(C.Structure):
+    _fields_ = [
+        ('steps', C.c_int32), ('n_coef', C.c_int32), ('coef', C.c_float * (3 * AGX_ORTH_MAX_STEPS)),
+        ('eps', C.c_float), ('reserved', C.c_int32),
+    ]
+
+
+class MuonDesc(C.Structure):
+    _fields_ = [
+        ('w', C.c_void_p), ('g', C.c_void_p), ('m', C.c_void_p),
+        ('ldw', C.c_int64), ('ldg', C.c_int64), ('ldm', C.c_int64),
+        ('rows', C.c_int32), ('cols', C.c_int32), ('scale', C.c_float), ('reserved', C.c_int32),
+    ]
+
+
+class MuonOpts(C.Structure):
+    _fields_ = [
+        ('orth', OrthOpts), ('lr', C.c_float), ('momentum', C.c_float), ('weight_decay', C.c_float), ('nesterov', C.c_int32),
+    ]
+
+
 _vp, _i32, _i64, _f32, _u64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_uint64
 
 # name -> (restype, argtypes); every symbol include/agx.h declares
@@ -191,6 +242,15 @@ SIGNATURES = {
     'agx_affine_act': (C.c_int, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _f32]),
     'agx_bn_backward': (C.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _f32, _i32, _i32, _vp, _vp]),
     'agx_bn_moving_update': (C.c_int, [_vp, _vp, _vp, _vp, _vp, _f32, _i32]),
+    'agx_layernorm_ws_floats': (_i64, [_i64, _i64, _i32]),
+    'agx_layernorm_fwd': (C.c_int, [_vp, C.POINTER(NormDesc)]),
+    'agx_layernorm_bwd': (C.c_int, [_vp, C.POINTER(NormDesc)]),
+    'agx_layernorm_bwd2': (C.c_int, [_vp, C.POINTER(NormDesc)]),
+    'agx_orth_ws_bytes': (_i64, [C.POINTER(OrthDesc), _i32, _i32]),
+    'agx_orthogonalize': (C.c_int, [_vp, C.POINTER(OrthDesc), _i32, C.POINTER(OrthOpts), _vp, _i64]),
+    'agx_opt_muon_ws_bytes': (_i64, [C.POINTER(MuonDesc), _i32, C.POINTER(MuonOpts)]),
+    'agx_opt_muon': (C.c_int, [_vp, C.POINTER(MuonDesc), _i32, C.POINTER(MuonOpts), _vp, _i64]),
+    'agx_op_sizeof': (_i64, [_i32]),
     'agx_embed_concat_fwd': (C.c_int, [_vp, C.POINTER(EmbedDesc), _vp, _vp, _i32, _i32, _vp, _i32, _i32,
                                        _vp, _i32, _i32, _i32, _vp, _i32]),
     'agx_embed_bwd': (C.c_int, [_vp, C.POINTER(EmbedDesc), _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32]),

@@ -1,0 +1,633 @@
+// Layer normalisation over the rows of a matrix: forward, backward, and the backward of the backward pass.
+//
+// Row x of N values, mean() over the row (eps > 0):
+//   forward      mu = mean(x), r = (mean((x - mu)^2) + eps)^-1/2, h = (x - mu) r, n = gamma h + beta, y = act(n)
+//   backward     dn = act'(y) dy, g = gamma dn
+//                dx = r (g - mean(g) - h mean(g h)), dgamma = sum_rows dn h, dbeta = sum_rows dn
+//   second order (u: adjoint of dx)   q = r (u - mean(u) - h mean(u h))
+//                ddy = act'(y) gamma q, dgamma = sum_rows dn q
+//                dx = r^2 [h (3 mean(gh) mean(uh) + mean(g) mean(u) - mean(gu)) - mean(uh) (g - mean(g)) - mean(gh) (u - mean(u))]
+//   (act is a leaky ReLU of slope >= 0, whose derivative follows from the sign of its output y)
+//
+// All three are bound by HBM: 8 to 30 flops per element of 2 to 6 arrays.  A row is read ONCE and kept in registers by
+// the G threads that own it (16, 64: part of or one wave, no barrier; 256, 1024: a workgroup), C vectors of 16 bytes each,
+// so that the two passes of a centred variance and the 2 to 5 row means cost no second read.  Vectors are loaded at the
+// element's alignment (the hardware needs no more), so odd widths and strides take the same path as padded ones.
+// Parameter gradients: every thread owns fixed columns, sums its rows in registers, the groups of a workgroup meet in
+// LDS, and a second launch adds the workgroups' partial rows in a fixed order (no atomics: bit-reproducible).
+#include "agx_common.h"
+
+#include <algorithm>
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int V = 4;
+  typedef f32x4 __attribute__((aligned(4))) type;
+};
+template <> struct Vec<__bf16> {
+  static constexpr int V = 8;
+  typedef bf16x8 __attribute__((aligned(2))) type;
+};
+
+// V elements from p[i..] of a row of n elements; zeros behind the row's end
+template <typename T>
+__device__ __forceinline__ void load_vec(const T *__restrict__ p, int64_t i, int64_t n, float (&o)[Vec<T>::V]) {
+  constexpr int V = Vec<T>::V;
+  if (i + V <= n) {
+    const typename Vec<T>::type v = *reinterpret_cast<const typename Vec<T>::type *>(p + i);
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = (float)v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = i + k < n ? (float)p[i + k] : 0.f;
+  }
+}
+// (a 16-bit result is rounded once, to nearest even, from the 32-bit value)
+template <typename T>
+__device__ __forceinline__ void store_vec(T *__restrict__ p, int64_t i, int64_t n, const float (&o)[Vec<T>::V]) {
+  constexpr int V = Vec<T>::V;
+  if (i + V <= n) {
+    typename Vec<T>::type v;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = (T)o[k];
+    *reinterpret_cast<typename Vec<T>::type *>(p + i) = v;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (i + k < n) p[i + k] = (T)o[k];
+  }
+}
+// (parameter vectors: float, possibly absent)
+template <int V>
+__device__ __forceinline__ void load_param(const float *p, int64_t i, int64_t n, float absent, float (&o)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) o[k] = p && i + k < n ? p[i + k] : absent;
+}
+
+struct NormArgs {
+  const void *x, *dy, *u, *ym;   // ym: forward output whose sign is the activation's derivative (NULL: no activation)
+  void *y, *dx, *ddy;
+  const float *gamma, *beta;
+  float *mean, *rstd;
+  const float *mean_in, *rstd_in;
+  float *part;                   // [workgroups][2][width] partial parameter gradients (NULL: none wanted)
+  int64_t ldx, lddy, ldu, ldym, ldy, lddx, ldddy;
+  int64_t rows, n;
+  float eps, slope;
+  int act, add_dx;
+};
+
+// sums of K values over the G threads of a row's group; every thread gets them.  G > 64: `red` holds 2 * K * (G / 64)
+// floats and `flip` alternates between its halves, so that one barrier a call is enough.
+template <int G, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float *red, int &flip) {
+#pragma unroll
+  for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o, 64);
+  if constexpr (G > 64) {
+    constexpr int W = G / 64;
+    float *b = red + flip * K * W;
+    flip ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) b[k * W + (threadIdx.x >> 6)] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += b[k * W + w];
+      v[k] = s;
+    }
+  }
+}
+
+template <int G> constexpr int block_threads() { return G > 256 ? G : 256; }
+
+template <typename T, int G, int C>
+__global__ __launch_bounds__(block_threads<G>()) void ln_fwd_kernel(NormArgs a) {
+  constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
+  __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
+  int flip = 0;
+  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const float inv_n = 1.f / (float)a.n;
+  for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    float v[C][V];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      load_vec<T>(x, ((int64_t)c * G + t) * V, a.n, v[c]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) s[0] += v[c][k];
+    }
+    group_sum<G, 1>(s, red, flip);
+    const float mu = s[0] * inv_n;
+    s[0] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = v[c][k] - mu;
+        if (((int64_t)c * G + t) * V + k < a.n) s[0] += d * d;
+      }
+    group_sum<G, 1>(s, red, flip);
+    const float r = 1.f / sqrtf(s[0] * inv_n + a.eps);
+    if (t == 0) {
+      if (a.mean) a.mean[row] = mu;
+      if (a.rstd) a.rstd[row] = r;
+    }
+    T *y = reinterpret_cast<T *>(a.y) + row * a.ldy;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int64_t i = ((int64_t)c * G + t) * V;
+      if (i >= a.n) continue;
+      float ga[V], be[V];
+      load_param<V>(a.gamma, i, a.n, 1.f, ga);
+      load_param<V>(a.beta, i, a.n, 0.f, be);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float n = (v[c][k] - mu) * r * ga[k] + be[k];
+        v[c][k] = a.act ? (n > 0.f ? n : a.slope * n) : n;
+      }
+      store_vec<T>(y, i, a.n, v[c]);
+    }
+  }
+}
+
+// the workgroup's partial sums of NA parameter gradients: groups meet in LDS in a fixed order
+template <typename T, int G, int C, int NA>
+__device__ __forceinline__ void write_partials(float (&acc)[NA][C][Vec<T>::V], const NormArgs &a, float *lds) {
+  constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
+  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+#pragma unroll
+  for (int q = 0; q < NA; ++q) {
+    if constexpr (NG > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) lds[(grp * C + c) * G * V + t * V + k] = acc[q][c][k];
+      __syncthreads();
+    }
+    float *p = a.part + ((int64_t)blockIdx.x * 2 + q) * a.n;
+    if constexpr (NG > 1) {
+      for (int64_t i = threadIdx.x; i < a.n; i += block_threads<G>()) {
+        float s = 0.f;
+        for (int g = 0; g < NG; ++g) s += lds[g * C * G * V + i];
+        p[i] = s;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const int64_t i = ((int64_t)c * G + t) * V + k;
+          if (i < a.n) p[i] = acc[q][c][k];
+        }
+    }
+  }
+}
+
+template <typename T, int G, int C> constexpr int lds_floats() {
+  return block_threads<G>() / G > 1 ? block_threads<G>() * C * Vec<T>::V : 1;
+}
+
+template <typename T, int G, int C, bool PG>
+__global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) {
+  constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
+  __shared__ float red[G > 64 ? 2 * 2 * (G / 64) : 1];
+  __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
+  int flip = 0;
+  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const float inv_n = 1.f / (float)a.n;
+  float acc[2][C][V] = {};
+  for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
+    const T *ym = reinterpret_cast<const T *>(a.ym) + row * a.ldym;
+    const float mu = a.mean_in[row], r = a.rstd_in[row];
+    float h[C][V], g[C][V];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int64_t i = ((int64_t)c * G + t) * V;
+      load_vec<T>(x, i, a.n, h[c]);
+      load_vec<T>(dy, i, a.n, g[c]);
+      if (a.ym) {
+        float m[V];
+        load_vec<T>(ym, i, a.n, m);
+#pragma unroll
+        for (int k = 0; k < V; ++k) g[c][k] = m[k] > 0.f ? g[c][k] : a.slope * g[c][k];
+      }
+      float ga[V];
+      load_param<V>(a.gamma, i, a.n, 1.f, ga);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        h[c][k] = i + k < a.n ? (h[c][k] - mu) * r : 0.f;
+        if constexpr (PG) {
+          acc[0][c][k] += g[c][k] * h[c][k];
+          acc[1][c][k] += g[c][k];
+        }
+        g[c][k] *= ga[k];
+        s[0] += g[c][k];
+        s[1] += g[c][k] * h[c][k];
+      }
+    }
+    if (a.dx) {
+      group_sum<G, 2>(s, red, flip);
+      const float mg = s[0] * inv_n, mgh = s[1] * inv_n;
+      T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int64_t i = ((int64_t)c * G + t) * V;
+        if (i >= a.n) continue;
+        float o[V];
+        if (a.add_dx) load_vec<T>(dx, i, a.n, o);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = r * (g[c][k] - mg - h[c][k] * mgh);
+          o[k] = a.add_dx ? o[k] + d : d;
+        }
+        store_vec<T>(dx, i, a.n, o);
+      }
+    }
+  }
+  if constexpr (PG) write_partials<T, G, C, 2>(acc, a, lds);
+}
+
+template <typename T, int G, int C, bool PG>
+__global__ __launch_bounds__(block_threads<G>()) void ln_bwd2_kernel(NormArgs a) {
+  constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
+  __shared__ float red[G > 64 ? 2 * 5 * (G / 64) : 1];
+  __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
+  int flip = 0;
+  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const float inv_n = 1.f / (float)a.n;
+  float acc[1][C][V] = {};
+  for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
+    const T *up = reinterpret_cast<const T *>(a.u) + row * a.ldu;
+    const T *ym = reinterpret_cast<const T *>(a.ym) + row * a.ldym;
+    const float mu = a.mean_in[row], r = a.rstd_in[row];
+    float h[C][V], d[C][V], u[C][V];   // d: dn (before gamma)
+    uint32_t neg[C];                   // bit k: the activation's derivative is the slope
+    float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int64_t i = ((int64_t)c * G + t) * V;
+      load_vec<T>(x, i, a.n, h[c]);
+      load_vec<T>(dy, i, a.n, d[c]);
+      load_vec<T>(up, i, a.n, u[c]);
+      neg[c] = 0;
+      if (a.ym) {
+        float m[V];
+        load_vec<T>(ym, i, a.n, m);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (!(m[k] > 0.f)) {
+            neg[c] |= 1u << k;
+            d[c][k] *= a.slope;
+          }
+      }
+      float ga[V];
+      load_param<V>(a.gamma, i, a.n, 1.f, ga);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        h[c][k] = i + k < a.n ? (h[c][k] - mu) * r : 0.f;
+        const float g = d[c][k] * ga[k];
+        s[0] += g;
+        s[1] += g * h[c][k];
+        s[2] += u[c][k];
+        s[3] += u[c][k] * h[c][k];
+        s[4] += g * u[c][k];
+      }
+    }
+    group_sum<G, 5>(s, red, flip);
+    const float mg = s[0] * inv_n, mgh = s[1] * inv_n, mu_ = s[2] * inv_n, muh = s[3] * inv_n, mgu = s[4] * inv_n;
+    const float hc = 3.f * mgh * muh + mg * mu_ - mgu, r2 = r * r;
+    T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
+    T *ddy = reinterpret_cast<T *>(a.ddy) + row * a.ldddy;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int64_t i = ((int64_t)c * G + t) * V;
+      if (i >= a.n) continue;
+      float ga[V], o[V], e[V];
+      load_param<V>(a.gamma, i, a.n, 1.f, ga);
+      if (a.dx && a.add_dx) load_vec<T>(dx, i, a.n, o);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float q = r * (u[c][k] - mu_ - h[c][k] * muh);
+        if constexpr (PG) acc[0][c][k] += d[c][k] * q;
+        e[k] = ga[k] * q;
+        if (neg[c] >> k & 1) e[k] *= a.slope;
+        const float b = r2 * (h[c][k] * hc - muh * (d[c][k] * ga[k] - mg) - mgh * (u[c][k] - mu_));
+        o[k] = a.add_dx ? o[k] + b : b;
+      }
+      if (a.dx) store_vec<T>(dx, i, a.n, o);
+      if (a.ddy) store_vec<T>(ddy, i, a.n, e);
+    }
+  }
+  if constexpr (PG) write_partials<T, G, C, 1>(acc, a, lds);
+}
+
+// Rows wider than the registers of a workgroup hold: one workgroup a row, the row read again for each pass (it stays in
+// L2 between them).  Partial parameter gradients are added to the workgroup's own row of `part`, each column by one thread.
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(NormArgs a) {
+  __shared__ float red[2 * 16];
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    float s[1] = {0.f};
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) s[0] += (float)x[i];
+    group_sum<1024, 1>(s, red, flip);
+    const float mu = s[0] / (float)a.n;
+    s[0] = 0.f;
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+      const float d = (float)x[i] - mu;
+      s[0] += d * d;
+    }
+    group_sum<1024, 1>(s, red, flip);
+    const float r = 1.f / sqrtf(s[0] / (float)a.n + a.eps);
+    if (threadIdx.x == 0) {
+      if (a.mean) a.mean[row] = mu;
+      if (a.rstd) a.rstd[row] = r;
+    }
+    T *y = reinterpret_cast<T *>(a.y) + row * a.ldy;
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+      const float n = ((float)x[i] - mu) * r * (a.gamma ? a.gamma[i] : 1.f) + (a.beta ? a.beta[i] : 0.f);
+      y[i] = (T)(a.act ? (n > 0.f ? n : a.slope * n) : n);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(NormArgs a) {
+  __shared__ float red[2 * 2 * 16];
+  int flip = 0;
+  float *p0 = a.part ? a.part + (int64_t)blockIdx.x * 2 * a.n : nullptr, *p1 = a.part ? p0 + a.n : nullptr;
+  bool first = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
+    const T *ym = a.ym ? reinterpret_cast<const T *>(a.ym) + row * a.ldym : nullptr;
+    const float mu = a.mean_in[row], r = a.rstd_in[row];
+    float s[2] = {0.f, 0.f};
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+      float d = (float)dy[i];
+      if (ym && !((float)ym[i] > 0.f)) d *= a.slope;
+      const float h = ((float)x[i] - mu) * r;
+      if (p0) {
+        p0[i] = (first ? 0.f : p0[i]) + d * h;
+        p1[i] = (first ? 0.f : p1[i]) + d;
+      }
+      const float g = d * (a.gamma ? a.gamma[i] : 1.f);
+      s[0] += g;
+      s[1] += g * h;
+    }
+    first = false;
+    if (!a.dx) continue;
+    group_sum<1024, 2>(s, red, flip);
+    const float mg = s[0] / (float)a.n, mgh = s[1] / (float)a.n;
+    T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+      float d = (float)dy[i];
+      if (ym && !((float)ym[i] > 0.f)) d *= a.slope;
+      const float h = ((float)x[i] - mu) * r;
+      const float o = r * (d * (a.gamma ? a.gamma[i] : 1.f) - mg - h * mgh);
+      dx[i] = (T)(a.add_dx ? (float)dx[i] + o : o);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd2_wide_kernel(NormArgs a) {
+  __shared__ float red[2 * 5 * 16];
+  int flip = 0;
+  float *p0 = a.part ? a.part + (int64_t)blockIdx.x * 2 * a.n : nullptr;
+  bool first = true;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
+    const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
+    const T *up = reinterpret_cast<const T *>(a.u) + row * a.ldu;
+    const T *ym = a.ym ? reinterpret_cast<const T *>(a.ym) + row * a.ldym : nullptr;
+    const float mu = a.mean_in[row], r = a.rstd_in[row];
+    float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+      float d = (float)dy[i];
+      if (ym && !((float)ym[i] > 0.f)) d *= a.slope;
+      const float h = ((float)x[i] - mu) * r, g = d * (a.gamma ? a.gamma[i] : 1.f), u = (float)up[i];
+      s[0] += g;
+      s[1] += g * h;
+      s[2] += u;
+      s[3] += u * h;
+      s[4] += g * u;
+    }
+    group_sum<1024, 5>(s, red, flip);
+    const float n = (float)a.n, mg = s[0] / n, mgh = s[1] / n, mu_ = s[2] / n, muh = s[3] / n, mgu = s[4] / n;
+    const float hc = 3.f * mgh * muh + mg * mu_ - mgu, r2 = r * r;
+    T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
+    T *ddy = reinterpret_cast<T *>(a.ddy) + row * a.ldddy;
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+      const bool neg = ym && !((float)ym[i] > 0.f);
+      const float d = neg ? (float)dy[i] * a.slope : (float)dy[i];
+      const float ga = a.gamma ? a.gamma[i] : 1.f, h = ((float)x[i] - mu) * r, u = (float)up[i];
+      const float q = r * (u - mu_ - h * muh);
+      if (p0) p0[i] = (first ? 0.f : p0[i]) + d * q;
+      if (a.dx) {
+        const float b = r2 * (h * hc - muh * (d * ga - mg) - mgh * (u - mu_));
+        dx[i] = (T)(a.add_dx ? (float)dx[i] + b : b);
+      }
+      if (a.ddy) ddy[i] = (T)(neg ? ga * q * a.slope : ga * q);
+    }
+    first = false;
+  }
+}
+
+// out_q[j] (+)= sum over workgroups b of part[b][q][j], b in a fixed order: 16 columns by 16 interleaved shares a workgroup
+__global__ __launch_bounds__(256) void ln_param_kernel(const float *__restrict__ part, int nb, int64_t n, float *dgamma,
+                                                       float *dbeta, int accumulate) {
+  __shared__ float red[16][17];
+  float *out = blockIdx.y ? dbeta : dgamma;
+  if (!out) return;
+  const int col = threadIdx.x & 15, sh = threadIdx.x >> 4;
+  const int64_t j = (int64_t)blockIdx.x * 16 + col;
+  float s = 0.f;
+  if (j < n)
+    for (int b = sh; b < nb; b += 16) s += part[((int64_t)b * 2 + blockIdx.y) * n + j];
+  red[sh][col] = s;
+  __syncthreads();
+  if (sh == 0 && j < n) {
+    s = accumulate ? out[j] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][col];
+    out[j] = s;
+  }
+}
+
+enum { FWD, BWD, BWD2 };
+
+template <int OP, typename T, int G, int C>
+void launch_cfg(hipStream_t st, const NormArgs &a, int blocks) {
+  const dim3 grid(blocks), thr(block_threads<G>());
+  if constexpr (OP == FWD) hipLaunchKernelGGL((ln_fwd_kernel<T, G, C>), grid, thr, 0, st, a);
+  else if constexpr (OP == BWD) {
+    if (a.part) hipLaunchKernelGGL((ln_bwd_kernel<T, G, C, true>), grid, thr, 0, st, a);
+    else hipLaunchKernelGGL((ln_bwd_kernel<T, G, C, false>), grid, thr, 0, st, a);
+  } else {
+    if (a.part) hipLaunchKernelGGL((ln_bwd2_kernel<T, G, C, true>), grid, thr, 0, st, a);
+    else hipLaunchKernelGGL((ln_bwd2_kernel<T, G, C, false>), grid, thr, 0, st, a);
+  }
+}
+
+// threads a row's group has (0: the wide kernels) and vectors each of them holds, by the row's vectors of 16 bytes
+struct Cfg { int g, c; };
+Cfg pick(int64_t width, int v) {
+  const int64_t nv = agx::cdiv64(width, v);
+  if (nv <= 16) return {16, 1};
+  if (nv <= 64) return {64, 1};
+  if (nv <= 128) return {64, 2};
+  if (nv <= 256) return {256, 1};
+  if (nv <= 512) return {256, 2};
+  if (nv <= 1024) return {256, 4};
+  if (nv <= 2048) return {1024, 2};
+  return {0, 0};
+}
+// workgroups of a launch: enough rows in flight to fill 256 CUs a few times over; with parameter gradients at most two
+// a CU, because each writes and the second launch reads a partial row
+int blocks_of(int64_t rows, const Cfg &c, bool params) {
+  const int ng = c.g == 0 || c.g >= 256 ? 1 : 256 / c.g;
+  const int64_t need = agx::cdiv64(rows, ng);
+  return (int)std::min<int64_t>(need, (int64_t)agx::num_cus() * (params ? 2 : 16));
+}
+
+template <int OP, typename T>
+int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int accumulate) {
+  const Cfg c = pick(a.n, Vec<T>::V);
+  const int blocks = blocks_of(a.rows, c, a.part != nullptr);
+  if (blocks > 0) {
+    if (c.g == 16) launch_cfg<OP, T, 16, 1>(st, a, blocks);
+    else if (c.g == 64 && c.c == 1) launch_cfg<OP, T, 64, 1>(st, a, blocks);
+    else if (c.g == 64) launch_cfg<OP, T, 64, 2>(st, a, blocks);
+    else if (c.g == 256 && c.c == 1) launch_cfg<OP, T, 256, 1>(st, a, blocks);
+    else if (c.g == 256 && c.c == 2) launch_cfg<OP, T, 256, 2>(st, a, blocks);
+    else if (c.g == 256) launch_cfg<OP, T, 256, 4>(st, a, blocks);
+    else if (c.g == 1024) launch_cfg<OP, T, 1024, 2>(st, a, blocks);
+    else if constexpr (OP == FWD) hipLaunchKernelGGL(ln_fwd_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
+    else if constexpr (OP == BWD) hipLaunchKernelGGL(ln_bwd_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(ln_bwd2_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
+    AGX_LAUNCH_CHECK();
+  }
+  if (dgamma || dbeta) {
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)agx::cdiv64(a.n, 16), 2), dim3(256), 0, st, a.part, blocks, a.n, dgamma,
+                       dbeta, accumulate);
+    AGX_LAUNCH_CHECK();
+  }
+  return AGX_OK;
+}
+
+int check_norm(const agx_norm_t *p, const char *who) {
+  AGX_CHECK_ARG(p, "%s: null argument", who);
+  AGX_CHECK_ARG(p->dtype == AGX_F32 || p->dtype == AGX_BF16, "%s: dtype %d", who, p->dtype);
+  AGX_CHECK_ARG(p->rows >= 0 && p->width > 0 && p->width <= (1 << 28), "%s: rows %lld, width %lld", who, (long long)p->rows,
+                (long long)p->width);
+  AGX_CHECK_ARG(p->slope >= 0.f && p->slope <= 1.f, "%s: slope must be in [0, 1]", who);
+  AGX_CHECK_ARG(p->act == 0 || p->act == 1, "%s: act %d", who, p->act);
+  return AGX_OK;
+}
+int check_mat(const agx_norm_t *p, const void *m, int64_t ld, const char *who, const char *name) {
+  AGX_CHECK_ARG(m && ld >= p->width, "%s: %s missing or its leading dimension below the width", who, name);
+  const uintptr_t al = p->dtype == AGX_F32 ? 3 : 1;
+  AGX_CHECK_ARG((reinterpret_cast<uintptr_t>(m) & al) == 0, "%s: %s not aligned to its elements", who, name);
+  return AGX_OK;
+}
+int check_back(const agx_norm_t *p, const char *who) {
+  AGX_TRY(check_mat(p, p->x, p->ldx, who, "x"));
+  AGX_TRY(check_mat(p, p->dy, p->lddy, who, "dy"));
+  AGX_CHECK_ARG(p->mean && p->rstd, "%s: mean / rstd missing", who);
+  if (p->act) AGX_TRY(check_mat(p, p->y, p->ldy, who, "y"));
+  if (p->dx) AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
+  if (p->dgamma || p->dbeta) {
+    const int64_t need = agx_layernorm_ws_floats(p->rows, p->width, p->dtype);
+    if (need > 0 && (!p->ws || p->ws_floats < need)) {
+      agx::set_error("%s: workspace of %lld floats, %lld needed", who, (long long)p->ws_floats, (long long)need);
+      return AGX_E_WORKSPACE;
+    }
+  }
+  return AGX_OK;
+}
+NormArgs back_args(const agx_norm_t *p) {
+  NormArgs a = {};
+  a.x = p->x; a.dy = p->dy; a.ym = p->act ? p->y : nullptr; a.dx = p->dx;
+  a.ldx = p->ldx; a.lddy = p->lddy; a.ldym = p->act ? p->ldy : 0; a.lddx = p->lddx;
+  a.gamma = p->gamma; a.mean_in = p->mean; a.rstd_in = p->rstd;
+  a.part = (p->dgamma || p->dbeta) ? p->ws : nullptr;
+  a.rows = p->rows; a.n = p->width; a.slope = p->slope; a.act = p->act; a.add_dx = p->accumulate_dx ? 1 : 0;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int64_t agx_layernorm_ws_floats(int64_t rows, int64_t width, int32_t dtype) {
+  if (rows <= 0 || width <= 0) return 0;
+  return (int64_t)blocks_of(rows, pick(width, dtype == AGX_BF16 ? 8 : 4), true) * 2 * width;
+}
+
+extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
+  AGX_TRY(check_norm(p, "agx_layernorm_fwd"));
+  AGX_CHECK_ARG(p->eps > 0.f, "agx_layernorm_fwd: eps must be positive");
+  if (p->rows == 0) return AGX_OK;
+  AGX_TRY(check_mat(p, p->x, p->ldx, "agx_layernorm_fwd", "x"));
+  AGX_TRY(check_mat(p, p->y, p->ldy, "agx_layernorm_fwd", "y"));
+  NormArgs a = {};
+  a.x = p->x; a.ldx = p->ldx; a.y = p->y; a.ldy = p->ldy;
+  a.gamma = p->gamma; a.beta = p->beta; a.mean = p->mean; a.rstd = p->rstd;
+  a.rows = p->rows; a.n = p->width; a.eps = p->eps; a.slope = p->slope; a.act = p->act;
+  return p->dtype == AGX_F32 ? launch<FWD, float>(agx::as_stream(stream), a, nullptr, nullptr, 0)
+                             : launch<FWD, __bf16>(agx::as_stream(stream), a, nullptr, nullptr, 0);
+}
+
+extern "C" int agx_layernorm_bwd(void *stream, const agx_norm_t *p) {
+  AGX_TRY(check_norm(p, "agx_layernorm_bwd"));
+  if (p->rows > 0) AGX_TRY(check_back(p, "agx_layernorm_bwd"));
+  AGX_CHECK_ARG(p->dx || p->dgamma || p->dbeta, "agx_layernorm_bwd: no output wanted");
+  const NormArgs a = back_args(p);
+  return p->dtype == AGX_F32
+             ? launch<BWD, float>(agx::as_stream(stream), a, p->dgamma, p->dbeta, p->accumulate_params)
+             : launch<BWD, __bf16>(agx::as_stream(stream), a, p->dgamma, p->dbeta, p->accumulate_params);
+}
+
+extern "C" int agx_layernorm_bwd2(void *stream, const agx_norm_t *p) {
+  AGX_TRY(check_norm(p, "agx_layernorm_bwd2"));
+  AGX_CHECK_ARG(!p->dbeta, "agx_layernorm_bwd2: the second-order pass has no term in beta");
+  AGX_CHECK_ARG(p->dx || p->ddy || p->dgamma, "agx_layernorm_bwd2: no output wanted");
+  if (p->rows > 0) {
+    AGX_TRY(check_back(p, "agx_layernorm_bwd2"));
+    AGX_TRY(check_mat(p, p->u, p->ldu, "agx_layernorm_bwd2", "u"));
+    if (p->ddy) AGX_TRY(check_mat(p, p->ddy, p->ldddy, "agx_layernorm_bwd2", "ddy"));
+  }
+  NormArgs a = back_args(p);
+  a.u = p->u; a.ldu = p->ldu; a.ddy = p->ddy; a.ldddy = p->ldddy;
+  return p->dtype == AGX_F32
+             ? launch<BWD2, float>(agx::as_stream(stream), a, p->dgamma, nullptr, p->accumulate_params)
+             : launch<BWD2, __bf16>(agx::as_stream(stream), a, p->dgamma, nullptr, p->accumulate_params);
+}
+
+extern "C" int64_t agx_op_sizeof(int32_t which) {
+  switch (which) {
+    case 0: return sizeof(agx_norm_t);
+    case 1: return sizeof(agx_orth_t);
+    case 2: return sizeof(agx_orth_opts_t);
+    case 3: return sizeof(agx_muon_t);
+    case 4: return sizeof(agx_muon_opts_t);
+    default: return -1;
+  }
+}

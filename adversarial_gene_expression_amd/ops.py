@@ -76,6 +76,144 @@ def dense_bn(x, W, b, M, N, K, *, gamma=None, beta=None, eps=1e-3, slope=0.0, ac
     return y, mean, std * std
 
 
+_DTYPES = {torch.float32: _lib.AGX_F32, torch.bfloat16: _lib.AGX_BF16}
+
+
+def _matrix(t, name, like=None):
+    """Row stride of a [rows, cols] operand of the normalisation / update operators; raises on what they do not take."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError('%s must be a 2-D tensor' % name)
+    if t.dtype not in _DTYPES:
+        raise ValueError('%s must be float32 or bfloat16, got %s' % (name, t.dtype))
+    rows, cols = t.shape
+    if cols == 0:
+        raise ValueError('%s has no columns' % name)
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError('%s must match the first operand: got %s %s on %s, expected %s %s on %s'
+                         % (name, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
+    ld = t.stride(0) if rows > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+        raise ValueError('%s must have contiguous rows that do not overlap (strides %s)' % (name, t.stride()))
+    return ld
+
+
+def _vector(t, name, n, like):
+    """A float32 vector of n entries on the operand's device, or None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError('%s must be a contiguous float32 vector of %d entries' % (name, n))
+    if t.device != like.device:
+        raise ValueError('%s is on %s, the rows on %s' % (name, t.device, like.device))
+    return t.data_ptr()
+
+
+def _on_current(t):
+    """Kernels run on the current device and stream: refuse operands that live elsewhere."""
+    if t.device != _dev.device():
+        raise ValueError('operands are on %s, the current device is cuda:%d' % (t.device, torch.cuda.current_device()))
+
+
+def _rows_like(x):
+    """Uninitialised [rows, width] result, rows 16-byte aligned as the package lays matrices out."""
+    rows, width = x.shape
+    q = 16 // x.element_size()
+    ld = (width + q - 1) // q * q
+    out = x.new_empty((rows, ld))
+    return out if ld == width else out[:, :width]
+
+
+def _norm_desc(x, act, slope):
+    d = _lib.NormDesc()
+    d.ldx = _matrix(x, 'x')
+    if act not in (0, 1) or not 0.0 <= slope <= 1.0:
+        raise ValueError('act must be 0 or 1 and slope in [0, 1]: got %r, %r' % (act, slope))
+    d.x, d.rows, d.width, d.dtype = x.data_ptr(), x.shape[0], x.shape[1], _DTYPES[x.dtype]
+    d.act, d.slope = act, slope
+    return d
+
+
+def layer_norm(x, gamma=None, beta=None, *, eps=1e-3, act=0, slope=0.0, out=None):
+    """Layer normalisation of every row of x [rows, width] (float32 or bfloat16), with the (leaky-)ReLU of `slope` behind
+    it when act=1: y = act(gamma * (x - mean) * rstd + beta), rstd = 1 / sqrt(var + eps), biased variance (Keras
+    LayerNormalization).  gamma / beta: float32 vectors or None (1 / 0).  Returns (y, mean, rstd), the statistics in
+    float32 for the backward passes.  out: where to write y (x itself is allowed).  The reference has no normalisation
+    layer (tf_utils.py:85-88)."""
+    d = _norm_desc(x, act, slope)
+    if not eps > 0.0:
+        raise ValueError('eps must be positive, got %r' % (eps,))
+    d.gamma, d.beta = _vector(gamma, 'gamma', x.shape[1], x), _vector(beta, 'beta', x.shape[1], x)
+    if out is not None:
+        d.ldy = _matrix(out, 'out', x)
+    _on_current(x)
+    if out is None:
+        out = _rows_like(x)
+        d.ldy = max(out.stride(0), out.shape[1])
+    stats = torch.empty((2, x.shape[0]), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    d.y, d.mean, d.rstd, d.eps = out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), eps
+    _lib.check(_lib.load().agx_layernorm_fwd(_dev.stream(), d), 'agx_layernorm_fwd')
+    return out, mean, rstd
+
+
+def _norm_back(d, dy, x, mean, rstd, gamma, y, act):
+    if mean is None or rstd is None:
+        raise ValueError('mean and rstd of the forward pass are needed')
+    d.lddy, d.dy = _matrix(dy, 'dy', x), dy.data_ptr()
+    d.mean, d.rstd = _vector(mean, 'mean', x.shape[0], x), _vector(rstd, 'rstd', x.shape[0], x)
+    d.gamma = _vector(gamma, 'gamma', x.shape[1], x)
+    if act:
+        if y is None:
+            raise ValueError('act=1 needs y, the forward result: the derivative is taken from its sign')
+        d.ldy, d.y = _matrix(y, 'y', x), y.data_ptr()
+    _on_current(x)
+
+
+def _norm_ws(d, x, lib):
+    n = int(lib.agx_layernorm_ws_floats(d.rows, d.width, d.dtype))
+    ws = torch.empty(max(n, 1), dtype=torch.float32, device=x.device)
+    d.ws, d.ws_floats = ws.data_ptr(), n
+    return ws
+
+
+def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, y=None, act=0, slope=0.0, param_grads=True):
+    """Backward of layer_norm: (dx, dgamma, dbeta) for the gradient dy of its result, dx in x's type, the parameter
+    gradients (sums over all rows in a fixed order) in float32 or None with param_grads=False.  mean / rstd: what the
+    forward returned; y: its result, needed with act=1."""
+    lib = _lib.load()
+    d = _norm_desc(x, act, slope)
+    _norm_back(d, dy, x, mean, rstd, gamma, y, act)
+    dx = _rows_like(x)
+    d.dx, d.lddx = dx.data_ptr(), max(dx.stride(0), dx.shape[1])
+    ws = dgamma = dbeta = None
+    if param_grads:
+        ws = _norm_ws(d, x, lib)
+        both = torch.empty((2, x.shape[1]), dtype=torch.float32, device=x.device)
+        dgamma, dbeta = both[0], both[1]
+        d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
+    _lib.check(lib.agx_layernorm_bwd(_dev.stream(), d), 'agx_layernorm_bwd')
+    return dx, dgamma, dbeta
+
+
+def layer_norm_backward2(u, dy, x, mean, rstd, gamma=None, *, y=None, act=0, slope=0.0, param_grads=True):
+    """Backward of layer_norm_backward's dx with respect to (dy, x, gamma): u is the gradient that arrives at dx, as under
+    a gradient penalty (tf_utils.py:154-171).  Returns (ddy, dx, dgamma)."""
+    lib = _lib.load()
+    d = _norm_desc(x, act, slope)
+    d.ldu, d.u = _matrix(u, 'u', x), u.data_ptr()
+    _norm_back(d, dy, x, mean, rstd, gamma, y, act)
+    dx, ddy = _rows_like(x), _rows_like(x)
+    d.dx, d.lddx = dx.data_ptr(), max(dx.stride(0), dx.shape[1])
+    d.ddy, d.ldddy = ddy.data_ptr(), max(ddy.stride(0), ddy.shape[1])
+    ws = dgamma = None
+    if param_grads:
+        ws = _norm_ws(d, x, lib)
+        dgamma = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+        d.dgamma = dgamma.data_ptr()
+    _lib.check(lib.agx_layernorm_bwd2(_dev.stream(), d), 'agx_layernorm_bwd2')
+    return ddy, dx, dgamma
+
+
 def colsum(A, r0, r1, H, out=None, accumulate=False):
     lib = _lib.load()
     if out is None:
@@ -94,6 +232,83 @@ def adam(w, g, m, v, lr_t, b1=0.9, b2=0.999, eps=1e-7, grad_scale=1.0):
     lib = _lib.load()
     _lib.check(lib.agx_opt_adam(_dev.stream(), ptr(w), ptr(g), ptr(m), ptr(v), w.numel(), lr_t, b1, b2, eps,
                                 grad_scale), 'agx_opt_adam')
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)   # a, b, c that bring singular values from about 0.01 up near 1 in five steps
+
+
+def _orth_opts(o, steps, coefficients, eps):
+    if int(steps) != steps or not 1 <= steps <= _lib.AGX_ORTH_MAX_STEPS:
+        raise ValueError('steps must be an integer in 1..%d, got %r' % (_lib.AGX_ORTH_MAX_STEPS, steps))
+    c = list(coefficients)
+    if len(c) == 3 and not hasattr(c[0], '__len__'):
+        c = [c]
+    if len(c) not in (1, steps) or any(len(t) != 3 for t in c):
+        raise ValueError('coefficients must be one triple (a, b, c) or one per step')
+    o.steps, o.n_coef, o.eps = int(steps), len(c), eps
+    for k, v in enumerate(v for t in c for v in t):
+        o.coef[k] = v
+    return o
+
+
+def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """Newton-Schulz orthogonalisation of a matrix (float32 or bfloat16), or of each of a list of them (one call's launches
+    are shared by up to 16): X_0 = x / (|x|_F + eps), then `steps` times X <- X (a I + b A + c A^2) with A = X^T X (from
+    the left with A = X X^T where rows < cols).  Products at float32 accuracy, one rounding to x's type at the end.  The
+    smaller side may be at most 4096.  coefficients: (a, b, c), or one such triple per step."""
+    one = isinstance(x, torch.Tensor)
+    xs = [x] if one else list(x)
+    o = _orth_opts(_lib.OrthOpts(), steps, coefficients, eps)
+    lds = [_matrix(t, 'x') for t in xs]
+    for t in xs:
+        _on_current(t)
+    lib, outs = _lib.load(), []
+    for lo in range(0, len(xs), _lib.AGX_MAX_ORTH):
+        part = xs[lo:lo + _lib.AGX_MAX_ORTH]
+        jobs = (_lib.OrthDesc * len(part))()
+        for j, t, ld in zip(jobs, part, lds[lo:]):
+            out = _rows_like(t)
+            outs.append(out)
+            j.x, j.out, j.ldx, j.ldo = t.data_ptr(), out.data_ptr(), ld, max(out.stride(0), out.shape[1])
+            j.rows, j.cols, j.dtype = t.shape[0], t.shape[1], _DTYPES[t.dtype]
+        n = int(lib.agx_orth_ws_bytes(jobs, len(part), o.steps))
+        _lib.check(0 if n >= 0 else n, 'agx_orth_ws_bytes')
+        ws = torch.empty(n, dtype=torch.uint8, device=part[0].device)
+        _lib.check(lib.agx_orthogonalize(_dev.stream(), jobs, len(part), o, ws.data_ptr(), n), 'agx_orthogonalize')
+    return outs[0] if one else outs
+
+
+def muon(w, g, m, lr, *, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
+         scale=None):
+    """One Muon step in place on float32 kernels w [in, out] (or lists of them) with gradients g and momentum buffers m:
+    m <- momentum m + g; u = g + momentum m (nesterov) or m; w <- (1 - lr weight_decay) w - lr scale orthogonalize(u).
+    scale: default sqrt(max(1, out / in)) per kernel; a number applies to all."""
+    ws_, gs, ms = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (w, g, m))
+    if not len(ws_) == len(gs) == len(ms):
+        raise ValueError('w, g and m must be as many: got %d, %d, %d' % (len(ws_), len(gs), len(ms)))
+    o = _lib.MuonOpts()
+    _orth_opts(o.orth, steps, coefficients, eps)
+    o.lr, o.momentum, o.weight_decay, o.nesterov = lr, momentum, weight_decay, int(bool(nesterov))
+    lds = []
+    for a, b, c in zip(ws_, gs, ms):
+        if not isinstance(a, torch.Tensor) or a.dtype != torch.float32:
+            raise ValueError('w must be float32')
+        lds.append((_matrix(a, 'w'), _matrix(b, 'g', a), _matrix(c, 'm', a)))
+    for a in ws_:
+        _on_current(a)
+    lib = _lib.load()
+    for lo in range(0, len(ws_), _lib.AGX_MAX_ORTH):
+        part = list(zip(ws_, gs, ms, lds))[lo:lo + _lib.AGX_MAX_ORTH]
+        jobs = (_lib.MuonDesc * len(part))()
+        for j, (a, b, c, ld) in zip(jobs, part):
+            j.w, j.g, j.m = a.data_ptr(), b.data_ptr(), c.data_ptr()
+            j.ldw, j.ldg, j.ldm = ld
+            j.rows, j.cols = a.shape
+            j.scale = max(1.0, a.shape[1] / a.shape[0]) ** 0.5 if scale is None else scale
+        n = int(lib.agx_opt_muon_ws_bytes(jobs, len(part), o))
+        _lib.check(0 if n >= 0 else n, 'agx_opt_muon_ws_bytes')
+        ws = torch.empty(n, dtype=torch.uint8, device=part[0][0].device)
+        _lib.check(lib.agx_opt_muon(_dev.stream(), jobs, len(part), o, ws.data_ptr(), n), 'agx_opt_muon')
 
 
 def rng(n, seed, offset=0, normal=True):

@@ -155,6 +155,82 @@ int agx_bn_backward(void *stream, float *dz, int32_t lddz, const float *x, int32
 int agx_bn_moving_update(void *stream, float *moving_mean, float *moving_var, const float *mean, const float *std,
                          float momentum, int32_t N);
 
+/* ---- layer normalisation of hidden layers (no reference counterpart: tf_utils.py:85-88 has no normalisation) ----
+ * Rows [rows, width] of fp32 or bf16 values with a leading dimension in ELEMENTS; parameters, statistics and parameter
+ * gradients are fp32.  With h = (x - mean) * rstd, n = gamma * h + beta, y = act(n), mean(.) over a row:
+ *   fwd   writes y and, where given, mean / rstd (rstd = 1 / sqrt(mean((x - mean)^2) + eps))
+ *   bwd   dn = act'(y) dy, g = gamma dn:  dx = rstd (g - mean(g) - h mean(g h)), dgamma = sum dn h, dbeta = sum dn
+ *   bwd2  the backward of bwd with respect to (dy, x, gamma), u = adjoint of dx (what a critic's gradient penalty asks):
+ *         q = rstd (u - mean(u) - h mean(u h)):  ddy = act'(y) gamma q,  dgamma = sum dn q,
+ *         dx = rstd^2 (h (3 mean(gh) mean(uh) + mean(g) mean(u) - mean(gu)) - mean(uh) (g - mean(g)) - mean(gh) (u - mean(u)))
+ * act: 1 = leaky ReLU of `slope` (its derivative is taken from the sign of y, which bwd / bwd2 then need), 0 = none.
+ * Any output but mean / rstd may be NULL in bwd / bwd2; an output may be the same array as an input of its own shape.
+ * ws: needed where dgamma / dbeta are wanted (agx_layernorm_ws_floats).  Sums in a fixed order.                       */
+#define AGX_F32 0
+#define AGX_BF16 1
+typedef struct agx_norm {
+  const void *x, *dy, *u;
+  void *y, *dx, *ddy;
+  const float *gamma, *beta;   /* NULL: 1 / 0 */
+  float *mean, *rstd;
+  float *dgamma, *dbeta;
+  float *ws;
+  int64_t ws_floats;
+  int64_t ldx, lddy, ldu, ldy, lddx, ldddy;
+  int64_t rows, width;
+  float eps, slope;
+  int32_t dtype, act;
+  int32_t accumulate_dx;       /* dx += instead of dx =         (bwd, bwd2) */
+  int32_t accumulate_params;   /* dgamma / dbeta += instead of = (bwd, bwd2) */
+} agx_norm_t;
+int64_t agx_layernorm_ws_floats(int64_t rows, int64_t width, int32_t dtype);
+int agx_layernorm_fwd(void *stream, const agx_norm_t *p);
+int agx_layernorm_bwd(void *stream, const agx_norm_t *p);
+int agx_layernorm_bwd2(void *stream, const agx_norm_t *p);
+
+/* ---- orthogonalised updates (no reference counterpart: its optimizers are RMSprop / Adam, tf_utils.py:285-288) ----
+ * X_0 = x / (|x|_F + eps); X <- X (a I + b A + c A^2), A = X^T X, `steps` times (A = X X^T from the left where
+ * rows < cols): Newton-Schulz steps that bring the singular values of x towards 1.  n_coef: 1 (the same a, b, c for
+ * every step) or `steps` triples.  min(rows, cols) <= AGX_ORTH_MAX_SIDE.  Products are fp32-accurate.                 */
+#define AGX_MAX_ORTH 16
+#define AGX_ORTH_MAX_SIDE 4096
+#define AGX_ORTH_MAX_STEPS 16
+typedef struct agx_orth {
+  const void *x;
+  void *out;                   /* same type as x; not x itself */
+  int64_t ldx, ldo;
+  int32_t rows, cols, dtype, reserved;
+} agx_orth_t;
+typedef struct agx_orth_opts {
+  int32_t steps, n_coef;
+  float coef[3 * AGX_ORTH_MAX_STEPS];
+  float eps;
+  int32_t reserved;
+} agx_orth_opts_t;
+/* workspace of a call over these matrices (sizes and types are read, no pointer); -1: they are refused */
+int64_t agx_orth_ws_bytes(const agx_orth_t *jobs, int32_t n, int32_t steps);
+int agx_orthogonalize(void *stream, const agx_orth_t *jobs, int32_t n, const agx_orth_opts_t *o, void *ws, int64_t ws_size);
+/* One Muon step over n fp32 matrices: m <- momentum m + g; u = g + momentum m (nesterov) or m;
+ * w <- (1 - lr weight_decay) w - lr scale orth(u).  w, g, m: different arrays.                                         */
+typedef struct agx_muon {
+  float *w;
+  const float *g;
+  float *m;
+  int64_t ldw, ldg, ldm;
+  int32_t rows, cols;
+  float scale;
+  int32_t reserved;
+} agx_muon_t;
+typedef struct agx_muon_opts {
+  agx_orth_opts_t orth;
+  float lr, momentum, weight_decay;
+  int32_t nesterov;
+} agx_muon_opts_t;
+int64_t agx_opt_muon_ws_bytes(const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o);
+int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o, void *ws, int64_t ws_size);
+/* sizeof() of agx_norm_t (0), agx_orth_t (1), agx_orth_opts_t (2), agx_muon_t (3), agx_muon_opts_t (4), -1 otherwise */
+int64_t agx_op_sizeof(int32_t which);
+
 /* ---- embeddings: tf_utils.py:64-76, 120-131 ---------------------------- */
 typedef struct agx_embed {
   int32_t n_cat;

@@ -1,0 +1,161 @@
+"""Layer normalisation kernels against the float64 formulas on the same inputs.
+
+Tolerances: with e = 2^-24 and S the sum of the absolute terms of a result (oracle `*_size`), an element is a tree of at
+most 16 serial additions a lane, 6 levels across a wave and 16 wave sums, each adding e of S, plus a few roundings of the
+factors and, for dx of the second order, a product of two such sums: 128 e S covers all of them.  Sums over rows run
+serially over a workgroup's rows, then over its groups and the workgroups: e per addition, at most rows of them on the
+longest path, counted below.  A result stored in bf16 adds half a step, 2^-8 of its value."""
+import pytest
+import torch
+
+from oracle import norm_oracle as N
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+EPS = 1e-3
+
+# widths around every change of the row's thread group, for both types: part of a wave, a wave, 256 and 1024 threads, the
+# form that reads rows again; odd ones; one value; rows: none, one, fewer than a workgroup holds, more than the grid
+SHAPES = [(1, 1), (3, 1), (5, 2), (4, 63), (7, 64), (33, 65), (64, 128), (32, 256), (9, 257), (1536, 256), (17, 512), (6, 513),
+          (5, 1024), (4, 1025), (3, 1077), (3, 2048), (2, 2050), (5, 4096), (3, 4297), (2, 8192), (2, 8193), (3, 16384),
+          (2, 16400), (2, 18154), (40000, 5), (9000, 129)]
+
+
+def make(rows, width, dtype, seed, ld_extra=0):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device='cuda')  # noqa: E731
+
+    def mat(v):
+        t = torch.full((rows, width + ld_extra), 7.0, device='cuda', dtype=dtype)[:, :width]
+        t.copy_(v)
+        return t
+    x = mat(r(rows, width) + 0.5 + 0.5 * r(width))
+    return x, mat(r(rows, width)), mat(r(rows, width)), 1 + 0.2 * r(width), 0.2 * r(width)
+
+
+def half_step(dtype):
+    return 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+
+
+def near(got, want, size, dtype, factor=128):
+    got = N.t64(got)
+    bad = (got - want).abs() - (factor * E * size + half_step(dtype) * want.abs() + 1e-38)
+    assert bool((bad <= 0).all()), (float(bad.max()), int((bad > 0).sum()))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,width', SHAPES)
+def test_forward(gpu, rows, width, dtype):
+    from adversarial_gene_expression_amd import ops
+    x, _, _, ga, be = make(rows, width, dtype, rows * 7 + width, ld_extra=(rows + width) % 3)
+    for on, slope in ((0, 0.0), (1, 0.0), (1, 0.2)):
+        y, mean, rstd = ops.layer_norm(x, ga, be, eps=EPS, act=on, slope=slope)
+        X, G, B = N.t64(x), N.t64(ga), N.t64(be)
+        wy, wm, wr = N.forward(X, G, B, EPS, slope, on)
+        assert y.dtype == dtype and y.shape == x.shape
+        size = N.forward_size(X, G, B, wr)
+        near(y, wy, size, dtype)
+        near(mean, wm, X.abs().mean(1), torch.float32)
+        # rstd: relative error of the variance (its terms' cancelled size over it), halved by the root
+        var = 1 / wr ** 2
+        near(rstd, wr, wr * (1 + ((X.abs() + wm.abs()[:, None]) ** 2).mean(1) / var), torch.float32)
+    y, _, _ = ops.layer_norm(x)                                  # no parameters, default eps, no activation
+    near(y, N.forward(X, G * 0 + 1, B * 0, 1e-3)[0], N.forward_size(X, G * 0 + 1, B * 0, wr), dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,width', SHAPES)
+def test_backward(gpu, rows, width, dtype):
+    from adversarial_gene_expression_amd import ops
+    x, dy, u, ga, be = make(rows, width, dtype, rows * 5 + width, ld_extra=(rows + width) % 2)
+    deep = 128 + rows
+    for on, slope in ((0, 0.0), (1, 0.2)):
+        y, mean, rstd = ops.layer_norm(x, ga, be, eps=EPS, act=on, slope=slope)
+        args = [N.t64(t) for t in (dy, x, mean, rstd, ga, y)]
+        dx, dg, db = ops.layer_norm_backward(dy, x, mean, rstd, ga, y=y, act=on, slope=slope)
+        want, size = N.backward(*args, slope, on), N.backward_size(*args, slope, on)
+        near(dx, want[0], size[0], dtype)
+        near(dg, want[1], size[1], torch.float32, deep)
+        near(db, want[2], size[2], torch.float32, deep)
+        dx2, none, _ = ops.layer_norm_backward(dy, x, mean, rstd, ga, y=y, act=on, slope=slope, param_grads=False)
+        assert none is None and torch.equal(dx2, dx)
+        ddy, d2, dg2 = ops.layer_norm_backward2(u, dy, x, mean, rstd, ga, y=y, act=on, slope=slope)
+        want, size = N.backward2(N.t64(u), *args, slope, on), N.backward2_size(N.t64(u), *args, slope, on)
+        near(ddy, want[0], size[0], dtype)
+        near(d2, want[1], size[1], dtype)
+        near(dg2, want[2], size[2], torch.float32, deep)
+
+
+def test_no_rows_and_results_are_reproducible(gpu):
+    from adversarial_gene_expression_amd import ops
+    x = torch.zeros(0, 24, device='cuda')
+    y, mean, rstd = ops.layer_norm(x)
+    assert y.shape == (0, 24) and mean.numel() == rstd.numel() == 0
+    dx, dg, db = ops.layer_norm_backward(x, x, mean, rstd)
+    assert dx.shape == (0, 24) and not dg.any() and not db.any()
+    assert not ops.layer_norm_backward2(x, x, x, mean, rstd)[2].any()
+    x, dy, u, ga, be = make(5000, 300, torch.float32, 4)
+    y, mean, rstd = ops.layer_norm(x, ga, be, act=1)
+    a = ops.layer_norm_backward(dy, x, mean, rstd, ga, y=y, act=1)
+    b = ops.layer_norm_backward(dy, x, mean, rstd, ga, y=y, act=1)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize('width', [40, 256, 1025, 20000])
+def test_rows_do_not_touch_each_other_and_padding_stays(gpu, width):
+    """A row of NaN, one of infinities and one constant row leave the others as they are; columns behind the width keep
+    their values; the result may be written over the input."""
+    from adversarial_gene_expression_amd import ops
+    g = torch.Generator(device='cuda').manual_seed(1)
+    buf = torch.randn(9, width + 5, generator=g, device='cuda')
+    x = buf[:, :width]
+    want = ops.layer_norm(x.contiguous(), act=1)[0]
+    keep = buf[:, width:].clone()
+    bad = buf.clone()
+    bad[2, :width] = float('nan')
+    bad[4, 3] = float('inf')
+    bad[6, :width] = 2.5
+    y, mean, rstd = ops.layer_norm(bad[:, :width], out=bad[:, :width], act=1)
+    ok = [0, 1, 3, 5, 7, 8]
+    assert torch.equal(y[ok], want[ok]) and y.data_ptr() == bad.data_ptr()
+    assert torch.isnan(y[2]).all() and torch.isnan(y[4]).all()
+    assert not y[6].any() and abs(float(rstd[6]) - 1e-3 ** -0.5) < 1e-5
+    assert torch.equal(bad[:, width:], keep)
+
+
+def test_captured_forward_and_backward_replay(gpu):
+    """Forward, backward and second order recorded into one graph: every replay equals the eager calls on its inputs."""
+    from adversarial_gene_expression_amd import ops
+    x, dy, u, ga, be = make(200, 256, torch.float32, 9)
+
+    def run():
+        y, m, r = ops.layer_norm(x, ga, be, act=1, slope=0.2)
+        return [y, *ops.layer_norm_backward(dy, x, m, r, ga, y=y, act=1, slope=0.2),
+                *ops.layer_norm_backward2(u, dy, x, m, r, ga, y=y, act=1, slope=0.2)]
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for k in range(4):
+        x.add_(0.25)
+        dy.mul_(-1.5)
+        want = [t.clone() for t in run()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_side_stream(gpu):
+    from adversarial_gene_expression_amd import ops
+    x, dy, _, ga, be = make(3000, 512, torch.float32, 2)
+    y, m, r = ops.layer_norm(x, ga, be)
+    want = ops.layer_norm_backward(dy, x, m, r, ga)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        y2, m2, r2 = ops.layer_norm(x, ga, be)
+        got = ops.layer_norm_backward(dy, x, m2, r2, ga)
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(got, want))
