@@ -11,6 +11,7 @@ namespace agx {
 void set_error(const char *fmt, ...);
 int num_cus();
 int gemm_prepare_device();
+int orth_prepare_device();
 
 // Optimizer update fused into a weight-gradient GEMM epilogue (internal: captured single-GPU
 // iteration only).  w / s1 point at the element that corresponds to C[0,0] (same leading
