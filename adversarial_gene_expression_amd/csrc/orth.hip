@@ -14,8 +14,9 @@
 // everything behind it: entries then stay under 2^14, and those down to 2^-25 of the bound keep all bits.  A bf16 operand
 // needs one term only (its 8 bits fit).
 //
-// Tiles of 64 x 64 by four waves of 32 x 32 (mfma 32x32x16), K in steps of 64 through LDS, next step's global loads in
-// flight during the products.
+// Tiles of 128 x 128 (eight waves of 64 x 32, mfma 32x32x16) where there are enough of them for the chip, of 64 x 64 below:
+// a larger tile splits and stages every element for more products.  K goes through two LDS buffers, the next
+// step's global loads in flight.
 #include "agx_common.h"
 
 #include <algorithm>
@@ -32,14 +33,15 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
-constexpr int T = 64, BK = 64, LDK = BK + 8;   // (LDS rows of 144 bytes: 16 rows start in 16 different bank groups)
+constexpr int T = 64;                          // n x n matrices are padded to T or to a multiple of 2 T
 constexpr int PHASE = 3;                       // steps between two Gram matrices
 constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ONE_BLOCK = 128;                 // largest padded side for a phase in one workgroup (LDS)
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
+constexpr int64_t BIG_TILES = 128;             // tiles of 2 T from which the product with the long side takes them
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
-// n x n matrix as two fp16 planes of np x np (np: n rounded up to T, zeros behind), value = (hi + lo) 2^-e
+// n x n matrix as two fp16 planes of np x np (np: n rounded up to T or a multiple of 2 T, zeros behind), value = (hi + lo) 2^-e
 struct Planes {
   _Float16 *hi;
   int32_t e, np;
@@ -75,29 +77,26 @@ struct PrepArgs {
   int nesterov;
 };
 
-// four consecutive values of a row (n of them valid)
-__device__ __forceinline__ void load4(const float *p, int n, float (&v)[4]) {
-  if (n == 4) {
-    const f32x4u w = *reinterpret_cast<const f32x4u *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = w[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
-  }
-}
-__device__ __forceinline__ void load4(const __bf16 *p, int n, float (&v)[4]) {
-  if (n == 4) {
-    const bf16x4u w = *reinterpret_cast<const bf16x4u *>(p);
+template <typename E> struct Vec4;
+template <> struct Vec4<float> { typedef f32x4u type; };
+template <> struct Vec4<__bf16> { typedef bf16x4u type; };
+// four values at p, zeros from the n-th on
+template <typename E>
+__device__ __forceinline__ f32x4 load4z(const E *p, int n) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (n >= 4) {
+    const typename Vec4<E>::type w = *reinterpret_cast<const typename Vec4<E>::type *>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)w[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+    for (int i = 0; i < 3; ++i)
+      if (i < n) v[i] = (float)p[i];
   }
+  return v;
 }
-__device__ __forceinline__ void store4(float *p, int n, const float (&v)[4]) {
-  if (n == 4) {
+__device__ __forceinline__ void store4(float *p, int n, f32x4 v) {
+  if (n >= 4) {
     f32x4u w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = v[i];
@@ -120,12 +119,10 @@ __global__ __launch_bounds__(256) void orth_prep_kernel(PrepArgs a) {
   for (uint32_t it = blockIdx.x * 256 + threadIdx.x; it < items; it += step) {
     const uint32_t r = it / per_row;
     const int c = (int)(it - r * per_row) * 4, n = min(4, j.cols - c);
-    float v[4];
-    if (j.dtype == AGX_F32) load4(reinterpret_cast<const float *>(j.x) + (int64_t)r * j.ldx + c, n, v);
-    else load4(reinterpret_cast<const __bf16 *>(j.x) + (int64_t)r * j.ldx + c, n, v);
+    f32x4 v = j.dtype == AGX_F32 ? load4z(reinterpret_cast<const float *>(j.x) + (int64_t)r * j.ldx + c, n)
+                                 : load4z(reinterpret_cast<const __bf16 *>(j.x) + (int64_t)r * j.ldx + c, n);
     if (j.m) {
-      float m[4];
-      load4(j.m + (int64_t)r * j.ldm + c, n, m);
+      f32x4 m = load4z(j.m + (int64_t)r * j.ldm + c, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         m[i] = a.mu * m[i] + v[i];
@@ -151,180 +148,226 @@ __device__ __forceinline__ void upper_tile(int t, int nt, int &ti, int &tj) {
   tj = ti + t;
 }
 
-// scale exponent of a matrix from its partial maxima; every thread of the 256 gets it
+// scale exponent of a matrix from its partial maxima; every thread of the workgroup (of up to 8 waves) gets it
 __device__ __forceinline__ int scale_exponent(const uint32_t *maxb, int nb, uint32_t *red) {
   uint32_t mx = 0;
-  for (int i = threadIdx.x; i < nb; i += 256) mx = max(mx, maxb[i]);
+  for (int i = threadIdx.x; i < nb; i += blockDim.x) mx = max(mx, maxb[i]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
   __syncthreads();
-  mx = max(max(red[0], red[1]), max(red[2], red[3]));
+  mx = 0;
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) mx = max(mx, red[i]);
   return TARGET - exponent_of(mx);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// tile product: operands in LDS as [64 rows][64 k] fp16 planes
+// tile product: operands in LDS as [TT rows][BK k] fp16 planes, TT = 64 or 128
 // ---------------------------------------------------------------------------------------------------------------------
-struct Tile {
-  _Float16 hi[T * LDK], lo[T * LDK];
+template <int TT> struct Geo {
+  static constexpr int BK = 64;                        // k of a step: 16 values a thread and operand
+  static constexpr int LD = BK + 8;                    // LDS rows of 144 bytes: 16 rows start in 16 different bank groups
+  static constexpr int PL = TT * LD;                   // halves of a plane
+  static constexpr int NT = TT * 4;                    // threads: 4 waves of 32 x 32 or 8 of 64 x 32
+  static constexpr int WC = TT / 32;                   // waves along the columns (two along the rows)
+  static constexpr int F = TT / 64;                    // 32 x 32 fragments of a wave, one above the other
 };
+template <int TT> constexpr int tile_lds() { return 2 * 2 * 2 * Geo<TT>::PL * 2; }   // buffers, operands, planes
 
+__device__ __forceinline__ f32x4 scale4(f32x4 v, int e) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(v[i], e);
+  return v;
+}
+
+// The loaders keep one 64-bit base a tile, the same for all lanes, and 32-bit offsets of their own (the host checks that 128
+// rows of a leading dimension fit them).
 // rows r0.. of a planes matrix, k contiguous (a symmetric matrix: also its columns)
-struct LoadPlanes {
+template <int TT> struct LoadPlanes {
   static constexpr bool two = true;
+  using G = Geo<TT>;
   const _Float16 *hi, *lo;
-  int64_t ld;
+  int ld;
   half8 v[4];
   __device__ __forceinline__ explicit LoadPlanes(const Planes &m) : hi(m.hi), lo(m.lo()), ld(m.np) {}
-  __device__ __forceinline__ void fetch(int r0, int64_t k0) {
-    const int row = threadIdx.x >> 3, k = (threadIdx.x & 7) * 8;
+  __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
+    const _Float16 *bh = hi + r0 * ld + k0, *bl = lo + r0 * ld + k0;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int64_t o = (int64_t)(r0 + row + 32 * p) * ld + k0 + k;
-      v[2 * p] = *reinterpret_cast<const half8 *>(hi + o);
-      v[2 * p + 1] = *reinterpret_cast<const half8 *>(lo + o);
+      const int o = ((threadIdx.x >> 3) + TT / 2 * p) * ld + (threadIdx.x & 7) * 8;
+      v[2 * p] = *reinterpret_cast<const half8 *>(bh + o);
+      v[2 * p + 1] = *reinterpret_cast<const half8 *>(bl + o);
     }
   }
-  __device__ __forceinline__ void store(Tile &t) const {
-    const int row = threadIdx.x >> 3, k = (threadIdx.x & 7) * 8;
+  __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      *reinterpret_cast<half8 *>(&t.hi[(row + 32 * p) * LDK + k]) = v[2 * p];
-      *reinterpret_cast<half8 *>(&t.lo[(row + 32 * p) * LDK + k]) = v[2 * p + 1];
+      const int o = ((threadIdx.x >> 3) + TT / 2 * p) * G::LD + (threadIdx.x & 7) * 8;
+      *reinterpret_cast<half8 *>(t + o) = v[2 * p];
+      *reinterpret_cast<half8 *>(t + G::PL + o) = v[2 * p + 1];
     }
   }
 };
 
+// (raw vectors are kept until they are stored: a conversion would wait for the load.  Tiles inside the matrix, which are
+// nearly all, take plain loads; at its edges every element is looked at.)
 // rows r0.. of a caller's matrix, k contiguous; zeros outside [rows) x [kmax)
-template <typename E> struct LoadK {
+template <int TT, typename E> struct LoadK {
   static constexpr bool two = sizeof(E) == 4;
+  using G = Geo<TT>;
+  using V = typename Vec4<E>::type;
   const E *p;
   int64_t ld, rows, kmax;
   int e;
-  float v[4][4];
+  V v[4];
   __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
-    const int64_t k = k0 + (threadIdx.x & 15) * 4;
+    const E *b = p + r0 * ld + k0;
+    const int row = threadIdx.x >> 4, k = (threadIdx.x & 15) * 4;
+    if (r0 + TT <= rows && k0 + G::BK <= kmax) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t row = r0 + (threadIdx.x >> 4) + 16 * q;
-      const E *s = p + row * ld + k;
-      if (row < rows && k + 4 <= kmax) {
-        if constexpr (sizeof(E) == 4) {
-          const f32x4u w = *reinterpret_cast<const f32x4u *>(s);
+      for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const V *>(b + (row + TT / 4 * q) * (int)ld + k);
+    } else {
+      const int nk = (int)min((int64_t)G::BK, kmax - k0) - k, nr = (int)min((int64_t)TT, rows - r0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[q][i] = w[i];
-        } else {
-          const bf16x4u w = *reinterpret_cast<const bf16x4u *>(s);
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[q][i] = (float)w[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[q][i] = row < rows && k + i < kmax ? (float)s[i] : 0.f;
-      }
+        for (int i = 0; i < 4; ++i) v[q][i] = row + TT / 4 * q < nr && i < nk ? b[(row + TT / 4 * q) * (int)ld + k + i] : (E)0.f;
     }
   }
-  __device__ __forceinline__ void store(Tile &t) const {
-    const int k = (threadIdx.x & 15) * 4;
+  __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int row = (threadIdx.x >> 4) + 16 * q;
+      const int o = ((threadIdx.x >> 4) + TT / 4 * q) * G::LD + (threadIdx.x & 15) * 4;
+      const V w = v[q];
       half4 hi, lo;
-      f32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __builtin_ldexpf(v[q][i], e);
-      split4(w, hi, lo);
-      *reinterpret_cast<half4 *>(&t.hi[row * LDK + k]) = hi;
-      if (two) *reinterpret_cast<half4 *>(&t.lo[row * LDK + k]) = lo;
+      split4(scale4(f32x4{(float)w[0], (float)w[1], (float)w[2], (float)w[3]}, e), hi, lo);
+      *reinterpret_cast<half4 *>(t + o) = hi;
+      if (two) *reinterpret_cast<half4 *>(t + G::PL + o) = lo;
     }
   }
 };
 
-// columns r0.. of a caller's matrix whose rows are k: element (r, k) at p[k * ld + r]
-template <typename E> struct LoadT {
+// columns r0.. of a caller's matrix whose rows are k: element (r, k) at p[k * ld + r].  A thread takes a block of 4 x 4: four
+// k's of four columns, so that loads and LDS writes are both vectors; a wave covers 32 columns of 32 k's (64 bytes or more
+// of a row, and LDS writes without bank conflicts).
+template <int TT, typename E> struct LoadT {
   static constexpr bool two = sizeof(E) == 4;
+  using G = Geo<TT>;
+  using V = typename Vec4<E>::type;
   const E *p;
   int64_t ld, rows, kmax;
   int e;
-  float v[2][8];
+  V v[4];                                              // v[k][column]
+  __device__ __forceinline__ int col() const { return (threadIdx.x >> 7) * 32 + (threadIdx.x & 7) * 4; }
+  __device__ __forceinline__ int kk() const { return (threadIdx.x >> 3 & 15) * 4; }
   __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
-    const int64_t row = r0 + (threadIdx.x & 63);
+    const E *b = p + k0 * ld + r0;
+    const int c = col(), k = kk();
+    if (r0 + TT <= rows && k0 + G::BK <= kmax) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const V *>(b + (k + i) * (int)ld + c);
+    } else {
+      const int nr = (int)min((int64_t)TT, rows - r0) - c, nk = (int)min((int64_t)G::BK, kmax - k0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t k = k0 + ((threadIdx.x >> 6) + 4 * q) * 8 + i;
-        v[q][i] = row < rows && k < kmax ? (float)p[k * ld + row] : 0.f;
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[i][q] = k + i < nk && q < nr ? b[(k + i) * (int)ld + c + q] : (E)0.f;
+    }
   }
-  __device__ __forceinline__ void store(Tile &t) const {
+  __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int o = (threadIdx.x & 63) * LDK + ((threadIdx.x >> 6) + 4 * q) * 8;
-      half4 hi[2], lo[2];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        f32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __builtin_ldexpf(v[q][4 * p + i], e);
-        split4(w, hi[p], lo[p]);
-      }
-      *reinterpret_cast<half8 *>(&t.hi[o]) = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      if (two) *reinterpret_cast<half8 *>(&t.lo[o]) = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int i = 0; i < 4; ++i) {
+      const int o = (col() + i) * G::LD + kk();
+      half4 hi, lo;
+      split4(scale4(f32x4{(float)v[0][i], (float)v[1][i], (float)v[2][i], (float)v[3][i]}, e), hi, lo);
+      *reinterpret_cast<half4 *>(t + o) = hi;
+      if (two) *reinterpret_cast<half4 *>(t + G::PL + o) = lo;
     }
   }
 };
 
-// acc = A-tile (rows ra..) . B-tile (rows rb..)^T over k in [k0, k1), k1 - k0 a multiple of BK.  The matrix cores add 64
-// k's, vector additions the steps of 64, and the small terms of the split have an accumulator of their own: a long chain
-// of additions to one fp32 sum would lose what the split keeps.
-template <class LA, class LB>
-__device__ __forceinline__ void tile_product(LA &la, LB &lb, int64_t ra, int64_t rb, int64_t k0, int64_t k1, Tile &ta, Tile &tb,
-                                             f32x16 &acc) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int fa = ((wave >> 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8;
-  const int fb = ((wave & 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8;
-  f32x16 cross = {};
-  acc = cross;
-  la.fetch(ra, k0);
-  lb.fetch(rb, k0);
-  for (int64_t k = k0; k < k1; k += BK) {
-    __syncthreads();
-    la.store(ta);
-    lb.store(tb);
-    __syncthreads();
-    if (k + BK < k1) {
-      la.fetch(ra, k + BK);
-      lb.fetch(rb, k + BK);
-    }
-    f32x16 sum = {};
+// acc = A-tile (rows ra..) . B-tile (rows rb..)^T over k in [k0, k1), whole steps.  The matrix cores add a step's products,
+// the split's small terms first, and vector additions the steps: a long chain of additions to one fp32 sum would lose what
+// the split keeps.  same: both operands are the same rows, loaded once.
+// late(): called when the first loads are on their way (sets the scale exponents the stores use).
+template <int TT, class LA, class LB, class Late>
+__device__ __forceinline__ void tile_product(LA &la, LB &lb, int64_t ra, int64_t rb, int64_t k0, int64_t k1, _Float16 *lds,
+                                             f32x16 (&acc)[Geo<TT>::F], bool same, Late late) {
+  using G = Geo<TT>;
+  constexpr int F = G::F, BUF = 4 * G::PL;             // a buffer: operand A's two planes, operand B's
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / G::WC, wc = wave % G::WC;
+  const int fa = (wr * 32 * F + (lane & 31)) * G::LD + (lane >> 5) * 8;
+  const int fb = (wc * 32 + (lane & 31)) * G::LD + (lane >> 5) * 8 + (same ? 0 : 2 * G::PL);
+  const int n = (int)((k1 - k0) / G::BK);
 #pragma unroll
-    for (int s = 0; s < BK; s += 16) {
-      const half8 ah = *reinterpret_cast<const half8 *>(&ta.hi[fa + s]);
-      const half8 bh = *reinterpret_cast<const half8 *>(&tb.hi[fb + s]);
-      sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, sum, 0, 0, 0);
-      if constexpr (LB::two) {
-        const half8 bl = *reinterpret_cast<const half8 *>(&tb.lo[fb + s]);
-        cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, cross, 0, 0, 0);
+  for (int i = 0; i < F; ++i) acc[i] = f32x16{};
+  auto fetch = [&](int step) {
+    la.fetch(ra, k0 + (int64_t)step * G::BK);
+    if (!same) lb.fetch(rb, k0 + (int64_t)step * G::BK);
+  };
+  auto store = [&](_Float16 *t) {
+    la.store(t);
+    if (!same) lb.store(t + 2 * G::PL);
+  };
+  auto at = [](const _Float16 *t) { return *reinterpret_cast<const half8 *>(t); };
+  auto compute = [&](const _Float16 *t) {
+    f32x16 sum[F] = {};
+#pragma unroll
+    for (int k = 0; k < G::BK; k += 32) {
+      half8 ah[2][F], bh[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int o = k + h * 16;
+        bh[h] = at(t + fb + o);
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+          ah[h][i] = at(t + fa + i * 32 * G::LD + o);
+          if constexpr (LA::two)
+            sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + G::PL + fa + i * 32 * G::LD + o), bh[h], sum[i], 0, 0, 0);
+        }
+        if constexpr (LB::two) {
+          const half8 bl = at(t + G::PL + fb + o);
+#pragma unroll
+          for (int i = 0; i < F; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[h][i], bl, sum[i], 0, 0, 0);
+        }
       }
-      if constexpr (LA::two) {
-        const half8 al = *reinterpret_cast<const half8 *>(&ta.lo[fa + s]);
-        cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, cross, 0, 0, 0);
-      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < F; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[h][i], bh[h], sum[i], 0, 0, 0);
     }
-    acc += sum;
+#pragma unroll
+    for (int i = 0; i < F; ++i) acc[i] += sum[i];
+  };
+  fetch(0);
+  late();
+  store(lds);
+  if (n > 1) fetch(1);
+  __syncthreads();
+  // (a step's products and the next one's conversion are one straight piece of code, in which they overlap; the loads of the
+  //  step behind that have one step's time)
+  for (int s = 0; s + 1 < n; ++s) {
+    compute(lds + (s & 1) * BUF);
+    store(lds + (s & 1 ^ 1) * BUF);
+    if (s + 2 < n) fetch(s + 2);
+    __syncthreads();
   }
-  acc += cross;
+  compute(lds + (n - 1 & 1) * BUF);
 }
-// accumulator element i of a lane: row frag_row(i) + wave row, column lane & 31 + wave column
-__device__ __forceinline__ int frag_row(int i) {
-  return ((threadIdx.x >> 7) * 32) + 8 * (i >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (i & 3);
+// calls f(row, column, value) for a lane's elements of the tile
+template <int TT, class Fn>
+__device__ __forceinline__ void each_element(const f32x16 (&acc)[Geo<TT>::F], Fn f) {
+  using G = Geo<TT>;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < G::F; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      f((wave / G::WC * G::F + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), wave % G::WC * 32 + (lane & 31), acc[i][e]);
 }
-__device__ __forceinline__ int frag_col() { return ((threadIdx.x >> 6) & 1) * 32 + (threadIdx.x & 31); }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Gram matrix of the long side, K split over workgroups: partial tiles [tile][slice][64][64] of the scaled matrix
+// Gram matrix of the long side, K split over workgroups: partial tiles [tile][slice][TT][TT] of the scaled matrix
 // ---------------------------------------------------------------------------------------------------------------------
 struct GramJob {
   const void *x;
@@ -340,48 +383,59 @@ struct GramArgs {
   int n;
 };
 
-template <class L>
-__device__ __forceinline__ void gram_tile(const GramJob &j, int ti, int tj, int64_t k0, int64_t k1, int e, Tile &ta, Tile &tb,
-                                          f32x16 &acc) {
+template <int TT, class L>
+__device__ __forceinline__ void gram_tile(const GramJob &j, int ti, int tj, int64_t k0, int64_t k1, uint32_t *red, _Float16 *lds,
+                                          f32x16 (&acc)[Geo<TT>::F]) {
   L la, lb;
   la.p = reinterpret_cast<decltype(la.p)>(j.x);
-  la.ld = j.ld; la.rows = j.n; la.kmax = j.K; la.e = e;
-  lb = la;
-  tile_product(la, lb, (int64_t)ti * T, (int64_t)tj * T, k0, k1, ta, tb, acc);
+  la.ld = j.ld; la.rows = j.n; la.kmax = j.K;
+  lb.p = la.p; lb.ld = la.ld; lb.rows = la.rows; lb.kmax = la.kmax;
+  tile_product<TT>(la, lb, (int64_t)ti * TT, (int64_t)tj * TT, k0, k1, lds, acc, ti == tj,
+                   [&] { la.e = lb.e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
 }
 
-__global__ __launch_bounds__(256) void orth_gram_kernel(GramArgs a) {
-  __shared__ Tile ta, tb;
-  __shared__ uint32_t red[4];
-  __shared__ float tr[4];
+// KIND: what all of a launch's matrices are (bit 0: wide, bit 1: bf16), or ANY: one loader's registers instead of the
+// largest of four let twice as many workgroups of a CU wait for memory at a time
+constexpr int ANY = 4;
+__device__ __host__ __forceinline__ bool is_kind(int kind, bool tall, int dtype) { return kind == (tall ? 0 : 1) + (dtype == AGX_F32 ? 0 : 2); }
+
+template <int TT, int KIND>
+__global__ __launch_bounds__(TT * 4, 2) void orth_gram_kernel(GramArgs a) {
+  extern __shared__ _Float16 lds[];
+  __shared__ uint32_t red[8];
+  __shared__ float tr[8];
+  // (the tiles of one slice follow each other on one XCD, whose L2 then reads the slice once)
+  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
-  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
+  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const GramJob &j = a.job[q];
-  const int local = blockIdx.x - j.first, tile = local / j.slices, slice = local % j.slices;
+  const int tiles = j.nt * (j.nt + 1) / 2, slice = (id - j.first) / tiles, tile = (id - j.first) % tiles;
   int ti, tj;
   upper_tile(tile, j.nt, ti, tj);
-  const int64_t k0 = (int64_t)slice * j.kper, k1 = k0 + j.kper;   // (slices end inside K rounded up; loads stop at K)
-  const int e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e;
-  f32x16 acc;
-  if (j.dtype == AGX_F32) {
-    if (j.tall) gram_tile<LoadT<float>>(j, ti, tj, k0, k1, e, ta, tb, acc);
-    else gram_tile<LoadK<float>>(j, ti, tj, k0, k1, e, ta, tb, acc);
-  } else {
-    if (j.tall) gram_tile<LoadT<__bf16>>(j, ti, tj, k0, k1, e, ta, tb, acc);
-    else gram_tile<LoadK<__bf16>>(j, ti, tj, k0, k1, e, ta, tb, acc);
-  }
-  float *p = j.part + ((int64_t)tile * j.slices + slice) * T * T;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) p[frag_row(i) * T + frag_col()] = acc[i];
+  const int64_t k0 = (int64_t)slice * j.kper, k1 = min(k0 + j.kper, (j.K + Geo<TT>::BK - 1) / Geo<TT>::BK * Geo<TT>::BK);
+  f32x16 acc[Geo<TT>::F];
+  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
+  if (is(0)) gram_tile<TT, LoadT<TT, float>>(j, ti, tj, k0, k1, red, lds, acc);
+  else if (is(1)) gram_tile<TT, LoadK<TT, float>>(j, ti, tj, k0, k1, red, lds, acc);
+  else if (is(2)) gram_tile<TT, LoadT<TT, __bf16>>(j, ti, tj, k0, k1, red, lds, acc);
+  else gram_tile<TT, LoadK<TT, __bf16>>(j, ti, tj, k0, k1, red, lds, acc);
+  float *p = j.part + ((int64_t)tile * j.slices + slice) * TT * TT;
+  float d = 0.f;
+  const int wave = threadIdx.x >> 6;
+  if (ti != tj || wave / Geo<TT>::WC <= wave % Geo<TT>::WC * 2 / Geo<TT>::WC)   // (not the quarter below the diagonal)
+  each_element<TT>(acc, [&](int r, int c, float v) {
+    p[r * TT + c] = v;
+    if (r == c) d += v;
+  });
   if (ti == tj) {
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) d += frag_row(i) == frag_col() ? acc[i] : 0.f;
     d = agx::wave_sum(d);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) tr[threadIdx.x >> 6] = d;
     __syncthreads();
-    if (threadIdx.x == 0) j.trace[ti * j.slices + slice] = tr[0] + tr[1] + tr[2] + tr[3];
+    if (threadIdx.x == 0) {
+      d = 0.f;
+      for (int i = 0; i < Geo<TT>::NT / 64; ++i) d += tr[i];
+      j.trace[ti * j.slices + slice] = d;
+    }
   }
 }
 
@@ -426,7 +480,6 @@ __device__ __forceinline__ void store_planes4(_Float16 *hi, _Float16 *lo, int ld
   pairs(l, lo);
 }
 
-constexpr int RCH = T * T / 256;   // workgroups a tile
 // A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase; the scaled matrix's trace is |X|_F^2) or
 // without a divisor (later phases).  Every workgroup sums the trace itself, in the same order.
 struct ReduceJob {
@@ -434,7 +487,7 @@ struct ReduceJob {
   const uint32_t *maxb;
   double *invd;                 // 1 / d of the scaled matrix, for the product with the long side (phase 0)
   Planes A;
-  int32_t nt, slices, e, nb, normalise, first;
+  int32_t nt, slices, e, nb, normalise, side, first;   // side: of the partial tiles
 };
 struct ReduceArgs {
   ReduceJob job[AGX_MAX_ORTH];
@@ -442,18 +495,22 @@ struct ReduceArgs {
   float eps;
 };
 __global__ __launch_bounds__(256) void orth_reduce_kernel(ReduceArgs a) {
+  __shared__ float part[4][64];
   __shared__ uint32_t red[4];
   __shared__ double tr[4];
   int q = 0;
   while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
   const ReduceJob &j = a.job[q];
-  const int tile = (blockIdx.x - j.first) / RCH, z = (blockIdx.x - j.first) % RCH * 256 + threadIdx.x;
+  // (64 elements of a tile a workgroup, by four interleaved shares of the slices)
+  const int area = j.side * j.side, tile = (blockIdx.x - j.first) / (area / 64), grp = threadIdx.x >> 6;
+  const int z = (blockIdx.x - j.first) % (area / 64) * 64 + (threadIdx.x & 63);
   int ti, tj;
   upper_tile(tile, j.nt, ti, tj);
   float sum = 0.f;
-  const float *p = j.part + (int64_t)tile * j.slices * T * T + z;
+  const float *p = j.part + (int64_t)tile * j.slices * area + z;
 #pragma unroll 8
-  for (int c = 0; c < j.slices; ++c) sum += p[(int64_t)c * T * T];
+  for (int c = grp; c < j.slices; c += 4) sum += p[(int64_t)c * area];
+  part[grp][threadIdx.x & 63] = sum;
   double f;
   if (j.normalise) {
     const int e = scale_exponent(j.maxb, j.nb, red);
@@ -470,7 +527,10 @@ __global__ __launch_bounds__(256) void orth_reduce_kernel(ReduceArgs a) {
   } else {
     f = ldexp(1.0, j.A.e - 2 * j.e);
   }
-  store_symmetric(j.A, (int64_t)ti * T + z / T, (int64_t)tj * T + z % T, (float)((double)sum * f));
+  __syncthreads();
+  if (grp) return;
+  sum = part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+  store_symmetric(j.A, (int64_t)ti * j.side + z / j.side, (int64_t)tj * j.side + z % j.side, (float)((double)sum * f));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -487,26 +547,27 @@ struct ChainArgs {
 };
 static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 
-__global__ __launch_bounds__(256) void orth_chain_kernel(ChainArgs a) {
-  __shared__ Tile ta, tb;
+template <int TT>
+__global__ __launch_bounds__(TT * 4, 2) void orth_chain_kernel(ChainArgs a) {
+  extern __shared__ _Float16 lds[];
+  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
-  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
+  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const ChainJob &j = a.job[q];
   int ti, tj;
-  upper_tile(blockIdx.x - j.first, j.nt, ti, tj);
-  LoadPlanes la(j.L), lb(j.R);
-  f32x16 acc;
-  tile_product(la, lb, ti * T, tj * T, 0, j.C.np, ta, tb, acc);
+  upper_tile(id - j.first, j.nt, ti, tj);
+  LoadPlanes<TT> la(j.L), lb(j.R);
+  f32x16 acc[Geo<TT>::F];
+  tile_product<TT>(la, lb, ti * TT, tj * TT, 0, j.C.np, lds, acc, ti == tj && j.L.hi == j.R.hi, [] {});
   const float fa = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
   const float fb = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fi = __builtin_ldexpf(j.gamma, j.C.e);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t r = (int64_t)ti * T + frag_row(i), c = (int64_t)tj * T + frag_col(), o = r * j.C.np + c;
+  each_element<TT>(acc, [&](int tr, int tc, float v) {
+    const int64_t r = (int64_t)ti * TT + tr, c = (int64_t)tj * TT + tc;
+    if (r > c) return;
     float w = r == c && r < j.n ? fi : 0.f;
-    if (j.beta != 0.f) w = fmaf(fb, plane_value(j.E, o), w);
-    const float v = fmaf(fa, acc[i], w);
-    store_symmetric(j.C, r, c, v);
-  }
+    if (j.beta != 0.f) w = fmaf(fb, plane_value(j.E, r * j.C.np + c), w);
+    store_symmetric(j.C, r, c, fmaf(fa, v, w));
+  });
 }
 
 // The same for small matrices, where a launch is all latency: tiles of 32 x 32 (36 of them at n = 256), k dealt to the four
@@ -724,46 +785,81 @@ struct ApplyArgs {
   int n;
 };
 
-template <typename E>
-__device__ __forceinline__ void apply_tile(const ApplyJob &j, int tr, int tc, int e, Tile &ta, Tile &tb, f32x16 &acc) {
-  LoadPlanes lq(j.Q);
-  if (j.tall) {
-    LoadK<E> lx;
-    lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.rows; lx.kmax = j.cols; lx.e = e;
-    tile_product(lx, lq, (int64_t)tr * T, (int64_t)tc * T, 0, j.Q.np, ta, tb, acc);
+template <int TT, typename E, bool TALL>
+__device__ __forceinline__ void apply_tile(const ApplyJob &j, int tr, int tc, int &e, uint32_t *red, _Float16 *lds,
+                                           f32x16 (&acc)[Geo<TT>::F]) {
+  LoadPlanes<TT> lq(j.Q);
+  if constexpr (TALL) {
+    LoadK<TT, E> lx;
+    lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.rows; lx.kmax = j.cols;
+    tile_product<TT>(lx, lq, (int64_t)tr * TT, (int64_t)tc * TT, 0, j.Q.np, lds, acc, false,
+                     [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
   } else {
-    LoadT<E> lx;
-    lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.cols; lx.kmax = j.rows; lx.e = e;
-    tile_product(lq, lx, (int64_t)tr * T, (int64_t)tc * T, 0, j.Q.np, ta, tb, acc);
+    LoadT<TT, E> lx;
+    lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.cols; lx.kmax = j.rows;
+    tile_product<TT>(lq, lx, (int64_t)tr * TT, (int64_t)tc * TT, 0, j.Q.np, lds, acc, false,
+                     [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
   }
 }
 
-__global__ __launch_bounds__(256) void orth_apply_kernel(ApplyArgs a) {
-  __shared__ Tile ta, tb;
-  __shared__ uint32_t red[4];
+template <int TT, int KIND>
+__global__ __launch_bounds__(TT * 4, 2) void orth_apply_kernel(ApplyArgs a) {
+  extern __shared__ _Float16 lds[];
+  __shared__ uint32_t red[8];
+  // (tiles that read the same part of X follow each other on one XCD)
+  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
-  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
+  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const ApplyJob &j = a.job[q];
-  const int tr = (blockIdx.x - j.first) / j.tc, tc = (blockIdx.x - j.first) % j.tc;
-  const int e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e;
-  f32x16 acc;
-  if (j.dtype == AGX_F32) apply_tile<float>(j, tr, tc, e, ta, tb, acc);
-  else apply_tile<__bf16>(j, tr, tc, e, ta, tb, acc);
-  // (in 64 bits: 1 / d spans more than fp32's exponents for tiny matrices)
+  const int trs = (j.rows + TT - 1) / TT, local = id - j.first;
+  const int tr = j.tall ? local / j.tc : local % trs, tc = j.tall ? local % j.tc : local / trs;
+  int e;
+  f32x16 acc[Geo<TT>::F];
+  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
+  if (is(0)) apply_tile<TT, float, true>(j, tr, tc, e, red, lds, acc);
+  else if (is(1)) apply_tile<TT, float, false>(j, tr, tc, e, red, lds, acc);
+  else if (is(2)) apply_tile<TT, __bf16, true>(j, tr, tc, e, red, lds, acc);
+  else apply_tile<TT, __bf16, false>(j, tr, tc, e, red, lds, acc);
+  // (in 64 bits where the factor leaves fp32's normal range: tiny matrices)
   const double f = ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e);
+  const float ff = (float)f;
+  if (!(fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) && f != 0.0)
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t r = (int64_t)tr * T + frag_row(i), c = (int64_t)tc * T + frag_col();
-    if (r >= j.rows || c >= j.cols) continue;
-    const float y = (float)((double)acc[i] * f);
-    if (j.muon) {
-      float *w = reinterpret_cast<float *>(j.out) + r * j.ldo + c;
-      *w = j.decay * *w - j.step * y;
-    } else if (j.otype == AGX_F32) {
-      reinterpret_cast<float *>(j.out)[r * j.ldo + c] = y;
-    } else {
-      reinterpret_cast<__bf16 *>(j.out)[r * j.ldo + c] = (__bf16)y;
-    }
+    for (int i = 0; i < Geo<TT>::F; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[i][k] = (float)((double)acc[i][k] * f);
+  else
+#pragma unroll
+    for (int i = 0; i < Geo<TT>::F; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[i][k] *= ff;
+  const bool inside = (tr + 1) * TT <= j.rows && (tc + 1) * TT <= j.cols;
+  const int64_t at = (int64_t)tr * TT * j.ldo + (int64_t)tc * TT;
+  const int left = j.rows - tr * TT, right = j.cols - tc * TT, ldo = (int)j.ldo;
+  auto ok = [&](int r, int c) { return inside || (r < left && c < right); };
+  if (j.muon) {
+    float *w = reinterpret_cast<float *>(j.out) + at;
+    f32x16 old[Geo<TT>::F];
+    int n = 0;
+    each_element<TT>(acc, [&](int r, int c, float) {
+      old[n / 16][n % 16] = ok(r, c) ? w[r * ldo + c] : 0.f;
+      ++n;
+    });
+    n = 0;
+    each_element<TT>(acc, [&](int r, int c, float y) {
+      if (ok(r, c)) w[r * ldo + c] = j.decay * old[n / 16][n % 16] - j.step * y;
+      ++n;
+    });
+  } else if (j.otype == AGX_F32) {
+    float *o = reinterpret_cast<float *>(j.out) + at;
+    each_element<TT>(acc, [&](int r, int c, float y) {
+      if (ok(r, c)) o[r * ldo + c] = y;
+    });
+  } else {
+    __bf16 *o = reinterpret_cast<__bf16 *>(j.out) + at;
+    each_element<TT>(acc, [&](int r, int c, float y) {
+      if (ok(r, c)) o[r * ldo + c] = (__bf16)y;
+    });
   }
 }
 
@@ -780,11 +876,13 @@ struct Job {          // one matrix of a call
   int64_t ldm = 0;
   float decay = 0.f, step = 0.f;
   bool muon = false;
-  bool tall() const { return rows >= cols; }
+  bool square_wide = false;   // a square matrix is taken as the call's others are
+  bool tall() const { return rows > cols || (rows == cols && !square_wide); }
   int n() const { return std::min(rows, cols); }
   int64_t K() const { return std::max(rows, cols); }
-  int nt() const { return agx::cdiv(n(), T); }
-  int np() const { return nt() * T; }
+  int np() const { return n() <= T ? T : agx::cdiv(n(), 2 * T) * 2 * T; }
+  int side() const { return np() == T ? T : 2 * T; }             // of the Gram matrix's tiles
+  int tiles() const { const int nt = np() / side(); return nt * (nt + 1) / 2; }
 };
 
 struct Layout {       // workspace of one job, in bytes from its start
@@ -794,20 +892,36 @@ struct Layout {       // workspace of one job, in bytes from its start
 };
 int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
-// slices of a Gram product: about three workgroups a CU over all of the call's matrices
+// what all matrices of a launch are (orth_gram_kernel), one more of them taken in
+int joined_kind(int kind, bool tall, int dtype) {
+  const int k = (tall ? 0 : 1) + (dtype != AGX_F32 ? 2 : 0);
+  return kind < 0 || kind == k ? k : ANY;
+}
+template <class F> void by_kind(int kind, F f) {
+  switch (kind) {
+    case 0: f(std::integral_constant<int, 0>{}); break;
+    case 1: f(std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 2>{}); break;
+    case 3: f(std::integral_constant<int, 3>{}); break;
+    default: f(std::integral_constant<int, ANY>{});
+  }
+}
+
+// slices of a Gram product: about one workgroup a CU over all of the call's matrices (each writes, and the next launch
+// reads, a whole tile)
 void plan(const Job &j, int total_tiles, int phases, bool need_u, Layout &l) {
-  const int tiles = j.nt() * (j.nt() + 1) / 2;
-  const int64_t ksteps = agx::cdiv64(j.K(), BK);
-  const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() * 3 / std::max(1, total_tiles));
-  l.kper = agx::cdiv64(ksteps, std::min(ksteps, want)) * BK;
+  const int tiles = j.tiles(), bk = j.side() == T ? Geo<T>::BK : Geo<2 * T>::BK;
+  const int64_t ksteps = agx::cdiv64(j.K(), bk);
+  const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() / std::max(1, total_tiles));
+  l.kper = agx::cdiv64(ksteps, std::min(ksteps, want)) * bk;
   l.slices = (int)agx::cdiv64(j.K(), l.kper);
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
   l.maxb = take(MAXB * 4);
   l.invd = take(8);
   for (int64_t &m : l.mat) m = take((int64_t)j.np() * j.np() * 4);
-  l.part = take((int64_t)tiles * l.slices * T * T * 4);
-  l.trace = take((int64_t)j.nt() * l.slices * 4);
+  l.part = take((int64_t)tiles * l.slices * j.side() * j.side() * 4);
+  l.trace = take((int64_t)j.np() / j.side() * l.slices * 4);
   for (int k = 0; k < 2; ++k) l.x[k] = phases > 1 + k ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.u = need_u ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.end = off;
@@ -816,7 +930,7 @@ int phases_of(int steps) { return agx::cdiv(steps, PHASE); }
 
 int64_t ws_bytes(const Job *jobs, int n, int steps, bool need_u) {
   int tiles = 0;
-  for (int i = 0; i < n; ++i) tiles += jobs[i].nt() * (jobs[i].nt() + 1) / 2;
+  for (int i = 0; i < n; ++i) tiles += jobs[i].tiles();
   int64_t total = 0;
   for (int i = 0; i < n; ++i) {
     Layout l;
@@ -886,8 +1000,12 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     return AGX_E_WORKSPACE;
   }
   AGX_CHECK_ARG(agx::aligned16(ws), "%s: workspace must be 16-byte aligned", who);
-  int tiles = 0;
-  for (int i = 0; i < n; ++i) tiles += jobs[i].nt() * (jobs[i].nt() + 1) / 2;
+  int tiles = 0, wide = 0;
+  for (int i = 0; i < n; ++i) {
+    tiles += jobs[i].tiles();
+    wide += (jobs[i].rows < jobs[i].cols) - (jobs[i].rows > jobs[i].cols);
+  }
+  for (int i = 0; i < n; ++i) jobs[i].square_wide = wide > 0;
   const int phases = phases_of(o->steps);
   Layout lay[AGX_MAX_ORTH];
   char *base[AGX_MAX_ORTH];
@@ -942,30 +1060,41 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     const bool first = ph == 0, last = ph == phases - 1;
     const int ex = exponent_for(s);                 // scale of the iterate (later phases)
     {
-      GramArgs ga;
+      // (matrices of one tile of T and larger ones take different tiles: a launch for each kind that is there)
+      GramArgs ga[2];
       ReduceArgs ra;
-      ga.n = ra.n = n;
+      ga[0].n = ga[1].n = 0;
+      ra.n = n;
       ra.eps = o->eps;
-      int gb = 0, rb = 0;
+      int gb[2] = {0, 0}, rb = 0, kind[2] = {-1, -1};
       for (int i = 0; i < n; ++i) {
         const Job &j = jobs[i];
         const Layout &l = lay[i];
-        const int nt = j.nt(), tl = nt * (nt + 1) / 2;
-        GramJob &g = ga.job[i];
+        const int nt = j.np() / j.side(), tl = j.tiles(), w = j.side() == T ? 0 : 1;
+        GramJob &g = ga[w].job[ga[w].n++];
         g.x = x[i]; g.ld = ldx[i]; g.K = j.K(); g.kper = l.kper; g.n = j.n(); g.nt = nt; g.slices = l.slices; g.tall = j.tall();
         g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
         g.maxb = reinterpret_cast<const uint32_t *>(base[i] + l.maxb);
         g.part = reinterpret_cast<float *>(base[i] + l.part);
         g.trace = reinterpret_cast<float *>(base[i] + l.trace);
-        g.first = gb;
-        gb += tl * l.slices;
+        g.first = gb[w];
+        gb[w] += tl * l.slices;
+        kind[w] = joined_kind(kind[w], g.tall, g.dtype);
         ReduceJob &r = ra.job[i];
         r.part = g.part; r.trace = g.trace; r.maxb = g.maxb; r.invd = reinterpret_cast<double *>(base[i] + l.invd);
         r.A = planes(i, 0, exponent_for(s * s)); r.nt = nt; r.slices = l.slices; r.e = ex; r.nb = nb[i];
-        r.normalise = first; r.first = rb;
-        rb += tl * RCH;
+        r.normalise = first; r.side = j.side(); r.first = rb;
+        rb += tl * (j.side() * j.side() / 64);
       }
-      hipLaunchKernelGGL(orth_gram_kernel, dim3(gb), dim3(256), 0, st, ga);
+      if (ga[0].n)
+        by_kind(kind[0], [&](auto k) {
+          hipLaunchKernelGGL((orth_gram_kernel<T, decltype(k)::value>), dim3(gb[0]), dim3(256), tile_lds<T>(), st, ga[0]);
+        });
+      AGX_LAUNCH_CHECK();
+      if (ga[1].n)
+        by_kind(kind[1], [&](auto k) {
+          hipLaunchKernelGGL((orth_gram_kernel<2 * T, decltype(k)::value>), dim3(gb[1]), dim3(Geo<2 * T>::NT), tile_lds<2 * T>(), st, ga[1]);
+        });
       AGX_LAUNCH_CHECK();
       hipLaunchKernelGGL(orth_reduce_kernel, dim3(rb), dim3(256), 0, st, ra);
       AGX_LAUNCH_CHECK();
@@ -1027,12 +1156,12 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
           for (int w = 0; w < per && jobs[i].np() > ONE_BLOCK; ++w) {
             ChainJob &g = ca.job[ca.n++];
             memset(&g, 0, sizeof(g));
-            g.n = jobs[i].n(); g.nt = small ? jobs[i].np() / 32 : jobs[i].nt(); g.first = blocks; g.alpha = 1.f;
+            g.n = jobs[i].n(); g.nt = jobs[i].np() / (small ? 32 : T); g.first = blocks; g.alpha = 1.f;
             blocks += g.nt * (g.nt + 1) / 2;
             fill(g, i, w);
           }
         if (small) hipLaunchKernelGGL(orth_chain_small_kernel, dim3(blocks), dim3(256), 0, st, ca);
-        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(256), 0, st, ca);
+        else hipLaunchKernelGGL(orth_chain_kernel<T>, dim3(blocks), dim3(256), tile_lds<T>(), st, ca);
         AGX_LAUNCH_CHECK();
         return AGX_OK;
       };
@@ -1057,9 +1186,15 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
           g.C = planes(i, 0, eA[t + 1]);
         }));
     }
+    // tiles of 2 T where they fill the chip
+    int64_t big = 0;
+    for (int i = 0; i < n; ++i) big += agx::cdiv64(jobs[i].rows, 2 * T) * agx::cdiv64(jobs[i].cols, 2 * T);
+    bool use_big = big >= BIG_TILES;
+    for (int i = 0; i < n; ++i) use_big = use_big && jobs[i].np() > T;
+    const int side = use_big ? 2 * T : T;
     ApplyArgs aa;
     aa.n = n;
-    int blocks = 0;
+    int blocks = 0, kind = -1;
     for (int i = 0; i < n; ++i) {
       const Job &j = jobs[i];
       ApplyJob &g = aa.job[i];
@@ -1076,11 +1211,15 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         x[i] = g.out;
         ldx[i] = g.ldo;
       }
-      g.tc = agx::cdiv(j.cols, T);
+      kind = joined_kind(kind, g.tall, g.dtype);
+      g.tc = agx::cdiv(j.cols, side);
       g.first = blocks;
-      blocks += agx::cdiv(j.rows, T) * g.tc;
+      blocks += agx::cdiv(j.rows, side) * g.tc;
     }
-    hipLaunchKernelGGL(orth_apply_kernel, dim3(blocks), dim3(256), 0, st, aa);
+    by_kind(kind, [&](auto k) {
+      if (use_big) hipLaunchKernelGGL((orth_apply_kernel<2 * T, decltype(k)::value>), dim3(blocks), dim3(Geo<2 * T>::NT), tile_lds<2 * T>(), st, aa);
+      else hipLaunchKernelGGL((orth_apply_kernel<T, decltype(k)::value>), dim3(blocks), dim3(256), tile_lds<T>(), st, aa);
+    });
     AGX_LAUNCH_CHECK();
   }
   return AGX_OK;
@@ -1095,6 +1234,7 @@ int to_jobs(const agx_orth_t *j, int n, Job *out, const char *who) {
                   "%s: matrix %d is %d x %d; the smaller side is at most %d", who, i, a.rows, a.cols, AGX_ORTH_MAX_SIDE);
     AGX_CHECK_ARG((int64_t)a.rows * agx::cdiv64(a.cols, 4) < (1LL << 30) && agx::cdiv64(a.rows, T) * agx::cdiv64(a.cols, T) < (1 << 26),
                   "%s: matrix %d is too large", who, i);
+    AGX_CHECK_ARG(a.ldx < (1 << 23) && a.ldo < (1 << 23), "%s: matrix %d: leading dimension above 2^23", who, i);
     Job &b = out[i];
     b.x = a.x; b.out = a.out; b.ldx = a.ldx; b.ldo = a.ldo; b.rows = a.rows; b.cols = a.cols; b.dtype = a.dtype;
   }
@@ -1122,10 +1262,25 @@ int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, co
 
 }  // namespace
 
-// (a phase in one workgroup takes more LDS than the default limit of a launch)
+// (more LDS than the default limit of a launch)
+namespace {
+template <class K> hipError_t allow_lds(K *kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+}  // namespace
 int agx::orth_prepare_device() {
-  AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_phase_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              phase_lds(ONE_BLOCK)));
+  AGX_HIP(allow_lds(&orth_phase_kernel, phase_lds(ONE_BLOCK)));
+  AGX_HIP(allow_lds(&orth_chain_kernel<T>, tile_lds<T>()));
+  for (int kind = 0; kind <= ANY; ++kind) {
+    hipError_t e = hipSuccess;
+    by_kind(kind, [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      for (hipError_t r : {allow_lds(&orth_gram_kernel<T, K>, tile_lds<T>()), allow_lds(&orth_gram_kernel<2 * T, K>, tile_lds<2 * T>()),
+                           allow_lds(&orth_apply_kernel<T, K>, tile_lds<T>()), allow_lds(&orth_apply_kernel<2 * T, K>, tile_lds<2 * T>())})
+        if (r != hipSuccess) e = r;
+    });
+    AGX_HIP(e);
+  }
   return AGX_OK;
 }
 
@@ -1172,7 +1327,7 @@ extern "C" int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, con
   AGX_TRY(muon_jobs(jobs, n, o, j, who));
   for (int i = 0; i < n; ++i) {
     const agx_muon_t &a = jobs[i];
-    AGX_CHECK_ARG(a.w && a.g && a.m && a.ldw >= a.cols && a.ldg >= a.cols && a.ldm >= a.cols && std::isfinite(a.scale),
+    AGX_CHECK_ARG(a.w && a.g && a.m && a.ldw >= a.cols && a.ldg >= a.cols && a.ldm >= a.cols && a.ldm < (1 << 23) && std::isfinite(a.scale),
                   "%s: matrix %d: null, leading dimension or scale", who, i);
     AGX_CHECK_ARG(((reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.g) | reinterpret_cast<uintptr_t>(a.m)) & 3) == 0,
                   "%s: matrix %d not aligned to its elements", who, i);
