@@ -14,7 +14,13 @@ def device():
     return torch.device('cuda', idx)
 
 
+# (the handle of the current stream without building a Stream object: 0.1 instead of 2.7 us a call)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
 def stream():
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 

@@ -354,6 +354,10 @@ def check(rc, what=''):
 _initialised = set()
 
 
+def is_initialised(device_index):
+    return device_index in _initialised
+
+
 def init_device(device_index):
     """agx_init on first use of a device (verifies gfx950, caches the CU count)."""
     if device_index not in _initialised:

@@ -9,15 +9,17 @@
 //                dx = r^2 [h (3 mean(gh) mean(uh) + mean(g) mean(u) - mean(gu)) - mean(uh) (g - mean(g)) - mean(gh) (u - mean(u))]
 //   (act is a leaky ReLU of slope >= 0, whose derivative follows from the sign of its output y)
 //
-// All three are bound by HBM: 8 to 30 flops per element of 2 to 6 arrays.  A row is read ONCE and kept in registers by
-// the G threads that own it (16, 64: part of or one wave, no barrier; 256, 1024: a workgroup), C vectors of 16 bytes each,
-// so that the two passes of a centred variance and the 2 to 5 row means cost no second read.  Vectors are loaded at the
-// element's alignment (the hardware needs no more), so odd widths and strides take the same path as padded ones.
+// All three are bound by HBM: 8 to 30 flops per element of 2 to 6 arrays.  A row is read ONCE and kept in registers, as it
+// was stored, by the G threads that own it (16, 64: part of or one wave, no barrier; 256, 1024: a workgroup), C vectors of
+// 16 bytes each, so that the two passes of a centred variance and the 2 to 5 row means cost no second read.  Vectors are
+// loaded at the element's alignment (the hardware needs no more), so odd widths and strides take the same path as padded
+// ones; the up to 7 elements behind the last whole vector are one more element of as many threads.
 // Parameter gradients: every thread owns fixed columns, sums its rows in registers, the groups of a workgroup meet in
 // LDS, and a second launch adds the workgroups' partial rows in a fixed order (no atomics: bit-reproducible).
 #include "agx_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -34,40 +36,74 @@ template <> struct Vec<__bf16> {
   typedef bf16x8 __attribute__((aligned(2))) type;
 };
 
-// V elements from p[i..] of a row of n elements; zeros behind the row's end
-template <typename T>
-__device__ __forceinline__ void load_vec(const T *__restrict__ p, int64_t i, int64_t n, float (&o)[Vec<T>::V]) {
-  constexpr int V = Vec<T>::V;
-  if (i + V <= n) {
-    const typename Vec<T>::type v = *reinterpret_cast<const typename Vec<T>::type *>(p + i);
-#pragma unroll
-    for (int k = 0; k < V; ++k) o[k] = (float)v[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) o[k] = i + k < n ? (float)p[i + k] : 0.f;
+// A row as its group holds it: C whole vectors a thread, and one element of the row's end in the first few threads
+template <typename T, int G, int C>
+struct Row {
+  static constexpr int V = Vec<T>::V;
+  typename Vec<T>::type v[C];
+  T end;
+};
+// where a thread's vectors and its end element are; the same for all rows of a launch
+template <typename T, int G, int C>
+struct Place {
+  static constexpr int V = Vec<T>::V;
+  int t, nv, last;               // thread of the group, whole vectors of a row, index of the end element or -1
+  __device__ __forceinline__ explicit Place(int64_t n) : t(threadIdx.x % G), nv((int)(n / V)) {
+    last = t < (int)(n - (int64_t)nv * V) ? nv * V + t : -1;
   }
-}
-// (a 16-bit result is rounded once, to nearest even, from the 32-bit value)
-template <typename T>
-__device__ __forceinline__ void store_vec(T *__restrict__ p, int64_t i, int64_t n, const float (&o)[Vec<T>::V]) {
-  constexpr int V = Vec<T>::V;
-  if (i + V <= n) {
-    typename Vec<T>::type v;
+  __device__ __forceinline__ bool in(int c) const { return c * G + t < nv; }
+  __device__ __forceinline__ int at(int c) const { return (c * G + t) * V; }
+  __device__ __forceinline__ void load(Row<T, G, C> &r, const T *__restrict__ p) const {
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = (T)o[k];
-    *reinterpret_cast<typename Vec<T>::type *>(p + i) = v;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (i + k < n) p[i + k] = (T)o[k];
+    for (int c = 0; c < C; ++c) {
+      r.v[c] = typename Vec<T>::type{};
+      if (in(c)) r.v[c] = *reinterpret_cast<const typename Vec<T>::type *>(p + at(c));
+    }
+    r.end = last >= 0 ? p[last] : (T)0.f;
   }
-}
-// (parameter vectors: float, possibly absent)
+};
+// V parameters from p[i..]
 template <int V>
-__device__ __forceinline__ void load_param(const float *p, int64_t i, int64_t n, float absent, float (&o)[V]) {
+__device__ __forceinline__ void load_param(const float *p, int i, float absent, float (&o)[V]) {
+  if (!p) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) o[k] = p && i + k < n ? p[i + k] : absent;
+    for (int k = 0; k < V; ++k) o[k] = absent;
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    const Vec<float>::type w = *reinterpret_cast<const Vec<float>::type *>(p + i + 4 * q);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[4 * q + k] = w[k];
+  }
 }
+// parameters of a thread's columns, kept over all its rows where they are few
+template <typename T, int G, int C>
+struct Params {
+  static constexpr int V = Vec<T>::V;
+  static constexpr bool KEEP = C * V <= 16;
+  const float *p;
+  float absent, kept[KEEP ? C : 1][V], end;
+  __device__ __forceinline__ Params(const float *p_, float absent_, const Place<T, G, C> &w) : p(p_), absent(absent_) {
+    end = p && w.last >= 0 ? p[w.last] : absent;
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) kept[c][k] = absent;
+        if (w.in(c)) load_param<V>(p, w.at(c), absent, kept[c]);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(const Place<T, G, C> &w, int c, float (&o)[V]) const {
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[k] = kept[c][k];
+    } else {
+      load_param<V>(p, w.in(c) ? w.at(c) : 0, absent, o);
+    }
+  }
+};
 
 struct NormArgs {
   const void *x, *dy, *u, *ym;   // ym: forward output whose sign is the activation's derivative (NULL: no activation)
@@ -115,88 +151,98 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_fwd_kernel(NormArgs a) 
   constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
   __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
   int flip = 0;
-  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const Place<T, G, C> w(a.n);
+  const int grp = threadIdx.x / G;
   const float inv_n = 1.f / (float)a.n;
+  const Params<T, G, C> gamma(a.gamma, 1.f, w), beta(a.beta, 0.f, w);
+  auto act = [&](float n) { return a.act ? (n > 0.f ? n : a.slope * n) : n; };
   for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
-    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
-    float v[C][V];
-    float s[1] = {0.f};
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      load_vec<T>(x, ((int64_t)c * G + t) * V, a.n, v[c]);
-#pragma unroll
-      for (int k = 0; k < V; ++k) s[0] += v[c][k];
-    }
-    group_sum<G, 1>(s, red, flip);
-    const float mu = s[0] * inv_n;
-    s[0] = 0.f;
+    Row<T, G, C> x;
+    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
+    float s[1] = {(float)x.end};
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
+      for (int k = 0; k < V; ++k) s[0] += (float)x.v[c][k];
+    group_sum<G, 1>(s, red, flip);
+    const float mu = s[0] * inv_n;
+    const float de = (float)x.end - mu;
+    s[0] = w.last >= 0 ? de * de : 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float q = 0.f;
+#pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float d = v[c][k] - mu;
-        if (((int64_t)c * G + t) * V + k < a.n) s[0] += d * d;
+        const float d = (float)x.v[c][k] - mu;
+        q += d * d;
       }
+      if (w.in(c)) s[0] += q;
+    }
     group_sum<G, 1>(s, red, flip);
     const float r = 1.f / sqrtf(s[0] * inv_n + a.eps);
-    if (t == 0) {
+    if (w.t == 0) {
       if (a.mean) a.mean[row] = mu;
       if (a.rstd) a.rstd[row] = r;
     }
     T *y = reinterpret_cast<T *>(a.y) + row * a.ldy;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = ((int64_t)c * G + t) * V;
-      if (i >= a.n) continue;
       float ga[V], be[V];
-      load_param<V>(a.gamma, i, a.n, 1.f, ga);
-      load_param<V>(a.beta, i, a.n, 0.f, be);
+      gamma.get(w, c, ga);
+      beta.get(w, c, be);
+      typename Vec<T>::type o;
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float n = (v[c][k] - mu) * r * ga[k] + be[k];
-        v[c][k] = a.act ? (n > 0.f ? n : a.slope * n) : n;
-      }
-      store_vec<T>(y, i, a.n, v[c]);
+      for (int k = 0; k < V; ++k) o[k] = (T)act(((float)x.v[c][k] - mu) * r * ga[k] + be[k]);
+      if (w.in(c)) *reinterpret_cast<typename Vec<T>::type *>(y + w.at(c)) = o;
     }
+    if (w.last >= 0) y[w.last] = (T)act(de * r * gamma.end + beta.end);
   }
 }
 
 // the workgroup's partial sums of NA parameter gradients: groups meet in LDS in a fixed order
 template <typename T, int G, int C, int NA>
-__device__ __forceinline__ void write_partials(float (&acc)[NA][C][Vec<T>::V], const NormArgs &a, float *lds) {
-  constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
-  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+__device__ __forceinline__ void write_partials(float (&acc)[NA][C][Vec<T>::V], float (&end)[NA], const Place<T, G, C> &w,
+                                               const NormArgs &a, float *lds) {
+  constexpr int V = Vec<T>::V, NG = block_threads<G>() / G, W = G * C * V + V;   // (a group's columns, then its end elements)
+  const int grp = threadIdx.x / G;
 #pragma unroll
   for (int q = 0; q < NA; ++q) {
+    float *p = a.part + ((int64_t)blockIdx.x * 2 + q) * a.n;
     if constexpr (NG > 1) {
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int k = 0; k < V; ++k) lds[(grp * C + c) * G * V + t * V + k] = acc[q][c][k];
+        for (int k = 0; k < V; ++k) lds[grp * W + w.at(c) + k] = acc[q][c][k];
+      if (w.t < V) lds[grp * W + G * C * V + w.t] = end[q];
       __syncthreads();
-    }
-    float *p = a.part + ((int64_t)blockIdx.x * 2 + q) * a.n;
-    if constexpr (NG > 1) {
-      for (int64_t i = threadIdx.x; i < a.n; i += block_threads<G>()) {
+      for (int i = threadIdx.x; i < a.n; i += block_threads<G>()) {
+        const int o = i < w.nv * V ? i : G * C * V + i - w.nv * V;
         float s = 0.f;
-        for (int g = 0; g < NG; ++g) s += lds[g * C * G * V + i];
+        for (int g = 0; g < NG; ++g) s += lds[g * W + o];
         p[i] = s;
       }
     } else {
 #pragma unroll
       for (int c = 0; c < C; ++c)
+        if (w.in(c))
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const int64_t i = ((int64_t)c * G + t) * V + k;
-          if (i < a.n) p[i] = acc[q][c][k];
-        }
+          for (int k = 0; k < V; ++k) p[w.at(c) + k] = acc[q][c][k];
+      if (w.last >= 0) p[w.last] = end[q];
     }
   }
 }
-
 template <typename T, int G, int C> constexpr int lds_floats() {
-  return block_threads<G>() / G > 1 ? block_threads<G>() * C * Vec<T>::V : 1;
+  return block_threads<G>() / G > 1 ? block_threads<G>() / G * (G * C * Vec<T>::V + Vec<T>::V) : 1;
+}
+
+// bit k of the result: the activation's derivative at element k is the slope (ym not positive)
+template <typename T>
+__device__ __forceinline__ uint32_t not_positive(const typename Vec<T>::type &m) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int k = 0; k < Vec<T>::V; ++k) b |= (float)m[k] > 0.f ? 0u : 1u << k;
+  return b;
 }
 
 template <typename T, int G, int C, bool PG>
@@ -205,39 +251,51 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) 
   __shared__ float red[G > 64 ? 2 * 2 * (G / 64) : 1];
   __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
   int flip = 0;
-  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const Place<T, G, C> w(a.n);
+  const int grp = threadIdx.x / G;
   const float inv_n = 1.f / (float)a.n;
-  float acc[2][C][V] = {};
+  const Params<T, G, C> gamma(a.gamma, 1.f, w);
+  float acc[2][C][V] = {}, aend[2] = {0.f, 0.f};
   for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
-    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
-    const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
-    const T *ym = reinterpret_cast<const T *>(a.ym) + row * a.ldym;
+    Row<T, G, C> x, dy;
+    uint32_t neg[C] = {}, nend = 0;
+    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
+    w.load(dy, reinterpret_cast<const T *>(a.dy) + row * a.lddy);
+    if (a.ym) {
+      Row<T, G, C> m;
+      w.load(m, reinterpret_cast<const T *>(a.ym) + row * a.ldym);
+#pragma unroll
+      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(m.v[c]);
+      nend = (float)m.end > 0.f ? 0u : 1u;
+    }
     const float mu = a.mean_in[row], r = a.rstd_in[row];
-    float h[C][V], g[C][V];
-    float s[2] = {0.f, 0.f};
+    auto hat = [&](int c, int k) { return ((float)x.v[c][k] - mu) * r; };
+    auto dn = [&](int c, int k) { return neg[c] >> k & 1 ? a.slope * (float)dy.v[c][k] : (float)dy.v[c][k]; };
+    const float he = w.last >= 0 ? ((float)x.end - mu) * r : 0.f, de = nend ? a.slope * (float)dy.end : (float)dy.end;
+    const float ge = de * gamma.end;
+    if constexpr (PG) {
+      aend[0] += de * he;
+      aend[1] += de;
+    }
+    float s[2] = {ge, ge * he};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = ((int64_t)c * G + t) * V;
-      load_vec<T>(x, i, a.n, h[c]);
-      load_vec<T>(dy, i, a.n, g[c]);
-      if (a.ym) {
-        float m[V];
-        load_vec<T>(ym, i, a.n, m);
-#pragma unroll
-        for (int k = 0; k < V; ++k) g[c][k] = m[k] > 0.f ? g[c][k] : a.slope * g[c][k];
-      }
-      float ga[V];
-      load_param<V>(a.gamma, i, a.n, 1.f, ga);
+      float ga[V], q[2] = {0.f, 0.f};
+      gamma.get(w, c, ga);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        h[c][k] = i + k < a.n ? (h[c][k] - mu) * r : 0.f;
+        const float h = hat(c, k), d = dn(c, k);
         if constexpr (PG) {
-          acc[0][c][k] += g[c][k] * h[c][k];
-          acc[1][c][k] += g[c][k];
+          acc[0][c][k] += d * h;
+          acc[1][c][k] += d;
         }
-        g[c][k] *= ga[k];
-        s[0] += g[c][k];
-        s[1] += g[c][k] * h[c][k];
+        const float g = d * ga[k];
+        q[0] += g;
+        q[1] += g * h;
+      }
+      if (w.in(c)) {       // (behind the row's end d is 0, but h may not be finite)
+        s[0] += q[0];
+        s[1] += q[1];
       }
     }
     if (a.dx) {
@@ -246,20 +304,24 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) 
       T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int64_t i = ((int64_t)c * G + t) * V;
-        if (i >= a.n) continue;
-        float o[V];
-        if (a.add_dx) load_vec<T>(dx, i, a.n, o);
+        float ga[V];
+        gamma.get(w, c, ga);
+        typename Vec<T>::type o = {};
+        if (a.add_dx && w.in(c)) o = *reinterpret_cast<const typename Vec<T>::type *>(dx + w.at(c));
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float d = r * (g[c][k] - mg - h[c][k] * mgh);
-          o[k] = a.add_dx ? o[k] + d : d;
+          const float d = r * (dn(c, k) * ga[k] - mg - hat(c, k) * mgh);
+          o[k] = (T)(a.add_dx ? (float)o[k] + d : d);
         }
-        store_vec<T>(dx, i, a.n, o);
+        if (w.in(c)) *reinterpret_cast<typename Vec<T>::type *>(dx + w.at(c)) = o;
+      }
+      if (w.last >= 0) {
+        const float d = r * (ge - mg - he * mgh);
+        dx[w.last] = (T)(a.add_dx ? (float)dx[w.last] + d : d);
       }
     }
   }
-  if constexpr (PG) write_partials<T, G, C, 2>(acc, a, lds);
+  if constexpr (PG) write_partials<T, G, C, 2>(acc, aend, w, a, lds);
 }
 
 template <typename T, int G, int C, bool PG>
@@ -268,74 +330,79 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd2_kernel(NormArgs a)
   __shared__ float red[G > 64 ? 2 * 5 * (G / 64) : 1];
   __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
   int flip = 0;
-  const int t = threadIdx.x % G, grp = threadIdx.x / G;
+  const Place<T, G, C> w(a.n);
+  const int grp = threadIdx.x / G;
   const float inv_n = 1.f / (float)a.n;
-  float acc[1][C][V] = {};
+  const Params<T, G, C> gamma(a.gamma, 1.f, w);
+  float acc[1][C][V] = {}, aend[1] = {0.f};
   for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
-    const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
-    const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
-    const T *up = reinterpret_cast<const T *>(a.u) + row * a.ldu;
-    const T *ym = reinterpret_cast<const T *>(a.ym) + row * a.ldym;
+    Row<T, G, C> x, dy, u;
+    uint32_t neg[C] = {}, nend = 0;
+    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
+    w.load(dy, reinterpret_cast<const T *>(a.dy) + row * a.lddy);
+    w.load(u, reinterpret_cast<const T *>(a.u) + row * a.ldu);
+    if (a.ym) {
+      Row<T, G, C> m;
+      w.load(m, reinterpret_cast<const T *>(a.ym) + row * a.ldym);
+#pragma unroll
+      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(m.v[c]);
+      nend = (float)m.end > 0.f ? 0u : 1u;
+    }
     const float mu = a.mean_in[row], r = a.rstd_in[row];
-    float h[C][V], d[C][V], u[C][V];   // d: dn (before gamma)
-    uint32_t neg[C];                   // bit k: the activation's derivative is the slope
-    float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+    auto hat = [&](int c, int k) { return ((float)x.v[c][k] - mu) * r; };
+    auto dn = [&](int c, int k) { return neg[c] >> k & 1 ? a.slope * (float)dy.v[c][k] : (float)dy.v[c][k]; };
+    const float he = w.last >= 0 ? ((float)x.end - mu) * r : 0.f, de = nend ? a.slope * (float)dy.end : (float)dy.end;
+    const float ge = de * gamma.end, ue = (float)u.end;
+    float s[5] = {ge, ge * he, ue, ue * he, ge * ue};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = ((int64_t)c * G + t) * V;
-      load_vec<T>(x, i, a.n, h[c]);
-      load_vec<T>(dy, i, a.n, d[c]);
-      load_vec<T>(up, i, a.n, u[c]);
-      neg[c] = 0;
-      if (a.ym) {
-        float m[V];
-        load_vec<T>(ym, i, a.n, m);
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (!(m[k] > 0.f)) {
-            neg[c] |= 1u << k;
-            d[c][k] *= a.slope;
-          }
-      }
-      float ga[V];
-      load_param<V>(a.gamma, i, a.n, 1.f, ga);
+      float ga[V], q[5] = {};
+      gamma.get(w, c, ga);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        h[c][k] = i + k < a.n ? (h[c][k] - mu) * r : 0.f;
-        const float g = d[c][k] * ga[k];
-        s[0] += g;
-        s[1] += g * h[c][k];
-        s[2] += u[c][k];
-        s[3] += u[c][k] * h[c][k];
-        s[4] += g * u[c][k];
+        const float h = hat(c, k), g = dn(c, k) * ga[k], uu = (float)u.v[c][k];
+        q[0] += g;
+        q[1] += g * h;
+        q[2] += uu;
+        q[3] += uu * h;
+        q[4] += g * uu;
       }
+      if (w.in(c))
+#pragma unroll
+        for (int k = 0; k < 5; ++k) s[k] += q[k];
     }
     group_sum<G, 5>(s, red, flip);
     const float mg = s[0] * inv_n, mgh = s[1] * inv_n, mu_ = s[2] * inv_n, muh = s[3] * inv_n, mgu = s[4] * inv_n;
     const float hc = 3.f * mgh * muh + mg * mu_ - mgu, r2 = r * r;
     T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
     T *ddy = reinterpret_cast<T *>(a.ddy) + row * a.ldddy;
+    auto second = [&](float h, float g, float uu) { return r2 * (h * hc - muh * (g - mg) - mgh * (uu - mu_)); };
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int64_t i = ((int64_t)c * G + t) * V;
-      if (i >= a.n) continue;
-      float ga[V], o[V], e[V];
-      load_param<V>(a.gamma, i, a.n, 1.f, ga);
-      if (a.dx && a.add_dx) load_vec<T>(dx, i, a.n, o);
+      float ga[V];
+      gamma.get(w, c, ga);
+      typename Vec<T>::type o = {}, e;
+      if (a.dx && a.add_dx && w.in(c)) o = *reinterpret_cast<const typename Vec<T>::type *>(dx + w.at(c));
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float q = r * (u[c][k] - mu_ - h[c][k] * muh);
-        if constexpr (PG) acc[0][c][k] += d[c][k] * q;
-        e[k] = ga[k] * q;
-        if (neg[c] >> k & 1) e[k] *= a.slope;
-        const float b = r2 * (h[c][k] * hc - muh * (d[c][k] * ga[k] - mg) - mgh * (u[c][k] - mu_));
-        o[k] = a.add_dx ? o[k] + b : b;
+        const float h = hat(c, k), d = dn(c, k), uu = (float)u.v[c][k];
+        const float q = r * (uu - mu_ - h * muh);
+        if constexpr (PG) acc[0][c][k] += d * q;
+        e[k] = (T)(neg[c] >> k & 1 ? ga[k] * q * a.slope : ga[k] * q);
+        const float b = second(h, d * ga[k], uu);
+        o[k] = (T)(a.add_dx ? (float)o[k] + b : b);
       }
-      if (a.dx) store_vec<T>(dx, i, a.n, o);
-      if (a.ddy) store_vec<T>(ddy, i, a.n, e);
+      if (a.dx && w.in(c)) *reinterpret_cast<typename Vec<T>::type *>(dx + w.at(c)) = o;
+      if (a.ddy && w.in(c)) *reinterpret_cast<typename Vec<T>::type *>(ddy + w.at(c)) = e;
+    }
+    if (w.last >= 0) {
+      const float q = r * (ue - mu_ - he * muh), b = second(he, ge, ue);
+      if constexpr (PG) aend[0] += de * q;
+      if (a.dx) dx[w.last] = (T)(a.add_dx ? (float)dx[w.last] + b : b);
+      if (a.ddy) ddy[w.last] = (T)(nend ? gamma.end * q * a.slope : gamma.end * q);
     }
   }
-  if constexpr (PG) write_partials<T, G, C, 1>(acc, a, lds);
+  if constexpr (PG) write_partials<T, G, C, 1>(acc, aend, w, a, lds);
 }
 
 // Rows wider than the registers of a workgroup hold: one workgroup a row, the row read again for each pass (it stays in
@@ -452,28 +519,31 @@ __global__ __launch_bounds__(1024) void ln_bwd2_wide_kernel(NormArgs a) {
   }
 }
 
-// out_q[j] (+)= sum over workgroups b of part[b][q][j], b in a fixed order: 16 columns by 16 interleaved shares a workgroup
-__global__ __launch_bounds__(256) void ln_param_kernel(const float *__restrict__ part, int nb, int64_t n, float *dgamma,
-                                                       float *dbeta, int accumulate) {
-  __shared__ float red[16][17];
+// out_q[j] (+)= sum over workgroups b of part[b][q][j], b in a fixed order: 32 columns by 32 interleaved shares a workgroup
+__global__ __launch_bounds__(1024) void ln_param_kernel(const float *__restrict__ part, int nb, int64_t n, float *dgamma,
+                                                        float *dbeta, int accumulate) {
+  __shared__ float red[32][33];
   float *out = blockIdx.y ? dbeta : dgamma;
   if (!out) return;
-  const int col = threadIdx.x & 15, sh = threadIdx.x >> 4;
-  const int64_t j = (int64_t)blockIdx.x * 16 + col;
+  const int col = threadIdx.x & 31, sh = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + col;
   float s = 0.f;
-  if (j < n)
-    for (int b = sh; b < nb; b += 16) s += part[((int64_t)b * 2 + blockIdx.y) * n + j];
+  if (j < n) {
+#pragma unroll 8
+    for (int b = sh; b < nb; b += 32) s += part[((int64_t)b * 2 + blockIdx.y) * n + j];
+  }
   red[sh][col] = s;
   __syncthreads();
   if (sh == 0 && j < n) {
     s = accumulate ? out[j] : 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += red[k][col];
+    for (int k = 0; k < 32; ++k) s += red[k][col];
     out[j] = s;
   }
 }
 
 enum { FWD, BWD, BWD2 };
+constexpr int PARAM_BLOCKS = 4;
 
 template <int OP, typename T, int G, int C>
 void launch_cfg(hipStream_t st, const NormArgs &a, int blocks) {
@@ -488,25 +558,22 @@ void launch_cfg(hipStream_t st, const NormArgs &a, int blocks) {
   }
 }
 
-// threads a row's group has (0: the wide kernels) and vectors each of them holds, by the row's vectors of 16 bytes
+// threads a row's group has (0: the wide kernels) and vectors each of them holds, by the row's whole vectors of 16 bytes
 struct Cfg { int g, c; };
 Cfg pick(int64_t width, int v) {
-  const int64_t nv = agx::cdiv64(width, v);
+  const int64_t nv = std::max<int64_t>(1, width / v);
   if (nv <= 16) return {16, 1};
-  if (nv <= 64) return {64, 1};
-  if (nv <= 128) return {64, 2};
-  if (nv <= 256) return {256, 1};
-  if (nv <= 512) return {256, 2};
-  if (nv <= 1024) return {256, 4};
-  if (nv <= 2048) return {1024, 2};
+  if (nv <= 64 * 4) return {64, (int)agx::cdiv64(nv, 64)};
+  if (nv <= 256 * 4) return {256, (int)agx::cdiv64(nv, 256)};
+  if (nv <= 1024 * 4) return {1024, (int)agx::cdiv64(nv, 1024)};
   return {0, 0};
 }
-// workgroups of a launch: enough rows in flight to fill 256 CUs a few times over; with parameter gradients at most two
+// workgroups of a launch: enough rows in flight to fill 256 CUs a few times over; with parameter gradients at most four
 // a CU, because each writes and the second launch reads a partial row
 int blocks_of(int64_t rows, const Cfg &c, bool params) {
   const int ng = c.g == 0 || c.g >= 256 ? 1 : 256 / c.g;
   const int64_t need = agx::cdiv64(rows, ng);
-  return (int)std::min<int64_t>(need, (int64_t)agx::num_cus() * (params ? 2 : 16));
+  return (int)std::min<int64_t>(need, (int64_t)agx::num_cus() * (params ? PARAM_BLOCKS : c.g == 64 || c.g == 16 ? 8 : 16));
 }
 
 template <int OP, typename T>
@@ -514,20 +581,24 @@ int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int a
   const Cfg c = pick(a.n, Vec<T>::V);
   const int blocks = blocks_of(a.rows, c, a.part != nullptr);
   if (blocks > 0) {
+    auto by_c = [&](auto g) {
+      constexpr int G = decltype(g)::value;
+      if (c.c == 1) launch_cfg<OP, T, G, 1>(st, a, blocks);
+      else if (c.c == 2) launch_cfg<OP, T, G, 2>(st, a, blocks);
+      else if (c.c == 3) launch_cfg<OP, T, G, 3>(st, a, blocks);
+      else launch_cfg<OP, T, G, 4>(st, a, blocks);
+    };
     if (c.g == 16) launch_cfg<OP, T, 16, 1>(st, a, blocks);
-    else if (c.g == 64 && c.c == 1) launch_cfg<OP, T, 64, 1>(st, a, blocks);
-    else if (c.g == 64) launch_cfg<OP, T, 64, 2>(st, a, blocks);
-    else if (c.g == 256 && c.c == 1) launch_cfg<OP, T, 256, 1>(st, a, blocks);
-    else if (c.g == 256 && c.c == 2) launch_cfg<OP, T, 256, 2>(st, a, blocks);
-    else if (c.g == 256) launch_cfg<OP, T, 256, 4>(st, a, blocks);
-    else if (c.g == 1024) launch_cfg<OP, T, 1024, 2>(st, a, blocks);
+    else if (c.g == 64) by_c(std::integral_constant<int, 64>{});
+    else if (c.g == 256) by_c(std::integral_constant<int, 256>{});
+    else if (c.g == 1024) by_c(std::integral_constant<int, 1024>{});
     else if constexpr (OP == FWD) hipLaunchKernelGGL(ln_fwd_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
     else if constexpr (OP == BWD) hipLaunchKernelGGL(ln_bwd_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL(ln_bwd2_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
     AGX_LAUNCH_CHECK();
   }
   if (dgamma || dbeta) {
-    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)agx::cdiv64(a.n, 16), 2), dim3(256), 0, st, a.part, blocks, a.n, dgamma,
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)agx::cdiv64(a.n, 32), 2), dim3(1024), 0, st, a.part, blocks, a.n, dgamma,
                        dbeta, accumulate);
     AGX_LAUNCH_CHECK();
   }

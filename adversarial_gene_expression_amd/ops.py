@@ -110,8 +110,9 @@ def _vector(t, name, n, like):
 
 def _on_current(t):
     """Kernels run on the current device and stream: refuse operands that live elsewhere."""
-    if t.device != _dev.device():
-        raise ValueError('operands are on %s, the current device is cuda:%d' % (t.device, torch.cuda.current_device()))
+    if not t.is_cuda or not _lib.is_initialised(t.get_device()) or t.get_device() != torch.cuda.current_device():
+        if t.device != _dev.device():
+            raise ValueError('operands are on %s, the current device is cuda:%d' % (t.device, torch.cuda.current_device()))
 
 
 def _rows_like(x):
@@ -149,8 +150,7 @@ def layer_norm(x, gamma=None, beta=None, *, eps=1e-3, act=0, slope=0.0, out=None
     if out is None:
         out = _rows_like(x)
         d.ldy = max(out.stride(0), out.shape[1])
-    stats = torch.empty((2, x.shape[0]), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    mean, rstd = torch.empty((2, x.shape[0]), dtype=torch.float32, device=x.device).unbind(0)
     d.y, d.mean, d.rstd, d.eps = out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), eps
     _lib.check(_lib.load().agx_layernorm_fwd(_dev.stream(), d), 'agx_layernorm_fwd')
     return out, mean, rstd
@@ -188,8 +188,7 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, y=None, act=0, slope=0
     ws = dgamma = dbeta = None
     if param_grads:
         ws = _norm_ws(d, x, lib)
-        both = torch.empty((2, x.shape[1]), dtype=torch.float32, device=x.device)
-        dgamma, dbeta = both[0], both[1]
+        dgamma, dbeta = torch.empty((2, x.shape[1]), dtype=torch.float32, device=x.device).unbind(0)
         d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
     _lib.check(lib.agx_layernorm_bwd(_dev.stream(), d), 'agx_layernorm_bwd')
     return dx, dgamma, dbeta

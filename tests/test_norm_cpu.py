@@ -93,7 +93,7 @@ def test_workspace_query():
     for rows, width in ((1, 1), (5, 257), (100000, 256), (3, 40000)):
         for dt in (0, 1):
             n = lib.agx_layernorm_ws_floats(rows, width, dt)
-            assert n % (2 * width) == 0 and 2 * width <= n <= 512 * 2 * width
+            assert n % (2 * width) == 0 and 2 * width <= n <= 1024 * 2 * width
 
 
 @pytest.mark.parametrize('on,slope', [(0, 0.0), (1, 0.0), (1, 0.2)])
