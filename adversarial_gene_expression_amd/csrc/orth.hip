@@ -39,6 +39,7 @@ constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ONE_BLOCK = 128;                 // largest padded side for a phase in one workgroup (LDS)
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
 constexpr int64_t BIG_TILES = 128;             // tiles of 2 T from which the product with the long side takes them
+constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
 // n x n matrix as two fp16 planes of np x np (np: n rounded up to T or a multiple of 2 T, zeros behind), value = (hi + lo) 2^-e
@@ -51,12 +52,8 @@ struct Planes {
 __device__ __forceinline__ int exponent_of(uint32_t absbits) {   // e with |v| < 2^e for the float of these bits
   return absbits == 0 ? 0 : (int)(absbits >> 23) - 126;
 }
-// v = hi + lo, each rounded to nearest
-__device__ __forceinline__ void split(float v, _Float16 &hi, _Float16 &lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
-}
-__device__ __forceinline__ void split4(f32x4 v, half4 &hi, half4 &lo) {   // (two values an instruction)
+// v = hi + lo, each rounded to nearest (two values an instruction)
+__device__ __forceinline__ void split4(f32x4 v, half4 &hi, half4 &lo) {
   hi = __builtin_convertvector(v, half4);
   lo = __builtin_convertvector(v - __builtin_convertvector(hi, f32x4), half4);
 }
@@ -148,7 +145,7 @@ __device__ __forceinline__ void upper_tile(int t, int nt, int &ti, int &tj) {
   tj = ti + t;
 }
 
-// scale exponent of a matrix from its partial maxima; every thread of the workgroup (of up to 8 waves) gets it
+// scale exponent of a matrix from its partial maxima; every thread of the workgroup gets it (red: a word a wave)
 __device__ __forceinline__ int scale_exponent(const uint32_t *maxb, int nb, uint32_t *red) {
   uint32_t mx = 0;
   for (int i = threadIdx.x; i < nb; i += blockDim.x) mx = max(mx, maxb[i]);
@@ -439,23 +436,9 @@ __global__ __launch_bounds__(TT * 4, 2) void orth_gram_kernel(GramArgs a) {
   }
 }
 
-// value (hi + lo) 2^-e of element o of a planes matrix, scaled by 2^e
-__device__ __forceinline__ float plane_value(const Planes &m, int64_t o) { return (float)m.hi[o] + (float)m.lo()[o]; }
-__device__ __forceinline__ void plane_store(const Planes &m, int64_t o, float scaled) {
-  _Float16 h, l;
-  split(scaled, h, l);
-  m.hi[o] = h;
-  m.lo()[o] = l;
-}
-
-// An element on or above the diagonal and its mirror image.  Products of matrices that are symmetric up to rounding are not
-// symmetric themselves, and the iteration would multiply the difference (rank-deficient matrices: 50 times the error).
-__device__ __forceinline__ void store_symmetric(const Planes &m, int64_t r, int64_t c, float scaled) {
-  if (r > c) return;
-  plane_store(m, r * m.np + c, scaled);
-  if (r != c) plane_store(m, c * m.np + r, scaled);
-}
-
+// Symmetric results are made symmetric to the last bit, from what is on and above the diagonal: products of matrices that are
+// symmetric up to rounding are not, and the iteration would multiply the difference (rank-deficient matrices: 50 times the
+// error).
 // A lane's four rows r.. of column c of a 32 x 32 tile, and their mirror image, into planes of row stride ld (global memory
 // or LDS).  The mirror image is contiguous; the rows themselves go out as pairs of columns, which two neighbouring lanes
 // exchange (the even one takes the first two rows, the odd one the others).  A tile on the diagonal comes symmetric: its
@@ -482,55 +465,98 @@ __device__ __forceinline__ void store_planes4(_Float16 *hi, _Float16 *lo, int ld
 
 // A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase; the scaled matrix's trace is |X|_F^2) or
 // without a divisor (later phases).  Every workgroup sums the trace itself, in the same order.
+// A workgroup takes R rows of a square of 32 x 32 on or above the diagonal: interleaved shares of the slices meet in LDS, from
+// where the piece and its mirror image go out as vectors.  R = 32 (4 shares) where the slices are few, 4 (8 shares) where
+// they are many: 18161 x 256 with 71 slices 5.0 us instead of 8.0, 1000 x 4297 with 7 slices 10 us instead of 17.
 struct ReduceJob {
   const float *part, *trace;
   const uint32_t *maxb;
   double *invd;                 // 1 / d of the scaled matrix, for the product with the long side (phase 0)
   Planes A;
-  int32_t nt, slices, e, nb, normalise, side, first;   // side: of the partial tiles
+  int32_t nt, slices, e, nb, normalise, side, first;   // nt, side: of the partial tiles
 };
 struct ReduceArgs {
   ReduceJob job[AGX_MAX_ORTH];
   int n;
   float eps;
 };
-__global__ __launch_bounds__(256) void orth_reduce_kernel(ReduceArgs a) {
-  __shared__ float part[4][64];
-  __shared__ uint32_t red[4];
-  __shared__ double tr[4];
+template <int R> constexpr int reduce_threads() { return R == 32 ? 1024 : 256; }
+template <int R>
+__global__ __launch_bounds__(reduce_threads<R>()) void orth_reduce_kernel(ReduceArgs a) {
+  constexpr int NT = reduce_threads<R>(), NG = NT / (R * 8);   // shares
+  __shared__ float piece[NG][R][33];
+  __shared__ uint32_t red[16];
+  __shared__ double tr[16];
   int q = 0;
   while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
   const ReduceJob &j = a.job[q];
-  // (64 elements of a tile a workgroup, by four interleaved shares of the slices)
-  const int area = j.side * j.side, tile = (blockIdx.x - j.first) / (area / 64), grp = threadIdx.x >> 6;
-  const int z = (blockIdx.x - j.first) % (area / 64) * 64 + (threadIdx.x & 63);
-  int ti, tj;
-  upper_tile(tile, j.nt, ti, tj);
-  float sum = 0.f;
-  const float *p = j.part + (int64_t)tile * j.slices * area + z;
+  int pi, pj;                                          // square of the n x n matrix, and where it is in the partial tiles
+  upper_tile((blockIdx.x - j.first) / (32 / R), j.A.np / 32, pi, pj);
+  const int r0 = (blockIdx.x - j.first) % (32 / R) * R;
+  const int per = j.side / 32, ti = pi / per, tj = pj / per, area = j.side * j.side;
+  const int tile = ti * j.nt - ti * (ti - 1) / 2 + tj - ti;
+  const int grp = threadIdx.x / (R * 8), r = (threadIdx.x >> 3) % R, c = (threadIdx.x & 7) * 4;
+  const float *p = j.part + (int64_t)tile * j.slices * area + (pi % per * 32 + r0 + r) * j.side + pj % per * 32 + c;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int c = grp; c < j.slices; c += 4) sum += p[(int64_t)c * area];
-  part[grp][threadIdx.x & 63] = sum;
+  for (int z = grp; z < j.slices; z += NG) sum += *reinterpret_cast<const f32x4 *>(p + (int64_t)z * area);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) piece[grp][r][c + i] = sum[i];
   double f;
   if (j.normalise) {
     const int e = scale_exponent(j.maxb, j.nb, red);
     double s = 0.0;
-    for (int i = threadIdx.x; i < j.nt * j.slices; i += 256) s += (double)j.trace[i];
+    for (int i = threadIdx.x; i < j.nt * j.slices; i += NT) s += (double)j.trace[i];
     s = agx::wave_sum(s);
     if ((threadIdx.x & 63) == 0) tr[threadIdx.x >> 6] = s;
     __syncthreads();
-    s = tr[0] + tr[1] + tr[2] + tr[3];
+    s = 0.0;
+    for (int i = 0; i < NT / 64; ++i) s += tr[i];
     const double d = sqrt(s) + ldexp((double)a.eps, e);
     const double inv = s == 0.0 ? 0.0 : 1.0 / d;                    // (a matrix of zeros gives zeros)
     f = ldexp(inv * inv, j.A.e);
-    if (blockIdx.x == j.first && threadIdx.x == 0) *j.invd = inv;
+    if ((int)blockIdx.x == j.first && threadIdx.x == 0) *j.invd = inv;
   } else {
     f = ldexp(1.0, j.A.e - 2 * j.e);
   }
   __syncthreads();
-  if (grp) return;
-  sum = part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
-  store_symmetric(j.A, (int64_t)ti * j.side + z / j.side, (int64_t)tj * j.side + z % j.side, (float)((double)sum * f));
+  auto total = [&](int y, int x) {
+    float t = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) t += piece[g][y][x];
+    return (float)((double)t * f);
+  };
+  // the first threads write the piece, the next its mirror image
+  const int y0 = pi * 32 + r0, x0 = pj * 32, np = j.A.np;
+  f32x4 v;
+  half4 h, l;
+  int o;
+  if (grp == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = total(r, c + i);
+    o = (y0 + r) * np + x0 + c;
+  } else if (grp == 1) {                               // (32 rows of R columns)
+    const int x = threadIdx.x % (R * 8) / (R / 4), y = threadIdx.x % (R / 4) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = total(y + i, x);
+    o = (x0 + x) * np + y0 + y;
+  } else {
+    return;
+  }
+  split4(v, h, l);
+  if (pi != pj) {
+    *reinterpret_cast<half4 *>(j.A.hi + o) = h;
+    *reinterpret_cast<half4 *>(j.A.lo() + o) = l;
+  } else {                                             // what is on and above the diagonal, and its mirror image
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = o / np, col = o % np + i;
+      if (grp == 0 ? row <= col : row > col) {
+        j.A.hi[o + i] = h[i];
+        j.A.lo()[o + i] = l[i];
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -547,8 +573,11 @@ struct ChainArgs {
 };
 static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 
-template <int TT>
-__global__ __launch_bounds__(TT * 4, 2) void orth_chain_kernel(ChainArgs a) {
+// (tiles of 64 x 64: an n of 1000 has 136 of them, less than a CU's worth each, so that latency counts: four steps' loads are
+//  in flight)
+__global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
+  using G = Geo<T>;
+  constexpr int DEPTH = 4, BUF = 4 * G::PL;
   extern __shared__ _Float16 lds[];
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
@@ -556,18 +585,82 @@ __global__ __launch_bounds__(TT * 4, 2) void orth_chain_kernel(ChainArgs a) {
   const ChainJob &j = a.job[q];
   int ti, tj;
   upper_tile(id - j.first, j.nt, ti, tj);
-  LoadPlanes<TT> la(j.L), lb(j.R);
-  f32x16 acc[Geo<TT>::F];
-  tile_product<TT>(la, lb, ti * TT, tj * TT, 0, j.C.np, lds, acc, ti == tj && j.L.hi == j.R.hi, [] {});
-  const float fa = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
-  const float fb = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fi = __builtin_ldexpf(j.gamma, j.C.e);
-  each_element<TT>(acc, [&](int tr, int tc, float v) {
-    const int64_t r = (int64_t)ti * TT + tr, c = (int64_t)tj * TT + tc;
-    if (r > c) return;
-    float w = r == c && r < j.n ? fi : 0.f;
-    if (j.beta != 0.f) w = fmaf(fb, plane_value(j.E, r * j.C.np + c), w);
-    store_symmetric(j.C, r, c, fmaf(fa, v, w));
-  });
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, np = j.C.np, n = np / G::BK;
+  LoadPlanes<T> la[DEPTH] = {LoadPlanes<T>(j.L), LoadPlanes<T>(j.L), LoadPlanes<T>(j.L), LoadPlanes<T>(j.L)};
+  LoadPlanes<T> lb[DEPTH] = {LoadPlanes<T>(j.R), LoadPlanes<T>(j.R), LoadPlanes<T>(j.R), LoadPlanes<T>(j.R)};
+  static_assert(DEPTH == 4, "");
+  f32x16 acc = {};
+  const int fa = ((wave >> 1) * 32 + (lane & 31)) * G::LD + (lane >> 5) * 8;
+  const int fb = ((wave & 1) * 32 + (lane & 31)) * G::LD + (lane >> 5) * 8 + 2 * G::PL;
+  auto at = [](const _Float16 *t) { return *reinterpret_cast<const half8 *>(t); };
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u)
+    if (u < n) {
+      la[u].fetch(ti * T, u * G::BK);
+      lb[u].fetch(tj * T, u * G::BK);
+    }
+  for (int s = 0; s < n; s += DEPTH)
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (s + u < n) {                                 // (one barrier a step: a buffer is written two steps after it was read)
+        _Float16 *t = lds + (u & 1) * BUF;
+        la[u].store(t);
+        lb[u].store(t + 2 * G::PL);
+        if (s + u + DEPTH < n) {
+          la[u].fetch(ti * T, (s + u + DEPTH) * G::BK);
+          lb[u].fetch(tj * T, (s + u + DEPTH) * G::BK);
+        }
+        __syncthreads();
+        f32x16 sum = {};
+        half8 ah[4], bh[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          ah[k] = at(t + fa + k * 16);
+          bh[k] = at(t + fb + k * 16);
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + G::PL + fa + k * 16), bh[k], sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], at(t + G::PL + fb + k * 16), sum, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], bh[k], sum, 0, 0, 0);
+        acc += sum;
+      }
+  // a wave's 32 x 32 results, as in the other forms
+  const int fi = ti * 2 + (wave >> 1), fj = tj * 2 + (wave & 1), c = fj * 32 + (lane & 31), r0 = fi * 32 + 4 * (lane >> 5);
+  const bool diag = fi == fj;
+  const float fl = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
+  const float fe = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fd = __builtin_ldexpf(j.gamma, j.C.e);
+  float v[16];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    half4 eh = {}, el = {};
+    if (j.beta != 0.f) {                               // (E is symmetric: its mirror image is one vector)
+      eh = *reinterpret_cast<const half4 *>(&j.E.hi[c * np + r0 + 8 * p]);
+      el = *reinterpret_cast<const half4 *>(&j.E.lo()[c * np + r0 + 8 * p]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[4 * p + i] = fmaf(fl, acc[4 * p + i], fmaf(fe, (float)eh[i] + (float)el[i], r0 + 8 * p + i == c && c < j.n ? fd : 0.f));
+  }
+  __syncthreads();
+  if (fi > fj) return;
+  if (diag) {                                          // below the diagonal: what is above it, through the wave's own 4 KB
+    float *scratch = reinterpret_cast<float *>(lds) + wave * 32 * 33;
+    const int lr = 4 * (lane >> 5), lc = lane & 31;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) scratch[(lr + 8 * (i >> 2) + (i & 3)) * 33 + lc] = v[i];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = lr + 8 * (i >> 2) + (i & 3);
+      const float m = scratch[lc * 33 + row];
+      v[i] = row > lc ? m : v[i];
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    store_planes4(j.C.hi, j.C.lo(), np, r0 + 8 * p, c, diag, f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]});
 }
 
 // The same for small matrices, where a launch is all latency: tiles of 32 x 32 (36 of them at n = 256), k dealt to the four
@@ -1066,7 +1159,9 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       ga[0].n = ga[1].n = 0;
       ra.n = n;
       ra.eps = o->eps;
-      int gb[2] = {0, 0}, rb = 0, kind[2] = {-1, -1};
+      int gb[2] = {0, 0}, rb = 0, kind[2] = {-1, -1}, most = 0;
+      for (int i = 0; i < n; ++i) most = std::max(most, lay[i].slices);
+      const int pieces = most > FEW_SLICES ? 8 : 1;     // of a square of 32 x 32
       for (int i = 0; i < n; ++i) {
         const Job &j = jobs[i];
         const Layout &l = lay[i];
@@ -1084,7 +1179,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         r.part = g.part; r.trace = g.trace; r.maxb = g.maxb; r.invd = reinterpret_cast<double *>(base[i] + l.invd);
         r.A = planes(i, 0, exponent_for(s * s)); r.nt = nt; r.slices = l.slices; r.e = ex; r.nb = nb[i];
         r.normalise = first; r.side = j.side(); r.first = rb;
-        rb += tl * (j.side() * j.side() / 64);
+        rb += j.np() / 32 * (j.np() / 32 + 1) / 2 * pieces;
       }
       if (ga[0].n)
         by_kind(kind[0], [&](auto k) {
@@ -1096,7 +1191,8 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
           hipLaunchKernelGGL((orth_gram_kernel<2 * T, decltype(k)::value>), dim3(gb[1]), dim3(Geo<2 * T>::NT), tile_lds<2 * T>(), st, ga[1]);
         });
       AGX_LAUNCH_CHECK();
-      hipLaunchKernelGGL(orth_reduce_kernel, dim3(rb), dim3(256), 0, st, ra);
+      if (pieces == 8) hipLaunchKernelGGL(orth_reduce_kernel<4>, dim3(rb), dim3(reduce_threads<4>()), 0, st, ra);
+      else hipLaunchKernelGGL(orth_reduce_kernel<32>, dim3(rb), dim3(reduce_threads<32>()), 0, st, ra);
       AGX_LAUNCH_CHECK();
     }
     // matrices: 0 A, 1 P, 2 A P, 3 / 4 Q (which of the two: 3 after an odd number of steps).  Matrices of np <= ONE_BLOCK take
@@ -1161,7 +1257,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
             fill(g, i, w);
           }
         if (small) hipLaunchKernelGGL(orth_chain_small_kernel, dim3(blocks), dim3(256), 0, st, ca);
-        else hipLaunchKernelGGL(orth_chain_kernel<T>, dim3(blocks), dim3(256), tile_lds<T>(), st, ca);
+        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(256), tile_lds<T>(), st, ca);
         AGX_LAUNCH_CHECK();
         return AGX_OK;
       };
@@ -1270,7 +1366,7 @@ template <class K> hipError_t allow_lds(K *kernel, int bytes) {
 }  // namespace
 int agx::orth_prepare_device() {
   AGX_HIP(allow_lds(&orth_phase_kernel, phase_lds(ONE_BLOCK)));
-  AGX_HIP(allow_lds(&orth_chain_kernel<T>, tile_lds<T>()));
+  AGX_HIP(allow_lds(&orth_chain_kernel, tile_lds<T>()));
   for (int kind = 0; kind <= ANY; ++kind) {
     hipError_t e = hipSuccess;
     by_kind(kind, [&](auto k) {
