@@ -439,28 +439,28 @@ __global__ __launch_bounds__(TT * 4, 2) void orth_gram_kernel(GramArgs a) {
 // Symmetric results are made symmetric to the last bit, from what is on and above the diagonal: products of matrices that are
 // symmetric up to rounding are not, and the iteration would multiply the difference (rank-deficient matrices: 50 times the
 // error).
-// A lane's four rows r.. of column c of a 32 x 32 tile, and their mirror image, into planes of row stride ld (global memory
-// or LDS).  The mirror image is contiguous; the rows themselves go out as pairs of columns, which two neighbouring lanes
-// exchange (the even one takes the first two rows, the odd one the others).  A tile on the diagonal comes symmetric: its
-// mirror image is all of it.
+// A lane's four rows r.. of column c go out as pairs of columns, which two neighbouring lanes exchange (the even one takes the
+// first two rows, the odd one the others)
+__device__ __forceinline__ void store_pairs4(_Float16 *p, int ld, int r, int c, half4 x) {
+  const bool odd = threadIdx.x & 1;
+  const uint2 w = __builtin_bit_cast(uint2, x);        // rows (0, 1) and (2, 3) of this lane's column
+  const uint32_t mine = odd ? w.y : w.x, give = odd ? w.x : w.y;
+  const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0xb1, 0xf, 0xf, true);   // lanes 2 k <-> 2 k + 1
+  const uint32_t a = odd ? got : mine, b = odd ? mine : got;
+  uint32_t *q = reinterpret_cast<uint32_t *>(p + (r + (odd ? 2 : 0)) * ld + (c & ~1));
+  q[0] = (a & 0xffffu) | (b << 16);
+  *reinterpret_cast<uint32_t *>(reinterpret_cast<_Float16 *>(q) + ld) = (a >> 16) | (b & 0xffff0000u);
+}
+// The same of a 32 x 32 tile with their mirror image, which is contiguous, into planes of row stride ld (global memory or
+// LDS).  A tile on the diagonal comes symmetric: its mirror image is all of it.
 __device__ __forceinline__ void store_planes4(_Float16 *hi, _Float16 *lo, int ld, int r, int c, bool diag, f32x4 v) {
   half4 h, l;
   split4(v, h, l);
   *reinterpret_cast<half4 *>(&hi[c * ld + r]) = h;
   *reinterpret_cast<half4 *>(&lo[c * ld + r]) = l;
   if (diag) return;                                    // (uniform over the wave)
-  const bool odd = threadIdx.x & 1;
-  auto pairs = [&](half4 x, _Float16 *p) {
-    const uint2 w = __builtin_bit_cast(uint2, x);      // rows (0, 1) and (2, 3) of this lane's column
-    const uint32_t mine = odd ? w.y : w.x, give = odd ? w.x : w.y;
-    const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0xb1, 0xf, 0xf, true);   // lanes 2 k <-> 2 k + 1
-    const uint32_t a = odd ? got : mine, b = odd ? mine : got;
-    uint32_t *q = reinterpret_cast<uint32_t *>(p + (r + (odd ? 2 : 0)) * ld + (c & ~1));
-    q[0] = (a & 0xffffu) | (b << 16);
-    *reinterpret_cast<uint32_t *>(reinterpret_cast<_Float16 *>(q) + ld) = (a >> 16) | (b & 0xffff0000u);
-  };
-  pairs(h, hi);
-  pairs(l, lo);
+  store_pairs4(hi, ld, r, c, h);
+  store_pairs4(lo, ld, r, c, l);
 }
 
 // A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase; the scaled matrix's trace is |X|_F^2) or
@@ -860,6 +860,163 @@ __global__ __launch_bounds__(PW * 64) void orth_phase_kernel(PhaseArgs a) {
 }
 static_assert(ONE_BLOCK == 2 * T, "one-workgroup phases are written for one or two tiles a side");
 
+// One step in one launch for np = 256.  Rows of a polynomial of A need A alone: r.A, (r.A).A, ... with r a row of A or Q, so
+// that a workgroup takes 16 rows of A (or of Q) through the whole step by itself,
+//   S = a r + b r A + c r A^2,  next A = a S + b S A + c S A^2  (four products; Q: the first two),
+// with A in its waves' registers (32 columns a wave: 128 registers of 512 threads hold all 256 KB of it) and the running
+// rows in LDS.  More flops than the symmetric products (6 n^3 a step against 1.5 to 2), but one launch of 11 us where three
+// of 6 us stood.
+constexpr int STEP_NP = 256, STEP_ROWS = 16, STEP_LD = STEP_NP + 8;   // (16 rows start in 16 different bank groups)
+struct StepJob {
+  Planes A, An, Q, Qn;
+  int32_t n, first;
+};
+struct StepArgs {
+  StepJob job[AGX_MAX_ORTH];
+  int n;
+  int32_t more, has_q;          // a further step follows (A is wanted); Q exists (otherwise the step's own polynomial is Q)
+  float a, b, c;
+  int32_t e1, eS, e3, q1;       // scale exponents of the running rows: r A, S, S A; of Q's r A
+};
+
+__global__ __launch_bounds__(512, 2) void orth_step_kernel(StepArgs a) {
+  __shared__ _Float16 panel[2][2][STEP_ROWS * STEP_LD];                // [buffer][plane]
+  int q = 0;
+  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
+  const StepJob &j = a.job[q];
+  constexpr int PANELS = STEP_NP / STEP_ROWS;
+  const int local = blockIdx.x - j.first, i0 = local % PANELS * STEP_ROWS;
+  const bool rows_of_q = local >= PANELS;
+  if (rows_of_q ? !a.has_q : a.has_q && !a.more) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
+  // the rows themselves, and A's columns (= rows: it is symmetric) wave * 32 ..; k runs in an order of its own, the same for
+  // both operands: a lane's vectors of two steps are neighbours in memory
+  const Planes &R = rows_of_q ? j.Q : j.A;
+  const int pr = threadIdx.x >> 5, pc = (threadIdx.x & 31) * 8;
+  const half8 rh = *reinterpret_cast<const half8 *>(R.hi + (i0 + pr) * STEP_NP + pc);
+  const half8 rl = *reinterpret_cast<const half8 *>(R.lo() + (i0 + pr) * STEP_NP + pc);
+  half8 bh[2][8], bl[2][8];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int o = (wave * 32 + t * 16 + cl) * STEP_NP + (k >> 1) * 64 + g * 16 + (k & 1) * 8;
+      bh[t][k] = *reinterpret_cast<const half8 *>(j.A.hi + o);
+      bl[t][k] = *reinterpret_cast<const half8 *>(j.A.lo() + o);
+    }
+  *reinterpret_cast<half8 *>(&panel[0][0][pr * STEP_LD + pc]) = rh;
+  *reinterpret_cast<half8 *>(&panel[0][1][pr * STEP_LD + pc]) = rl;
+  __syncthreads();
+  int buf = 0;
+  typedef f32x4 Rows[2];        // a lane's results: rows 4 g .. of columns wave * 32 + 16 t + cl
+  auto multiply = [&](int e, Rows &out) {              // out = (rows in the panel, of scale e) . A
+    const _Float16 *ph = panel[buf][0] + cl * STEP_LD + g * 16, *pl = panel[buf][1] + cl * STEP_LD + g * 16;
+    f32x4 acc[2] = {};
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      f32x4 sum[2] = {};
+      half8 x[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int o = (k + h >> 1) * 64 + (h & 1) * 8;
+        x[h] = *reinterpret_cast<const half8 *>(ph + o);
+        const half8 y = *reinterpret_cast<const half8 *>(pl + o);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, bh[t][k + h], sum[t], 0, 0, 0);
+          sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], bl[t][k + h], sum[t], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], bh[t][k + h], sum[t], 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[t] += sum[t];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) out[t] = scale4(acc[t], -e - j.A.e);
+  };
+  auto put = [&](const Rows &r, int e) {               // rows into the other panel, which is then the current one
+    buf ^= 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      half4 h, l;
+      split4(scale4(r[t], e), h, l);
+      store_pairs4(panel[buf][0], STEP_LD, 4 * g, wave * 32 + t * 16 + cl, h);
+      store_pairs4(panel[buf][1], STEP_LD, 4 * g, wave * 32 + t * 16 + cl, l);
+    }
+    __syncthreads();
+  };
+  auto write_rows = [&](const Planes &m) {             // the current panel
+    *reinterpret_cast<half8 *>(m.hi + (i0 + pr) * STEP_NP + pc) = *reinterpret_cast<const half8 *>(&panel[buf][0][pr * STEP_LD + pc]);
+    *reinterpret_cast<half8 *>(m.lo() + (i0 + pr) * STEP_NP + pc) = *reinterpret_cast<const half8 *>(&panel[buf][1][pr * STEP_LD + pc]);
+  };
+  Rows r, x1, x2, s;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int o = (4 * g + i) * STEP_LD + wave * 32 + t * 16 + cl;
+      r[t][i] = __builtin_ldexpf((float)panel[0][0][o] + (float)panel[0][1][o], -R.e);
+    }
+  multiply(R.e, x1);
+  if (!rows_of_q && !a.has_q) {                        // Q = a I + b A + c A^2
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = i0 + 4 * g + i, col = wave * 32 + t * 16 + cl;
+        s[t][i] = a.c * x1[t][i] + (a.b * r[t][i] + (row == col && row < j.n ? a.a : 0.f));
+      }
+    put(s, j.Qn.e);
+    write_rows(j.Qn);
+    if (!a.more) return;
+  }
+  put(x1, rows_of_q ? a.q1 : a.e1);
+  multiply(rows_of_q ? a.q1 : a.e1, x2);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = a.a * r[t][i] + (a.b * x1[t][i] + a.c * x2[t][i]);
+  if (rows_of_q) {
+    put(s, j.Qn.e);
+    write_rows(j.Qn);
+    return;
+  }
+  put(s, a.eS);
+  multiply(a.eS, x1);
+  put(x1, a.e3);
+  multiply(a.e3, x2);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = a.a * s[t][i] + (a.b * x1[t][i] + a.c * x2[t][i]);
+  put(s, j.An.e);
+  // the rows from the diagonal on, and their mirror image behind it
+  const int from = pc - i0;
+  if (from >= STEP_ROWS) {
+    write_rows(j.An);
+  } else if (from >= 0) {                              // (the square on the diagonal: symmetric from what is above it)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = from + k, y = min(pr, c), x = max(pr, c);
+      j.An.hi[(i0 + pr) * STEP_NP + i0 + c] = panel[buf][0][y * STEP_LD + i0 + x];
+      j.An.lo()[(i0 + pr) * STEP_NP + i0 + c] = panel[buf][1][y * STEP_LD + i0 + x];
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int col = wave * 32 + t * 16 + cl;
+    if (col >= i0 + STEP_ROWS) {
+      half4 h, l;
+      split4(scale4(s[t], j.An.e), h, l);
+      *reinterpret_cast<half4 *>(j.An.hi + col * STEP_NP + i0 + 4 * g) = h;
+      *reinterpret_cast<half4 *>(j.An.lo() + col * STEP_NP + i0 + 4 * g) = l;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // product with the long side: Y = X Q / d, or from the left for a wide matrix
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1146,8 +1303,14 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     p.np = jobs[i].np();
     return p;
   };
-  bool small = true;
-  for (int i = 0; i < n; ++i) small = small && jobs[i].np() <= SMALL;
+  // matrices of np <= ONE_BLOCK take a launch a phase, of np = STEP_NP a launch a step, the others three a step
+  auto by_products = [&](int i) { return jobs[i].np() > ONE_BLOCK && jobs[i].np() != STEP_NP; };
+  bool small = true, any_steps = false, any_products = false;
+  for (int i = 0; i < n; ++i) {
+    small = small && jobs[i].np() <= SMALL;
+    any_steps = any_steps || jobs[i].np() == STEP_NP;
+    any_products = any_products || by_products(i);
+  }
   double s = 1.0;       // bound on the iterate's singular values (|X_0| <= |X_0|_F <= 1)
   for (int ph = 0, k = 0; ph < phases; ++ph) {
     const bool first = ph == 0, last = ph == phases - 1;
@@ -1195,18 +1358,20 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       else hipLaunchKernelGGL(orth_reduce_kernel<32>, dim3(rb), dim3(reduce_threads<32>()), 0, st, ra);
       AGX_LAUNCH_CHECK();
     }
-    // matrices: 0 A, 1 P, 2 A P, 3 / 4 Q (which of the two: 3 after an odd number of steps).  Matrices of np <= ONE_BLOCK take
-    // the one-workgroup form, the others a launch per product
+    // matrices: 0 A, 1 P, 2 A P, 3 / 4 Q (which of the two: 3 after an odd number of steps); a launch a step: 0 / 1 A
     const int steps = std::min(PHASE, o->steps - k);
     PhaseArgs pa;
     memset(&pa, 0, sizeof(pa));
     float coef[3 * PHASE];
     int eA[PHASE + 1], eP[PHASE], eS[PHASE], eQ[PHASE];              // scale exponents per step
+    int e1[PHASE], e3[PHASE], q1[PHASE];                             // of the running rows of a launch a step
     double bQ = 1.0;                                                 // |Q| <= bQ
     for (int t = 0; t < steps; ++t) {
       const float *c = o->coef + (o->n_coef == 1 ? 0 : 3 * (k + t));
       const Bounds b = bounds_of(s, c[0], c[1], c[2]);
       memcpy(coef + 3 * t, c, 3 * sizeof(float));
+      const double L = s * s;
+      e1[t] = exponent_for(L * L); e3[t] = exponent_for(L * b.S); q1[t] = exponent_for(bQ * L);
       bQ *= b.P;
       eA[t] = exponent_for(s * s); eP[t] = exponent_for(b.P); eS[t] = exponent_for(b.S); eQ[t] = exponent_for(bQ);
       s = b.next;
@@ -1242,14 +1407,33 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       hipLaunchKernelGGL(orth_phase_kernel, dim3(nblock), dim3(PW * 64), lds, st, pa);
       AGX_LAUNCH_CHECK();
     }
-    for (int t = 0; t < steps && nblock < n; ++t) {
+    for (int t = 0; t < steps && any_steps; ++t) {
+      StepArgs sa;
+      memset(&sa, 0, sizeof(sa));
+      sa.more = t + 1 < steps; sa.has_q = t > 0;
+      sa.a = coef[3 * t]; sa.b = coef[3 * t + 1]; sa.c = coef[3 * t + 2];
+      sa.e1 = e1[t]; sa.eS = eS[t]; sa.e3 = e3[t]; sa.q1 = q1[t];
+      int blocks = 0;
+      for (int i = 0; i < n; ++i)
+        if (jobs[i].np() == STEP_NP) {
+          StepJob &g = sa.job[sa.n++];
+          g.A = planes(i, t & 1, eA[t]); g.An = planes(i, t & 1 ^ 1, eA[t + 1]);
+          g.Q = planes(i, t & 1 ? 3 : 4, eQ[t > 0 ? t - 1 : 0]); g.Qn = planes(i, t & 1 ? 4 : 3, eQ[t]);
+          g.n = jobs[i].n(); g.first = blocks;
+          // (rows of A where they or the first Q are wanted, then rows of Q)
+          blocks += STEP_NP / STEP_ROWS * 2;
+        }
+      hipLaunchKernelGGL(orth_step_kernel, dim3(blocks), dim3(512), 0, st, sa);
+      AGX_LAUNCH_CHECK();
+    }
+    for (int t = 0; t < steps && any_products; ++t) {
       const int in = t & 1 ? 3 : 4, out = t & 1 ? 4 : 3, iP = t == 0 ? out : 1;   // the first step's P is Q too
       auto launch = [&](int per, auto fill) -> int {
         ChainArgs ca;
         int blocks = 0;
         ca.n = 0;
         for (int i = 0; i < n; ++i)
-          for (int w = 0; w < per && jobs[i].np() > ONE_BLOCK; ++w) {
+          for (int w = 0; w < per && by_products(i); ++w) {
             ChainJob &g = ca.job[ca.n++];
             memset(&g, 0, sizeof(g));
             g.n = jobs[i].n(); g.nt = jobs[i].np() / (small ? 32 : T); g.first = blocks; g.alpha = 1.f;
