@@ -14,9 +14,10 @@
 // everything behind it: entries then stay under 2^14, and those down to 2^-25 of the bound keep all bits.  A bf16 operand
 // needs one term only (its 8 bits fit).
 //
-// Tiles of 128 x 128 (eight waves of 64 x 32, mfma 32x32x16) where there are enough of them for the chip, of 64 x 64 below:
-// a larger tile splits and stages every element for more products.  K goes through two LDS buffers, the next
-// step's global loads in flight.
+// Tiles of 64 x 64 by four waves of 32 x 32 (mfma 32x32x16), K in steps of 64 through one LDS buffer, the next step's global
+// loads in flight: four workgroups of a CU overlap each other's loads, conversions and products.  (Tiles of 128 x 128 with
+// two buffers convert every element half as often, but leave one workgroup a CU, whose phases nothing covers: 18161 x 256
+// 166 us against 158.)
 #include "agx_common.h"
 
 #include <algorithm>
@@ -33,16 +34,16 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
-constexpr int T = 64;                          // n x n matrices are padded to T or to a multiple of 2 T
+constexpr int T = 64;                          // n x n matrices are padded to T, 2 T, 4 T or a multiple of T above
 constexpr int PHASE = 3;                       // steps between two Gram matrices
 constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ONE_BLOCK = 128;                 // largest padded side for a phase in one workgroup (LDS)
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
-constexpr int64_t BIG_TILES = 128;             // tiles of 2 T from which the product with the long side takes them
+constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram product
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
-// n x n matrix as two fp16 planes of np x np (np: n rounded up to T or a multiple of 2 T, zeros behind), value = (hi + lo) 2^-e
+// n x n matrix as two fp16 planes of np x np (np: n rounded up, zeros behind), value = (hi + lo) 2^-e
 struct Planes {
   _Float16 *hi;
   int32_t e, np;
@@ -159,18 +160,10 @@ __device__ __forceinline__ int scale_exponent(const uint32_t *maxb, int nb, uint
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// tile product: operands in LDS as [TT rows][BK k] fp16 planes, TT = 64 or 128
+// tile product: operands in LDS as [64 rows][64 k] fp16 planes
 // ---------------------------------------------------------------------------------------------------------------------
-template <int TT> struct Geo {
-  static constexpr int BK = 64;                        // k of a step: 16 values a thread and operand
-  static constexpr int LD = BK + 8;                    // LDS rows of 144 bytes: 16 rows start in 16 different bank groups
-  static constexpr int PL = TT * LD;                   // halves of a plane
-  static constexpr int NT = TT * 4;                    // threads: 4 waves of 32 x 32 or 8 of 64 x 32
-  static constexpr int WC = TT / 32;                   // waves along the columns (two along the rows)
-  static constexpr int F = TT / 64;                    // 32 x 32 fragments of a wave, one above the other
-};
-template <int TT> constexpr int tile_lds() { return 2 * 2 * 2 * Geo<TT>::PL * 2; }   // buffers, operands, planes
-
+constexpr int BK = 64, LDK = BK + 8, PL = T * LDK;   // k of a step; LDS rows of 144 bytes (16 of them start in 16 different bank
+                                                     // groups); halves of a plane
 __device__ __forceinline__ f32x4 scale4(f32x4 v, int e) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(v[i], e);
@@ -180,9 +173,8 @@ __device__ __forceinline__ f32x4 scale4(f32x4 v, int e) {
 // The loaders keep one 64-bit base a tile, the same for all lanes, and 32-bit offsets of their own (the host checks that 128
 // rows of a leading dimension fit them).
 // rows r0.. of a planes matrix, k contiguous (a symmetric matrix: also its columns)
-template <int TT> struct LoadPlanes {
+struct LoadPlanes {
   static constexpr bool two = true;
-  using G = Geo<TT>;
   const _Float16 *hi, *lo;
   int ld;
   half8 v[4];
@@ -191,7 +183,7 @@ template <int TT> struct LoadPlanes {
     const _Float16 *bh = hi + r0 * ld + k0, *bl = lo + r0 * ld + k0;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int o = ((threadIdx.x >> 3) + TT / 2 * p) * ld + (threadIdx.x & 7) * 8;
+      const int o = ((threadIdx.x >> 3) + 32 * p) * ld + (threadIdx.x & 7) * 8;
       v[2 * p] = *reinterpret_cast<const half8 *>(bh + o);
       v[2 * p + 1] = *reinterpret_cast<const half8 *>(bl + o);
     }
@@ -199,9 +191,9 @@ template <int TT> struct LoadPlanes {
   __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int o = ((threadIdx.x >> 3) + TT / 2 * p) * G::LD + (threadIdx.x & 7) * 8;
+      const int o = ((threadIdx.x >> 3) + 32 * p) * LDK + (threadIdx.x & 7) * 8;
       *reinterpret_cast<half8 *>(t + o) = v[2 * p];
-      *reinterpret_cast<half8 *>(t + G::PL + o) = v[2 * p + 1];
+      *reinterpret_cast<half8 *>(t + PL + o) = v[2 * p + 1];
     }
   }
 };
@@ -209,9 +201,8 @@ template <int TT> struct LoadPlanes {
 // (raw vectors are kept until they are stored: a conversion would wait for the load.  Tiles inside the matrix, which are
 // nearly all, take plain loads; at its edges every element is looked at.)
 // rows r0.. of a caller's matrix, k contiguous; zeros outside [rows) x [kmax)
-template <int TT, typename E> struct LoadK {
+template <typename E> struct LoadK {
   static constexpr bool two = sizeof(E) == 4;
-  using G = Geo<TT>;
   using V = typename Vec4<E>::type;
   const E *p;
   int64_t ld, rows, kmax;
@@ -220,26 +211,26 @@ template <int TT, typename E> struct LoadK {
   __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
     const E *b = p + r0 * ld + k0;
     const int row = threadIdx.x >> 4, k = (threadIdx.x & 15) * 4;
-    if (r0 + TT <= rows && k0 + G::BK <= kmax) {
+    if (r0 + T <= rows && k0 + BK <= kmax) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const V *>(b + (row + TT / 4 * q) * (int)ld + k);
+      for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const V *>(b + (row + 16 * q) * (int)ld + k);
     } else {
-      const int nk = (int)min((int64_t)G::BK, kmax - k0) - k, nr = (int)min((int64_t)TT, rows - r0);
+      const int nk = (int)min((int64_t)BK, kmax - k0) - k, nr = (int)min((int64_t)T, rows - r0);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[q][i] = row + TT / 4 * q < nr && i < nk ? b[(row + TT / 4 * q) * (int)ld + k + i] : (E)0.f;
+        for (int i = 0; i < 4; ++i) v[q][i] = row + 16 * q < nr && i < nk ? b[(row + 16 * q) * (int)ld + k + i] : (E)0.f;
     }
   }
   __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int o = ((threadIdx.x >> 4) + TT / 4 * q) * G::LD + (threadIdx.x & 15) * 4;
+      const int o = ((threadIdx.x >> 4) + 16 * q) * LDK + (threadIdx.x & 15) * 4;
       const V w = v[q];
       half4 hi, lo;
       split4(scale4(f32x4{(float)w[0], (float)w[1], (float)w[2], (float)w[3]}, e), hi, lo);
       *reinterpret_cast<half4 *>(t + o) = hi;
-      if (two) *reinterpret_cast<half4 *>(t + G::PL + o) = lo;
+      if (two) *reinterpret_cast<half4 *>(t + PL + o) = lo;
     }
   }
 };
@@ -247,9 +238,8 @@ template <int TT, typename E> struct LoadK {
 // columns r0.. of a caller's matrix whose rows are k: element (r, k) at p[k * ld + r].  A thread takes a block of 4 x 4: four
 // k's of four columns, so that loads and LDS writes are both vectors; a wave covers 32 columns of 32 k's (64 bytes or more
 // of a row, and LDS writes without bank conflicts).
-template <int TT, typename E> struct LoadT {
+template <typename E> struct LoadT {
   static constexpr bool two = sizeof(E) == 4;
-  using G = Geo<TT>;
   using V = typename Vec4<E>::type;
   const E *p;
   int64_t ld, rows, kmax;
@@ -260,11 +250,11 @@ template <int TT, typename E> struct LoadT {
   __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
     const E *b = p + k0 * ld + r0;
     const int c = col(), k = kk();
-    if (r0 + TT <= rows && k0 + G::BK <= kmax) {
+    if (r0 + T <= rows && k0 + BK <= kmax) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const V *>(b + (k + i) * (int)ld + c);
     } else {
-      const int nr = (int)min((int64_t)TT, rows - r0) - c, nk = (int)min((int64_t)G::BK, kmax - k0);
+      const int nr = (int)min((int64_t)T, rows - r0) - c, nk = (int)min((int64_t)BK, kmax - k0);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -274,11 +264,11 @@ template <int TT, typename E> struct LoadT {
   __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int o = (col() + i) * G::LD + kk();
+      const int o = (col() + i) * LDK + kk();
       half4 hi, lo;
       split4(scale4(f32x4{(float)v[0][i], (float)v[1][i], (float)v[2][i], (float)v[3][i]}, e), hi, lo);
       *reinterpret_cast<half4 *>(t + o) = hi;
-      if (two) *reinterpret_cast<half4 *>(t + G::PL + o) = lo;
+      if (two) *reinterpret_cast<half4 *>(t + PL + o) = lo;
     }
   }
 };
@@ -287,84 +277,55 @@ template <int TT, typename E> struct LoadT {
 // the split's small terms first, and vector additions the steps: a long chain of additions to one fp32 sum would lose what
 // the split keeps.  same: both operands are the same rows, loaded once.
 // late(): called when the first loads are on their way (sets the scale exponents the stores use).
-template <int TT, class LA, class LB, class Late>
-__device__ __forceinline__ void tile_product(LA &la, LB &lb, int64_t ra, int64_t rb, int64_t k0, int64_t k1, _Float16 *lds,
-                                             f32x16 (&acc)[Geo<TT>::F], bool same, Late late) {
-  using G = Geo<TT>;
-  constexpr int F = G::F, BUF = 4 * G::PL;             // a buffer: operand A's two planes, operand B's
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / G::WC, wc = wave % G::WC;
-  const int fa = (wr * 32 * F + (lane & 31)) * G::LD + (lane >> 5) * 8;
-  const int fb = (wc * 32 + (lane & 31)) * G::LD + (lane >> 5) * 8 + (same ? 0 : 2 * G::PL);
-  const int n = (int)((k1 - k0) / G::BK);
-#pragma unroll
-  for (int i = 0; i < F; ++i) acc[i] = f32x16{};
-  auto fetch = [&](int step) {
-    la.fetch(ra, k0 + (int64_t)step * G::BK);
-    if (!same) lb.fetch(rb, k0 + (int64_t)step * G::BK);
+template <class LA, class LB, class Late>
+__device__ __forceinline__ f32x16 tile_product(LA &la, LB &lb, int64_t ra, int64_t rb, int64_t k0, int64_t k1, _Float16 *lds,
+                                               bool same, Late late) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int fa = ((wave >> 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8;
+  const int fb = ((wave & 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8 + (same ? 0 : 2 * PL);
+  f32x16 acc = {};
+  auto fetch = [&](int64_t k) {
+    la.fetch(ra, k);
+    if (!same) lb.fetch(rb, k);
   };
-  auto store = [&](_Float16 *t) {
-    la.store(t);
-    if (!same) lb.store(t + 2 * G::PL);
-  };
-  auto at = [](const _Float16 *t) { return *reinterpret_cast<const half8 *>(t); };
-  auto compute = [&](const _Float16 *t) {
-    f32x16 sum[F] = {};
-#pragma unroll
-    for (int k = 0; k < G::BK; k += 32) {
-      half8 ah[2][F], bh[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int o = k + h * 16;
-        bh[h] = at(t + fb + o);
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-          ah[h][i] = at(t + fa + i * 32 * G::LD + o);
-          if constexpr (LA::two)
-            sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + G::PL + fa + i * 32 * G::LD + o), bh[h], sum[i], 0, 0, 0);
-        }
-        if constexpr (LB::two) {
-          const half8 bl = at(t + G::PL + fb + o);
-#pragma unroll
-          for (int i = 0; i < F; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[h][i], bl, sum[i], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < F; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[h][i], bh[h], sum[i], 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < F; ++i) acc[i] += sum[i];
-  };
-  fetch(0);
+  auto at = [&](int o) { return *reinterpret_cast<const half8 *>(lds + o); };
+  fetch(k0);
   late();
-  store(lds);
-  if (n > 1) fetch(1);
-  __syncthreads();
-  // (a step's products and the next one's conversion are one straight piece of code, in which they overlap; the loads of the
-  //  step behind that have one step's time)
-  for (int s = 0; s + 1 < n; ++s) {
-    compute(lds + (s & 1) * BUF);
-    store(lds + (s & 1 ^ 1) * BUF);
-    if (s + 2 < n) fetch(s + 2);
+  for (int64_t k = k0; k < k1; k += BK) {
+    la.store(lds);
+    if (!same) lb.store(lds + 2 * PL);
+    if (k + BK < k1) fetch(k + BK);
+    __syncthreads();
+    f32x16 sum = {};
+#pragma unroll
+    for (int i = 0; i < BK; i += 32) {
+      const half8 a0 = at(fa + i), a1 = at(fa + i + 16), b0 = at(fb + i), b1 = at(fb + i + 16);
+      if constexpr (LA::two) {
+        sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(PL + fa + i), b0, sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(PL + fa + i + 16), b1, sum, 0, 0, 0);
+      }
+      if constexpr (LB::two) {
+        sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, at(PL + fb + i), sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, at(PL + fb + i + 16), sum, 0, 0, 0);
+      }
+      sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0, b0, sum, 0, 0, 0);
+      sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1, b1, sum, 0, 0, 0);
+    }
+    acc += sum;
     __syncthreads();
   }
-  compute(lds + (n - 1 & 1) * BUF);
+  return acc;
 }
 // calls f(row, column, value) for a lane's elements of the tile
-template <int TT, class Fn>
-__device__ __forceinline__ void each_element(const f32x16 (&acc)[Geo<TT>::F], Fn f) {
-  using G = Geo<TT>;
+template <class Fn>
+__device__ __forceinline__ void each_element(const f32x16 &acc, Fn f) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
-  for (int i = 0; i < G::F; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      f((wave / G::WC * G::F + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), wave % G::WC * 32 + (lane & 31), acc[i][e]);
+  for (int e = 0; e < 16; ++e) f((wave >> 1) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), (wave & 1) * 32 + (lane & 31), acc[e]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Gram matrix of the long side, K split over workgroups: partial tiles [tile][slice][TT][TT] of the scaled matrix
+// Gram matrix of the long side, K split over workgroups: partial tiles [tile][slice][64][64] of the scaled matrix
 // ---------------------------------------------------------------------------------------------------------------------
 struct GramJob {
   const void *x;
@@ -380,15 +341,14 @@ struct GramArgs {
   int n;
 };
 
-template <int TT, class L>
-__device__ __forceinline__ void gram_tile(const GramJob &j, int ti, int tj, int64_t k0, int64_t k1, uint32_t *red, _Float16 *lds,
-                                          f32x16 (&acc)[Geo<TT>::F]) {
+template <class L>
+__device__ __forceinline__ f32x16 gram_tile(const GramJob &j, int ti, int tj, int64_t k0, int64_t k1, uint32_t *red, _Float16 *lds) {
   L la, lb;
   la.p = reinterpret_cast<decltype(la.p)>(j.x);
   la.ld = j.ld; la.rows = j.n; la.kmax = j.K;
   lb.p = la.p; lb.ld = la.ld; lb.rows = la.rows; lb.kmax = la.kmax;
-  tile_product<TT>(la, lb, (int64_t)ti * TT, (int64_t)tj * TT, k0, k1, lds, acc, ti == tj,
-                   [&] { la.e = lb.e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
+  return tile_product(la, lb, (int64_t)ti * T, (int64_t)tj * T, k0, k1, lds, ti == tj,
+                      [&] { la.e = lb.e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
 }
 
 // KIND: what all of a launch's matrices are (bit 0: wide, bit 1: bf16), or ANY: one loader's registers instead of the
@@ -396,11 +356,11 @@ __device__ __forceinline__ void gram_tile(const GramJob &j, int ti, int tj, int6
 constexpr int ANY = 4;
 __device__ __host__ __forceinline__ bool is_kind(int kind, bool tall, int dtype) { return kind == (tall ? 0 : 1) + (dtype == AGX_F32 ? 0 : 2); }
 
-template <int TT, int KIND>
-__global__ __launch_bounds__(TT * 4, 2) void orth_gram_kernel(GramArgs a) {
-  extern __shared__ _Float16 lds[];
-  __shared__ uint32_t red[8];
-  __shared__ float tr[8];
+template <int KIND>
+__global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
+  __shared__ __align__(16) _Float16 lds[4 * PL];
+  __shared__ uint32_t red[4];
+  __shared__ float tr[4];
   // (the tiles of one slice follow each other on one XCD, whose L2 then reads the slice once)
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
@@ -409,30 +369,24 @@ __global__ __launch_bounds__(TT * 4, 2) void orth_gram_kernel(GramArgs a) {
   const int tiles = j.nt * (j.nt + 1) / 2, slice = (id - j.first) / tiles, tile = (id - j.first) % tiles;
   int ti, tj;
   upper_tile(tile, j.nt, ti, tj);
-  const int64_t k0 = (int64_t)slice * j.kper, k1 = min(k0 + j.kper, (j.K + Geo<TT>::BK - 1) / Geo<TT>::BK * Geo<TT>::BK);
-  f32x16 acc[Geo<TT>::F];
+  const int64_t k0 = (int64_t)slice * j.kper, k1 = min(k0 + j.kper, (j.K + BK - 1) / BK * BK);
+  f32x16 acc;
   auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
-  if (is(0)) gram_tile<TT, LoadT<TT, float>>(j, ti, tj, k0, k1, red, lds, acc);
-  else if (is(1)) gram_tile<TT, LoadK<TT, float>>(j, ti, tj, k0, k1, red, lds, acc);
-  else if (is(2)) gram_tile<TT, LoadT<TT, __bf16>>(j, ti, tj, k0, k1, red, lds, acc);
-  else gram_tile<TT, LoadK<TT, __bf16>>(j, ti, tj, k0, k1, red, lds, acc);
-  float *p = j.part + ((int64_t)tile * j.slices + slice) * TT * TT;
+  if (is(0)) acc = gram_tile<LoadT<float>>(j, ti, tj, k0, k1, red, lds);
+  else if (is(1)) acc = gram_tile<LoadK<float>>(j, ti, tj, k0, k1, red, lds);
+  else if (is(2)) acc = gram_tile<LoadT<__bf16>>(j, ti, tj, k0, k1, red, lds);
+  else acc = gram_tile<LoadK<__bf16>>(j, ti, tj, k0, k1, red, lds);
+  float *p = j.part + ((int64_t)tile * j.slices + slice) * T * T;
   float d = 0.f;
-  const int wave = threadIdx.x >> 6;
-  if (ti != tj || wave / Geo<TT>::WC <= wave % Geo<TT>::WC * 2 / Geo<TT>::WC)   // (not the quarter below the diagonal)
-  each_element<TT>(acc, [&](int r, int c, float v) {
-    p[r * TT + c] = v;
+  each_element(acc, [&](int r, int c, float v) {
+    p[r * T + c] = v;
     if (r == c) d += v;
   });
   if (ti == tj) {
     d = agx::wave_sum(d);
     if ((threadIdx.x & 63) == 0) tr[threadIdx.x >> 6] = d;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      d = 0.f;
-      for (int i = 0; i < Geo<TT>::NT / 64; ++i) d += tr[i];
-      j.trace[ti * j.slices + slice] = d;
-    }
+    if (threadIdx.x == 0) j.trace[ti * j.slices + slice] = tr[0] + tr[1] + tr[2] + tr[3];
   }
 }
 
@@ -473,7 +427,7 @@ struct ReduceJob {
   const uint32_t *maxb;
   double *invd;                 // 1 / d of the scaled matrix, for the product with the long side (phase 0)
   Planes A;
-  int32_t nt, slices, e, nb, normalise, side, first;   // nt, side: of the partial tiles
+  int32_t nt, slices, e, nb, normalise, first;         // nt: partial tiles along a side
 };
 struct ReduceArgs {
   ReduceJob job[AGX_MAX_ORTH];
@@ -493,13 +447,14 @@ __global__ __launch_bounds__(reduce_threads<R>()) void orth_reduce_kernel(Reduce
   int pi, pj;                                          // square of the n x n matrix, and where it is in the partial tiles
   upper_tile((blockIdx.x - j.first) / (32 / R), j.A.np / 32, pi, pj);
   const int r0 = (blockIdx.x - j.first) % (32 / R) * R;
-  const int per = j.side / 32, ti = pi / per, tj = pj / per, area = j.side * j.side;
+  constexpr int per = T / 32, area = T * T;
+  const int ti = pi / per, tj = pj / per;
   const int tile = ti * j.nt - ti * (ti - 1) / 2 + tj - ti;
   const int grp = threadIdx.x / (R * 8), r = (threadIdx.x >> 3) % R, c = (threadIdx.x & 7) * 4;
-  const float *p = j.part + (int64_t)tile * j.slices * area + (pi % per * 32 + r0 + r) * j.side + pj % per * 32 + c;
+  const float *p = j.part + (int64_t)tile * j.slices * area + (pi % per * 32 + r0 + r) * T + pj % per * 32 + c;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int z = grp; z < j.slices; z += NG) sum += *reinterpret_cast<const f32x4 *>(p + (int64_t)z * area);
+  for (int z = grp; z < (tj < j.nt ? j.slices : 0); z += NG) sum += *reinterpret_cast<const f32x4 *>(p + (int64_t)z * area);
 #pragma unroll
   for (int i = 0; i < 4; ++i) piece[grp][r][c + i] = sum[i];
   double f;
@@ -575,9 +530,9 @@ static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 
 // (tiles of 64 x 64: an n of 1000 has 136 of them, less than a CU's worth each, so that latency counts: four steps' loads are
 //  in flight)
+constexpr int CHAIN_LDS = 2 * 4 * PL * 2;             // two buffers of both operands' planes
 __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
-  using G = Geo<T>;
-  constexpr int DEPTH = 4, BUF = 4 * G::PL;
+  constexpr int DEPTH = 4, BUF = 4 * PL;
   extern __shared__ _Float16 lds[];
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
@@ -585,19 +540,19 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
   const ChainJob &j = a.job[q];
   int ti, tj;
   upper_tile(id - j.first, j.nt, ti, tj);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, np = j.C.np, n = np / G::BK;
-  LoadPlanes<T> la[DEPTH] = {LoadPlanes<T>(j.L), LoadPlanes<T>(j.L), LoadPlanes<T>(j.L), LoadPlanes<T>(j.L)};
-  LoadPlanes<T> lb[DEPTH] = {LoadPlanes<T>(j.R), LoadPlanes<T>(j.R), LoadPlanes<T>(j.R), LoadPlanes<T>(j.R)};
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, np = j.C.np, n = np / BK;
+  LoadPlanes la[DEPTH] = {LoadPlanes(j.L), LoadPlanes(j.L), LoadPlanes(j.L), LoadPlanes(j.L)};
+  LoadPlanes lb[DEPTH] = {LoadPlanes(j.R), LoadPlanes(j.R), LoadPlanes(j.R), LoadPlanes(j.R)};
   static_assert(DEPTH == 4, "");
   f32x16 acc = {};
-  const int fa = ((wave >> 1) * 32 + (lane & 31)) * G::LD + (lane >> 5) * 8;
-  const int fb = ((wave & 1) * 32 + (lane & 31)) * G::LD + (lane >> 5) * 8 + 2 * G::PL;
+  const int fa = ((wave >> 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8;
+  const int fb = ((wave & 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8 + 2 * PL;
   auto at = [](const _Float16 *t) { return *reinterpret_cast<const half8 *>(t); };
 #pragma unroll
   for (int u = 0; u < DEPTH; ++u)
     if (u < n) {
-      la[u].fetch(ti * T, u * G::BK);
-      lb[u].fetch(tj * T, u * G::BK);
+      la[u].fetch(ti * T, u * BK);
+      lb[u].fetch(tj * T, u * BK);
     }
   for (int s = 0; s < n; s += DEPTH)
 #pragma unroll
@@ -605,10 +560,10 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
       if (s + u < n) {                                 // (one barrier a step: a buffer is written two steps after it was read)
         _Float16 *t = lds + (u & 1) * BUF;
         la[u].store(t);
-        lb[u].store(t + 2 * G::PL);
+        lb[u].store(t + 2 * PL);
         if (s + u + DEPTH < n) {
-          la[u].fetch(ti * T, (s + u + DEPTH) * G::BK);
-          lb[u].fetch(tj * T, (s + u + DEPTH) * G::BK);
+          la[u].fetch(ti * T, (s + u + DEPTH) * BK);
+          lb[u].fetch(tj * T, (s + u + DEPTH) * BK);
         }
         __syncthreads();
         f32x16 sum = {};
@@ -617,8 +572,8 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
         for (int k = 0; k < 4; ++k) {
           ah[k] = at(t + fa + k * 16);
           bh[k] = at(t + fb + k * 16);
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + G::PL + fa + k * 16), bh[k], sum, 0, 0, 0);
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], at(t + G::PL + fb + k * 16), sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + PL + fa + k * 16), bh[k], sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], at(t + PL + fb + k * 16), sum, 0, 0, 0);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], bh[k], sum, 0, 0, 0);
@@ -1035,79 +990,71 @@ struct ApplyArgs {
   int n;
 };
 
-template <int TT, typename E, bool TALL>
-__device__ __forceinline__ void apply_tile(const ApplyJob &j, int tr, int tc, int &e, uint32_t *red, _Float16 *lds,
-                                           f32x16 (&acc)[Geo<TT>::F]) {
-  LoadPlanes<TT> lq(j.Q);
+template <typename E, bool TALL>
+__device__ __forceinline__ f32x16 apply_tile(const ApplyJob &j, int tr, int tc, int &e, uint32_t *red, _Float16 *lds) {
+  LoadPlanes lq(j.Q);
   if constexpr (TALL) {
-    LoadK<TT, E> lx;
+    LoadK<E> lx;
     lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.rows; lx.kmax = j.cols;
-    tile_product<TT>(lx, lq, (int64_t)tr * TT, (int64_t)tc * TT, 0, j.Q.np, lds, acc, false,
-                     [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
+    return tile_product(lx, lq, (int64_t)tr * T, (int64_t)tc * T, 0, j.Q.np, lds, false,
+                        [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
   } else {
-    LoadT<TT, E> lx;
+    LoadT<E> lx;
     lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.cols; lx.kmax = j.rows;
-    tile_product<TT>(lq, lx, (int64_t)tr * TT, (int64_t)tc * TT, 0, j.Q.np, lds, acc, false,
-                     [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
+    return tile_product(lq, lx, (int64_t)tr * T, (int64_t)tc * T, 0, j.Q.np, lds, false,
+                        [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
   }
 }
 
-template <int TT, int KIND>
-__global__ __launch_bounds__(TT * 4, 2) void orth_apply_kernel(ApplyArgs a) {
-  extern __shared__ _Float16 lds[];
-  __shared__ uint32_t red[8];
+template <int KIND>
+__global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
+  __shared__ __align__(16) _Float16 lds[4 * PL];
+  __shared__ uint32_t red[4];
   // (tiles that read the same part of X follow each other on one XCD)
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
   while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const ApplyJob &j = a.job[q];
-  const int trs = (j.rows + TT - 1) / TT, local = id - j.first;
+  const int trs = (j.rows + T - 1) / T, local = id - j.first;
   const int tr = j.tall ? local / j.tc : local % trs, tc = j.tall ? local % j.tc : local / trs;
   int e;
-  f32x16 acc[Geo<TT>::F];
+  f32x16 acc;
   auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
-  if (is(0)) apply_tile<TT, float, true>(j, tr, tc, e, red, lds, acc);
-  else if (is(1)) apply_tile<TT, float, false>(j, tr, tc, e, red, lds, acc);
-  else if (is(2)) apply_tile<TT, __bf16, true>(j, tr, tc, e, red, lds, acc);
-  else apply_tile<TT, __bf16, false>(j, tr, tc, e, red, lds, acc);
+  if (is(0)) acc = apply_tile<float, true>(j, tr, tc, e, red, lds);
+  else if (is(1)) acc = apply_tile<float, false>(j, tr, tc, e, red, lds);
+  else if (is(2)) acc = apply_tile<__bf16, true>(j, tr, tc, e, red, lds);
+  else acc = apply_tile<__bf16, false>(j, tr, tc, e, red, lds);
   // (in 64 bits where the factor leaves fp32's normal range: tiny matrices)
   const double f = ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e);
   const float ff = (float)f;
-  if (!(fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) && f != 0.0)
+  const bool wide = !(fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) && f != 0.0;
 #pragma unroll
-    for (int i = 0; i < Geo<TT>::F; ++i)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) acc[i][k] = (float)((double)acc[i][k] * f);
-  else
-#pragma unroll
-    for (int i = 0; i < Geo<TT>::F; ++i)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) acc[i][k] *= ff;
-  const bool inside = (tr + 1) * TT <= j.rows && (tc + 1) * TT <= j.cols;
-  const int64_t at = (int64_t)tr * TT * j.ldo + (int64_t)tc * TT;
-  const int left = j.rows - tr * TT, right = j.cols - tc * TT, ldo = (int)j.ldo;
+  for (int k = 0; k < 16; ++k) acc[k] = wide ? (float)((double)acc[k] * f) : acc[k] * ff;
+  const bool inside = (tr + 1) * T <= j.rows && (tc + 1) * T <= j.cols;
+  const int64_t at = (int64_t)tr * T * j.ldo + (int64_t)tc * T;
+  const int left = j.rows - tr * T, right = j.cols - tc * T, ldo = (int)j.ldo;
   auto ok = [&](int r, int c) { return inside || (r < left && c < right); };
   if (j.muon) {
     float *w = reinterpret_cast<float *>(j.out) + at;
-    f32x16 old[Geo<TT>::F];
+    f32x16 old;
     int n = 0;
-    each_element<TT>(acc, [&](int r, int c, float) {
-      old[n / 16][n % 16] = ok(r, c) ? w[r * ldo + c] : 0.f;
+    each_element(acc, [&](int r, int c, float) {
+      old[n] = ok(r, c) ? w[r * ldo + c] : 0.f;
       ++n;
     });
     n = 0;
-    each_element<TT>(acc, [&](int r, int c, float y) {
-      if (ok(r, c)) w[r * ldo + c] = j.decay * old[n / 16][n % 16] - j.step * y;
+    each_element(acc, [&](int r, int c, float y) {
+      if (ok(r, c)) w[r * ldo + c] = j.decay * old[n] - j.step * y;
       ++n;
     });
   } else if (j.otype == AGX_F32) {
     float *o = reinterpret_cast<float *>(j.out) + at;
-    each_element<TT>(acc, [&](int r, int c, float y) {
+    each_element(acc, [&](int r, int c, float y) {
       if (ok(r, c)) o[r * ldo + c] = y;
     });
   } else {
     __bf16 *o = reinterpret_cast<__bf16 *>(j.out) + at;
-    each_element<TT>(acc, [&](int r, int c, float y) {
+    each_element(acc, [&](int r, int c, float y) {
       if (ok(r, c)) o[r * ldo + c] = (__bf16)y;
     });
   }
@@ -1130,9 +1077,9 @@ struct Job {          // one matrix of a call
   bool tall() const { return rows > cols || (rows == cols && !square_wide); }
   int n() const { return std::min(rows, cols); }
   int64_t K() const { return std::max(rows, cols); }
-  int np() const { return n() <= T ? T : agx::cdiv(n(), 2 * T) * 2 * T; }
-  int side() const { return np() == T ? T : 2 * T; }             // of the Gram matrix's tiles
-  int tiles() const { const int nt = np() / side(); return nt * (nt + 1) / 2; }
+  int np() const { return n() <= T ? T : n() <= 2 * T ? 2 * T : n() <= STEP_NP ? STEP_NP : agx::cdiv(n(), T) * T; }
+  int nt() const { return agx::cdiv(n(), T); }                   // tiles along the small side that hold anything
+  int tiles() const { return nt() * (nt() + 1) / 2; }
 };
 
 struct Layout {       // workspace of one job, in bytes from its start
@@ -1157,21 +1104,21 @@ template <class F> void by_kind(int kind, F f) {
   }
 }
 
-// slices of a Gram product: about one workgroup a CU over all of the call's matrices (each writes, and the next launch
-// reads, a whole tile)
+// slices of a Gram product: about GRAM_BLOCKS workgroups a CU over all of the call's matrices (each writes, and the next
+// launch reads, a whole tile)
 void plan(const Job &j, int total_tiles, int phases, bool need_u, Layout &l) {
-  const int tiles = j.tiles(), bk = j.side() == T ? Geo<T>::BK : Geo<2 * T>::BK;
-  const int64_t ksteps = agx::cdiv64(j.K(), bk);
-  const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() / std::max(1, total_tiles));
-  l.kper = agx::cdiv64(ksteps, std::min(ksteps, want)) * bk;
+  const int tiles = j.tiles();
+  const int64_t ksteps = agx::cdiv64(j.K(), BK);
+  const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() * GRAM_BLOCKS / std::max(1, total_tiles));
+  l.kper = std::max<int64_t>(std::min<int64_t>(ksteps, 2), agx::cdiv64(ksteps, want)) * BK;   // (two steps at least)
   l.slices = (int)agx::cdiv64(j.K(), l.kper);
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
   l.maxb = take(MAXB * 4);
   l.invd = take(8);
   for (int64_t &m : l.mat) m = take((int64_t)j.np() * j.np() * 4);
-  l.part = take((int64_t)tiles * l.slices * j.side() * j.side() * 4);
-  l.trace = take((int64_t)j.np() / j.side() * l.slices * 4);
+  l.part = take((int64_t)tiles * l.slices * T * T * 4);
+  l.trace = take((int64_t)j.nt() * l.slices * 4);
   for (int k = 0; k < 2; ++k) l.x[k] = phases > 1 + k ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.u = need_u ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.end = off;
@@ -1316,43 +1263,35 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     const bool first = ph == 0, last = ph == phases - 1;
     const int ex = exponent_for(s);                 // scale of the iterate (later phases)
     {
-      // (matrices of one tile of T and larger ones take different tiles: a launch for each kind that is there)
-      GramArgs ga[2];
+      GramArgs ga;
       ReduceArgs ra;
-      ga[0].n = ga[1].n = 0;
-      ra.n = n;
+      ga.n = ra.n = n;
       ra.eps = o->eps;
-      int gb[2] = {0, 0}, rb = 0, kind[2] = {-1, -1}, most = 0;
+      int gb = 0, rb = 0, kind = -1, most = 0;
       for (int i = 0; i < n; ++i) most = std::max(most, lay[i].slices);
       const int pieces = most > FEW_SLICES ? 8 : 1;     // of a square of 32 x 32
       for (int i = 0; i < n; ++i) {
         const Job &j = jobs[i];
         const Layout &l = lay[i];
-        const int nt = j.np() / j.side(), tl = j.tiles(), w = j.side() == T ? 0 : 1;
-        GramJob &g = ga[w].job[ga[w].n++];
+        const int nt = j.nt();
+        GramJob &g = ga.job[i];
         g.x = x[i]; g.ld = ldx[i]; g.K = j.K(); g.kper = l.kper; g.n = j.n(); g.nt = nt; g.slices = l.slices; g.tall = j.tall();
         g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
         g.maxb = reinterpret_cast<const uint32_t *>(base[i] + l.maxb);
         g.part = reinterpret_cast<float *>(base[i] + l.part);
         g.trace = reinterpret_cast<float *>(base[i] + l.trace);
-        g.first = gb[w];
-        gb[w] += tl * l.slices;
-        kind[w] = joined_kind(kind[w], g.tall, g.dtype);
+        g.first = gb;
+        gb += j.tiles() * l.slices;
+        kind = joined_kind(kind, g.tall, g.dtype);
         ReduceJob &r = ra.job[i];
         r.part = g.part; r.trace = g.trace; r.maxb = g.maxb; r.invd = reinterpret_cast<double *>(base[i] + l.invd);
         r.A = planes(i, 0, exponent_for(s * s)); r.nt = nt; r.slices = l.slices; r.e = ex; r.nb = nb[i];
-        r.normalise = first; r.side = j.side(); r.first = rb;
+        r.normalise = first; r.first = rb;
         rb += j.np() / 32 * (j.np() / 32 + 1) / 2 * pieces;
       }
-      if (ga[0].n)
-        by_kind(kind[0], [&](auto k) {
-          hipLaunchKernelGGL((orth_gram_kernel<T, decltype(k)::value>), dim3(gb[0]), dim3(256), tile_lds<T>(), st, ga[0]);
-        });
-      AGX_LAUNCH_CHECK();
-      if (ga[1].n)
-        by_kind(kind[1], [&](auto k) {
-          hipLaunchKernelGGL((orth_gram_kernel<2 * T, decltype(k)::value>), dim3(gb[1]), dim3(Geo<2 * T>::NT), tile_lds<2 * T>(), st, ga[1]);
-        });
+      by_kind(kind, [&](auto k) {
+        hipLaunchKernelGGL(orth_gram_kernel<decltype(k)::value>, dim3(gb), dim3(256), 0, st, ga);
+      });
       AGX_LAUNCH_CHECK();
       if (pieces == 8) hipLaunchKernelGGL(orth_reduce_kernel<4>, dim3(rb), dim3(reduce_threads<4>()), 0, st, ra);
       else hipLaunchKernelGGL(orth_reduce_kernel<32>, dim3(rb), dim3(reduce_threads<32>()), 0, st, ra);
@@ -1441,7 +1380,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
             fill(g, i, w);
           }
         if (small) hipLaunchKernelGGL(orth_chain_small_kernel, dim3(blocks), dim3(256), 0, st, ca);
-        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(256), tile_lds<T>(), st, ca);
+        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(256), CHAIN_LDS, st, ca);
         AGX_LAUNCH_CHECK();
         return AGX_OK;
       };
@@ -1466,12 +1405,6 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
           g.C = planes(i, 0, eA[t + 1]);
         }));
     }
-    // tiles of 2 T where they fill the chip
-    int64_t big = 0;
-    for (int i = 0; i < n; ++i) big += agx::cdiv64(jobs[i].rows, 2 * T) * agx::cdiv64(jobs[i].cols, 2 * T);
-    bool use_big = big >= BIG_TILES;
-    for (int i = 0; i < n; ++i) use_big = use_big && jobs[i].np() > T;
-    const int side = use_big ? 2 * T : T;
     ApplyArgs aa;
     aa.n = n;
     int blocks = 0, kind = -1;
@@ -1492,13 +1425,12 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         ldx[i] = g.ldo;
       }
       kind = joined_kind(kind, g.tall, g.dtype);
-      g.tc = agx::cdiv(j.cols, side);
+      g.tc = agx::cdiv(j.cols, T);
       g.first = blocks;
-      blocks += agx::cdiv(j.rows, side) * g.tc;
+      blocks += agx::cdiv(j.rows, T) * g.tc;
     }
     by_kind(kind, [&](auto k) {
-      if (use_big) hipLaunchKernelGGL((orth_apply_kernel<2 * T, decltype(k)::value>), dim3(blocks), dim3(Geo<2 * T>::NT), tile_lds<2 * T>(), st, aa);
-      else hipLaunchKernelGGL((orth_apply_kernel<T, decltype(k)::value>), dim3(blocks), dim3(256), tile_lds<T>(), st, aa);
+      hipLaunchKernelGGL(orth_apply_kernel<decltype(k)::value>, dim3(blocks), dim3(256), 0, st, aa);
     });
     AGX_LAUNCH_CHECK();
   }
@@ -1543,24 +1475,11 @@ int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, co
 }  // namespace
 
 // (more LDS than the default limit of a launch)
-namespace {
-template <class K> hipError_t allow_lds(K *kernel, int bytes) {
-  return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-}  // namespace
 int agx::orth_prepare_device() {
-  AGX_HIP(allow_lds(&orth_phase_kernel, phase_lds(ONE_BLOCK)));
-  AGX_HIP(allow_lds(&orth_chain_kernel, tile_lds<T>()));
-  for (int kind = 0; kind <= ANY; ++kind) {
-    hipError_t e = hipSuccess;
-    by_kind(kind, [&](auto k) {
-      constexpr int K = decltype(k)::value;
-      for (hipError_t r : {allow_lds(&orth_gram_kernel<T, K>, tile_lds<T>()), allow_lds(&orth_gram_kernel<2 * T, K>, tile_lds<2 * T>()),
-                           allow_lds(&orth_apply_kernel<T, K>, tile_lds<T>()), allow_lds(&orth_apply_kernel<2 * T, K>, tile_lds<2 * T>())})
-        if (r != hipSuccess) e = r;
-    });
-    AGX_HIP(e);
-  }
+  AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_phase_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              phase_lds(ONE_BLOCK)));
+  AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_chain_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              CHAIN_LDS));
   return AGX_OK;
 }
 
