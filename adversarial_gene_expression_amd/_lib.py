@@ -73,6 +73,8 @@ class MlpDesc(C.Structure):
         ('bn', C.c_int32), ('bn_eps', C.c_float), ('bn_momentum', C.c_float),
         ('bn_gamma_off', C.c_int64 * AGX_MAX_LAYERS), ('bn_beta_off', C.c_int64 * AGX_MAX_LAYERS),
         ('bn_mean_off', C.c_int64 * AGX_MAX_LAYERS), ('bn_var_off', C.c_int64 * AGX_MAX_LAYERS),
+        ('ln', C.c_int32), ('ln_eps', C.c_float),
+        ('ln_gamma_off', C.c_int64 * AGX_MAX_LAYERS), ('ln_beta_off', C.c_int64 * AGX_MAX_LAYERS),
     ]
 
 

@@ -108,6 +108,9 @@ int ff_hx(void *stream, const float *hrows, int ldh, int HL, float *X, int ldx, 
 // epilogue, without split-K (then fused and unfused runs sum in the same order: bit-identical)
 bool gemm_can_fuse_opt(int M, int N, int K, int64_t ws_floats);
 int fill_zero(void *stream, float *p, int64_t n);   // elementwise.hip
+// real += (1 - alpha[b]) d, fake += alpha[b] d over B rows of H values, all with leading dimension ld: the backward of
+// agx_gp_interp into gradients that are there already (elementwise.hip)
+int interp_back(void *stream, const float *d, float *real, float *fake, int ld, const float *alpha, int B, int H);
 int colstats_scratch_init();   // corr.hip: address of the static scratch of agx_colstats_noalloc on the current device
 // Loss-log snapshot done by the last small-gradient launch of a captured iteration: n floats from
 // src to the address stored at *dst_slot (left there by iter_stage; NULL address: no copy).

@@ -81,6 +81,14 @@ struct agx_cgan {
   float *bn_scale = nullptr, *bn_shift = nullptr;
   double *bn_ws = nullptr;
   int64_t bn_ws_doubles = 0;
+  // layer normalisation (cfg.gen.ln / cfg.disc.ln; eager step functions only): values in front of it and the rows'
+  // statistics - the generator's in gpre / g_mean / g_rstd, the critic's in P / d_mean / d_rstd; N: gradients behind it;
+  // lnU: one layer's B rows of the penalty's second-order chain; ln_ws: the parameter gradients' partial rows
+  float *P[AGX_MAX_LAYERS + 1] = {}, *N[AGX_MAX_LAYERS + 1] = {};   // [3Bm, ldh]
+  float *d_mean[AGX_MAX_LAYERS + 1] = {}, *d_rstd[AGX_MAX_LAYERS + 1] = {};   // [3Bm]
+  float *g_mean[AGX_MAX_LAYERS + 1] = {}, *g_rstd[AGX_MAX_LAYERS + 1] = {};   // [Bm]
+  float *lnU = nullptr, *ln_ws = nullptr;
+  int64_t ln_ws_floats = 0;
   float *F = nullptr;                       // [S*Bm, ldsx] fake rows of a whole captured iteration
   int ldgh[AGX_MAX_LAYERS + 1] = {};
   // staging for the captured iteration (agx_cgan_iter_*)
@@ -126,6 +134,13 @@ int validate_mlp(const agx_mlp_desc_t &m, const char *name, int want_in, int wan
       for (const int64_t off : {m.bn_gamma_off[l], m.bn_beta_off[l], m.bn_mean_off[l], m.bn_var_off[l]})
         AGX_CHECK_ARG(off >= 0 && off % 4 == 0 && off + m.dims[l + 1] <= m.n_flat, "%s: batch-norm vector of layer %d outside the flat buffer", name, l);
   }
+  if (m.ln) {
+    AGX_CHECK_ARG(!m.bn, "%s: batch-norm and layer normalisation at once", name);
+    AGX_CHECK_ARG(m.ln_eps > 0.f, "%s: layer normalisation eps", name);
+    for (int l = 0; l < m.n_layers - 1; ++l)
+      for (const int64_t off : {m.ln_gamma_off[l], m.ln_beta_off[l]})
+        AGX_CHECK_ARG(off >= 0 && off % 4 == 0 && off + m.dims[l + 1] <= m.n_flat, "%s: layer normalisation vector of layer %d outside the flat buffer", name, l);
+  }
   for (int l = 0; l < m.n_layers; ++l) {
     AGX_CHECK_ARG(m.dims[l + 1] > 0 && m.ldw[l] >= m.dims[l + 1], "%s: layer %d ldw", name, l);
     AGX_CHECK_ARG(m.w_off[l] >= 0 && m.w_off[l] % 4 == 0 && m.w_off[l] + (int64_t)m.dims[l] * m.ldw[l] <= m.n_flat,
@@ -166,8 +181,9 @@ void carve(agx_cgan *h, float *base) {
   const int L = c.disc.n_layers - 1;
   for (int l = 1; l <= L; ++l) {
     h->ldh[l] = r4(c.disc.dims[l]);
-    h->A[l] = cv.take((int64_t)3 * Bm * h->ldh[l]);
-    h->D[l] = cv.take((int64_t)(3 * Bm + (l == 1 ? h->HD : 0)) * h->ldh[l]);
+    const int64_t blocks = c.disc.ln ? 4 : 3;         // (critic_core_ln keeps a fourth block of rows)
+    h->A[l] = cv.take(blocks * Bm * h->ldh[l]);
+    h->D[l] = cv.take((blocks * Bm + (l == 1 ? h->HD : 0)) * h->ldh[l]);
     if (l == 1 && h->D[l]) h->D[l] += (size_t)h->HD * h->ldh[l];
   }
   h->out = cv.take(4 * 3 * Bm);                      // up to 4 partial dot products per row (column-split tails)
@@ -210,6 +226,28 @@ void carve(agx_cgan *h, float *base) {
     h->bn_ws_doubles = wsd;
     h->bn_ws = reinterpret_cast<double *>(cv.take(2 * wsd));
   }
+  {
+    int64_t lnw = 0, maxh = 0;
+    if (c.gen.ln)
+      for (int l = 1; l <= Lg; ++l) {
+        h->gpre[l] = cv.take((int64_t)Bm * h->ldgh[l]);
+        h->g_mean[l] = cv.take(Bm);
+        h->g_rstd[l] = cv.take(Bm);
+        lnw = std::max(lnw, agx_layernorm_ws_floats(Bm, c.gen.dims[l], AGX_F32));
+      }
+    if (c.disc.ln)
+      for (int l = 1; l <= L; ++l) {
+        h->P[l] = cv.take((int64_t)3 * Bm * h->ldh[l]);
+        h->N[l] = cv.take((int64_t)3 * Bm * h->ldh[l]);
+        h->d_mean[l] = cv.take(3 * Bm);
+        h->d_rstd[l] = cv.take(3 * Bm);
+        lnw = std::max(lnw, agx_layernorm_ws_floats(2 * Bm, c.disc.dims[l], AGX_F32));
+        maxh = std::max<int64_t>(maxh, h->ldh[l]);
+      }
+    h->lnU = cv.take(Bm * maxh);
+    h->ln_ws = cv.take(lnw);
+    h->ln_ws_floats = lnw;
+  }
   h->ldsx = r4(c.x_dim);
   h->F = cv.take((int64_t)S * Bm * h->ldsx);
   h->snum = cv.take((int64_t)Bm * std::max(c.gen.n_num, 1));
@@ -232,6 +270,7 @@ void carve(agx_cgan *h, float *base) {
       need = std::max(need, agx_gemm_ws_floats(3 * B, c.disc.dims[l], c.disc.dims[l + 1]));
       need = std::max(need, agx_gemm_ws_floats(B, c.disc.dims[l], c.disc.dims[l + 1]));
       need = std::max(need, agx_gemm_ws_floats(c.disc.dims[l], c.disc.dims[l + 1], 3 * B));
+      if (c.disc.ln) need = std::max(need, agx_gemm_ws_floats(c.disc.dims[l], c.disc.dims[l + 1], 4 * B));
     }
     need = std::max(need, (int64_t)2 * B * c.disc.dims[1]);  // layer 1 always goes through the slab reduce
     // Gram form of the penalty: W_g^T W_g, d_1 . M, d_1^T (f d_1), and the layer-1 product over 2B + H1 rows
@@ -314,6 +353,35 @@ bool tn_fuse() {
   static const bool v = getenv("AGX_NO_TN_FUSE") == nullptr;
   return v;
 }
+
+// Layer normalisation behind hidden layer l (0-based) of net m with the flat parameters p, gradients g
+struct Norm {
+  agx_norm_t n;
+  Norm(const agx_cgan *h, const agx_mlp_desc_t &m, const float *p, int l, int R, const float *x, int ldx, float *mean,
+       float *rstd, const float *y) {
+    memset(&n, 0, sizeof(n));
+    n.x = x; n.ldx = ldx; n.rows = R; n.width = m.dims[l + 1];
+    n.gamma = p + m.ln_gamma_off[l]; n.beta = p + m.ln_beta_off[l];
+    n.mean = mean; n.rstd = rstd;
+    n.y = const_cast<float *>(y); n.ldy = ldx;
+    n.eps = m.ln_eps; n.slope = h->cfg.slope; n.dtype = AGX_F32; n.act = 1;
+    n.ws = h->ln_ws; n.ws_floats = h->ln_ws_floats;
+  }
+  Norm &params(float *dgamma, float *dbeta, bool add) {
+    n.dgamma = dgamma; n.dbeta = dbeta; n.accumulate_params = add;
+    return *this;
+  }
+  int fwd(hipStream_t st) { return agx_layernorm_fwd(st, &n); }
+  int bwd(hipStream_t st, const float *dy, float *dx, bool add = false) {
+    n.dy = dy; n.dx = dx; n.lddy = n.lddx = n.ldx; n.accumulate_dx = add;
+    return agx_layernorm_bwd(st, &n);
+  }
+  int bwd2(hipStream_t st, const float *u, const float *dy, float *ddy, float *dx) {
+    n.u = u; n.dy = dy; n.ddy = ddy; n.dx = dx; n.ldu = n.lddy = n.ldddy = n.lddx = n.ldx;
+    return agx_layernorm_bwd2(st, &n);
+  }
+};
+
 // generator layer-1 input rows [0, R): [z | num | emb], covariates of source row r % B
 int gen_input(agx_cgan *h, hipStream_t st, const float *z, const int32_t *cat, const float *num, int R,
               int B) {
@@ -360,6 +428,20 @@ int gen_layers(agx_cgan *h, hipStream_t st, int R, float *out, int ldo, const ag
       ldin = ldo_l;
     }
     l0 = m.n_layers - 1;
+  } else if (m.ln) {
+    // (the training-mode forward keeps what gen_core's backward reads; any other normalises in place)
+    AGX_CHECK_ARG(!training || R <= h->Bm, "generator layer normalisation: %d rows > max_batch %d", R, h->Bm);
+    for (int l = 0; l < m.n_layers - 1; ++l) {
+      float *o = h->gh[l + 1], *pre = training ? h->gpre[l + 1] : o;
+      const int ldo_l = h->ldgh[l + 1];
+      AGX_TRY(Gemm(h, in, ldin, 0, h->gp + m.w_off[l], m.ldw[l], 0, pre, ldo_l, R, m.dims[l + 1], m.dims[l])
+                  .bias(h->gp + m.b_off[l]).id(AGX_K_GEN_FWD_HID).run(st));
+      AGX_TRY(Norm(h, m, h->gp, l, R, pre, ldo_l, training ? h->g_mean[l + 1] : nullptr,
+                   training ? h->g_rstd[l + 1] : nullptr, o).fwd(st));
+      in = o;
+      ldin = ldo_l;
+    }
+    l0 = m.n_layers - 1;
   } else
   if (gen_tail && m.n_layers == 3 && m.dims[0] <= 128 && m.dims[1] <= 256 && m.dims[2] <= 256 && (batch > 0 ? batch : R) <= 64) {
     // small batches: both hidden layers in ONE launch (tail.hip mode 2; always 4 column groups, so that a row's
@@ -400,7 +482,7 @@ bool tail_ok(const agx_cgan *h, int rows) {
   static const bool off = getenv("AGX_NO_TAIL") != nullptr;
   // (any batch: at 512 rows the tails still beat reduce + Dense + Dense(1) launches, 176.6 k vs 172.0 k samples/s)
   // (mode 1 zeroes the covariate columns of a row with one 256-thread group: ncov <= 256)
-  return !off && m.n_layers == 3 && m.dims[1] <= 256 && m.dims[2] <= 256 && h->ncov <= 256;
+  return !off && !m.ln && m.n_layers == 3 && m.dims[1] <= 256 && m.dims[2] <= 256 && h->ncov <= 256;
 }
 
 // Gram form of the gradient penalty (critic_core), for batches of at least the first hidden width (gram_ratio2): the
@@ -484,6 +566,19 @@ int tail_forward(agx_cgan *h, hipStream_t st, int splitk, int m_slab, int interp
   return agx::critic_tail(st, 0, t);
 }
 
+// critic with layer normalisation: the Dense product of hidden layer l (0-based) in front of it; the normalisation of
+// the R rows from row p0 of P (its statistics' rows too) into / by the sign of the rows from row a0 of A
+int ln_dense(agx_cgan *h, hipStream_t st, int l, const float *in, int ldin, int R, float *out) {
+  const agx_mlp_desc_t &m = h->cfg.disc;
+  return Gemm(h, in, ldin, 0, h->dp + m.w_off[l], m.ldw[l], 0, out, h->ldh[l + 1], R, m.dims[l + 1], m.dims[l])
+      .bias(h->dp + m.b_off[l]).id(l == 0 ? AGX_K_DISC_FWD_IN : AGX_K_DISC_FWD_HID).run(st);
+}
+Norm ln_norm(agx_cgan *h, int l, int R, int p0, int a0) {
+  const int ld = h->ldh[l + 1];
+  return Norm(h, h->cfg.disc, h->dp, l, R, h->P[l + 1] + (size_t)p0 * ld, ld, h->d_mean[l + 1] + p0, h->d_rstd[l + 1] + p0,
+              h->A[l + 1] + (size_t)a0 * ld);
+}
+
 // critic Dense stack from layer index l0 over R rows (input of layer l0 already in place),
 // then Dense(1) + seed of the backward chain D[L] = act'(A_L) * c(r) * w_out
 int disc_layers_from(agx_cgan *h, hipStream_t st, int l0, int R, int n0, int n1, float c0, float c1,
@@ -500,13 +595,19 @@ int disc_layers_from(agx_cgan *h, hipStream_t st, int l0, int R, int n0, int n1,
   for (int l = l0; l < L; ++l) {
     const float *in = l == 0 ? h->X : h->A[l];
     const int ldin = l == 0 ? h->ldx : h->ldh[l];
+    if (m.ln) {
+      AGX_TRY(ln_dense(h, st, l, in, ldin, R, h->P[l + 1]));
+      AGX_TRY(ln_norm(h, l, R, 0, 0).fwd(st));
+      continue;
+    }
     Gemm g(h, in, ldin, 0, h->dp + m.w_off[l], m.ldw[l], 0, h->A[l + 1], h->ldh[l + 1], R,
         m.dims[l + 1], m.dims[l]);
     g.bias(h->dp + m.b_off[l]).act().id(l == 0 ? AGX_K_DISC_FWD_IN : AGX_K_DISC_FWD_HID);
     AGX_TRY(g.run(st));
   }
+  // (layer normalisation: its backward takes act' itself, the seed is c(r) * w_out alone - a slope of 1 - into N[L])
   return agx_critic_head(st, h->A[L], h->ldh[L], h->dp + m.w_off[L], h->dp + m.b_off[L], h->out,
-                         h->D[L], h->ldh[L], R, m.dims[L], n0, n1, c0, c1, c2, h->cfg.slope);
+                         m.ln ? h->N[L] : h->D[L], h->ldh[L], R, m.dims[L], n0, n1, c0, c1, c2, m.ln ? 1.f : h->cfg.slope);
 }
 
 int disc_cov_columns(agx_cgan *h, hipStream_t st, const int32_t *cat, const float *num, int R, int B) {
@@ -519,6 +620,16 @@ int disc_cov_columns(agx_cgan *h, hipStream_t st, const int32_t *cat, const floa
 int disc_backward_chain(agx_cgan *h, hipStream_t st, int R) {
   const agx_mlp_desc_t &m = h->cfg.disc;
   const int L = m.n_layers - 1;
+  if (m.ln) {
+    // N[l] = gradients behind the normalisation, D[l] = in front of it (no parameter gradients: the generator's step)
+    for (int l = L; l >= 1; --l) {
+      AGX_TRY(ln_norm(h, l - 1, R, 0, 0).bwd(st, h->N[l], h->D[l]));
+      if (l > 1)
+        AGX_TRY(Gemm(h, h->D[l], h->ldh[l], 0, h->dp + m.w_off[l - 1], m.ldw[l - 1], 1, h->N[l - 1], h->ldh[l - 1], R,
+                     m.dims[l - 1], m.dims[l]).id(AGX_K_DISC_CHAIN).run(st));
+    }
+    return AGX_OK;
+  }
   for (int l = L; l >= 2; --l) {
     // D[l-1] = act'(A[l-1]) * (D[l] . W_{l-1}^T);  W_{l-1}: [d_{l-1}, d_l]
     Gemm g(h, h->D[l], h->ldh[l], 0, h->dp + m.w_off[l - 1], m.ldw[l - 1], 1, h->D[l - 1],
@@ -527,6 +638,97 @@ int disc_backward_chain(agx_cgan *h, hipStream_t st, int R) {
     AGX_TRY(g.run(st));
   }
   return AGX_OK;
+}
+
+// Critic gradients with layer normalisation, given X rows [0,2B) = [real; fake].  The Dense -> norm -> act layers are
+// curved in their input, so the penalty reaches every parameter through the interpolated rows' forward pass too.
+// Per layer l on the interpolated rows, P = values in front of the norm, a = behind the activation:
+//   first order   N_l = dD/da_l,  delta_l = bwd(N_l; P_l),  N_{l-1} = delta_l W_l^T,  g = delta_1 W_1[:G]^T
+//   up            u_1 = (f g) W_1[:G];  (E_l, p_l) = bwd2(u_l; N_l, P_l);  u_{l+1} = E_l W_{l+1}
+//   down          p_l += bwd(p_{l+1} W_{l+1}^T; P_l)        with E_l, p_l = the penalty's gradients by N_l and P_l
+//   dW_l = a_{l-1}^T p_l + E_{l-1}^T delta_l,  dw_out = colsum(E_L);  bwd2 and the down pass add to dgamma, dbeta
+// Blocks of B rows, in an order that lets every product above and the weight gradients (one product over 4B rows per
+// layer) run over contiguous rows:
+//   A[l] = [a inter | a real | a fake | E],  D[l] = [p | delta real | delta fake | delta inter],
+//   P[l] and its statistics as A[l];  N[l] = [real | fake | inter], N[L] (written by the head) as A[L]
+// Layer 1: P is linear in the input, p_1 goes to the real and fake rows by (1 - alpha) and alpha (tf_utils.py:162-167).
+int critic_core_ln(agx_cgan *h, hipStream_t st, const int32_t *cat, int B, int B_global, const float *alpha,
+                   float gp_weight, float *losses) {
+  const agx_mlp_desc_t &m = h->cfg.disc;
+  const int L = m.n_layers - 1, G = h->G, ldx = h->ldx;
+  const float invb = 1.0f / (float)B_global;
+  float *Xi = h->X + (size_t)2 * B * ldx;
+  auto blk = [&](float *base, int l, int k) { return base + (size_t)k * B * h->ldh[l]; };
+  // forward: [real; fake] through the first product, the interpolated rows by its linearity
+  AGX_TRY(ln_dense(h, st, 0, h->X, ldx, 2 * B, blk(h->P[1], 1, 1)));
+  AGX_TRY(agx_gp_interp(st, blk(h->P[1], 1, 1), h->ldh[1], blk(h->P[1], 1, 2), h->ldh[1], alpha, h->P[1], h->ldh[1], B, m.dims[1]));
+  AGX_TRY(ln_norm(h, 0, 3 * B, 0, 0).fwd(st));
+  AGX_TRY(disc_layers_from(h, st, 1, 3 * B, B, B, 1.f, -invb, invb));
+  // first order
+  for (int l = L; l >= 1; --l) {
+    const int in = l == L ? 0 : 2, rf = l == L ? 1 : 0;
+    AGX_TRY(ln_norm(h, l - 1, 2 * B, B, B).params(h->dg + m.ln_gamma_off[l - 1], h->dg + m.ln_beta_off[l - 1], false)
+                .bwd(st, blk(h->N[l], l, rf), blk(h->D[l], l, 1)));
+    AGX_TRY(ln_norm(h, l - 1, B, 0, 0).bwd(st, blk(h->N[l], l, in), blk(h->D[l], l, 3)));
+    if (l > 1)
+      AGX_TRY(Gemm(h, blk(h->D[l], l, 1), h->ldh[l], 0, h->dp + m.w_off[l - 1], m.ldw[l - 1], 1, h->N[l - 1], h->ldh[l - 1],
+                   3 * B, m.dims[l - 1], m.dims[l]).id(AGX_K_DISC_CHAIN).run(st));
+  }
+  // g into the inter rows of X; slopes, f, delta_1 *= f, covariate columns of those rows to zero
+  float *D1i = blk(h->D[1], 1, 3);
+  AGX_TRY(Gemm(h, D1i, h->ldh[1], 0, h->dp + m.w_off[0], m.ldw[0], 1, Xi, ldx, B, G, m.dims[1])
+              .rowsq(h->rowsq, h->nslab).id(AGX_K_DISC_DX).run(st));
+  AGX_TRY(agx_gp_finalize(st, h->rowsq, h->nslab, h->nslab, h->slopes, h->fscale, D1i, h->ldh[1], m.dims[1], Xi + G, ldx,
+                          h->ncov, B, gp_weight * 2.0f * invb));
+  // up
+  for (int l = 1; l <= L; ++l) {
+    Gemm g(h, l == 1 ? Xi : blk(h->A[l - 1], l - 1, 3), l == 1 ? ldx : h->ldh[l - 1], 0, h->dp + m.w_off[l - 1],
+           m.ldw[l - 1], 0, h->lnU, h->ldh[l], B, m.dims[l], l == 1 ? G : m.dims[l - 1]);
+    if (l == 1) g.rowscale(h->fscale);
+    AGX_TRY(g.id(l == 1 ? AGX_K_GP2_IN : AGX_K_GP2_HID).run(st));
+    AGX_TRY(ln_norm(h, l - 1, B, 0, 0).params(h->dg + m.ln_gamma_off[l - 1], nullptr, true)
+                .bwd2(st, h->lnU, blk(h->N[l], l, l == L ? 0 : 2), blk(h->A[l], l, 3), h->D[l]));
+  }
+  // down
+  for (int l = L - 1; l >= 1; --l) {
+    AGX_TRY(Gemm(h, h->D[l + 1], h->ldh[l + 1], 0, h->dp + m.w_off[l], m.ldw[l], 1, h->lnU, h->ldh[l], B, m.dims[l],
+                 m.dims[l + 1]).id(AGX_K_DISC_CHAIN).run(st));
+    AGX_TRY(ln_norm(h, l - 1, B, 0, 0).params(h->dg + m.ln_gamma_off[l - 1], h->dg + m.ln_beta_off[l - 1], true)
+                .bwd(st, h->lnU, h->D[l], true));
+  }
+  AGX_TRY(agx::interp_back(st, h->D[1], blk(h->D[1], 1, 1), blk(h->D[1], 1, 2), h->ldh[1], alpha, B, m.dims[1]));
+  // kernel gradients, then everything small in one launch (as critic_core)
+  agx::TnJobs tn;
+  tn.n = 0;
+  for (int l = L - 1; l >= 0; --l) {
+    const float *in = l == 0 ? h->X : h->A[l], *d = l == 0 ? blk(h->D[1], 1, 1) : h->D[l + 1];
+    const int ldin = l == 0 ? ldx : h->ldh[l], R = l == 0 ? 3 * B : 4 * B;
+    if (l > 0 && tn_fuse() && agx::tn_job_ok(m.dims[l], m.dims[l + 1], R)) {
+      tn.job[tn.n++] = agx::TnJobs::Job{in, d, h->dg + m.w_off[l], ldin, h->ldh[l + 1], m.ldw[l], m.dims[l], m.dims[l + 1], R};
+      continue;
+    }
+    AGX_TRY(Gemm(h, in, ldin, 1, d, h->ldh[l + 1], 0, h->dg + m.w_off[l], m.ldw[l], m.dims[l], m.dims[l + 1], R)
+                .id(l == 0 ? AGX_K_DISC_DW_IN : AGX_K_DISC_DW_HID).run(st));
+  }
+  agx_small_grads_t j;
+  memset(&j, 0, sizeof(j));
+  j.n_colsum = L;
+  for (int l = 0; l < L; ++l) {
+    j.cs_A[l] = h->D[l + 1]; j.cs_lda[l] = h->ldh[l + 1]; j.cs_r0[l] = l == 0 ? B : 0; j.cs_r1[l] = 3 * B;
+    j.cs_H[l] = m.dims[l + 1]; j.cs_out[l] = h->dg + m.b_off[l];
+  }
+  j.w_A = blk(h->A[L], L, 1); j.w_lda = h->ldh[L]; j.w_R = 3 * B; j.w_H = m.dims[L]; j.w_n0 = B; j.w_n1 = B;
+  j.w_c0 = -invb; j.w_c1 = invb; j.w_c2 = 1.f;
+  j.w_out = h->dg + m.w_off[L]; j.w_bias_out = h->dg + m.b_off[L];
+  if (m.emb.n_cat > 0) {
+    j.emb_grad = h->dg; j.emb = m.emb; j.emb_D = blk(h->D[1], 1, 1); j.emb_ldd = h->ldh[1]; j.emb_H = m.dims[1];
+    j.emb_W = h->dp + m.w_off[0]; j.emb_ldw = m.ldw[0]; j.emb_col0 = G + m.n_num;
+    j.emb_cat = cat; j.emb_ld_cat = m.emb.n_cat; j.emb_B = B; j.emb_rows = 2 * B;
+  }
+  j.l_losses = losses; j.l_out = h->out + B; j.l_slopes = h->slopes; j.l_n0 = B; j.l_n1 = B; j.l_ns = B;
+  j.l_out_parts = 1; j.l_out_ld = 3 * h->Bm;
+  j.l_inv_b = invb; j.l_gp_weight = gp_weight; j.l_fake_sign = 1.f;
+  return agx::small_grads_run(st, &j, agx::LossCopy{nullptr, nullptr, 0}, &tn);
 }
 
 // Critic gradients given X rows [0,2B) = [real; fake] (gene + covariate columns in place).
@@ -773,7 +975,7 @@ int gen_core(agx_cgan *h, hipStream_t st, const int32_t *cat, int B, int B_globa
   int lddout = ldx;
   // small batches of the two-hidden-layer generator: split-K reduce + hidden delta product as one tail launch
   static const bool gen_tail_off = getenv("AGX_NO_GEN_TAIL") != nullptr;
-  const bool tail3 = !gen_tail_off && !fact && Lg == 2 && !gm.bn && B <= 64 && gm.dims[1] <= 256 && gm.dims[2] <= 256 &&
+  const bool tail3 = !gen_tail_off && !fact && Lg == 2 && !gm.bn && !gm.ln && B <= 64 && gm.dims[1] <= 256 && gm.dims[2] <= 256 &&
                      gm.ldw[1] % 4 == 0;
   for (int l = Lg; l >= 0; --l) {
     const float *in = l == 0 ? h->gin0 + (size_t)gen_row0 * h->ldg0 : h->gh[l] + (size_t)gen_row0 * h->ldgh[l];
@@ -837,8 +1039,12 @@ int gen_core(agx_cgan *h, hipStream_t st, const int32_t *cat, int B, int B_globa
              : (fact && l == Lg) ? Gemm(h, h->D[1], h->ldh[1], 0, h->genPT, h->ldpt, 0, h->gd[l], h->ldgh[l], B, HLg, H1c)
                                  : Gemm(h, dout, lddout, 0, h->gp + gm.w_off[l], gm.ldw[l], 1, h->gd[l], h->ldgh[l], B, gm.dims[l],
                                         gm.dims[l + 1]);
-      g.mask(in, ldin).id(l == Lg ? AGX_K_GEN_BWD_OUT : AGX_K_GEN_BWD_HID);
-      AGX_TRY(g.run(st));
+      if (!gm.ln) g.mask(in, ldin);
+      AGX_TRY(g.id(l == Lg ? AGX_K_GEN_BWD_OUT : AGX_K_GEN_BWD_HID).run(st));
+      if (gm.ln)   // (its backward takes act' by the sign of the activations) in place; gamma / beta gradients of hidden layer l - 1
+        AGX_TRY(Norm(h, gm, h->gp, l - 1, B, h->gpre[l], h->ldgh[l], h->g_mean[l], h->g_rstd[l], in)
+                    .params(h->gg + gm.ln_gamma_off[l - 1], h->gg + gm.ln_beta_off[l - 1], false)
+                    .bwd(st, h->gd[l], h->gd[l]));
       if (gm.bn)   // gd[l] = dL/d(normalised value) -> dL/d(Dense output), gamma / beta gradients of hidden layer l - 1
         AGX_TRY(agx_bn_backward(st, h->gd[l], h->ldgh[l], h->gpre[l], h->ldgh[l], h->bn_mean[l], h->bn_std[l],
                                 h->gp + gm.bn_gamma_off[l - 1], gm.bn_eps, B, gm.dims[l], h->gg + gm.bn_gamma_off[l - 1],
@@ -987,6 +1193,7 @@ extern "C" int agx_cgan_disc_grads(agx_cgan_t *h, void *stream, const agx_step_a
     AGX_TRY(agx_aug_add(st, Xr, ldx, a->aug_mask, a->aug_noise_real, G, 0, B, G));
   }
   AGX_TRY(disc_cov_columns(h, st, a->cat, a->num, 2 * B, B));
+  if (h->cfg.disc.ln) return critic_core_ln(h, st, a->cat, B, a->B_global, a->alpha, a->gp_weight, a->losses);
   return critic_core(h, st, a->cat, B, a->B_global, a->alpha, a->gp_weight, a->losses);
 }
 
@@ -1300,6 +1507,7 @@ extern "C" int agx_cgan_iter_capture(agx_cgan_t *h, void *stream, const agx_iter
   AGX_CHECK_ARG(!a->aug_mask_gen || a->aug_noise_gen, "agx_cgan_iter_capture: generator aug noise missing");
   AGX_CHECK_ARG(stream != nullptr, "agx_cgan_iter_capture: capture needs a non-default stream");
   AGX_CHECK_ARG(!h->cfg.gen.bn, "agx_cgan_iter_capture: batch-norm generators run through the eager step functions only");
+  AGX_CHECK_ARG(!h->cfg.gen.ln && !h->cfg.disc.ln, "agx_cgan_iter_capture: layer-normalised nets run through the eager step functions only");
   if (agx_prof_enabled()) {
     agx::set_error("agx_cgan_iter_capture: event brackets cannot be captured; call agx_prof_enable(-2) first");
     return AGX_E_STATE;
@@ -1423,6 +1631,7 @@ extern "C" int agx_cgan_iter_eager(agx_cgan_t *h, void *stream, const agx_iter_a
   AGX_CHECK_ARG(a->nb_critic >= 0 && a->nb_critic < h->S, "agx_cgan_iter_eager: nb_critic %d needs max_steps > %d", a->nb_critic, a->nb_critic);
   AGX_CHECK_ARG(!a->split, "agx_cgan_iter_eager: one-GPU form only");
   AGX_CHECK_ARG(!h->cfg.gen.bn, "agx_cgan_iter_eager: batch-norm generators run through the eager step functions only");
+  AGX_CHECK_ARG(!h->cfg.gen.ln && !h->cfg.disc.ln, "agx_cgan_iter_eager: layer-normalised nets run through the eager step functions only");
   AGX_CHECK_ARG(a->opt_kind == 1 ? (a->disc_m && a->disc_v && a->gen_m && a->gen_v && a->adam_lr_t_host)
                                  : (a->opt_kind == 0 && a->disc_rms && a->gen_rms),
                 "agx_cgan_iter_eager: optimizer slots (and adam_lr_t_host for Adam) required");

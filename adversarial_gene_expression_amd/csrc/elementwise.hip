@@ -93,6 +93,18 @@ __global__ void __launch_bounds__(256) gp_interp_kernel(const float *__restrict_
   }
 }
 
+__global__ void __launch_bounds__(256) interp_back_kernel(const float *__restrict__ d, float *__restrict__ real,
+                                                          float *__restrict__ fake, int ld,
+                                                          const float *__restrict__ alpha, int H) {
+  const size_t row = (size_t)blockIdx.y * ld;
+  const float a = alpha[blockIdx.y];
+  for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < H; j += gridDim.x * blockDim.x) {
+    const float v = d[row + j], f = a * v;
+    real[row + j] += v - f;
+    fake[row + j] += f;
+  }
+}
+
 __global__ void __launch_bounds__(256) aug_add_kernel(float *__restrict__ x, int ldx,
                                                       const float *__restrict__ mask,
                                                       const float *__restrict__ noise, int ldn,
@@ -1206,6 +1218,14 @@ extern "C" int agx_gp_interp(void *stream, const float *real, int32_t ldr, const
   if (B <= 0 || G <= 0) return AGX_OK;
   hipLaunchKernelGGL(gp_interp_kernel, dim3(std::min(agx::cdiv(G, 256), 64), B), dim3(256), 0,
                      agx::as_stream(stream), real, ldr, fake, ldf, alpha, inter, ldi, B, G);
+  AGX_LAUNCH_CHECK();
+  return AGX_OK;
+}
+
+int agx::interp_back(void *stream, const float *d, float *real, float *fake, int ld, const float *alpha, int B, int H) {
+  if (B <= 0 || H <= 0) return AGX_OK;
+  hipLaunchKernelGGL(interp_back_kernel, dim3(std::min(agx::cdiv(H, 256), 64), B), dim3(256), 0, agx::as_stream(stream), d,
+                     real, fake, ld, alpha, H);
   AGX_LAUNCH_CHECK();
   return AGX_OK;
 }

@@ -8,7 +8,9 @@ gradient penalty's double-backward) is derived by hand in csrc/cgan.hip.
 
 Differences a caller can see (all additive):
   * optimizers are ``RMSprop`` / ``Adam`` from this module (Keras-v2 formulas)
-    instead of ``tfk.optimizers.*``;
+    instead of ``tfk.optimizers.*``, and ``Muon``, which the reference lacks;
+  * ``make_generator`` / ``make_discriminator`` take ``layer_norm=True`` (the
+    generator also ``batch_norm=True``), which the reference lacks;
   * ``train_disc`` / ``train_gen`` / ``train`` / ``predict`` take optional
     keyword-only ``alpha=``, ``aug=`` (and ``z=`` where the reference already
     has it) to inject the random draws TF would make, which is how parity
@@ -33,7 +35,7 @@ import torch
 from . import _dev, _lib, ops
 from ._dev import DeviceArray, ptr
 
-tfk = SimpleNamespace()  # populated below with .optimizers.{RMSprop, Adam}
+tfk = SimpleNamespace()  # populated below with .optimizers.{RMSprop, Adam, Muon}
 
 CHECKPOINTS_DIR = '../checkpoints/'
 _LOSS_SLOTS = 64  # floats appended to every flat gradient buffer (loss scalars ride the gradient exchange)
@@ -100,7 +102,7 @@ class _Net:
     kind = None
 
     def __init__(self, x_dim, vocab_sizes, nb_numeric, h_dims, z_dim, slope=0.0, weights=None, seed=None,
-                 batch_norm=False, bn_epsilon=1e-3, bn_momentum=0.99):
+                 batch_norm=False, bn_epsilon=1e-3, bn_momentum=0.99, layer_norm=False, ln_epsilon=1e-3):
         if h_dims is None:
             h_dims = [256, 256]
         # optional BatchNormalization after every hidden Dense, before the activation (the
@@ -114,6 +116,14 @@ class _Net:
         if self.batch_norm and self.kind != 'gen':
             raise NotImplementedError('batch_norm is available for the generator only: the WGAN-GP critic is penalised per '
                                       'sample (tf_utils.py:154-171), batch statistics would couple the samples')
+        # optional LayerNormalization in the same place (the reference has none): a row's own statistics, so the critic
+        # may have it - the gradient penalty then differentiates through the normalisation - and data parallelism needs
+        # no exchange.  Eager step functions only.
+        self.layer_norm, self.ln_epsilon = bool(layer_norm), float(ln_epsilon)
+        if self.layer_norm and self.batch_norm:
+            raise ValueError('batch_norm and layer_norm exclude each other')
+        if self.layer_norm and not self.ln_epsilon > 0.0:
+            raise ValueError('ln_epsilon must be positive, got %r' % (ln_epsilon,))
         if len(h_dims) < 1 or len(h_dims) + 1 > _lib.AGX_MAX_LAYERS:
             raise ValueError('h_dims must have between 1 and %d entries' % (_lib.AGX_MAX_LAYERS - 1))
         if len(vocab_sizes) > _lib.AGX_MAX_CAT:
@@ -152,6 +162,7 @@ class _Net:
             off = a64(off + v * e)
         self.ldw, self.w_off, self.b_off = [], [], []
         self.bn_off = []      # per hidden layer: flat offsets of (gamma, beta, moving_mean, moving_variance)
+        self.ln_off = []      # per hidden layer: flat offsets of (gamma, beta)
         for l in range(len(self.dims) - 1):
             n = self.dims[l + 1]
             ld = 1 if n == 1 else _dev.r4(n)
@@ -166,6 +177,9 @@ class _Net:
                     four.append(off)
                     off = a64(off + n)
                 self.bn_off.append(tuple(four))
+            if self.layer_norm and l < len(self.dims) - 2:
+                self.ln_off.append((off, a64(off + n)))
+                off = a64(a64(off + n) + n)
         self.n_flat = off
         d = _lib.MlpDesc()
         d.n_layers = len(self.dims) - 1
@@ -182,6 +196,9 @@ class _Net:
         d.bn_eps, d.bn_momentum = self.bn_epsilon, self.bn_momentum
         for l, four in enumerate(self.bn_off):
             d.bn_gamma_off[l], d.bn_beta_off[l], d.bn_mean_off[l], d.bn_var_off[l] = four
+        d.ln, d.ln_eps = int(self.layer_norm), self.ln_epsilon
+        for l, two in enumerate(self.ln_off):
+            d.ln_gamma_off[l], d.ln_beta_off[l] = two
         self.desc = d
 
     def _initial_weights(self, seed):
@@ -196,11 +213,13 @@ class _Net:
             if self.batch_norm and l < len(self.dims) - 2:     # Keras BatchNormalization: gamma 1, beta 0, moving 0 / 1
                 n = self.dims[l + 1]
                 ws += [np.ones(n, np.float32), np.zeros(n, np.float32), np.zeros(n, np.float32), np.ones(n, np.float32)]
+            if self.layer_norm and l < len(self.dims) - 2:     # Keras LayerNormalization: gamma 1, beta 0
+                ws += [np.ones(self.dims[l + 1], np.float32), np.zeros(self.dims[l + 1], np.float32)]
         return ws
 
     def _segments(self):
         """(flat offset, rows, cols, ld) per variable in Keras `get_weights()` order (a batch-norm layer contributes
-        gamma, beta, moving_mean, moving_variance behind its Dense)."""
+        gamma, beta, moving_mean, moving_variance behind its Dense, a layer-norm layer gamma, beta)."""
         segs = [(o, v, e, e) for o, v, e in zip(self.emb_off, self.vocab_sizes, self.emb_dims)]
         self._vector_seg, self._frozen_seg = set(), set()
         for l in range(len(self.dims) - 1):
@@ -212,6 +231,10 @@ class _Net:
                     self._vector_seg.add(len(segs))
                     if q >= 2:
                         self._frozen_seg.add(len(segs))      # moving statistics: not trainable
+                    segs.append((o, 1, self.dims[l + 1], self.dims[l + 1]))
+            if l < len(self.ln_off):
+                for o in self.ln_off[l]:
+                    self._vector_seg.add(len(segs))
                     segs.append((o, 1, self.dims[l + 1], self.dims[l + 1]))
         return segs
 
@@ -258,6 +281,8 @@ class _Net:
             names += ['dense_%d/kernel' % l, 'dense_%d/bias' % l]
             if self.batch_norm and l < len(self.bn_off):
                 names += ['batch_normalization_%d/%s' % (l, q) for q in ('gamma', 'beta', 'moving_mean', 'moving_variance')]
+            if l < len(self.ln_off):
+                names += ['layer_normalization_%d/%s' % (l, q) for q in ('gamma', 'beta')]
         for n, (_, r, c, _) in zip(names, self._segments()):
             print('  %-22s %-16s %d' % (n, (r, c) if r > 1 or 'kernel' in n or 'emb' in n else (c,), r * c))
         print('Total params: {:,}'.format(self.count_params()))
@@ -271,6 +296,8 @@ class _Net:
                    nb_numeric=self.nb_numeric, h_dims=self.h_dims, slope=self.slope)
         if self.batch_norm:
             cfg.update(batch_norm=True, bn_epsilon=self.bn_epsilon, bn_momentum=self.bn_momentum)
+        if self.layer_norm:
+            cfg.update(layer_norm=True, ln_epsilon=self.ln_epsilon)
         np.savez(path, __config__=np.array(repr(cfg)), **{'w%03d' % i: w for i, w in enumerate(self.get_weights())})
 
     # -- forward (op-level ABI) ---------------------------------------------
@@ -290,6 +317,7 @@ class _Net:
         h, _ = self._embed_concat(lead, cc, nc, rows)
         acts = [h]
         nl = len(self.dims) - 1
+        kept = []          # layer normalisation: (values in front of it, mean, rstd) per hidden layer
         for l in range(nl):
             n, k = self.dims[l + 1], self.dims[l]
             w = self.params[self.w_off[l]:self.w_off[l] + k * self.ldw[l]].view(k, self.ldw[l])
@@ -298,11 +326,17 @@ class _Net:
                 ga, be, mm, mv = (self.params[o:o + n] for o in self.bn_off[l])
                 h = ops.dense_bn(h, w, b, rows, n, k, gamma=ga, beta=be, eps=self.bn_epsilon, slope=self.slope,
                                  running=(mm, mv))[0]
+            elif self.layer_norm and l < nl - 1:
+                pre = ops.gemm(h, w, rows, n, k, bias=b)
+                ga, be = (self.params[o:o + n] for o in self.ln_off[l])
+                h = torch.empty_like(pre) if keep else pre
+                _, mean, rstd = ops.layer_norm(pre[:, :n], ga, be, eps=self.ln_epsilon, act=1, slope=self.slope, out=h[:, :n])
+                kept.append((pre[:, :n], mean, rstd))
             else:
                 h = ops.gemm(h, w, rows, n, k, bias=b, act=1 if l < nl - 1 else 0, slope=self.slope)
             acts.append(h)
         out = h[:, :self.dims[-1]]
-        return (out, acts) if keep else out
+        return (out, acts, kept) if keep else out
 
     def __call__(self, inputs, training=False):
         lead, cc, nc = inputs
@@ -345,7 +379,8 @@ def load_model(path):
     cfg = _check_model_config(cfg)
     cls = Generator if cfg['kind'] == 'gen' else Critic
     return cls(cfg['x_dim'], cfg['vocab_sizes'], cfg['nb_numeric'], cfg['h_dims'], cfg['z_dim'],
-               slope=cfg['slope'], weights=ws, **{k: cfg[k] for k in ('batch_norm', 'bn_epsilon', 'bn_momentum') if k in cfg})
+               slope=cfg['slope'], weights=ws, **{k: cfg[k] for k in ('batch_norm', 'bn_epsilon', 'bn_momentum', 'layer_norm',
+                                                                      'ln_epsilon') if k in cfg})
 
 
 def _check_model_config(cfg):
@@ -365,6 +400,10 @@ def _check_model_config(cfg):
         if cfg['batch_norm'] is not True or not all(isinstance(cfg.get(k), float) and cfg[k] > 0 for k in ('bn_epsilon', 'bn_momentum')):
             raise ValueError('model file: malformed batch-norm entries in __config__ %r' % (cfg,))
         bn = dict(batch_norm=True, bn_epsilon=cfg['bn_epsilon'], bn_momentum=cfg['bn_momentum'])
+    if cfg.get('layer_norm', False):
+        if cfg['layer_norm'] is not True or bn or not (isinstance(cfg.get('ln_epsilon'), float) and cfg['ln_epsilon'] > 0):
+            raise ValueError('model file: malformed layer-norm entries in __config__ %r' % (cfg,))
+        bn = dict(layer_norm=True, ln_epsilon=cfg['ln_epsilon'])
     return dict(kind=cfg['kind'], x_dim=cfg['x_dim'], z_dim=cfg['z_dim'], nb_numeric=cfg['nb_numeric'],
                 vocab_sizes=list(cfg['vocab_sizes']), h_dims=list(cfg['h_dims']), slope=float(cfg.get('slope', 0.0)), **bn)
 
@@ -426,19 +465,25 @@ def _critic_input_gradient(disc, x, cc, nc):
     """d sum(D(x)) / d x for a ReLU critic, hand-derived chain on the op-level ABI."""
     lib = _lib.load()
     rows = x.shape[0]
-    _, acts = disc._forward(x, cc, nc, keep=True)
+    _, acts, kept = disc._forward(x, cc, nc, keep=True)
     L = len(disc.dims) - 2
     a = acts[L]
     d = _dev.empty(a.shape)
     w_out = disc.params.data_ptr() + 4 * disc.w_off[L]
+    # (with layer normalisation the derivative of the activation is layer_norm_backward's: a slope of 1 leaves it out here)
     _lib.check(lib.agx_delta_init(_dev.stream(), ptr(a), a.stride(0), w_out, ptr(d), d.stride(0), rows,
-                                  disc.dims[L], 0, 0, 0.0, 0.0, 1.0, disc.slope), 'agx_delta_init')
+                                  disc.dims[L], 0, 0, 0.0, 0.0, 1.0, 1.0 if disc.layer_norm else disc.slope), 'agx_delta_init')
     for l in range(L, 0, -1):
         n = disc.dims[l - 1] if l > 1 else disc.x_dim
         k = disc.dims[l]
+        if disc.layer_norm:
+            pre, mean, rstd = kept[l - 1]
+            o = disc.ln_off[l - 1][0]
+            d = ops.layer_norm_backward(d[:, :k], pre, mean, rstd, disc.params[o:o + k], y=acts[l][:, :k], act=1,
+                                        slope=disc.slope, param_grads=False)[0]
         w = disc.params[disc.w_off[l - 1]:disc.w_off[l - 1] + disc.dims[l - 1] * disc.ldw[l - 1]].view(
             disc.dims[l - 1], disc.ldw[l - 1])
-        d = ops.gemm(d, w, rows, n, k, tb=1, slope=disc.slope, mask=acts[l - 1] if l > 1 else None)
+        d = ops.gemm(d, w, rows, n, k, tb=1, slope=disc.slope, mask=acts[l - 1] if l > 1 and not disc.layer_norm else None)
     return d  # [rows, r4(x_dim)]
 
 
@@ -554,7 +599,65 @@ class Adam:
                 'v': net._unflatten(_gathered_slot(net, st[1]).cpu().numpy())}
 
 
-tfk.optimizers = SimpleNamespace(RMSprop=RMSprop, Adam=Adam)
+class Muon:
+    """Orthogonalised momentum for the Dense kernels (no reference counterpart: its optimizers are RMSprop and Adam,
+    tf_utils.py:285-288): ``m = momentum*m + g ; u = g + momentum*m (nesterov) or m ;
+    w -= lr * (sqrt(max(1, out / in)) * orthogonalize(u) + weight_decay * w)``, with ``steps`` Newton-Schulz steps over
+    all kernels of a net in one call.  What has no direction to orthogonalise - embedding tables, biases, normalisation
+    vectors, kernels with a side of 1 (the critic's Dense(1)) - and kernels whose smaller side exceeds
+    AGX_ORTH_MAX_SIDE take the ``fallback`` optimizer (default RMSprop(5e-4)).  train() runs it through the eager step
+    functions; under data parallelism the gradients are all-reduced and every rank takes the whole step."""
+
+    def __init__(self, learning_rate=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, epsilon=1e-7,
+                 coefficients=ops.NEWTON_SCHULZ, fallback=None, **kw):
+        self.learning_rate, self.momentum = float(kw.get('lr', learning_rate)), float(momentum)
+        self.nesterov, self.weight_decay = bool(nesterov), float(weight_decay)
+        self.steps, self.epsilon, self.coefficients = int(steps), float(epsilon), coefficients
+        self.fallback = RMSprop(5e-4) if fallback is None else fallback
+        if type(self.fallback) not in (RMSprop, Adam):
+            raise TypeError('fallback must be an RMSprop or Adam')
+        self._state = {}
+        self.iterations = 0
+
+    @staticmethod
+    def _plan(net):
+        """([(offset, rows, cols, ld)] of the orthogonalised kernels, [(offset, length)] of the ranges between them)."""
+        mats = [(o, r, c, ld) for o, r, c, ld in zip(net.w_off, net.dims, net.dims[1:], net.ldw)
+                if 1 < min(r, c) <= _lib.AGX_ORTH_MAX_SIDE]
+        gaps, lo = [], 0
+        for o, r, _, ld in mats:
+            gaps.append((lo, o - lo))
+            lo = o + (r * ld + 63) // 64 * 64
+        gaps.append((lo, net.n_flat - lo))
+        return mats, [(a, n) for a, n in gaps if n > 0]
+
+    def slot(self, net):
+        ent = self._state.get(id(net))
+        if ent is None or ent[0]() is not net:
+            ent = self._state[id(net)] = (weakref.ref(net), _dev.zeros(net.n_flat))
+        return ent[1]
+
+    def apply(self, net, grad_scale=1.0):
+        m = self.slot(net)
+        grads = net.grads if grad_scale == 1.0 else net.grads * grad_scale
+        mats, gaps = self._plan(net)
+        if mats:
+            view = lambda buf: [buf[o:o + r * ld].view(r, ld)[:, :c] for o, r, c, ld in mats]
+            ops.muon(view(net.params), view(grads), view(m), self.learning_rate, momentum=self.momentum,
+                     nesterov=self.nesterov, weight_decay=self.weight_decay, steps=self.steps,
+                     coefficients=self.coefficients, eps=self.epsilon)
+        for k, (lo, n) in enumerate(gaps):
+            self.fallback.apply_range(net, lo, n, grads[lo:lo + n], advance=k == 0)
+        self.iterations += 1
+
+    def state_arrays(self, net):
+        """Momentum and the fallback's slots in Keras variable order (zeros where the other one is in charge).  Every
+        rank of a data-parallel run holds all of them; a COLLECTIVE under torch.distributed all the same, since the
+        fallback's own is."""
+        return dict(self.fallback.state_arrays(net), momentum=net._unflatten(self.slot(net).cpu().numpy()))
+
+
+tfk.optimizers = SimpleNamespace(RMSprop=RMSprop, Adam=Adam, Muon=Muon)
 
 
 # ---------------------------------------------------------------------------
@@ -832,7 +935,13 @@ def _dp_update(net, opt):
     optimizer to that share only (the 94 MB RMSprop pass of the GTEx critic becomes 94/R MB per GPU; the
     optimizer slots of the other shares are never touched), all-gather the parameters.  Same bytes on the
     links as one all-reduce of the gradients.  The loss scalars sit in the slots behind the gradients: their
-    sums travel back in the parameter buffer's tail (net._pbuf[n_flat:])."""
+    sums travel back in the parameter buffer's tail (net._pbuf[n_flat:]).  Muon orthogonalises whole kernels, which no
+    shard holds: the gradients are all-reduced and every rank takes the same step."""
+    if type(opt) is Muon:
+        _allreduce_grads(net)
+        opt.apply(net)
+        net._pbuf[net.n_flat:net.n_flat + _LOSS_SLOTS].copy_(net.grads[net.n_flat:])
+        return
     world, rank = _world()
     pieces = _exchange_pieces(net, world, _dp_chunks(net, 0))   # (no overlap on this path: one piece unless AGX_DP_CHUNKS asks)
     key = (world, rank, len(pieces))
@@ -999,9 +1108,11 @@ def train_gen(z, cc, nc, gen, disc, gen_opt, p_aug=0, norm_scale=1, *, aug=None,
     return DeviceArray(gen.grads[gen.n_flat:gen.n_flat + 1].clone())
 
 
-def _graph_ok(gen_opt, disc_opt, world=1, gen=None):
+def _graph_ok(gen_opt, disc_opt, world=1, gen=None, disc=None):
     if gen is not None and getattr(gen, 'batch_norm', False):
         return False      # batch-norm generators: eager step functions (training-mode forward in train_gen only)
+    if getattr(gen, 'layer_norm', False) or getattr(disc, 'layer_norm', False):
+        return False      # layer-normalised nets: eager step functions
     if type(gen_opt) is RMSprop and type(disc_opt) is RMSprop:
         return gen_opt.rho == disc_opt.rho and gen_opt.epsilon == disc_opt.epsilon
     if type(gen_opt) is Adam and type(disc_opt) is Adam:
@@ -1036,17 +1147,17 @@ def train_iteration(x, cc, nc, gen, disc, gen_opt, disc_opt, nb_critic=5, grad_p
     captured as nb_critic+1 gradient segments; between them the flat gradient buffer is reduce-scattered
     over RCCL, each rank applies the optimizer to its 1/R shard and the parameters are all-gathered
     (``_dp_update``); draws are the global batch's, so R ranks reproduce the one-GPU big-batch run.
-    RMSprop (the reference default) or Adam on both nets; ``train`` falls back to the eager step
-    functions otherwise."""
+    RMSprop (the reference default) or Adam on both nets without normalisation layers; ``train`` falls back to the
+    eager step functions otherwise."""
     lib = _lib.load()
     x = _dev.to_dev(x)
     cc = _dev.to_dev(cc, torch.int32)
     nc = _dev.to_dev(nc)
     B = x.shape[0]
     world, _ = _world()
-    if not _graph_ok(gen_opt, disc_opt, gen=gen):
+    if not _graph_ok(gen_opt, disc_opt, gen=gen, disc=disc):
         raise ValueError('train_iteration needs the same optimizer class (RMSprop or Adam) with equal decay rates / '
-                         'epsilon on both networks, and a generator without batch-norm')
+                         'epsilon on both networks, and networks without batch-norm or layer-norm')
     Bg = int(batch_global) if batch_global else B * world
     if world == 1 and Bg != B:
         raise ValueError('batch_global differs from the local batch on a single GPU')
@@ -1143,7 +1254,7 @@ def train(dataset, cat_covs, num_covs, z_dim, epochs, batch_size, gen, disc, sco
             if hi_r <= lo_r:
                 raise ValueError('global batch of %d rows cannot be split over %d ranks' % (bg, world))
             x, cc, nc = data[lo_r:hi_r], ccs[lo_r:hi_r], ncs[lo_r:hi_r]
-            if use_graph and noise_fn is None and nb_critic > 0 and _graph_ok(gen_opt, disc_opt, gen=gen):
+            if use_graph and noise_fn is None and nb_critic > 0 and _graph_ok(gen_opt, disc_opt, gen=gen, disc=disc):
                 d_l, g_l = train_iteration(x, cc, nc, gen, disc, gen_opt, disc_opt, nb_critic, 10, p_aug, norm_scale,
                                            batch_global=bg, row_lo=lo_r - i)
                 dl.append(d_l)

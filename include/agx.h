@@ -464,6 +464,12 @@ typedef struct agx_mlp_desc {
   int32_t bn;
   float bn_eps, bn_momentum;        /* Keras defaults 1e-3, 0.99 */
   int64_t bn_gamma_off[AGX_MAX_LAYERS], bn_beta_off[AGX_MAX_LAYERS], bn_mean_off[AGX_MAX_LAYERS], bn_var_off[AGX_MAX_LAYERS];
+  /* optional LayerNormalization after every hidden Dense, before the activation (no reference counterpart either): a  */
+  /* row's own statistics, so the critic may have it and data parallelism needs no exchange.  Not together with bn;    */
+  /* eager step functions only.  Per hidden layer l two vectors of dims[l+1] floats: gamma, beta.                      */
+  int32_t ln;
+  float ln_eps;                     /* Keras default 1e-3 */
+  int64_t ln_gamma_off[AGX_MAX_LAYERS], ln_beta_off[AGX_MAX_LAYERS];
 } agx_mlp_desc_t;
 
 typedef struct agx_cgan_config {
