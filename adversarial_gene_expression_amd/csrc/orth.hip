@@ -35,7 +35,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int T = 64;                          // n x n matrices are padded to T, 2 T, 4 T or a multiple of T above
-constexpr int PHASE = 3;                       // steps between two Gram matrices
+constexpr int PHASE = 3;                       // most steps between two Gram matrices
 constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ONE_BLOCK = 128;                 // largest padded side for a phase in one workgroup (LDS)
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
@@ -43,12 +43,25 @@ constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram prod
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
-// n x n matrix as two fp16 planes of np x np (np: n rounded up, zeros behind), value = (hi + lo) 2^-e
+// n x n matrix as two fp16 planes of np x np (np: n rounded up, zeros behind), value = (hi + lo) 2^-e.  Row-major above
+// OPERAND_NP; up to it in the order of the matrix cores' operands, so that a wave's load of 16 rows and 32 k is one piece of
+// 1 KB: blocks of 16 rows by 64 k, in them (k / 8) % 2, then (k / 16) % 4, the row and k % 8.  (Row-major, each of those
+// loads asks for 16 bytes of 32 lines or more.)
+constexpr int OPERAND_NP = 256;
 struct Planes {
   _Float16 *hi;
   int32_t e, np;
   __device__ __forceinline__ _Float16 *lo() const { return hi + (int64_t)np * np; }
 };
+__device__ __forceinline__ int place(int np, int row, int k) {        // (eight k's from a multiple of 8 on are neighbours)
+  if (np > OPERAND_NP) return row * np + k;
+  return (((row >> 4) * (np >> 6) + (k >> 6)) * 2 + ((k >> 3) & 1)) * 512 + (((k >> 4) & 3) * 16 + (row & 15)) * 8 + (k & 7);
+}
+__device__ __forceinline__ void placed(int np, int piece, int &row, int &k) {   // of the piece-th eight values in operand order
+  const int block = piece >> 7;
+  row = block / (np >> 6) * 16 + (piece & 15);
+  k = block % (np >> 6) * 64 + (piece >> 4 & 3) * 16 + (piece >> 6 & 1) * 8;
+}
 
 __device__ __forceinline__ int exponent_of(uint32_t absbits) {   // e with |v| < 2^e for the float of these bits
   return absbits == 0 ? 0 : (int)(absbits >> 23) - 126;
@@ -485,28 +498,30 @@ __global__ __launch_bounds__(reduce_threads<R>()) void orth_reduce_kernel(Reduce
   const int y0 = pi * 32 + r0, x0 = pj * 32, np = j.A.np;
   f32x4 v;
   half4 h, l;
-  int o;
+  int row, col;
   if (grp == 0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = total(r, c + i);
-    o = (y0 + r) * np + x0 + c;
+    row = y0 + r;
+    col = x0 + c;
   } else if (grp == 1) {                               // (32 rows of R columns)
     const int x = threadIdx.x % (R * 8) / (R / 4), y = threadIdx.x % (R / 4) * 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = total(y + i, x);
-    o = (x0 + x) * np + y0 + y;
+    row = x0 + x;
+    col = y0 + y;
   } else {
     return;
   }
   split4(v, h, l);
+  const int o = place(np, row, col);
   if (pi != pj) {
     *reinterpret_cast<half4 *>(j.A.hi + o) = h;
     *reinterpret_cast<half4 *>(j.A.lo() + o) = l;
   } else {                                             // what is on and above the diagonal, and its mirror image
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = o / np, col = o % np + i;
-      if (grp == 0 ? row <= col : row > col) {
+      if (grp == 0 ? row <= col + i : row > col + i) {
         j.A.hi[o + i] = h[i];
         j.A.lo()[o + i] = l[i];
       }
@@ -714,8 +729,13 @@ __device__ __forceinline__ void phase_steps(const PhaseArgs &a, const PhaseJob &
   constexpr int nt = NP / 32, tri = nt * (nt + 1) / 2, LD = NP + 8, PL = NP * LD;   // (16 rows start in 16 bank groups)
   _Float16 *P = A + 2 * PL;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = (lane >> 5) * 8;
+  auto lds_place = [](int i) {
+    int row, k;
+    placed(NP, i / 8, row, k);
+    return row * LD + k;
+  };
   for (int i = threadIdx.x * 8; i < NP * NP; i += PW * 64 * 8) {
-    const int o = i / NP * LD + i % NP;
+    const int o = lds_place(i);
     *reinterpret_cast<half8 *>(&A[o]) = *reinterpret_cast<const half8 *>(j.A.hi + i);
     *reinterpret_cast<half8 *>(&A[PL + o]) = *reinterpret_cast<const half8 *>(j.A.lo() + i);
   }
@@ -802,7 +822,7 @@ __device__ __forceinline__ void phase_steps(const PhaseArgs &a, const PhaseJob &
   }
   const _Float16 *f = a.stages == 1 ? P : A;           // (one step: P is the product)
   for (int i = threadIdx.x * 8; i < NP * NP; i += PW * 64 * 8) {
-    const int o = i / NP * LD + i % NP;
+    const int o = lds_place(i);
     *reinterpret_cast<half8 *>(j.Q.hi + i) = *reinterpret_cast<const half8 *>(&f[o]);
     *reinterpret_cast<half8 *>(j.Q.lo() + i) = *reinterpret_cast<const half8 *>(&f[PL + o]);
   }
@@ -847,15 +867,16 @@ __global__ __launch_bounds__(512, 2) void orth_step_kernel(StepArgs a) {
   // the rows themselves, and A's columns (= rows: it is symmetric) wave * 32 ..; k runs in an order of its own, the same for
   // both operands: a lane's vectors of two steps are neighbours in memory
   const Planes &R = rows_of_q ? j.Q : j.A;
-  const int pr = threadIdx.x >> 5, pc = (threadIdx.x & 31) * 8;
-  const half8 rh = *reinterpret_cast<const half8 *>(R.hi + (i0 + pr) * STEP_NP + pc);
-  const half8 rl = *reinterpret_cast<const half8 *>(R.lo() + (i0 + pr) * STEP_NP + pc);
+  int pr, pc;                                          // this thread's eight values of them
+  placed(STEP_NP, threadIdx.x, pr, pc);
+  const int mine = i0 * STEP_NP + threadIdx.x * 8;
+  const half8 rh = *reinterpret_cast<const half8 *>(R.hi + mine), rl = *reinterpret_cast<const half8 *>(R.lo() + mine);
   half8 bh[2][8], bl[2][8];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int o = (wave * 32 + t * 16 + cl) * STEP_NP + (k >> 1) * 64 + g * 16 + (k & 1) * 8;
+      const int o = (wave * 2 + t) * 16 * STEP_NP + k * 512 + lane * 8;
       bh[t][k] = *reinterpret_cast<const half8 *>(j.A.hi + o);
       bl[t][k] = *reinterpret_cast<const half8 *>(j.A.lo() + o);
     }
@@ -904,8 +925,8 @@ __global__ __launch_bounds__(512, 2) void orth_step_kernel(StepArgs a) {
     __syncthreads();
   };
   auto write_rows = [&](const Planes &m) {             // the current panel
-    *reinterpret_cast<half8 *>(m.hi + (i0 + pr) * STEP_NP + pc) = *reinterpret_cast<const half8 *>(&panel[buf][0][pr * STEP_LD + pc]);
-    *reinterpret_cast<half8 *>(m.lo() + (i0 + pr) * STEP_NP + pc) = *reinterpret_cast<const half8 *>(&panel[buf][1][pr * STEP_LD + pc]);
+    *reinterpret_cast<half8 *>(m.hi + mine) = *reinterpret_cast<const half8 *>(&panel[buf][0][pr * STEP_LD + pc]);
+    *reinterpret_cast<half8 *>(m.lo() + mine) = *reinterpret_cast<const half8 *>(&panel[buf][1][pr * STEP_LD + pc]);
   };
   Rows r, x1, x2, s;
 #pragma unroll
@@ -956,8 +977,8 @@ __global__ __launch_bounds__(512, 2) void orth_step_kernel(StepArgs a) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int c = from + k, y = min(pr, c), x = max(pr, c);
-      j.An.hi[(i0 + pr) * STEP_NP + i0 + c] = panel[buf][0][y * STEP_LD + i0 + x];
-      j.An.lo()[(i0 + pr) * STEP_NP + i0 + c] = panel[buf][1][y * STEP_LD + i0 + x];
+      j.An.hi[mine + k] = panel[buf][0][y * STEP_LD + i0 + x];
+      j.An.lo()[mine + k] = panel[buf][1][y * STEP_LD + i0 + x];
     }
   }
 #pragma unroll
@@ -966,8 +987,9 @@ __global__ __launch_bounds__(512, 2) void orth_step_kernel(StepArgs a) {
     if (col >= i0 + STEP_ROWS) {
       half4 h, l;
       split4(scale4(s[t], j.An.e), h, l);
-      *reinterpret_cast<half4 *>(j.An.hi + col * STEP_NP + i0 + 4 * g) = h;
-      *reinterpret_cast<half4 *>(j.An.lo() + col * STEP_NP + i0 + 4 * g) = l;
+      const int o = place(STEP_NP, col, i0 + 4 * g);
+      *reinterpret_cast<half4 *>(j.An.hi + o) = h;
+      *reinterpret_cast<half4 *>(j.An.lo() + o) = l;
     }
   }
 }
@@ -983,12 +1005,53 @@ struct ApplyJob {
   const uint32_t *maxb;
   const double *invd;           // NULL: no divisor
   float decay, step;            // a Muon step: out <- decay * out - step * Y
-  int32_t rows, cols, tall, dtype, otype, e, nb, tc, muon, first;   // tc: tiles along the columns
+  int32_t rows, cols, tall, dtype, otype, e, nb, muon, first;
 };
 struct ApplyArgs {
   ApplyJob job[AGX_MAX_ORTH];
-  int n;
+  int n, per;                   // per: groups of lines a workgroup (orth_panel_kernel)
 };
+
+// a wave's 32 x 32 results of the scaled product, from row r0 and column c0 of Y on
+__device__ __forceinline__ void finish_tile(const ApplyJob &j, f32x16 acc, int e, int r0, int c0) {
+  const int lane = threadIdx.x & 63;
+  // (in 64 bits where the factor leaves fp32's normal range: tiny matrices)
+  const double f = ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e);
+  const float ff = (float)f;
+  if (__builtin_amdgcn_readfirstlane((fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) || f == 0.0)) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] *= ff;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] = (float)((double)acc[k] * f);
+  }
+  // (r0 and c0 are the wave's: scalar row pointers, one offset a lane)
+  const bool inside = r0 + 32 <= j.rows && c0 + 32 <= j.cols;
+  const int64_t at = (int64_t)r0 * j.ldo + c0;
+  const int lr = 4 * (lane >> 5), left = j.rows - r0 - lr, ldo = (int)j.ldo, off = lr * ldo + (lane & 31);
+  const bool column = (lane & 31) < j.cols - c0;
+  auto row = [](int k) { return 8 * (k >> 2) + (k & 3); };
+  auto ok = [&](int k) { return inside || (row(k) < left && column); };
+  if (j.muon) {
+    float *w = reinterpret_cast<float *>(j.out) + at;
+    f32x16 old;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) old[k] = ok(k) ? (w + row(k) * ldo)[off] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (ok(k)) (w + row(k) * ldo)[off] = j.decay * old[k] - j.step * acc[k];
+  } else if (j.otype == AGX_F32) {
+    float *o = reinterpret_cast<float *>(j.out) + at;
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (ok(k)) (o + row(k) * ldo)[off] = acc[k];
+  } else {
+    __bf16 *o = reinterpret_cast<__bf16 *>(j.out) + at;
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (ok(k)) (o + row(k) * ldo)[off] = (__bf16)acc[k];
+  }
+}
 
 template <typename E, bool TALL>
 __device__ __forceinline__ f32x16 apply_tile(const ApplyJob &j, int tr, int tc, int &e, uint32_t *red, _Float16 *lds) {
@@ -1015,8 +1078,8 @@ __global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
   int q = 0;
   while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const ApplyJob &j = a.job[q];
-  const int trs = (j.rows + T - 1) / T, local = id - j.first;
-  const int tr = j.tall ? local / j.tc : local % trs, tc = j.tall ? local % j.tc : local / trs;
+  const int trs = (j.rows + T - 1) / T, tcs = (j.cols + T - 1) / T, local = id - j.first;
+  const int tr = j.tall ? local / tcs : local % trs, tc = j.tall ? local % tcs : local / trs;
   int e;
   f32x16 acc;
   auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
@@ -1024,40 +1087,122 @@ __global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
   else if (is(1)) acc = apply_tile<float, false>(j, tr, tc, e, red, lds);
   else if (is(2)) acc = apply_tile<__bf16, true>(j, tr, tc, e, red, lds);
   else acc = apply_tile<__bf16, false>(j, tr, tc, e, red, lds);
-  // (in 64 bits where the factor leaves fp32's normal range: tiny matrices)
-  const double f = ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e);
-  const float ff = (float)f;
-  const bool wide = !(fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) && f != 0.0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  finish_tile(j, acc, e, tr * T + (wave >> 1) * 32, tc * T + (wave & 1) * 32);
+}
+
+// The same for np <= PANEL_NP.  Its eight waves hold all of Q in registers (32 columns each, over all of k; at np = 128 and 64
+// two and four groups of waves hold it), and the lines of X - rows of a tall matrix, columns of a wide one - go by in groups
+// of 8192 / np through two LDS buffers, converted once, the next group's loads in flight: one workgroup a CU.
+constexpr int PANEL_NP = OPERAND_NP, PANEL_LDS = 2 * 2 * 128 * (64 + 8) * 2;    // (np = 64 has the most padding)
+// a group's loads and LDS writes: 16 elements a thread, raw until they are stored
+template <typename E, bool TALL, int NP> struct PanelLines {
+  static constexpr int GL = 8192 / NP, LD = NP + 8;    // (rows that start in 16 different bank groups)
+  using V = typename Vec4<E>::type;
+  V v[4];
+  // tall: four vectors along k; wide: four k's of four lines
+  static __device__ __forceinline__ int line(int q) { return TALL ? (threadIdx.x + 512 * q) / (NP / 4) : threadIdx.x % (GL / 4) * 4; }
+  static __device__ __forceinline__ int k(int q) { return TALL ? threadIdx.x % (NP / 4) * 4 : threadIdx.x / (GL / 4) * 4 + q; }
+  __device__ __forceinline__ void fetch(const ApplyJob &j, int l0) {
+    const int lines = TALL ? j.rows : j.cols, n = TALL ? j.cols : j.rows, ld = (int)j.ldx;
+    const E *b = reinterpret_cast<const E *>(j.x) + (TALL ? (int64_t)l0 * j.ldx : (int64_t)l0);
+    if (l0 + GL <= lines && n == NP) {
 #pragma unroll
-  for (int k = 0; k < 16; ++k) acc[k] = wide ? (float)((double)acc[k] * f) : acc[k] * ff;
-  const bool inside = (tr + 1) * T <= j.rows && (tc + 1) * T <= j.cols;
-  const int64_t at = (int64_t)tr * T * j.ldo + (int64_t)tc * T;
-  const int left = j.rows - tr * T, right = j.cols - tc * T, ldo = (int)j.ldo;
-  auto ok = [&](int r, int c) { return inside || (r < left && c < right); };
-  if (j.muon) {
-    float *w = reinterpret_cast<float *>(j.out) + at;
-    f32x16 old;
-    int n = 0;
-    each_element(acc, [&](int r, int c, float) {
-      old[n] = ok(r, c) ? w[r * ldo + c] : 0.f;
-      ++n;
-    });
-    n = 0;
-    each_element(acc, [&](int r, int c, float y) {
-      if (ok(r, c)) w[r * ldo + c] = j.decay * old[n] - j.step * y;
-      ++n;
-    });
-  } else if (j.otype == AGX_F32) {
-    float *o = reinterpret_cast<float *>(j.out) + at;
-    each_element(acc, [&](int r, int c, float y) {
-      if (ok(r, c)) o[r * ldo + c] = y;
-    });
-  } else {
-    __bf16 *o = reinterpret_cast<__bf16 *>(j.out) + at;
-    each_element(acc, [&](int r, int c, float y) {
-      if (ok(r, c)) o[r * ldo + c] = (__bf16)y;
-    });
+      for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const V *>(b + (TALL ? line(q) * ld + k(q) : k(q) * ld + line(q)));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int l = line(q) + (TALL ? 0 : i), kk = k(q) + (TALL ? i : 0);
+          v[q][i] = l0 + l < lines && kk < n ? b[TALL ? l * ld + kk : kk * ld + l] : (E)0.f;
+        }
+    }
   }
+  __device__ __forceinline__ void store(_Float16 *hi, _Float16 *lo, int e) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      half4 h, l;
+      if (TALL) split4(scale4(f32x4{(float)v[q][0], (float)v[q][1], (float)v[q][2], (float)v[q][3]}, e), h, l);
+      else split4(scale4(f32x4{(float)v[0][q], (float)v[1][q], (float)v[2][q], (float)v[3][q]}, e), h, l);
+      const int o = TALL ? line(q) * LD + k(q) : (line(0) + q) * LD + k(0);
+      *reinterpret_cast<half4 *>(hi + o) = h;
+      if (sizeof(E) == 4) *reinterpret_cast<half4 *>(lo + o) = l;
+    }
+  }
+};
+template <typename E, bool TALL, int NP>
+__device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int g1, uint32_t *red, _Float16 *lds) {
+  typedef PanelLines<E, TALL, NP> X;
+  constexpr int CG = NP / 32, NB = NP / 32, PLANE = X::GL * X::LD;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cg = wave % CG, rg = wave / CG;
+  X x;
+  x.fetch(j, g0 * X::GL);
+  // (k runs in an order of its own, the same for both operands: a lane's two vectors of a block are neighbours in memory)
+  half8 qh[NB][2], ql[NB][2];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int o = place(NP, cg * 32 + (lane & 31), b * 32 + (lane >> 5) * 16 + i * 8);
+      qh[b][i] = *reinterpret_cast<const half8 *>(j.Q.hi + o);
+      ql[b][i] = *reinterpret_cast<const half8 *>(j.Q.lo() + o);
+    }
+  const int e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e;
+  x.store(lds, lds + PLANE, e);
+  for (int g = g0, buf = 0; g < g1; ++g, buf ^= 1) {   // (one barrier a group: a buffer is written a group after it was read)
+    if (g + 1 < g1) x.fetch(j, (g + 1) * X::GL);
+    __syncthreads();
+    const _Float16 *xl = lds + buf * 2 * PLANE + (rg * 32 + (lane & 31)) * X::LD + (lane >> 5) * 16;
+    auto at = [&](int o) { return *reinterpret_cast<const half8 *>(xl + o); };
+    f32x16 acc = {};
+#pragma unroll
+    for (int s = 0; s < NB; s += 2) {                  // (steps of 64 k, as in tile_product)
+      f32x16 sum = {};
+      auto mul = [&](half8 xv, half8 qv) {
+        sum = TALL ? __builtin_amdgcn_mfma_f32_32x32x16_f16(xv, qv, sum, 0, 0, 0)
+                   : __builtin_amdgcn_mfma_f32_32x32x16_f16(qv, xv, sum, 0, 0, 0);
+      };
+#pragma unroll
+      for (int b = s; b < s + 2; ++b) {
+        const half8 x0 = at(b * 32), x1 = at(b * 32 + 8);
+        mul(x0, ql[b][0]);
+        mul(x1, ql[b][1]);
+        if (sizeof(E) == 4) {
+          mul(at(PLANE + b * 32), qh[b][0]);
+          mul(at(PLANE + b * 32 + 8), qh[b][1]);
+        }
+        mul(x0, qh[b][0]);
+        mul(x1, qh[b][1]);
+      }
+      acc += sum;
+      asm volatile("" : "+v"(acc));                    // (put off to the epilogue, the sums would not fit the registers)
+    }
+    const int l = g * X::GL + rg * 32;
+    if (l < (TALL ? j.rows : j.cols) && cg * 32 < (TALL ? j.cols : j.rows)) finish_tile(j, acc, e, TALL ? l : cg * 32, TALL ? cg * 32 : l);
+    if (g + 1 < g1) x.store(lds + (buf ^ 1) * 2 * PLANE, lds + (buf ^ 1) * 2 * PLANE + PLANE, e);
+  }
+}
+template <typename E, bool TALL>
+__device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int per, uint32_t *red, _Float16 *lds) {
+  const int lines = TALL ? j.rows : j.cols, g1 = min(g0 + per, (lines + 8192 / j.Q.np - 1) / (8192 / j.Q.np));
+  if (j.Q.np == 64) panel_lines<E, TALL, 64>(j, g0, g1, red, lds);
+  else if (j.Q.np == 128) panel_lines<E, TALL, 128>(j, g0, g1, red, lds);
+  else panel_lines<E, TALL, 256>(j, g0, g1, red, lds);
+}
+template <int KIND>
+__global__ __launch_bounds__(512, 2) void orth_panel_kernel(ApplyArgs a) {
+  extern __shared__ _Float16 lds[];
+  __shared__ uint32_t red[8];
+  int q = 0;
+  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
+  const ApplyJob &j = a.job[q];
+  const int g0 = ((int)blockIdx.x - j.first) * a.per;
+  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
+  if (is(0)) panel_lines<float, true>(j, g0, a.per, red, lds);
+  else if (is(1)) panel_lines<float, false>(j, g0, a.per, red, lds);
+  else if (is(2)) panel_lines<__bf16, true>(j, g0, a.per, red, lds);
+  else panel_lines<__bf16, false>(j, g0, a.per, red, lds);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1123,7 +1268,12 @@ void plan(const Job &j, int total_tiles, int phases, bool need_u, Layout &l) {
   l.u = need_u ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.end = off;
 }
-int phases_of(int steps) { return agx::cdiv(steps, PHASE); }
+// steps between two Gram matrices
+int phase_of(const Job *jobs, int n) {
+  for (int i = 0; i < n; ++i)
+    if (jobs[i].np() <= PANEL_NP) return 2;
+  return PHASE;
+}
 
 int64_t ws_bytes(const Job *jobs, int n, int steps, bool need_u) {
   int tiles = 0;
@@ -1131,7 +1281,7 @@ int64_t ws_bytes(const Job *jobs, int n, int steps, bool need_u) {
   int64_t total = 0;
   for (int i = 0; i < n; ++i) {
     Layout l;
-    plan(jobs[i], tiles, phases_of(steps), need_u, l);
+    plan(jobs[i], tiles, agx::cdiv(steps, phase_of(jobs, n)), need_u, l);
     total += l.end;
   }
   return total;
@@ -1203,7 +1353,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     wide += (jobs[i].rows < jobs[i].cols) - (jobs[i].rows > jobs[i].cols);
   }
   for (int i = 0; i < n; ++i) jobs[i].square_wide = wide > 0;
-  const int phases = phases_of(o->steps);
+  const int phase = phase_of(jobs, n), phases = agx::cdiv(o->steps, phase);
   Layout lay[AGX_MAX_ORTH];
   char *base[AGX_MAX_ORTH];
   int nb[AGX_MAX_ORTH];
@@ -1298,7 +1448,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       AGX_LAUNCH_CHECK();
     }
     // matrices: 0 A, 1 P, 2 A P, 3 / 4 Q (which of the two: 3 after an odd number of steps); a launch a step: 0 / 1 A
-    const int steps = std::min(PHASE, o->steps - k);
+    const int steps = std::min(phase, o->steps - k);
     PhaseArgs pa;
     memset(&pa, 0, sizeof(pa));
     float coef[3 * PHASE];
@@ -1405,34 +1555,44 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
           g.C = planes(i, 0, eA[t + 1]);
         }));
     }
-    ApplyArgs aa;
-    aa.n = n;
-    int blocks = 0, kind = -1;
-    for (int i = 0; i < n; ++i) {
-      const Job &j = jobs[i];
-      ApplyJob &g = aa.job[i];
-      memset(&g, 0, sizeof(g));
-      g.x = x[i]; g.ldx = ldx[i]; g.Q = planes(i, iq, eQ[steps - 1]);
-      g.maxb = reinterpret_cast<const uint32_t *>(base[i] + lay[i].maxb);
-      g.invd = first ? reinterpret_cast<const double *>(base[i] + lay[i].invd) : nullptr;
-      g.rows = j.rows; g.cols = j.cols; g.tall = j.tall();
-      g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
-      if (last) {
-        g.out = j.out; g.ldo = j.ldo; g.otype = j.dtype; g.muon = j.muon; g.decay = j.decay; g.step = j.step;
-      } else {
-        g.out = base[i] + lay[i].x[ph & 1]; g.ldo = j.cols; g.otype = AGX_F32;
-        x[i] = g.out;
-        ldx[i] = g.ldo;
+    auto apply = [&](bool panel) -> int {
+      ApplyArgs aa;
+      aa.n = 0;
+      int blocks = 0, kind = -1, groups = 0;
+      auto groups_of = [](const Job &j) { return (int)agx::cdiv64(j.K(), 8192 / j.np()); };
+      for (int i = 0; i < n; ++i) groups += panel && jobs[i].np() <= PANEL_NP ? groups_of(jobs[i]) : 0;
+      aa.per = agx::cdiv(groups, agx::num_cus());
+      for (int i = 0; i < n; ++i) {
+        const Job &j = jobs[i];
+        if ((j.np() <= PANEL_NP) != panel) continue;
+        ApplyJob &g = aa.job[aa.n++];
+        memset(&g, 0, sizeof(g));
+        g.x = x[i]; g.ldx = ldx[i]; g.Q = planes(i, iq, eQ[steps - 1]);
+        g.maxb = reinterpret_cast<const uint32_t *>(base[i] + lay[i].maxb);
+        g.invd = first ? reinterpret_cast<const double *>(base[i] + lay[i].invd) : nullptr;
+        g.rows = j.rows; g.cols = j.cols; g.tall = j.tall();
+        g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
+        if (last) {
+          g.out = j.out; g.ldo = j.ldo; g.otype = j.dtype; g.muon = j.muon; g.decay = j.decay; g.step = j.step;
+        } else {
+          g.out = base[i] + lay[i].x[ph & 1]; g.ldo = j.cols; g.otype = AGX_F32;
+          x[i] = g.out;
+          ldx[i] = g.ldo;
+        }
+        kind = joined_kind(kind, g.tall, g.dtype);
+        g.first = blocks;
+        blocks += panel ? agx::cdiv(groups_of(j), aa.per) : agx::cdiv(j.rows, T) * agx::cdiv(j.cols, T);
       }
-      kind = joined_kind(kind, g.tall, g.dtype);
-      g.tc = agx::cdiv(j.cols, T);
-      g.first = blocks;
-      blocks += agx::cdiv(j.rows, T) * g.tc;
-    }
-    by_kind(kind, [&](auto k) {
-      hipLaunchKernelGGL(orth_apply_kernel<decltype(k)::value>, dim3(blocks), dim3(256), 0, st, aa);
-    });
-    AGX_LAUNCH_CHECK();
+      if (!blocks) return AGX_OK;
+      by_kind(kind, [&](auto k) {
+        if (panel) hipLaunchKernelGGL(orth_panel_kernel<decltype(k)::value>, dim3(blocks), dim3(512), PANEL_LDS, st, aa);
+        else hipLaunchKernelGGL(orth_apply_kernel<decltype(k)::value>, dim3(blocks), dim3(256), 0, st, aa);
+      });
+      AGX_LAUNCH_CHECK();
+      return AGX_OK;
+    };
+    AGX_TRY(apply(true));
+    AGX_TRY(apply(false));
   }
   return AGX_OK;
 }
@@ -1480,6 +1640,11 @@ int agx::orth_prepare_device() {
                               phase_lds(ONE_BLOCK)));
   AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_chain_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                               CHAIN_LDS));
+  for (int k = 0; k <= ANY; ++k) {
+    const void *f = nullptr;
+    by_kind(k, [&](auto kind) { f = reinterpret_cast<const void *>(&orth_panel_kernel<decltype(kind)::value>); });
+    AGX_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, PANEL_LDS));
+  }
   return AGX_OK;
 }
 
