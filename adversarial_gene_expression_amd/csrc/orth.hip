@@ -1012,45 +1012,52 @@ struct ApplyArgs {
   int n, per;                   // per: groups of lines a workgroup (orth_panel_kernel)
 };
 
-// a wave's 32 x 32 results of the scaled product, from row r0 and column c0 of Y on
-__device__ __forceinline__ void finish_tile(const ApplyJob &j, f32x16 acc, int e, int r0, int c0) {
-  const int lane = threadIdx.x & 63;
-  // (in 64 bits where the factor leaves fp32's normal range: tiny matrices)
-  const double f = ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e);
-  const float ff = (float)f;
-  if (__builtin_amdgcn_readfirstlane((fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) || f == 0.0)) {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) acc[k] *= ff;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) acc[k] = (float)((double)acc[k] * f);
+// from the scaled product to Y (in 64 bits where the factor leaves fp32's normal range: tiny matrices)
+struct Factor {
+  double f;
+  float ff;
+  bool plain;
+  __device__ __forceinline__ Factor(const ApplyJob &j, int e) : f(ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e)), ff((float)f) {
+    plain = __builtin_amdgcn_readfirstlane((fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) || f == 0.0);
   }
-  // (r0 and c0 are the wave's: scalar row pointers, one offset a lane)
-  const bool inside = r0 + 32 <= j.rows && c0 + 32 <= j.cols;
-  const int64_t at = (int64_t)r0 * j.ldo + c0;
-  const int lr = 4 * (lane >> 5), left = j.rows - r0 - lr, ldo = (int)j.ldo, off = lr * ldo + (lane & 31);
+};
+// a wave's 32 x 32 results of it, from row r0 and column c0 of Y on (scalar row pointers, one offset a lane)
+template <typename O, bool MUON, bool INSIDE>
+__device__ __forceinline__ void write_tile(O *o, const ApplyJob &j, const f32x16 &acc, int r0, int c0) {
+  const int lane = threadIdx.x & 63, lr = 4 * (lane >> 5), left = j.rows - r0 - lr, ldo = (int)j.ldo, off = lr * ldo + (lane & 31);
   const bool column = (lane & 31) < j.cols - c0;
+  const float decay = j.decay, step = j.step;
+  o += (int64_t)r0 * j.ldo + c0;
   auto row = [](int k) { return 8 * (k >> 2) + (k & 3); };
-  auto ok = [&](int k) { return inside || (row(k) < left && column); };
-  if (j.muon) {
-    float *w = reinterpret_cast<float *>(j.out) + at;
-    f32x16 old;
+  auto ok = [&](int k) { return INSIDE || (row(k) < left && column); };
+  f32x16 y = acc;
+  if constexpr (MUON) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) old[k] = ok(k) ? (w + row(k) * ldo)[off] : 0.f;
+    for (int k = 0; k < 16; ++k) y[k] = ok(k) ? (o + row(k) * ldo)[off] : 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (ok(k)) (w + row(k) * ldo)[off] = j.decay * old[k] - j.step * acc[k];
-  } else if (j.otype == AGX_F32) {
-    float *o = reinterpret_cast<float *>(j.out) + at;
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (ok(k)) (o + row(k) * ldo)[off] = acc[k];
-  } else {
-    __bf16 *o = reinterpret_cast<__bf16 *>(j.out) + at;
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (ok(k)) (o + row(k) * ldo)[off] = (__bf16)acc[k];
+    for (int k = 0; k < 16; ++k) y[k] = decay * y[k] - step * acc[k];
   }
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (ok(k)) (o + row(k) * ldo)[off] = (O)y[k];
+}
+template <bool INSIDE>
+__device__ __forceinline__ void write_tile(const ApplyJob &j, const f32x16 &acc, int r0, int c0) {
+  if (j.muon) write_tile<float, true, INSIDE>(reinterpret_cast<float *>(j.out), j, acc, r0, c0);
+  else if (j.otype == AGX_F32) write_tile<float, false, INSIDE>(reinterpret_cast<float *>(j.out), j, acc, r0, c0);
+  else write_tile<__bf16, false, INSIDE>(reinterpret_cast<__bf16 *>(j.out), j, acc, r0, c0);
+}
+__device__ __forceinline__ void finish_tile(const ApplyJob &j, const Factor &f, f32x16 acc, int r0, int c0) {
+  if (f.plain) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] *= f.ff;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] = (float)((double)acc[k] * f.f);
+  }
+  // (tiles inside the matrix, nearly all, without a condition per element: each would wait for what is in flight)
+  if (r0 + 32 <= j.rows && c0 + 32 <= j.cols) write_tile<true>(j, acc, r0, c0);
+  else write_tile<false>(j, acc, r0, c0);
 }
 
 template <typename E, bool TALL>
@@ -1088,7 +1095,7 @@ __global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
   else if (is(2)) acc = apply_tile<__bf16, true>(j, tr, tc, e, red, lds);
   else acc = apply_tile<__bf16, false>(j, tr, tc, e, red, lds);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  finish_tile(j, acc, e, tr * T + (wave >> 1) * 32, tc * T + (wave & 1) * 32);
+  finish_tile(j, Factor(j, e), acc, tr * T + (wave >> 1) * 32, tc * T + (wave & 1) * 32);
 }
 
 // The same for np <= PANEL_NP.  Its eight waves hold all of Q in registers (32 columns each, over all of k; at np = 128 and 64
@@ -1150,6 +1157,7 @@ __device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int g1, u
     }
   const int e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e;
   x.store(lds, lds + PLANE, e);
+  const Factor f(j, e);
   for (int g = g0, buf = 0; g < g1; ++g, buf ^= 1) {   // (one barrier a group: a buffer is written a group after it was read)
     if (g + 1 < g1) x.fetch(j, (g + 1) * X::GL);
     __syncthreads();
@@ -1179,7 +1187,7 @@ __device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int g1, u
       asm volatile("" : "+v"(acc));                    // (put off to the epilogue, the sums would not fit the registers)
     }
     const int l = g * X::GL + rg * 32;
-    if (l < (TALL ? j.rows : j.cols) && cg * 32 < (TALL ? j.cols : j.rows)) finish_tile(j, acc, e, TALL ? l : cg * 32, TALL ? cg * 32 : l);
+    if (l < (TALL ? j.rows : j.cols) && cg * 32 < (TALL ? j.cols : j.rows)) finish_tile(j, f, acc, TALL ? l : cg * 32, TALL ? cg * 32 : l);
     if (g + 1 < g1) x.store(lds + (buf ^ 1) * 2 * PLANE, lds + (buf ^ 1) * 2 * PLANE + PLANE, e);
   }
 }
