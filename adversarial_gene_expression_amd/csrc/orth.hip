@@ -37,7 +37,7 @@ typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 constexpr int T = 64;                          // n x n matrices are padded to T, 2 T, 4 T or a multiple of T above
 constexpr int PHASE = 3;                       // most steps between two Gram matrices
 constexpr int MAXB = 1024;                     // partial maxima of one matrix
-constexpr int ONE_BLOCK = 128;                 // largest padded side for a phase in one workgroup (LDS)
+constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
 constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram product
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
@@ -699,299 +699,242 @@ __global__ __launch_bounds__(256) void orth_chain_small_kernel(ChainArgs a) {
   store_planes4(j.C.hi, j.C.lo(), np, r, c, ti == tj, out);
 }
 
-// All products of a phase for np <= 128, one workgroup a matrix.  A wave owns one tile of 32 x 32 of every product (10 at
-// np = 128).  Two matrices fit the LDS: A and P; S = A P and the next A are written over A, and the product Q of the steps
-// is kept in its owners' registers and put where A was while it is multiplied.  The products are turns of ONE loop over the
-// same few kilobytes of code.  Bound by instruction issue of the one CU: 3 waves a SIMD, each of which turns 16 results a
-// lane into planes.
-struct PhaseStage {
-  int32_t what;                 // P: P = a I + b A + c A^2; S: A <- A P; A: A' = A P, held; Q: Q <- A P; W: no product
-  int32_t out;                  // what is written over A behind it (P: over P): the result, the held A', Q
-  int32_t first;                // P: it is Q too
-  float alpha, beta, gamma;     // of the scaled values: result = alpha (L R) + beta A + gamma I
-};
-enum { ST_P, ST_S, ST_A, ST_Q, ST_W };
-enum { OUT_RESULT, OUT_HELD, OUT_Q };
-struct PhaseJob {
-  Planes A, Q;
-  int32_t n;
-};
-struct PhaseArgs {
-  PhaseJob job[AGX_MAX_ORTH];
-  PhaseStage stage[4 * PHASE + 1];
-  int stages;
-};
-constexpr int PW = 10;          // waves of a phase's workgroup: the tiles of np = 128
-constexpr int phase_lds(int np) { return 4 * np * (np + 8) * 2 + np / 32 * 32 * 33 * 4; }
-
-template <int NP>
-__device__ __forceinline__ void phase_steps(const PhaseArgs &a, const PhaseJob &j, _Float16 *A) {
-  constexpr int nt = NP / 32, tri = nt * (nt + 1) / 2, LD = NP + 8, PL = NP * LD;   // (16 rows start in 16 bank groups)
-  _Float16 *P = A + 2 * PL;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = (lane >> 5) * 8;
-  auto lds_place = [](int i) {
-    int row, k;
-    placed(NP, i / 8, row, k);
-    return row * LD + k;
-  };
-  for (int i = threadIdx.x * 8; i < NP * NP; i += PW * 64 * 8) {
-    const int o = lds_place(i);
-    *reinterpret_cast<half8 *>(&A[o]) = *reinterpret_cast<const half8 *>(j.A.hi + i);
-    *reinterpret_cast<half8 *>(&A[PL + o]) = *reinterpret_cast<const half8 *>(j.A.lo() + i);
-  }
-  __syncthreads();
-  int ti = 0, tj = 0;
-  if (wave < tri) upper_tile(wave, nt, ti, tj);
-  const bool diag = ti == tj;
-  float *scratch = reinterpret_cast<float *>(A + 4 * PL) + ti * 32 * 33;
-  const int c = tj * 32 + (lane & 31), r0 = ti * 32 + 4 * (lane >> 5);
-  auto at = [](const _Float16 *p) { return *reinterpret_cast<const half8 *>(p); };
-  float Q[16], held[16];
-#pragma unroll 1
-  for (int st = 0; st < a.stages; ++st) {
-    const PhaseStage g = a.stage[st];
-    float v[16];
-    if (wave < tri && g.what != ST_W) {
-      const _Float16 *l = A + (ti * 32 + (lane & 31)) * LD + h, *r = (g.what == ST_P ? A : P) + c * LD + h;
-      f32x16 acc = {};
-      // (the split's small terms are added first, so that only one product in three rounds at the sum's magnitude)
-#pragma unroll
-      for (int k = 0; k < NP; k += 64) {
-        half8 x[4], y[4];
-        f32x16 s = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = at(l + k + i * 16);
-          y[i] = at(r + k + i * 16);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(l + PL + k + i * 16), y[i], s, 0, 0, 0);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], at(r + PL + k + i * 16), s, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], y[i], s, 0, 0, 0);
-        acc += s;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = g.alpha * acc[i];
-      if (g.what == ST_P) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {                  // (A is symmetric: its mirror image is one vector)
-          const half4 eh = *reinterpret_cast<const half4 *>(&A[c * LD + r0 + 8 * q]), el = *reinterpret_cast<const half4 *>(&A[PL + c * LD + r0 + 8 * q]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[4 * q + i] += fmaf(g.beta, (float)eh[i] + (float)el[i], r0 + 8 * q + i == c && c < j.n ? g.gamma : 0.f);
-        }
-      }
-      if (diag) {                                      // below the diagonal: what is above it (the wave's own 4 KB)
-        const int lr = r0 & 31, lc = lane & 31;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) scratch[(lr + 8 * (i >> 2) + (i & 3)) * 33 + lc] = v[i];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int row = lr + 8 * (i >> 2) + (i & 3);
-          const float m = scratch[lc * 33 + row];
-          v[i] = row > lc ? m : v[i];
-        }
-      }
-      if (g.first || g.what == ST_Q)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) Q[i] = v[i];
-      if (g.what == ST_A)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) held[i] = v[i];
-    }
-    if (g.out == OUT_Q) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = Q[i];
-    } else if (g.out == OUT_HELD) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = held[i];
-    }
-    __syncthreads();
-    if (wave < tri) {
-      _Float16 *o = g.what == ST_P ? P : A;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 w = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-        store_planes4(o, o + PL, LD, r0 + 8 * q, c, diag, w);
-      }
-    }
-    __syncthreads();
-  }
-  const _Float16 *f = a.stages == 1 ? P : A;           // (one step: P is the product)
-  for (int i = threadIdx.x * 8; i < NP * NP; i += PW * 64 * 8) {
-    const int o = lds_place(i);
-    *reinterpret_cast<half8 *>(j.Q.hi + i) = *reinterpret_cast<const half8 *>(&f[o]);
-    *reinterpret_cast<half8 *>(j.Q.lo() + i) = *reinterpret_cast<const half8 *>(&f[PL + o]);
-  }
-}
-__global__ __launch_bounds__(PW * 64) void orth_phase_kernel(PhaseArgs a) {
-  extern __shared__ _Float16 lds[];
-  const PhaseJob &j = a.job[blockIdx.x];
-  if (j.A.np == T) phase_steps<T>(a, j, lds);
-  else phase_steps<2 * T>(a, j, lds);
-}
-static_assert(ONE_BLOCK == 2 * T, "one-workgroup phases are written for one or two tiles a side");
-
-// One step in one launch for np = 256.  Rows of a polynomial of A need A alone: r.A, (r.A).A, ... with r a row of A or Q, so
-// that a workgroup takes 16 rows of A (or of Q) through the whole step by itself,
-//   S = a r + b r A + c r A^2,  next A = a S + b S A + c S A^2  (four products; Q: the first two),
-// with A in its waves' registers (32 columns a wave: 128 registers of 512 threads hold all 256 KB of it) and the running
-// rows in LDS.  More flops than the symmetric products (6 n^3 a step against 1.5 to 2), but one launch of 11 us where three
-// of 6 us stood.
-constexpr int STEP_NP = 256, STEP_ROWS = 16, STEP_LD = STEP_NP + 8;   // (16 rows start in 16 different bank groups)
-struct StepJob {
+// np <= OPERAND_NP: rows of a polynomial of A need A alone - r A, (r A) A, ... - so that a workgroup takes 16 rows through
+// many products by itself, with A in its waves' registers (256 KB of them at np = 256, 32 columns a wave) and the running
+// rows in LDS.  More flops than the symmetric products of whole matrices (6 n^3 a step against 1.5 to 2), but few launches.
+//   np = 256, a launch a step: S = a r + b r A + c r A^2, next A = a S + b S A + c S A^2 (four products, r rows of A) and
+//     Q = a r + b r A + c r A^2 (two, r rows of the Q before; the first step's Q is S without its A)
+//   np <= 128, a launch a phase of up to two steps: u = rows of P_0, then u P_1 with u A_1 = ((u A) P_0) P_0 (twelve products).
+//     (Errors of the first of those are multiplied by the later ones: the split's lo.lo products are taken too.  Three
+//     products: 23 x 61 off by 1.8e-6, four 1.0e-6, the plain fp32 iteration 0.8e-6.)
+constexpr int STEP_NP = 256, ROWS = 16;
+static_assert(STEP_NP == OPERAND_NP && ROWS_PHASE == 128, "the three sides that orth_rows_kernel is made for");
+enum { E_U, E_UA, E_UAA, E_W, E_WA, E_Y, E_YA, E_YAA, E_W2, E_WA2, E_COUNT };   // scales of the rows in a phase's panel
+struct RowsJob {
   Planes A, An, Q, Qn;
   int32_t n, first;
 };
-struct StepArgs {
-  StepJob job[AGX_MAX_ORTH];
+struct RowsArgs {
+  RowsJob job[AGX_MAX_ORTH];
   int n;
   int32_t more, has_q;          // a further step follows (A is wanted); Q exists (otherwise the step's own polynomial is Q)
   float a, b, c;
   int32_t e1, eS, e3, q1;       // scale exponents of the running rows: r A, S, S A; of Q's r A
+  int32_t steps;                // of a phase
+  float a2, b2, c2;             // its second step
+  int32_t e[E_COUNT];
 };
 
-__global__ __launch_bounds__(512, 2) void orth_step_kernel(StepArgs a) {
-  __shared__ _Float16 panel[2][2][STEP_ROWS * STEP_LD];                // [buffer][plane]
-  int q = 0;
-  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
-  const StepJob &j = a.job[q];
-  constexpr int PANELS = STEP_NP / STEP_ROWS;
-  const int local = blockIdx.x - j.first, i0 = local % PANELS * STEP_ROWS;
-  const bool rows_of_q = local >= PANELS;
-  if (rows_of_q ? !a.has_q : a.has_q && !a.more) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, cl = lane & 15;
-  // the rows themselves, and A's columns (= rows: it is symmetric) wave * 32 ..; k runs in an order of its own, the same for
-  // both operands: a lane's vectors of two steps are neighbours in memory
-  const Planes &R = rows_of_q ? j.Q : j.A;
-  int pr, pc;                                          // this thread's eight values of them
-  placed(STEP_NP, threadIdx.x, pr, pc);
-  const int mine = i0 * STEP_NP + threadIdx.x * 8;
-  const half8 rh = *reinterpret_cast<const half8 *>(R.hi + mine), rl = *reinterpret_cast<const half8 *>(R.lo() + mine);
-  half8 bh[2][8], bl[2][8];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int o = (wave * 2 + t) * 16 * STEP_NP + k * 512 + lane * 8;
-      bh[t][k] = *reinterpret_cast<const half8 *>(j.A.hi + o);
-      bl[t][k] = *reinterpret_cast<const half8 *>(j.A.lo() + o);
+template <int NP> struct RowsOf {
+  static constexpr int LD = NP + 8, CT = NP == 256 ? 2 : 1, KB = NP / 32, BUF = 2 * ROWS * LD;   // (16 rows start in 16 bank groups)
+  static constexpr bool FOUR = NP <= ROWS_PHASE;
+  typedef f32x4 Result[CT];     // a lane's results: rows 4 g .. of columns col(t)
+  half8 bh[CT][KB], bl[CT][KB];
+  _Float16 *panel;              // two of [plane][row][LD]
+  int buf, ea, i0, pr, pc;      // pr, pc: the row and the first of the eight k's of this thread's piece of a row block
+  bool works, piece;            // the wave has columns (np = 64: four of eight do); the thread has a piece
+  __device__ __forceinline__ int col(int t) const { return (threadIdx.x >> 6) * 16 * CT + t * 16 + (threadIdx.x & 15); }
+  __device__ __forceinline__ int row(int i) const { return 4 * (threadIdx.x >> 4 & 3) + i; }
+  __device__ __forceinline__ int mine() const { return i0 * NP + threadIdx.x * 8; }
+  // the rows from R, and all of A
+  __device__ __forceinline__ RowsOf(const Planes &R, const Planes &A, int first_row, _Float16 *lds) : panel(lds), buf(0), ea(A.e), i0(first_row) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    works = wave * 16 * CT < NP;
+    piece = (int)threadIdx.x < 2 * NP;
+    placed(NP, threadIdx.x, pr, pc);
+    half8 rh, rl;
+    if (piece) {
+      rh = *reinterpret_cast<const half8 *>(R.hi + mine());
+      rl = *reinterpret_cast<const half8 *>(R.lo() + mine());
     }
-  *reinterpret_cast<half8 *>(&panel[0][0][pr * STEP_LD + pc]) = rh;
-  *reinterpret_cast<half8 *>(&panel[0][1][pr * STEP_LD + pc]) = rl;
-  __syncthreads();
-  int buf = 0;
-  typedef f32x4 Rows[2];        // a lane's results: rows 4 g .. of columns wave * 32 + 16 t + cl
-  auto multiply = [&](int e, Rows &out) {              // out = (rows in the panel, of scale e) . A
-    const _Float16 *ph = panel[buf][0] + cl * STEP_LD + g * 16, *pl = panel[buf][1] + cl * STEP_LD + g * 16;
-    f32x4 acc[2] = {};
+    // (k runs in an order of its own, the same for both operands: a wave's vectors are what place() keeps together)
+    if (works)
 #pragma unroll
-    for (int k = 0; k < 8; k += 4) {
-      f32x4 sum[2] = {};
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+          const int o = (wave * CT + t) * 16 * NP + k * 512 + lane * 8;
+          bh[t][k] = *reinterpret_cast<const half8 *>(A.hi + o);
+          bl[t][k] = *reinterpret_cast<const half8 *>(A.lo() + o);
+        }
+    if (piece) {
+      *reinterpret_cast<half8 *>(&panel[pr * LD + pc]) = rh;
+      *reinterpret_cast<half8 *>(&panel[ROWS * LD + pr * LD + pc]) = rl;
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ _Float16 *plane(int lo) const { return panel + buf * BUF + lo * ROWS * LD; }
+  __device__ __forceinline__ void values(int e, Result &out) const {    // the rows in the panel, of scale e
+    if (!works) return;
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int o = row(i) * LD + col(t);
+        out[t][i] = __builtin_ldexpf((float)plane(0)[o] + (float)plane(1)[o], -e);
+      }
+  }
+  __device__ __forceinline__ void multiply(int e, Result &out) const {  // out = (rows in the panel, of scale e) . A
+    if (!works) return;
+    const int at = (threadIdx.x & 15) * LD + (threadIdx.x >> 4 & 3) * 16;
+    const _Float16 *ph = plane(0) + at, *pl = plane(1) + at;
+    f32x4 acc[CT] = {};
+#pragma unroll
+    for (int k = 0; k < KB; k += KB < 4 ? KB : 4) {
+      f32x4 sum[CT] = {};
       half8 x[4];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
+      for (int h = 0; h < (KB < 4 ? KB : 4); ++h) {
         const int o = (k + h >> 1) * 64 + (h & 1) * 8;
         x[h] = *reinterpret_cast<const half8 *>(ph + o);
         const half8 y = *reinterpret_cast<const half8 *>(pl + o);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < CT; ++t) {
+          if (FOUR) sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, bl[t][k + h], sum[t], 0, 0, 0);
           sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, bh[t][k + h], sum[t], 0, 0, 0);
           sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], bl[t][k + h], sum[t], 0, 0, 0);
         }
       }
 #pragma unroll
-      for (int h = 0; h < 4; ++h)
+      for (int h = 0; h < (KB < 4 ? KB : 4); ++h)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], bh[t][k + h], sum[t], 0, 0, 0);
+        for (int t = 0; t < CT; ++t) sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], bh[t][k + h], sum[t], 0, 0, 0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) acc[t] += sum[t];
+      for (int t = 0; t < CT; ++t) acc[t] += sum[t];
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) out[t] = scale4(acc[t], -e - j.A.e);
-  };
-  auto put = [&](const Rows &r, int e) {               // rows into the other panel, which is then the current one
+    for (int t = 0; t < CT; ++t) out[t] = scale4(acc[t], -e - ea);
+  }
+  __device__ __forceinline__ void put(const Result &r, int e) {         // rows into the other panel, which is then the current one
     buf ^= 1;
+    if (works)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      half4 h, l;
-      split4(scale4(r[t], e), h, l);
-      store_pairs4(panel[buf][0], STEP_LD, 4 * g, wave * 32 + t * 16 + cl, h);
-      store_pairs4(panel[buf][1], STEP_LD, 4 * g, wave * 32 + t * 16 + cl, l);
-    }
-    __syncthreads();
-  };
-  auto write_rows = [&](const Planes &m) {             // the current panel
-    *reinterpret_cast<half8 *>(m.hi + mine) = *reinterpret_cast<const half8 *>(&panel[buf][0][pr * STEP_LD + pc]);
-    *reinterpret_cast<half8 *>(m.lo() + mine) = *reinterpret_cast<const half8 *>(&panel[buf][1][pr * STEP_LD + pc]);
-  };
-  Rows r, x1, x2, s;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int o = (4 * g + i) * STEP_LD + wave * 32 + t * 16 + cl;
-      r[t][i] = __builtin_ldexpf((float)panel[0][0][o] + (float)panel[0][1][o], -R.e);
-    }
-  multiply(R.e, x1);
-  if (!rows_of_q && !a.has_q) {                        // Q = a I + b A + c A^2
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = i0 + 4 * g + i, col = wave * 32 + t * 16 + cl;
-        s[t][i] = a.c * x1[t][i] + (a.b * r[t][i] + (row == col && row < j.n ? a.a : 0.f));
+      for (int t = 0; t < CT; ++t) {
+        half4 h, l;
+        split4(scale4(r[t], e), h, l);
+        store_pairs4(plane(0), LD, row(0), col(t), h);
+        store_pairs4(plane(1), LD, row(0), col(t), l);
       }
-    put(s, j.Qn.e);
-    write_rows(j.Qn);
+    __syncthreads();
+  }
+  __device__ __forceinline__ void write(const Planes &m) const {        // the current panel
+    if (!piece) return;
+    *reinterpret_cast<half8 *>(m.hi + mine()) = *reinterpret_cast<const half8 *>(plane(0) + pr * LD + pc);
+    *reinterpret_cast<half8 *>(m.lo() + mine()) = *reinterpret_cast<const half8 *>(plane(1) + pr * LD + pc);
+  }
+  // out = a v + b v1 + c v2, a on the diagonal where v is the identity's rows
+  template <class V>
+  __device__ __forceinline__ void combine(float a, V v, float b, const Result &v1, float c, const Result &v2, Result &out) const {
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[t][i] = fmaf(a, v(t, i), fmaf(b, v1[t][i], c * v2[t][i]));
+  }
+  __device__ __forceinline__ void combine(float a, const Result &v, float b, const Result &v1, float c, const Result &v2, Result &out) const {
+    combine(a, [&](int t, int i) { return v[t][i]; }, b, v1, c, v2, out);
+  }
+  // rows of P_0: a I + b r + c r A, r = rows of A in the panel
+  __device__ __forceinline__ void polynomial(const RowsArgs &p, int n, const Result &r, const Result &x1, Result &out) const {
+    combine(p.a, [&](int t, int i) { return i0 + row(i) == col(t) && col(t) < n ? 1.f : 0.f; }, p.b, r, p.c, x1, out);
+  }
+};
+
+// one step of np = 256; local: 16 workgroups for rows of A (where they or the first Q are wanted), then 16 for rows of Q
+__device__ __forceinline__ void rows_step(const RowsArgs &a, const RowsJob &j, int local, _Float16 *lds) {
+  typedef RowsOf<STEP_NP> R;
+  const bool rows_of_q = local >= STEP_NP / ROWS;
+  if (rows_of_q ? !a.has_q : a.has_q && !a.more) return;
+  const Planes &from = rows_of_q ? j.Q : j.A;
+  R x(from, j.A, local % (STEP_NP / ROWS) * ROWS, lds);
+  R::Result r, x1, x2, s;
+  x.values(from.e, r);
+  x.multiply(from.e, x1);
+  if (!rows_of_q && !a.has_q) {
+    x.polynomial(a, j.n, r, x1, s);
+    x.put(s, j.Qn.e);
+    x.write(j.Qn);
     if (!a.more) return;
   }
-  put(x1, rows_of_q ? a.q1 : a.e1);
-  multiply(rows_of_q ? a.q1 : a.e1, x2);
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[t][i] = a.a * r[t][i] + (a.b * x1[t][i] + a.c * x2[t][i]);
+  const int e1 = rows_of_q ? a.q1 : a.e1;
+  x.put(x1, e1);
+  x.multiply(e1, x2);
+  x.combine(a.a, r, a.b, x1, a.c, x2, s);
   if (rows_of_q) {
-    put(s, j.Qn.e);
-    write_rows(j.Qn);
+    x.put(s, j.Qn.e);
+    x.write(j.Qn);
     return;
   }
-  put(s, a.eS);
-  multiply(a.eS, x1);
-  put(x1, a.e3);
-  multiply(a.e3, x2);
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[t][i] = a.a * s[t][i] + (a.b * x1[t][i] + a.c * x2[t][i]);
-  put(s, j.An.e);
+  x.put(s, a.eS);
+  x.multiply(a.eS, x1);
+  x.put(x1, a.e3);
+  x.multiply(a.e3, x2);
+  x.combine(a.a, s, a.b, x1, a.c, x2, s);
+  x.put(s, j.An.e);
   // the rows from the diagonal on, and their mirror image behind it
-  const int from = pc - i0;
-  if (from >= STEP_ROWS) {
-    write_rows(j.An);
-  } else if (from >= 0) {                              // (the square on the diagonal: symmetric from what is above it)
+  const int from_diagonal = x.pc - x.i0;
+  if (from_diagonal >= ROWS) {
+    x.write(j.An);
+  } else if (from_diagonal >= 0) {                     // (the square on the diagonal: symmetric from what is above it)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int c = from + k, y = min(pr, c), x = max(pr, c);
-      j.An.hi[mine + k] = panel[buf][0][y * STEP_LD + i0 + x];
-      j.An.lo()[mine + k] = panel[buf][1][y * STEP_LD + i0 + x];
+      const int c = from_diagonal + k, o = min(x.pr, c) * R::LD + x.i0 + max(x.pr, c);
+      j.An.hi[x.mine() + k] = x.plane(0)[o];
+      j.An.lo()[x.mine() + k] = x.plane(1)[o];
     }
   }
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int col = wave * 32 + t * 16 + cl;
-    if (col >= i0 + STEP_ROWS) {
+  for (int t = 0; t < R::CT; ++t) {
+    if (x.col(t) >= x.i0 + ROWS) {
       half4 h, l;
       split4(scale4(s[t], j.An.e), h, l);
-      const int o = place(STEP_NP, col, i0 + 4 * g);
+      const int o = place(STEP_NP, x.col(t), x.i0 + x.row(0));
       *reinterpret_cast<half4 *>(j.An.hi + o) = h;
       *reinterpret_cast<half4 *>(j.An.lo() + o) = l;
     }
   }
+}
+// a phase of np <= 128, one workgroup for 16 rows of its Q
+template <int NP>
+__device__ __forceinline__ void rows_phase(const RowsArgs &a, const RowsJob &j, int local, _Float16 *lds) {
+  typedef RowsOf<NP> R;
+  R x(j.A, j.A, local * ROWS, lds);
+  typename R::Result u, v, v1, v2, y1;
+  x.values(j.A.e, v);
+  x.multiply(j.A.e, v1);
+  x.polynomial(a, j.n, v, v1, u);
+  if (a.steps > 1) {
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {                      // u A_1, (u A_1) A_1
+      const int32_t *e = a.e + 5 * k;
+      if (k == 0) x.put(u, e[0]);
+      else x.put(y1, e[0]);
+      x.multiply(e[0], v);
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {                    // . P_0, twice
+        x.put(v, e[1 + 2 * i]);
+        x.multiply(e[1 + 2 * i], v1);
+        x.put(v1, e[2 + 2 * i]);
+        x.multiply(e[2 + 2 * i], v2);
+        x.combine(a.a, v, a.b, v1, a.c, v2, v);
+      }
+      if (k == 0)
+#pragma unroll
+        for (int t = 0; t < R::CT; ++t) y1[t] = v[t];
+    }
+    x.combine(a.a2, u, a.b2, y1, a.c2, v, u);
+  }
+  x.put(u, j.Qn.e);
+  x.write(j.Qn);
+}
+__global__ __launch_bounds__(512, 2) void orth_rows_kernel(RowsArgs a) {
+  __shared__ __align__(16) _Float16 lds[2 * RowsOf<STEP_NP>::BUF];
+  int q = 0;
+  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
+  const RowsJob &j = a.job[q];
+  const int local = (int)blockIdx.x - j.first;
+  if (j.A.np == STEP_NP) rows_step(a, j, local, lds);
+  else if (j.A.np == ROWS_PHASE) rows_phase<ROWS_PHASE>(a, j, local, lds);
+  else rows_phase<T>(a, j, local, lds);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1408,11 +1351,12 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     p.np = jobs[i].np();
     return p;
   };
-  // matrices of np <= ONE_BLOCK take a launch a phase, of np = STEP_NP a launch a step, the others three a step
-  auto by_products = [&](int i) { return jobs[i].np() > ONE_BLOCK && jobs[i].np() != STEP_NP; };
-  bool small = true, any_steps = false, any_products = false;
+  // matrices of np <= ROWS_PHASE take a launch a phase, of np = STEP_NP a launch a step, the others three a step
+  auto by_products = [&](int i) { return jobs[i].np() > STEP_NP; };
+  bool small = true, any_phases = false, any_steps = false, any_products = false;
   for (int i = 0; i < n; ++i) {
     small = small && jobs[i].np() <= SMALL;
+    any_phases = any_phases || jobs[i].np() <= ROWS_PHASE;
     any_steps = any_steps || jobs[i].np() == STEP_NP;
     any_products = any_products || by_products(i);
   }
@@ -1457,11 +1401,10 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     }
     // matrices: 0 A, 1 P, 2 A P, 3 / 4 Q (which of the two: 3 after an odd number of steps); a launch a step: 0 / 1 A
     const int steps = std::min(phase, o->steps - k);
-    PhaseArgs pa;
-    memset(&pa, 0, sizeof(pa));
     float coef[3 * PHASE];
     int eA[PHASE + 1], eP[PHASE], eS[PHASE], eQ[PHASE];              // scale exponents per step
     int e1[PHASE], e3[PHASE], q1[PHASE];                             // of the running rows of a launch a step
+    int32_t er[E_COUNT] = {};                                        // and of a launch a phase
     double bQ = 1.0;                                                 // |Q| <= bQ
     for (int t = 0; t < steps; ++t) {
       const float *c = o->coef + (o->n_coef == 1 ? 0 : 3 * (k + t));
@@ -1469,6 +1412,12 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       memcpy(coef + 3 * t, c, 3 * sizeof(float));
       const double L = s * s;
       e1[t] = exponent_for(L * L); e3[t] = exponent_for(L * b.S); q1[t] = exponent_for(bQ * L);
+      if (t == 0) {
+        const double N = b.next * b.next;
+        const double bound[E_COUNT] = {b.P, b.P * L, b.P * L * L, b.P * b.S, b.P * b.S * L,
+                                       b.P * N, b.P * N * L, b.P * N * L * L, b.P * N * b.S, b.P * N * b.S * L};
+        for (int i = 0; i < E_COUNT; ++i) er[i] = exponent_for(bound[i]);
+      }
       bQ *= b.P;
       eA[t] = exponent_for(s * s); eP[t] = exponent_for(b.P); eS[t] = exponent_for(b.S); eQ[t] = exponent_for(bQ);
       s = b.next;
@@ -1476,51 +1425,31 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     eA[steps] = exponent_for(s * s);
     k += steps;
     const int iq = steps & 1 ? 3 : 4;
-    for (int t = 0; t < steps; ++t) {
-      const bool more = t + 1 < steps;
-      auto stage = [&](int what, int e, int out) -> PhaseStage & {
-        PhaseStage &g = pa.stage[pa.stages++];
-        g.what = what; g.alpha = std::ldexp(1.f, e); g.out = out;
-        return g;
-      };
-      PhaseStage &p = stage(ST_P, 0, OUT_RESULT);
-      p.alpha = std::ldexp(coef[3 * t + 2], eP[t] - 2 * eA[t]);
-      p.beta = std::ldexp(coef[3 * t + 1], eP[t] - eA[t]);
-      p.gamma = std::ldexp(coef[3 * t], eP[t]);
-      p.first = t == 0;
-      if (more) stage(ST_S, eS[t] - eA[t] - eP[t], OUT_RESULT);
-      if (more) stage(ST_A, eA[t + 1] - eS[t] - eP[t], t > 0 ? OUT_Q : OUT_RESULT);
-      if (t > 0 && !more) stage(ST_W, 0, OUT_Q);
-      if (t > 0) stage(ST_Q, eQ[t] - eQ[t - 1] - eP[t], more ? OUT_HELD : OUT_Q);
-    }
-    int nblock = 0, lds = 0;
-    for (int i = 0; i < n; ++i)
-      if (jobs[i].np() <= ONE_BLOCK) {
-        PhaseJob &g = pa.job[nblock++];
-        g.A = planes(i, 0, 0); g.Q = planes(i, iq, 0); g.n = jobs[i].n();
-        lds = std::max(lds, phase_lds(jobs[i].np()));
-      }
-    if (nblock) {
-      hipLaunchKernelGGL(orth_phase_kernel, dim3(nblock), dim3(PW * 64), lds, st, pa);
-      AGX_LAUNCH_CHECK();
-    }
-    for (int t = 0; t < steps && any_steps; ++t) {
-      StepArgs sa;
-      memset(&sa, 0, sizeof(sa));
-      sa.more = t + 1 < steps; sa.has_q = t > 0;
-      sa.a = coef[3 * t]; sa.b = coef[3 * t + 1]; sa.c = coef[3 * t + 2];
-      sa.e1 = e1[t]; sa.eS = eS[t]; sa.e3 = e3[t]; sa.q1 = q1[t];
+    for (int t = 0; t < (any_steps ? steps : any_phases ? 1 : 0); ++t) {
+      RowsArgs ra;
+      memset(&ra, 0, sizeof(ra));
+      ra.more = t + 1 < steps; ra.has_q = t > 0; ra.steps = steps;
+      ra.a = coef[3 * t]; ra.b = coef[3 * t + 1]; ra.c = coef[3 * t + 2];
+      ra.e1 = e1[t]; ra.eS = eS[t]; ra.e3 = e3[t]; ra.q1 = q1[t];
+      if (steps > 1) { ra.a2 = coef[3]; ra.b2 = coef[4]; ra.c2 = coef[5]; }
+      memcpy(ra.e, er, sizeof(er));
       int blocks = 0;
-      for (int i = 0; i < n; ++i)
-        if (jobs[i].np() == STEP_NP) {
-          StepJob &g = sa.job[sa.n++];
+      for (int i = 0; i < n; ++i) {
+        const int np = jobs[i].np();
+        if (by_products(i) || (np <= ROWS_PHASE && t > 0)) continue;
+        RowsJob &g = ra.job[ra.n++];
+        g.n = jobs[i].n();
+        g.first = blocks;
+        if (np == STEP_NP) {
           g.A = planes(i, t & 1, eA[t]); g.An = planes(i, t & 1 ^ 1, eA[t + 1]);
           g.Q = planes(i, t & 1 ? 3 : 4, eQ[t > 0 ? t - 1 : 0]); g.Qn = planes(i, t & 1 ? 4 : 3, eQ[t]);
-          g.n = jobs[i].n(); g.first = blocks;
-          // (rows of A where they or the first Q are wanted, then rows of Q)
-          blocks += STEP_NP / STEP_ROWS * 2;
+          blocks += STEP_NP / ROWS * 2;
+        } else {
+          g.A = planes(i, 0, eA[0]); g.Qn = planes(i, iq, eQ[steps - 1]);
+          blocks += np / ROWS;
         }
-      hipLaunchKernelGGL(orth_step_kernel, dim3(blocks), dim3(512), 0, st, sa);
+      }
+      hipLaunchKernelGGL(orth_rows_kernel, dim3(blocks), dim3(512), 0, st, ra);
       AGX_LAUNCH_CHECK();
     }
     for (int t = 0; t < steps && any_products; ++t) {
@@ -1644,8 +1573,6 @@ int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, co
 
 // (more LDS than the default limit of a launch)
 int agx::orth_prepare_device() {
-  AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_phase_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              phase_lds(ONE_BLOCK)));
   AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_chain_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                               CHAIN_LDS));
   for (int k = 0; k <= ANY; ++k) {
