@@ -18,9 +18,10 @@ def device():
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 
 
-def stream():
+def stream(device=None):
+    """Handle of the current stream of the current device (given its index, without asking for it)."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(torch.cuda.current_device() if device is None else device)
     return torch.cuda.current_stream().cuda_stream
 
 

@@ -83,16 +83,18 @@ def _matrix(t, name, like=None):
     """Row stride of a [rows, cols] operand of the normalisation / update operators; raises on what they do not take."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError('%s must be a 2-D tensor' % name)
-    if t.dtype not in _DTYPES:
-        raise ValueError('%s must be float32 or bfloat16, got %s' % (name, t.dtype))
-    rows, cols = t.shape
+    dtype, shape = t.dtype, t.shape
+    if dtype not in _DTYPES:
+        raise ValueError('%s must be float32 or bfloat16, got %s' % (name, dtype))
+    rows, cols = shape
     if cols == 0:
         raise ValueError('%s has no columns' % name)
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (shape != like.shape or dtype is not like.dtype or t.device != like.device):
         raise ValueError('%s must match the first operand: got %s %s on %s, expected %s %s on %s'
-                         % (name, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype, like.device))
-    ld = t.stride(0) if rows > 1 else cols
-    if (cols > 1 and t.stride(1) != 1) or ld < cols:
+                         % (name, tuple(shape), dtype, t.device, tuple(like.shape), like.dtype, like.device))
+    step, each = t.stride()
+    ld = step if rows > 1 else cols
+    if (each != 1 and cols > 1) or ld < cols:
         raise ValueError('%s must have contiguous rows that do not overlap (strides %s)' % (name, t.stride()))
     return ld
 
@@ -109,19 +111,25 @@ def _vector(t, name, n, like):
 
 
 def _on_current(t):
-    """Kernels run on the current device and stream: refuse operands that live elsewhere."""
-    if not t.is_cuda or not _lib.is_initialised(t.get_device()) or t.get_device() != torch.cuda.current_device():
+    """The current stream.  Kernels run on the current device: refuse operands that live elsewhere."""
+    i = t.get_device()
+    if i < 0 or i != torch.cuda.current_device() or not _lib.is_initialised(i):
         if t.device != _dev.device():
             raise ValueError('operands are on %s, the current device is cuda:%d' % (t.device, torch.cuda.current_device()))
+    return _dev.stream(i)
 
 
 def _rows_like(x):
-    """Uninitialised [rows, width] result, rows 16-byte aligned as the package lays matrices out."""
+    """Uninitialised [rows, width] result, rows 16-byte aligned as the package lays matrices out, and its row stride."""
     rows, width = x.shape
-    q = 16 // x.element_size()
-    ld = (width + q - 1) // q * q
+    q = 3 if x.dtype is torch.float32 else 7
+    ld = (width + q) & ~q
     out = x.new_empty((rows, ld))
-    return out if ld == width else out[:, :width]
+    return (out if ld == width else out[:, :width]), ld
+
+
+def _f32(n, x):
+    return torch.empty(n, dtype=torch.float32, device=x.device)
 
 
 def _norm_desc(x, act, slope):
@@ -146,13 +154,12 @@ def layer_norm(x, gamma=None, beta=None, *, eps=1e-3, act=0, slope=0.0, out=None
     d.gamma, d.beta = _vector(gamma, 'gamma', x.shape[1], x), _vector(beta, 'beta', x.shape[1], x)
     if out is not None:
         d.ldy = _matrix(out, 'out', x)
-    _on_current(x)
+    stream = _on_current(x)
     if out is None:
-        out = _rows_like(x)
-        d.ldy = max(out.stride(0), out.shape[1])
-    mean, rstd = torch.empty((2, x.shape[0]), dtype=torch.float32, device=x.device).unbind(0)
+        out, d.ldy = _rows_like(x)
+    mean, rstd = _f32(d.rows, x), _f32(d.rows, x)
     d.y, d.mean, d.rstd, d.eps = out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), eps
-    _lib.check(_lib.load().agx_layernorm_fwd(_dev.stream(), d), 'agx_layernorm_fwd')
+    _lib.check(_lib.load().agx_layernorm_fwd(stream, d), 'agx_layernorm_fwd')
     return out, mean, rstd
 
 
@@ -166,12 +173,12 @@ def _norm_back(d, dy, x, mean, rstd, gamma, y, act):
         if y is None:
             raise ValueError('act=1 needs y, the forward result: the derivative is taken from its sign')
         d.ldy, d.y = _matrix(y, 'y', x), y.data_ptr()
-    _on_current(x)
+    return _on_current(x)
 
 
 def _norm_ws(d, x, lib):
-    n = int(lib.agx_layernorm_ws_floats(d.rows, d.width, d.dtype))
-    ws = torch.empty(max(n, 1), dtype=torch.float32, device=x.device)
+    n = lib.agx_layernorm_ws_floats(d.rows, d.width, d.dtype)
+    ws = _f32(n, x)
     d.ws, d.ws_floats = ws.data_ptr(), n
     return ws
 
@@ -182,15 +189,15 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, y=None, act=0, slope=0
     forward returned; y: its result, needed with act=1."""
     lib = _lib.load()
     d = _norm_desc(x, act, slope)
-    _norm_back(d, dy, x, mean, rstd, gamma, y, act)
-    dx = _rows_like(x)
-    d.dx, d.lddx = dx.data_ptr(), max(dx.stride(0), dx.shape[1])
+    stream = _norm_back(d, dy, x, mean, rstd, gamma, y, act)
+    dx, d.lddx = _rows_like(x)
+    d.dx = dx.data_ptr()
     ws = dgamma = dbeta = None
     if param_grads:
         ws = _norm_ws(d, x, lib)
-        dgamma, dbeta = torch.empty((2, x.shape[1]), dtype=torch.float32, device=x.device).unbind(0)
+        dgamma, dbeta = _f32(d.width, x), _f32(d.width, x)
         d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
-    _lib.check(lib.agx_layernorm_bwd(_dev.stream(), d), 'agx_layernorm_bwd')
+    _lib.check(lib.agx_layernorm_bwd(stream, d), 'agx_layernorm_bwd')
     return dx, dgamma, dbeta
 
 
@@ -200,16 +207,15 @@ def layer_norm_backward2(u, dy, x, mean, rstd, gamma=None, *, y=None, act=0, slo
     lib = _lib.load()
     d = _norm_desc(x, act, slope)
     d.ldu, d.u = _matrix(u, 'u', x), u.data_ptr()
-    _norm_back(d, dy, x, mean, rstd, gamma, y, act)
-    dx, ddy = _rows_like(x), _rows_like(x)
-    d.dx, d.lddx = dx.data_ptr(), max(dx.stride(0), dx.shape[1])
-    d.ddy, d.ldddy = ddy.data_ptr(), max(ddy.stride(0), ddy.shape[1])
+    stream = _norm_back(d, dy, x, mean, rstd, gamma, y, act)
+    (dx, d.lddx), (ddy, d.ldddy) = _rows_like(x), _rows_like(x)
+    d.dx, d.ddy = dx.data_ptr(), ddy.data_ptr()
     ws = dgamma = None
     if param_grads:
         ws = _norm_ws(d, x, lib)
-        dgamma = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+        dgamma = _f32(d.width, x)
         d.dgamma = dgamma.data_ptr()
-    _lib.check(lib.agx_layernorm_bwd2(_dev.stream(), d), 'agx_layernorm_bwd2')
+    _lib.check(lib.agx_layernorm_bwd2(stream, d), 'agx_layernorm_bwd2')
     return ddy, dx, dgamma
 
 
@@ -266,9 +272,9 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
         part = xs[lo:lo + _lib.AGX_MAX_ORTH]
         jobs = (_lib.OrthDesc * len(part))()
         for j, t, ld in zip(jobs, part, lds[lo:]):
-            out = _rows_like(t)
+            out, j.ldo = _rows_like(t)
             outs.append(out)
-            j.x, j.out, j.ldx, j.ldo = t.data_ptr(), out.data_ptr(), ld, max(out.stride(0), out.shape[1])
+            j.x, j.out, j.ldx = t.data_ptr(), out.data_ptr(), ld
             j.rows, j.cols, j.dtype = t.shape[0], t.shape[1], _DTYPES[t.dtype]
         n = int(lib.agx_orth_ws_bytes(jobs, len(part), o.steps))
         _lib.check(0 if n >= 0 else n, 'agx_orth_ws_bytes')
