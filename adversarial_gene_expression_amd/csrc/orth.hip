@@ -40,6 +40,7 @@ constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
 constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram product
+constexpr int ONE_SLICE = 8;                   // longest K, in steps of 64, that is not split over workgroups
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
@@ -73,14 +74,15 @@ __device__ __forceinline__ void split4(f32x4 v, half4 &hi, half4 &lo) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// largest |x|; with a momentum step in front where m is given: m <- mu m + g, u = g + mu m (nesterov) or m
+// largest |x| and sum of squares; with a momentum step in front where m is given: m <- mu m + g, u = g + mu m (nesterov) or m
 // ---------------------------------------------------------------------------------------------------------------------
 struct PrepJob {
   const void *x;        // matrix (g with momentum)
   float *m, *u;         // momentum buffer; where u goes (NULL: u is m)
   int64_t ldx, ldm, ldu;
   int32_t rows, cols, dtype, nb;
-  uint32_t *maxb;
+  uint32_t *maxb;       // a workgroup's share of each
+  double *squares;
 };
 struct PrepArgs {
   PrepJob job[AGX_MAX_ORTH];
@@ -123,7 +125,9 @@ __global__ __launch_bounds__(256) void orth_prep_kernel(PrepArgs a) {
   const PrepJob j = a.job[blockIdx.y];
   if ((int)blockIdx.x >= j.nb) return;
   __shared__ uint32_t red[4];
+  __shared__ double sums[4];
   uint32_t mx = 0;
+  double sq = 0.0;
   const uint32_t per_row = (uint32_t)(j.cols + 3) / 4;               // (host: rows * per_row < 2^31)
   const uint32_t items = per_row * (uint32_t)j.rows, step = (uint32_t)j.nb * 256;
 #pragma unroll 4
@@ -143,13 +147,23 @@ __global__ __launch_bounds__(256) void orth_prep_kernel(PrepArgs a) {
       if (j.u) store4(j.u + (int64_t)r * j.ldu + c, n, v);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);   // (as integers: infinities and NaN win)
+    for (int i = 0; i < 4; ++i) {
+      mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);              // (as integers: infinities and NaN win)
+      sq = fma((double)v[i], (double)v[i], sq);                        // (64 bits: no overflow or underflow to look after)
+    }
   }
+  sq = agx::wave_sum(sq);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = mx;
+    sums[threadIdx.x >> 6] = sq;
+  }
   __syncthreads();
-  if (threadIdx.x == 0) j.maxb[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+  if (threadIdx.x == 0) {
+    j.maxb[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+    j.squares[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
 }
 
 // tile (ti <= tj) of linear index t over the upper triangle of nt x nt tiles (nt is small: no square root)
@@ -170,6 +184,20 @@ __device__ __forceinline__ int scale_exponent(const uint32_t *maxb, int nb, uint
   mx = 0;
   for (int i = 0; i < (int)blockDim.x / 64; ++i) mx = max(mx, red[i]);
   return TARGET - exponent_of(mx);
+}
+
+// 1 / (|X|_F + eps) of the matrix scaled by 2^e, the same in every thread and workgroup (sums: a word a wave).  A matrix of
+// zeros gives zeros, one with an infinity or NaN NaN throughout.
+__device__ __forceinline__ double normaliser(const double *squares, int nb, float eps, int e, double *sums) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < nb; i += blockDim.x) s += squares[i];
+  s = agx::wave_sum(s);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) s += sums[i];
+  if (!(s < __builtin_huge_val())) return __builtin_nan("");
+  return s == 0.0 ? 0.0 : 1.0 / ldexp(sqrt(s) + (double)eps, e);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -346,61 +374,26 @@ struct GramJob {
   int32_t n, nt, slices, tall;  // n: small side, nt: tiles along it; tall: element (i, k) at x[k * ld + i]
   int32_t dtype, e, nb;         // e: scale exponent where nb == 0, otherwise from the partial maxima
   const uint32_t *maxb;
-  float *part, *trace;          // trace[ti * slices + slice]: sums of the diagonal of the partial diagonal tiles
+  float *part;
+  const double *squares;        // (one slice) as in ReduceJob
+  double *invd;
+  Planes A;
   int32_t first;                // first workgroup of the job
 };
 struct GramArgs {
   GramJob job[AGX_MAX_ORTH];
   int n;
+  float eps;
 };
 
 template <class L>
-__device__ __forceinline__ f32x16 gram_tile(const GramJob &j, int ti, int tj, int64_t k0, int64_t k1, uint32_t *red, _Float16 *lds) {
+__device__ __forceinline__ f32x16 gram_tile(const GramJob &j, int ti, int tj, int64_t k0, int64_t k1, int &e, uint32_t *red, _Float16 *lds) {
   L la, lb;
   la.p = reinterpret_cast<decltype(la.p)>(j.x);
   la.ld = j.ld; la.rows = j.n; la.kmax = j.K;
   lb.p = la.p; lb.ld = la.ld; lb.rows = la.rows; lb.kmax = la.kmax;
   return tile_product(la, lb, (int64_t)ti * T, (int64_t)tj * T, k0, k1, lds, ti == tj,
-                      [&] { la.e = lb.e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
-}
-
-// KIND: what all of a launch's matrices are (bit 0: wide, bit 1: bf16), or ANY: one loader's registers instead of the
-// largest of four let twice as many workgroups of a CU wait for memory at a time
-constexpr int ANY = 4;
-__device__ __host__ __forceinline__ bool is_kind(int kind, bool tall, int dtype) { return kind == (tall ? 0 : 1) + (dtype == AGX_F32 ? 0 : 2); }
-
-template <int KIND>
-__global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
-  __shared__ __align__(16) _Float16 lds[4 * PL];
-  __shared__ uint32_t red[4];
-  __shared__ float tr[4];
-  // (the tiles of one slice follow each other on one XCD, whose L2 then reads the slice once)
-  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
-  int q = 0;
-  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
-  const GramJob &j = a.job[q];
-  const int tiles = j.nt * (j.nt + 1) / 2, slice = (id - j.first) / tiles, tile = (id - j.first) % tiles;
-  int ti, tj;
-  upper_tile(tile, j.nt, ti, tj);
-  const int64_t k0 = (int64_t)slice * j.kper, k1 = min(k0 + j.kper, (j.K + BK - 1) / BK * BK);
-  f32x16 acc;
-  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
-  if (is(0)) acc = gram_tile<LoadT<float>>(j, ti, tj, k0, k1, red, lds);
-  else if (is(1)) acc = gram_tile<LoadK<float>>(j, ti, tj, k0, k1, red, lds);
-  else if (is(2)) acc = gram_tile<LoadT<__bf16>>(j, ti, tj, k0, k1, red, lds);
-  else acc = gram_tile<LoadK<__bf16>>(j, ti, tj, k0, k1, red, lds);
-  float *p = j.part + ((int64_t)tile * j.slices + slice) * T * T;
-  float d = 0.f;
-  each_element(acc, [&](int r, int c, float v) {
-    p[r * T + c] = v;
-    if (r == c) d += v;
-  });
-  if (ti == tj) {
-    d = agx::wave_sum(d);
-    if ((threadIdx.x & 63) == 0) tr[threadIdx.x >> 6] = d;
-    __syncthreads();
-    if (threadIdx.x == 0) j.trace[ti * j.slices + slice] = tr[0] + tr[1] + tr[2] + tr[3];
-  }
+                      [&] { la.e = lb.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
 }
 
 // Symmetric results are made symmetric to the last bit, from what is on and above the diagonal: products of matrices that are
@@ -418,8 +411,8 @@ __device__ __forceinline__ void store_pairs4(_Float16 *p, int ld, int r, int c, 
   q[0] = (a & 0xffffu) | (b << 16);
   *reinterpret_cast<uint32_t *>(reinterpret_cast<_Float16 *>(q) + ld) = (a >> 16) | (b & 0xffff0000u);
 }
-// The same of a 32 x 32 tile with their mirror image, which is contiguous, into planes of row stride ld (global memory or
-// LDS).  A tile on the diagonal comes symmetric: its mirror image is all of it.
+// The same of a 32 x 32 tile with their mirror image, which is contiguous, into row-major planes.  A tile on the diagonal
+// comes symmetric: its mirror image is all of it.
 __device__ __forceinline__ void store_planes4(_Float16 *hi, _Float16 *lo, int ld, int r, int c, bool diag, f32x4 v) {
   half4 h, l;
   split4(v, h, l);
@@ -430,14 +423,90 @@ __device__ __forceinline__ void store_planes4(_Float16 *hi, _Float16 *lo, int ld
   store_pairs4(lo, ld, r, c, l);
 }
 
-// A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase; the scaled matrix's trace is |X|_F^2) or
-// without a divisor (later phases).  Every workgroup sums the trace itself, in the same order.
+// A lane's results of a 32 x 32 tile on the diagonal (rows lr + 8 (i / 4) + i % 4 of column lc): what is below it from what
+// is above, through 32 * 33 words of the wave's own
+__device__ __forceinline__ void mirror(float *v, float *scratch) {
+  const int lane = threadIdx.x & 63, lr = 4 * (lane >> 5), lc = lane & 31;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) scratch[(lr + 8 * (i >> 2) + (i & 3)) * 33 + lc] = v[i];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = lr + 8 * (i >> 2) + (i & 3);
+    const float m = scratch[lc * 33 + row];
+    v[i] = row > lc ? m : v[i];
+  }
+}
+
+// KIND: what all of a launch's matrices are (bit 0: wide, bit 1: bf16), or ANY: one loader's registers instead of the
+// largest of four let twice as many workgroups of a CU wait for memory at a time
+constexpr int ANY = 4;
+__device__ __host__ __forceinline__ bool is_kind(int kind, bool tall, int dtype) { return kind == (tall ? 0 : 1) + (dtype == AGX_F32 ? 0 : 2); }
+
+// ONE: the job is one slice, and its tiles (of all np x np) go out as A_0 itself, without a launch that adds slices
+template <int KIND, bool ONE>
+__global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
+  __shared__ __align__(16) _Float16 lds[4 * PL];
+  __shared__ uint32_t red[4];
+  // (the tiles of one slice follow each other on one XCD, whose L2 then reads the slice once)
+  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
+  int q = 0;
+  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
+  const GramJob &j = a.job[q];
+  const int tiles = j.nt * (j.nt + 1) / 2, slice = ONE ? 0 : (id - j.first) / tiles, tile = (id - j.first) % tiles;
+  int ti, tj, e;
+  upper_tile(tile, j.nt, ti, tj);
+  const int64_t k0 = (int64_t)slice * j.kper, k1 = min(k0 + j.kper, (j.K + BK - 1) / BK * BK);
+  f32x16 acc;
+  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
+  if (is(0)) acc = gram_tile<LoadT<float>>(j, ti, tj, k0, k1, e, red, lds);
+  else if (is(1)) acc = gram_tile<LoadK<float>>(j, ti, tj, k0, k1, e, red, lds);
+  else if (is(2)) acc = gram_tile<LoadT<__bf16>>(j, ti, tj, k0, k1, e, red, lds);
+  else acc = gram_tile<LoadK<__bf16>>(j, ti, tj, k0, k1, e, red, lds);
+  if constexpr (!ONE) {
+    float *p = j.part + ((int64_t)tile * j.slices + slice) * T * T;
+    each_element(acc, [&](int r, int c, float v) { p[r * T + c] = v; });
+  } else {
+    __shared__ double sums[4];
+    double f = ldexp(1.0, j.A.e - 2 * e);
+    if (j.nb) {
+      const double inv = normaliser(j.squares, j.nb, a.eps, e, sums);
+      f = ldexp(inv * inv, j.A.e);
+      if (tile == 0 && threadIdx.x == 0) *j.invd = inv;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fi = 2 * ti + (wave >> 1), fj = 2 * tj + (wave & 1);
+    if (fi > fj) return;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = (float)((double)acc[i] * f);
+    if (fi == fj) mirror(v, reinterpret_cast<float *>(lds) + wave * 32 * 33);
+    const int r = fi * 32 + 4 * (lane >> 5), c = fj * 32 + (lane & 31), np = j.A.np;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      half4 h, l;
+      split4(f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]}, h, l);
+      const int o = place(np, c, r + 8 * p);
+      *reinterpret_cast<half4 *>(j.A.hi + o) = h;
+      *reinterpret_cast<half4 *>(j.A.lo() + o) = l;
+      if (fi != fj) {
+        const int m = place(np, r + 8 * p, c & ~1), next_row = np > OPERAND_NP ? np : 8;
+        store_pairs4(j.A.hi + m, next_row, 0, 0, h);
+        store_pairs4(j.A.lo() + m, next_row, 0, 0, l);
+      }
+    }
+  }
+}
+
+// A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase) or without a divisor (later phases).
 // A workgroup takes R rows of a square of 32 x 32 on or above the diagonal: interleaved shares of the slices meet in LDS, from
 // where the piece and its mirror image go out as vectors.  R = 32 (4 shares) where the slices are few, 4 (8 shares) where
 // they are many: 18161 x 256 with 71 slices 5.0 us instead of 8.0, 1000 x 4297 with 7 slices 10 us instead of 17.
 struct ReduceJob {
-  const float *part, *trace;
+  const float *part;
   const uint32_t *maxb;
+  const double *squares;
   double *invd;                 // 1 / d of the scaled matrix, for the product with the long side (phase 0)
   Planes A;
   int32_t nt, slices, e, nb, normalise, first;         // nt: partial tiles along a side
@@ -473,15 +542,7 @@ __global__ __launch_bounds__(reduce_threads<R>()) void orth_reduce_kernel(Reduce
   double f;
   if (j.normalise) {
     const int e = scale_exponent(j.maxb, j.nb, red);
-    double s = 0.0;
-    for (int i = threadIdx.x; i < j.nt * j.slices; i += NT) s += (double)j.trace[i];
-    s = agx::wave_sum(s);
-    if ((threadIdx.x & 63) == 0) tr[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = 0.0;
-    for (int i = 0; i < NT / 64; ++i) s += tr[i];
-    const double d = sqrt(s) + ldexp((double)a.eps, e);
-    const double inv = s == 0.0 ? 0.0 : 1.0 / d;                    // (a matrix of zeros gives zeros)
+    const double inv = normaliser(j.squares, j.nb, a.eps, e, tr);
     f = ldexp(inv * inv, j.A.e);
     if ((int)blockIdx.x == j.first && threadIdx.x == 0) *j.invd = inv;
   } else {
@@ -613,21 +674,7 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
   }
   __syncthreads();
   if (fi > fj) return;
-  if (diag) {                                          // below the diagonal: what is above it, through the wave's own 4 KB
-    float *scratch = reinterpret_cast<float *>(lds) + wave * 32 * 33;
-    const int lr = 4 * (lane >> 5), lc = lane & 31;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) scratch[(lr + 8 * (i >> 2) + (i & 3)) * 33 + lc] = v[i];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = lr + 8 * (i >> 2) + (i & 3);
-      const float m = scratch[lc * 33 + row];
-      v[i] = row > lc ? m : v[i];
-    }
-  }
+  if (diag) mirror(v, reinterpret_cast<float *>(lds) + wave * 32 * 33);
 #pragma unroll
   for (int p = 0; p < 4; ++p)
     store_planes4(j.C.hi, j.C.lo(), np, r0 + 8 * p, c, diag, f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]});
@@ -1179,7 +1226,7 @@ struct Job {          // one matrix of a call
 };
 
 struct Layout {       // workspace of one job, in bytes from its start
-  int64_t maxb, invd, mat[5], part, trace, x[2], u, end;
+  int64_t maxb, squares, invd, mat[5], part, x[2], u, end;
   int slices;
   int64_t kper;
 };
@@ -1200,21 +1247,27 @@ template <class F> void by_kind(int kind, F f) {
   }
 }
 
+int64_t longest(const Job *jobs, int n) {               // steps of the longest of a call's Gram products
+  int64_t k = 0;
+  for (int i = 0; i < n; ++i) k = std::max(k, agx::cdiv64(jobs[i].K(), BK));
+  return k;
+}
 // slices of a Gram product: about GRAM_BLOCKS workgroups a CU over all of the call's matrices (each writes, and the next
 // launch reads, a whole tile)
-void plan(const Job &j, int total_tiles, int phases, bool need_u, Layout &l) {
+// (most_steps: longest())
+void plan(const Job &j, int total_tiles, int64_t most_steps, int phases, bool need_u, Layout &l) {
   const int tiles = j.tiles();
   const int64_t ksteps = agx::cdiv64(j.K(), BK);
   const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() * GRAM_BLOCKS / std::max(1, total_tiles));
-  l.kper = std::max<int64_t>(std::min<int64_t>(ksteps, 2), agx::cdiv64(ksteps, want)) * BK;   // (two steps at least)
+  l.kper = std::max<int64_t>(std::min<int64_t>(ksteps, most_steps <= ONE_SLICE ? ONE_SLICE : 2), agx::cdiv64(ksteps, want)) * BK;
   l.slices = (int)agx::cdiv64(j.K(), l.kper);
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = up256(off + bytes); return o; };
   l.maxb = take(MAXB * 4);
+  l.squares = take(MAXB * 8);
   l.invd = take(8);
   for (int64_t &m : l.mat) m = take((int64_t)j.np() * j.np() * 4);
   l.part = take((int64_t)tiles * l.slices * T * T * 4);
-  l.trace = take((int64_t)j.nt() * l.slices * 4);
   for (int k = 0; k < 2; ++k) l.x[k] = phases > 1 + k ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.u = need_u ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.end = off;
@@ -1232,7 +1285,7 @@ int64_t ws_bytes(const Job *jobs, int n, int steps, bool need_u) {
   int64_t total = 0;
   for (int i = 0; i < n; ++i) {
     Layout l;
-    plan(jobs[i], tiles, agx::cdiv(steps, phase_of(jobs, n)), need_u, l);
+    plan(jobs[i], tiles, longest(jobs, n), agx::cdiv(steps, phase_of(jobs, n)), need_u, l);
     total += l.end;
   }
   return total;
@@ -1316,7 +1369,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     int gx = 1;
     for (int i = 0; i < n; ++i) {
       Job &j = jobs[i];
-      plan(j, tiles, phases, need_u && j.muon, lay[i]);
+      plan(j, tiles, longest(jobs, n), phases, need_u && j.muon, lay[i]);
       base[i] = ws;
       ws += lay[i].end;
       nb[i] = (int)std::min<int64_t>(MAXB, agx::cdiv64((int64_t)j.rows * agx::cdiv(j.cols, 4), 512));
@@ -1324,6 +1377,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       PrepJob &p = pa.job[i];
       p.x = j.x; p.ldx = j.ldx; p.rows = j.rows; p.cols = j.cols; p.dtype = j.dtype; p.nb = nb[i];
       p.maxb = reinterpret_cast<uint32_t *>(base[i] + lay[i].maxb);
+      p.squares = reinterpret_cast<double *>(base[i] + lay[i].squares);
       if (j.muon) {
         p.m = j.m;
         p.ldm = j.ldm;
@@ -1368,34 +1422,39 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       GramArgs ga;
       ReduceArgs ra;
       ga.n = ra.n = n;
-      ra.eps = o->eps;
+      ga.eps = ra.eps = o->eps;
       int gb = 0, rb = 0, kind = -1, most = 0;
       for (int i = 0; i < n; ++i) most = std::max(most, lay[i].slices);
+      const bool one = most == 1;                       // nothing to add
       const int pieces = most > FEW_SLICES ? 8 : 1;     // of a square of 32 x 32
       for (int i = 0; i < n; ++i) {
         const Job &j = jobs[i];
         const Layout &l = lay[i];
-        const int nt = j.nt();
+        const int nt = one ? j.np() / T : j.nt();
         GramJob &g = ga.job[i];
         g.x = x[i]; g.ld = ldx[i]; g.K = j.K(); g.kper = l.kper; g.n = j.n(); g.nt = nt; g.slices = l.slices; g.tall = j.tall();
         g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
         g.maxb = reinterpret_cast<const uint32_t *>(base[i] + l.maxb);
         g.part = reinterpret_cast<float *>(base[i] + l.part);
-        g.trace = reinterpret_cast<float *>(base[i] + l.trace);
+        g.squares = reinterpret_cast<const double *>(base[i] + l.squares);
+        g.invd = reinterpret_cast<double *>(base[i] + l.invd);
+        g.A = planes(i, 0, exponent_for(s * s));
         g.first = gb;
-        gb += j.tiles() * l.slices;
+        gb += nt * (nt + 1) / 2 * l.slices;
         kind = joined_kind(kind, g.tall, g.dtype);
         ReduceJob &r = ra.job[i];
-        r.part = g.part; r.trace = g.trace; r.maxb = g.maxb; r.invd = reinterpret_cast<double *>(base[i] + l.invd);
-        r.A = planes(i, 0, exponent_for(s * s)); r.nt = nt; r.slices = l.slices; r.e = ex; r.nb = nb[i];
+        r.part = g.part; r.squares = g.squares; r.maxb = g.maxb; r.invd = g.invd;
+        r.A = g.A; r.nt = nt; r.slices = l.slices; r.e = ex; r.nb = nb[i];
         r.normalise = first; r.first = rb;
         rb += j.np() / 32 * (j.np() / 32 + 1) / 2 * pieces;
       }
       by_kind(kind, [&](auto k) {
-        hipLaunchKernelGGL(orth_gram_kernel<decltype(k)::value>, dim3(gb), dim3(256), 0, st, ga);
+        if (one) hipLaunchKernelGGL((orth_gram_kernel<decltype(k)::value, true>), dim3(gb), dim3(256), 0, st, ga);
+        else hipLaunchKernelGGL((orth_gram_kernel<decltype(k)::value, false>), dim3(gb), dim3(256), 0, st, ga);
       });
       AGX_LAUNCH_CHECK();
-      if (pieces == 8) hipLaunchKernelGGL(orth_reduce_kernel<4>, dim3(rb), dim3(reduce_threads<4>()), 0, st, ra);
+      if (one) {}
+      else if (pieces == 8) hipLaunchKernelGGL(orth_reduce_kernel<4>, dim3(rb), dim3(reduce_threads<4>()), 0, st, ra);
       else hipLaunchKernelGGL(orth_reduce_kernel<32>, dim3(rb), dim3(reduce_threads<32>()), 0, st, ra);
       AGX_LAUNCH_CHECK();
     }
