@@ -40,7 +40,7 @@ constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
 constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
 constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram product
-constexpr int ONE_SLICE = 8;                   // longest K, in steps of 64, that is not split over workgroups
+constexpr int ONE_SLICE = 4;                   // longest K, in steps of 64 (1.5 us each), that is not split over workgroups
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
@@ -1252,7 +1252,8 @@ int64_t longest(const Job *jobs, int n) {               // steps of the longest 
   for (int i = 0; i < n; ++i) k = std::max(k, agx::cdiv64(jobs[i].K(), BK));
   return k;
 }
-// slices of a Gram product: about GRAM_BLOCKS workgroups a CU over all of the call's matrices (each writes, and the next
+// slices of a Gram product.  Up to ONE_SLICE steps one, whose launch gives the matrix itself (256 x 256 92 us instead of 97,
+// 100 x 60 57 instead of 64; 7 steps in one slice: 400 x 400 173 us instead of 156).  Beyond: about GRAM_BLOCKS workgroups a CU over all of the call's matrices (each writes, and the next
 // launch reads, a whole tile)
 // (most_steps: longest())
 void plan(const Job &j, int total_tiles, int64_t most_steps, int phases, bool need_u, Layout &l) {
