@@ -219,12 +219,13 @@ struct LoadPlanes {
   const _Float16 *hi, *lo;
   int ld;
   half8 v[4];
+  static __device__ __forceinline__ int tid() { return threadIdx.x & 255; }    // (orth_chain_kernel has two sets of 256)
   __device__ __forceinline__ explicit LoadPlanes(const Planes &m) : hi(m.hi), lo(m.lo()), ld(m.np) {}
   __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
     const _Float16 *bh = hi + r0 * ld + k0, *bl = lo + r0 * ld + k0;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int o = ((threadIdx.x >> 3) + 32 * p) * ld + (threadIdx.x & 7) * 8;
+      const int o = ((tid() >> 3) + 32 * p) * ld + (threadIdx.x & 7) * 8;
       v[2 * p] = *reinterpret_cast<const half8 *>(bh + o);
       v[2 * p + 1] = *reinterpret_cast<const half8 *>(bl + o);
     }
@@ -232,7 +233,7 @@ struct LoadPlanes {
   __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int o = ((threadIdx.x >> 3) + 32 * p) * LDK + (threadIdx.x & 7) * 8;
+      const int o = ((tid() >> 3) + 32 * p) * LDK + (threadIdx.x & 7) * 8;
       *reinterpret_cast<half8 *>(t + o) = v[2 * p];
       *reinterpret_cast<half8 *>(t + PL + o) = v[2 * p + 1];
     }
@@ -604,10 +605,10 @@ struct ChainArgs {
 };
 static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 
-// (tiles of 64 x 64: an n of 1000 has 136 of them, less than a CU's worth each, so that latency counts: four steps' loads are
-//  in flight)
-constexpr int CHAIN_LDS = 2 * 4 * PL * 2;             // two buffers of both operands' planes
-__global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
+// (tiles of 64 x 64: an n of 1000 has 136 of them, less than a CU's worth each, so that latency counts: two sets of four
+//  waves take every other step of 64 k, each with four steps' loads in flight and LDS of its own, and meet at the end)
+constexpr int CHAIN_LDS = 2 * 2 * 4 * PL * 2;         // two sets' two buffers of both operands' planes
+__global__ __launch_bounds__(512, 2) void orth_chain_kernel(ChainArgs a) {
   constexpr int DEPTH = 4, BUF = 4 * PL;
   extern __shared__ _Float16 lds[];
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
@@ -616,7 +617,8 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
   const ChainJob &j = a.job[q];
   int ti, tj;
   upper_tile(id - j.first, j.nt, ti, tj);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, np = j.C.np, n = np / BK;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int set = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), np = j.C.np, n = np / BK;
   LoadPlanes la[DEPTH] = {LoadPlanes(j.L), LoadPlanes(j.L), LoadPlanes(j.L), LoadPlanes(j.L)};
   LoadPlanes lb[DEPTH] = {LoadPlanes(j.R), LoadPlanes(j.R), LoadPlanes(j.R), LoadPlanes(j.R)};
   static_assert(DEPTH == 4, "");
@@ -624,39 +626,56 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
   const int fa = ((wave >> 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8;
   const int fb = ((wave & 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8 + 2 * PL;
   auto at = [](const _Float16 *t) { return *reinterpret_cast<const half8 *>(t); };
+  _Float16 *own = lds + set * 2 * BUF;
+  auto step = [&](int turn) { return 2 * turn + set; };
 #pragma unroll
   for (int u = 0; u < DEPTH; ++u)
-    if (u < n) {
-      la[u].fetch(ti * T, u * BK);
-      lb[u].fetch(tj * T, u * BK);
+    if (step(u) < n) {
+      la[u].fetch(ti * T, step(u) * BK);
+      lb[u].fetch(tj * T, step(u) * BK);
     }
-  for (int s = 0; s < n; s += DEPTH)
+  for (int s = 0; 2 * s < n; s += DEPTH)               // (the barriers are both sets': the same turns for both)
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u)
-      if (s + u < n) {                                 // (one barrier a step: a buffer is written two steps after it was read)
-        _Float16 *t = lds + (u & 1) * BUF;
-        la[u].store(t);
-        lb[u].store(t + 2 * PL);
-        if (s + u + DEPTH < n) {
-          la[u].fetch(ti * T, (s + u + DEPTH) * BK);
-          lb[u].fetch(tj * T, (s + u + DEPTH) * BK);
+      if (2 * (s + u) < n) {                           // (one barrier a turn: a buffer is written two turns after it was read)
+        _Float16 *t = own + (u & 1) * BUF;
+        const bool works = step(s + u) < n;
+        if (works) {
+          la[u].store(t);
+          lb[u].store(t + 2 * PL);
+        }
+        if (step(s + u + DEPTH) < n) {
+          la[u].fetch(ti * T, step(s + u + DEPTH) * BK);
+          lb[u].fetch(tj * T, step(s + u + DEPTH) * BK);
         }
         __syncthreads();
-        f32x16 sum = {};
-        half8 ah[4], bh[4];
+        if (works) {
+          f32x16 sum = {};
+          half8 ah[4], bh[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          ah[k] = at(t + fa + k * 16);
-          bh[k] = at(t + fb + k * 16);
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + PL + fa + k * 16), bh[k], sum, 0, 0, 0);
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], at(t + PL + fb + k * 16), sum, 0, 0, 0);
+          for (int k = 0; k < 4; ++k) {
+            ah[k] = at(t + fa + k * 16);
+            bh[k] = at(t + fb + k * 16);
+            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + PL + fa + k * 16), bh[k], sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], at(t + PL + fb + k * 16), sum, 0, 0, 0);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], bh[k], sum, 0, 0, 0);
+          acc += sum;
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], bh[k], sum, 0, 0, 0);
-        acc += sum;
       }
-  // a wave's 32 x 32 results, as in the other forms
+  __syncthreads();
+  float *meet = reinterpret_cast<float *>(lds) + wave * 16 * 64 + lane;
+  if (set) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) meet[i * 64] = acc[i];
+  }
+  __syncthreads();
   const int fi = ti * 2 + (wave >> 1), fj = tj * 2 + (wave & 1), c = fj * 32 + (lane & 31), r0 = fi * 32 + 4 * (lane >> 5);
+  if (set || fi > fj) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] += meet[i * 64];
+  // a wave's 32 x 32 results, as in the other forms
   const bool diag = fi == fj;
   const float fl = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
   const float fe = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fd = __builtin_ldexpf(j.gamma, j.C.e);
@@ -672,9 +691,7 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
     for (int i = 0; i < 4; ++i)
       v[4 * p + i] = fmaf(fl, acc[4 * p + i], fmaf(fe, (float)eh[i] + (float)el[i], r0 + 8 * p + i == c && c < j.n ? fd : 0.f));
   }
-  __syncthreads();
-  if (fi > fj) return;
-  if (diag) mirror(v, reinterpret_cast<float *>(lds) + wave * 32 * 33);
+  if (diag) mirror(v, reinterpret_cast<float *>(lds) + 4 * 16 * 64 + wave * 32 * 33);
 #pragma unroll
   for (int p = 0; p < 4; ++p)
     store_planes4(j.C.hi, j.C.lo(), np, r0 + 8 * p, c, diag, f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]});
@@ -1527,7 +1544,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
             fill(g, i, w);
           }
         if (small) hipLaunchKernelGGL(orth_chain_small_kernel, dim3(blocks), dim3(256), 0, st, ca);
-        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(256), CHAIN_LDS, st, ca);
+        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(512), CHAIN_LDS, st, ca);
         AGX_LAUNCH_CHECK();
         return AGX_OK;
       };
