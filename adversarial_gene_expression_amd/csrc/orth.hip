@@ -38,24 +38,21 @@ constexpr int T = 64;                          // n x n matrices are padded to T
 constexpr int PHASE = 3;                       // most steps between two Gram matrices
 constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
-constexpr int SMALL = 512;                     // largest padded side for the chain's latency form
 constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram product
 constexpr int ONE_SLICE = 4;                   // longest K, in steps of 64 (1.5 us each), that is not split over workgroups
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
-// n x n matrix as two fp16 planes of np x np (np: n rounded up, zeros behind), value = (hi + lo) 2^-e.  Row-major above
-// OPERAND_NP; up to it in the order of the matrix cores' operands, so that a wave's load of 16 rows and 32 k is one piece of
-// 1 KB: blocks of 16 rows by 64 k, in them (k / 8) % 2, then (k / 16) % 4, the row and k % 8.  (Row-major, each of those
-// loads asks for 16 bytes of 32 lines or more.)
-constexpr int OPERAND_NP = 256;
+// n x n matrix as two fp16 planes of np x np (np: n rounded up, zeros behind), value = (hi + lo) 2^-e, in the order of the
+// matrix cores' operands, so that a wave's load of 16 rows and 32 k is one piece of 1 KB: blocks of 16 rows by 64 k, in them
+// (k / 8) % 2, then (k / 16) % 4, the row and k % 8.  (Row-major, each of those loads asks for 16 bytes of 32 lines or more.)
 struct Planes {
   _Float16 *hi;
   int32_t e, np;
   __device__ __forceinline__ _Float16 *lo() const { return hi + (int64_t)np * np; }
 };
+constexpr int NEXT_ROW = 8;                    // from a place to the same k of the next row, inside a block
 __device__ __forceinline__ int place(int np, int row, int k) {        // (eight k's from a multiple of 8 on are neighbours)
-  if (np > OPERAND_NP) return row * np + k;
   return (((row >> 4) * (np >> 6) + (k >> 6)) * 2 + ((k >> 3) & 1)) * 512 + (((k >> 4) & 3) * 16 + (row & 15)) * 8 + (k & 7);
 }
 __device__ __forceinline__ void placed(int np, int piece, int &row, int &k) {   // of the piece-th eight values in operand order
@@ -217,15 +214,14 @@ __device__ __forceinline__ f32x4 scale4(f32x4 v, int e) {
 struct LoadPlanes {
   static constexpr bool two = true;
   const _Float16 *hi, *lo;
-  int ld;
+  int np;
   half8 v[4];
-  static __device__ __forceinline__ int tid() { return threadIdx.x & 255; }    // (orth_chain_kernel has two sets of 256)
-  __device__ __forceinline__ explicit LoadPlanes(const Planes &m) : hi(m.hi), lo(m.lo()), ld(m.np) {}
+  __device__ __forceinline__ explicit LoadPlanes(const Planes &m) : hi(m.hi), lo(m.lo()), np(m.np) {}
   __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
-    const _Float16 *bh = hi + r0 * ld + k0, *bl = lo + r0 * ld + k0;
+    const _Float16 *bh = hi + r0 * np + k0 * 16, *bl = lo + r0 * np + k0 * 16;      // (block (r0, k0) of 16 x 64)
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int o = ((tid() >> 3) + 32 * p) * ld + (threadIdx.x & 7) * 8;
+      const int o = ((threadIdx.x >> 7) + 2 * p) * 16 * np + (threadIdx.x & 127) * 8;
       v[2 * p] = *reinterpret_cast<const half8 *>(bh + o);
       v[2 * p + 1] = *reinterpret_cast<const half8 *>(bl + o);
     }
@@ -233,7 +229,9 @@ struct LoadPlanes {
   __device__ __forceinline__ void store(_Float16 *t) const {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int o = ((tid() >> 3) + 32 * p) * LDK + (threadIdx.x & 7) * 8;
+      int row, k;
+      placed(BK, threadIdx.x + 256 * p, row, k);
+      const int o = row * LDK + k;
       *reinterpret_cast<half8 *>(t + o) = v[2 * p];
       *reinterpret_cast<half8 *>(t + PL + o) = v[2 * p + 1];
     }
@@ -412,18 +410,18 @@ __device__ __forceinline__ void store_pairs4(_Float16 *p, int ld, int r, int c, 
   q[0] = (a & 0xffffu) | (b << 16);
   *reinterpret_cast<uint32_t *>(reinterpret_cast<_Float16 *>(q) + ld) = (a >> 16) | (b & 0xffff0000u);
 }
-// The same of a 32 x 32 tile with their mirror image, which is contiguous, into row-major planes.  A tile on the diagonal
-// comes symmetric: its mirror image is all of it.
-__device__ __forceinline__ void store_planes4(_Float16 *hi, _Float16 *lo, int ld, int r, int c, bool diag, f32x4 v) {
+// The same of a symmetric matrix, into planes with their mirror image, which is contiguous.  diag: the tile's mirror image is
+// all of it.
+__device__ __forceinline__ void store_planes4(const Planes &m, int r, int c, bool diag, f32x4 v) {
   half4 h, l;
   split4(v, h, l);
-  *reinterpret_cast<half4 *>(&hi[c * ld + r]) = h;
-  *reinterpret_cast<half4 *>(&lo[c * ld + r]) = l;
+  const int o = place(m.np, c, r), x = place(m.np, r, c & ~1);
+  *reinterpret_cast<half4 *>(m.hi + o) = h;
+  *reinterpret_cast<half4 *>(m.lo() + o) = l;
   if (diag) return;                                    // (uniform over the wave)
-  store_pairs4(hi, ld, r, c, h);
-  store_pairs4(lo, ld, r, c, l);
+  store_pairs4(m.hi + x, NEXT_ROW, 0, 0, h);
+  store_pairs4(m.lo() + x, NEXT_ROW, 0, 0, l);
 }
-
 // A lane's results of a 32 x 32 tile on the diagonal (rows lr + 8 (i / 4) + i % 4 of column lc): what is below it from what
 // is above, through 32 * 33 words of the wave's own
 __device__ __forceinline__ void mirror(float *v, float *scratch) {
@@ -483,20 +481,9 @@ __global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = (float)((double)acc[i] * f);
     if (fi == fj) mirror(v, reinterpret_cast<float *>(lds) + wave * 32 * 33);
-    const int r = fi * 32 + 4 * (lane >> 5), c = fj * 32 + (lane & 31), np = j.A.np;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      half4 h, l;
-      split4(f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]}, h, l);
-      const int o = place(np, c, r + 8 * p);
-      *reinterpret_cast<half4 *>(j.A.hi + o) = h;
-      *reinterpret_cast<half4 *>(j.A.lo() + o) = l;
-      if (fi != fj) {
-        const int m = place(np, r + 8 * p, c & ~1), next_row = np > OPERAND_NP ? np : 8;
-        store_pairs4(j.A.hi + m, next_row, 0, 0, h);
-        store_pairs4(j.A.lo() + m, next_row, 0, 0, l);
-      }
-    }
+    for (int p = 0; p < 4; ++p)
+      store_planes4(j.A, fi * 32 + 4 * (lane >> 5) + 8 * p, fj * 32 + (lane & 31), fi == fj, f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]});
   }
 }
 
@@ -605,165 +592,97 @@ struct ChainArgs {
 };
 static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 
-// (tiles of 64 x 64: an n of 1000 has 136 of them, less than a CU's worth each, so that latency counts: two sets of four
-//  waves take every other step of 64 k, each with four steps' loads in flight and LDS of its own, and meet at the end)
-constexpr int CHAIN_LDS = 2 * 2 * 4 * PL * 2;         // two sets' two buffers of both operands' planes
-__global__ __launch_bounds__(512, 2) void orth_chain_kernel(ChainArgs a) {
-  constexpr int DEPTH = 4, BUF = 4 * PL;
-  extern __shared__ _Float16 lds[];
+// A workgroup has a tile of 64 x 32 on or above the diagonal, its four waves every fourth step of 64 k of all of it: operands
+// go straight from L2 to the matrix cores' registers, each byte once a workgroup, without LDS or barriers until the waves'
+// sums meet.  (Tiles through LDS, four or eight waves at a barrier a step: 16.5 us at n = 1024 instead of CHAIN_US.)
+__global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
+  __shared__ float part[4][32][64];                    // [wave][element][lane]
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
   int q = 0;
   while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const ChainJob &j = a.job[q];
-  int ti, tj;
-  upper_tile(id - j.first, j.nt, ti, tj);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-  const int set = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), np = j.C.np, n = np / BK;
-  LoadPlanes la[DEPTH] = {LoadPlanes(j.L), LoadPlanes(j.L), LoadPlanes(j.L), LoadPlanes(j.L)};
-  LoadPlanes lb[DEPTH] = {LoadPlanes(j.R), LoadPlanes(j.R), LoadPlanes(j.R), LoadPlanes(j.R)};
-  static_assert(DEPTH == 4, "");
-  f32x16 acc = {};
-  const int fa = ((wave >> 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8;
-  const int fb = ((wave & 1) * 32 + (lane & 31)) * LDK + (lane >> 5) * 8 + 2 * PL;
-  auto at = [](const _Float16 *t) { return *reinterpret_cast<const half8 *>(t); };
-  _Float16 *own = lds + set * 2 * BUF;
-  auto step = [&](int turn) { return 2 * turn + set; };
+  int ti = 0, tj = id - j.first;                       // row ti of tiles starts at column 2 ti
+  while (tj >= 2 * (j.nt - ti)) tj -= 2 * (j.nt - ti++);
+  tj += 2 * ti;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), np = j.C.np, steps = np / BK;
+  // (k runs in an order of its own, the same for both operands)
+  const int at = (lane & 31) / 16 * 16 * np + (lane >> 5) * 128 + (lane & 15) * 8;
+  const _Float16 *ah = j.L.hi + (int64_t)ti * 64 * np, *al = j.L.lo() + (int64_t)ti * 64 * np;
+  const _Float16 *bh = j.R.hi + (int64_t)tj * 32 * np, *bl = j.R.lo() + (int64_t)tj * 32 * np;
+  half8 x[2][2][2][2], y[2][2][2];                     // [half of a step][rows 32 ..][plane][vector], [half][plane][vector]
+  auto fetch = [&](int s, int h) {
 #pragma unroll
-  for (int u = 0; u < DEPTH; ++u)
-    if (step(u) < n) {
-      la[u].fetch(ti * T, step(u) * BK);
-      lb[u].fetch(tj * T, step(u) * BK);
-    }
-  for (int s = 0; 2 * s < n; s += DEPTH)               // (the barriers are both sets': the same turns for both)
+    for (int i = 0; i < 2; ++i) {
+      const int o = at + s * 1024 + h * 256 + i * 512;
 #pragma unroll
-    for (int u = 0; u < DEPTH; ++u)
-      if (2 * (s + u) < n) {                           // (one barrier a turn: a buffer is written two turns after it was read)
-        _Float16 *t = own + (u & 1) * BUF;
-        const bool works = step(s + u) < n;
-        if (works) {
-          la[u].store(t);
-          lb[u].store(t + 2 * PL);
-        }
-        if (step(s + u + DEPTH) < n) {
-          la[u].fetch(ti * T, step(s + u + DEPTH) * BK);
-          lb[u].fetch(tj * T, step(s + u + DEPTH) * BK);
-        }
-        __syncthreads();
-        if (works) {
-          f32x16 sum = {};
-          half8 ah[4], bh[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            ah[k] = at(t + fa + k * 16);
-            bh[k] = at(t + fb + k * 16);
-            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(at(t + PL + fa + k * 16), bh[k], sum, 0, 0, 0);
-            sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], at(t + PL + fb + k * 16), sum, 0, 0, 0);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k], bh[k], sum, 0, 0, 0);
-          acc += sum;
-        }
+      for (int t = 0; t < 2; ++t) {
+        x[h][t][0][i] = *reinterpret_cast<const half8 *>(ah + t * 32 * np + o);
+        x[h][t][1][i] = *reinterpret_cast<const half8 *>(al + t * 32 * np + o);
       }
-  __syncthreads();
-  float *meet = reinterpret_cast<float *>(lds) + wave * 16 * 64 + lane;
-  if (set) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) meet[i * 64] = acc[i];
+      y[h][0][i] = *reinterpret_cast<const half8 *>(bh + o);
+      y[h][1][i] = *reinterpret_cast<const half8 *>(bl + o);
+    }
+  };
+  f32x16 acc[2] = {};
+  if (wave < steps) {
+    fetch(wave, 0);
+    fetch(wave, 1);
   }
-  __syncthreads();
-  const int fi = ti * 2 + (wave >> 1), fj = tj * 2 + (wave & 1), c = fj * 32 + (lane & 31), r0 = fi * 32 + 4 * (lane >> 5);
-  if (set || fi > fj) return;
+  for (int s = wave; s < steps; s += 4) {
+    f32x16 sum[2] = {};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] += meet[i * 64];
-  // a wave's 32 x 32 results, as in the other forms
-  const bool diag = fi == fj;
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          sum[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][t][1][i], y[h][0][i], sum[t], 0, 0, 0);
+          sum[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][t][0][i], y[h][1][i], sum[t], 0, 0, 0);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sum[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][t][0][i], y[h][0][i], sum[t], 0, 0, 0);
+      if (s + 4 < steps) fetch(s + 4, h);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) acc[t] += sum[t];
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[wave][t * 16 + i][lane] = acc[t][i];
+  __syncthreads();
+  // a wave finishes half of a 32 x 32 tile: accumulator element f is row 8 (f / 4) + 4 (lane / 32) + f % 4
+  const int t = wave >> 1, fi = 2 * ti + t, c = tj * 32 + (lane & 31);
+  if (fi > tj) return;
   const float fl = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
   const float fe = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fd = __builtin_ldexpf(j.gamma, j.C.e);
-  float v[16];
+  auto total = [&](int f, int l) { return (part[0][t * 16 + f][l] + part[1][t * 16 + f][l]) + (part[2][t * 16 + f][l] + part[3][t * 16 + f][l]); };
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
+  for (int p = 0; p < 2; ++p) {
+    const int f0 = 8 * (wave & 1) + 4 * p, r = fi * 32 + 2 * f0 + 4 * (lane >> 5);
     half4 eh = {}, el = {};
     if (j.beta != 0.f) {                               // (E is symmetric: its mirror image is one vector)
-      eh = *reinterpret_cast<const half4 *>(&j.E.hi[c * np + r0 + 8 * p]);
-      el = *reinterpret_cast<const half4 *>(&j.E.lo()[c * np + r0 + 8 * p]);
+      const int o = place(np, c, r);
+      eh = *reinterpret_cast<const half4 *>(j.E.hi + o);
+      el = *reinterpret_cast<const half4 *>(j.E.lo() + o);
     }
+    f32x4 v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[4 * p + i] = fmaf(fl, acc[4 * p + i], fmaf(fe, (float)eh[i] + (float)el[i], r0 + 8 * p + i == c && c < j.n ? fd : 0.f));
+    for (int i = 0; i < 4; ++i) {
+      float sum = total(f0 + i, lane);
+      if (fi == tj && r + i > c) {                     // below the diagonal: what is above it
+        const int cc = lane & 31;
+        sum = total((cc & 3) + 4 * (cc >> 3), (r + i & 31) + 32 * (cc >> 2 & 1));
+      }
+      v[i] = fmaf(fl, sum, fmaf(fe, (float)eh[i] + (float)el[i], r + i == c && c < j.n ? fd : 0.f));
+    }
+    store_planes4(j.C, r, c, fi == tj, v);
   }
-  if (diag) mirror(v, reinterpret_cast<float *>(lds) + 4 * 16 * 64 + wave * 32 * 33);
-#pragma unroll
-  for (int p = 0; p < 4; ++p)
-    store_planes4(j.C.hi, j.C.lo(), np, r0 + 8 * p, c, diag, f32x4{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]});
 }
 
-// The same for small matrices, where a launch is all latency: tiles of 32 x 32 (36 of them at n = 256), k dealt to the four
-// waves in blocks of 32, operands straight from L2 to the matrix cores' registers - every load of a wave's k range is
-// in flight at once up to n = 256 - and the waves' sums met in LDS.
-// (k runs in an order of its own, the same for both operands: a lane's two vectors of a block are neighbours in memory)
-__global__ __launch_bounds__(256) void orth_chain_small_kernel(ChainArgs a) {
-  __shared__ float part[4][16][64];
-  int q = 0;
-  while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
-  const ChainJob &j = a.job[q];
-  const int np = j.C.np, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int ti, tj;
-  upper_tile(blockIdx.x - j.first, np / 32, ti, tj);
-  const int64_t oa = (int64_t)(ti * 32 + (lane & 31)) * np + (lane >> 5) * 16, ob = (int64_t)(tj * 32 + (lane & 31)) * np + (lane >> 5) * 16;
-  const _Float16 *ah = j.L.hi + oa, *al = j.L.lo() + oa, *bh = j.R.hi + ob, *bl = j.R.lo() + ob;
-  auto at = [](const _Float16 *p, int k) { return *reinterpret_cast<const half8 *>(p + k); };
-  const int r = ti * 32 + 8 * wave + 4 * (lane >> 5), c = tj * 32 + (lane & 31);   // the four elements this lane finishes
-  float ev[4] = {};
-  if (j.beta != 0.f)
-  {                                                    // (E is symmetric: its mirror image is one vector)
-    const half4 eh = *reinterpret_cast<const half4 *>(&j.E.hi[c * np + r]), el = *reinterpret_cast<const half4 *>(&j.E.lo()[c * np + r]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ev[i] = (float)eh[i] + (float)el[i];
-  }
-  f32x16 sum = {}, cross = {};
-  for (int k = wave * 32; k < np; k += 256) {          // two blocks of 32 a turn
-    half8 v[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (k + 128 * h < np) {
-        const int o = k + 128 * h;
-        v[h][0] = at(ah, o); v[h][1] = at(ah, o + 8); v[h][2] = at(al, o); v[h][3] = at(al, o + 8);
-        v[h][4] = at(bh, o); v[h][5] = at(bh, o + 8); v[h][6] = at(bl, o); v[h][7] = at(bl, o + 8);
-      }
-    f32x16 s = {};
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (k + 128 * h < np) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[h][i], v[h][4 + i], s, 0, 0, 0);
-          cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[h][i], v[h][6 + i], cross, 0, 0, 0);
-          cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[h][2 + i], v[h][4 + i], cross, 0, 0, 0);
-        }
-      }
-    sum += s;
-  }
-  sum += cross;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) part[wave][i][lane] = sum[i];
-  __syncthreads();
-  const float fa = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
-  const float fb = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fi = __builtin_ldexpf(j.gamma, j.C.e);
-  f32x4 out;
-  auto total = [&](int f, int l) { return part[0][f][l] + part[1][f][l] + part[2][f][l] + part[3][f][l]; };
-#pragma unroll
-  for (int i = 0; i < 4; ++i)                          // accumulator element f: row 8 (f / 4) + 4 (lane / 32) + f % 4
-    out[i] = fmaf(fa, total(wave * 4 + i, lane), fmaf(fb, ev[i], r + i == c && c < j.n ? fi : 0.f));
-  if (ti == tj) {                                      // below the diagonal: what is above it (E is symmetric)
-    const int cc = lane & 31, rr = r & 31;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (r + i > c) out[i] = fmaf(fa, total((cc & 3) + 4 * (cc >> 3), rr + i + 32 * (cc >> 2 & 1)), fb * ev[i]);
-  }
-  store_planes4(j.C.hi, j.C.lo(), np, r, c, ti == tj, out);
-}
-
-// np <= OPERAND_NP: rows of a polynomial of A need A alone - r A, (r A) A, ... - so that a workgroup takes 16 rows through
+// np <= STEP_NP: rows of a polynomial of A need A alone - r A, (r A) A, ... - so that a workgroup takes 16 rows through
 // many products by itself, with A in its waves' registers (256 KB of them at np = 256, 32 columns a wave) and the running
 // rows in LDS.  More flops than the symmetric products of whole matrices (6 n^3 a step against 1.5 to 2), but few launches.
 //   np = 256, a launch a step: S = a r + b r A + c r A^2, next A = a S + b S A + c S A^2 (four products, r rows of A) and
@@ -772,7 +691,7 @@ __global__ __launch_bounds__(256) void orth_chain_small_kernel(ChainArgs a) {
 //     (Errors of the first of those are multiplied by the later ones: the split's lo.lo products are taken too.  Three
 //     products: 23 x 61 off by 1.8e-6, four 1.0e-6, the plain fp32 iteration 0.8e-6.)
 constexpr int STEP_NP = 256, ROWS = 16;
-static_assert(STEP_NP == OPERAND_NP && ROWS_PHASE == 128, "the three sides that orth_rows_kernel is made for");
+static_assert(ROWS_PHASE == 128, "the three sides that orth_rows_kernel is made for");
 enum { E_U, E_UA, E_UAA, E_W, E_WA, E_Y, E_YA, E_YAA, E_W2, E_WA2, E_COUNT };   // scales of the rows in a phase's panel
 struct RowsJob {
   Planes A, An, Q, Qn;
@@ -1108,7 +1027,7 @@ __global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
 // The same for np <= PANEL_NP.  Its eight waves hold all of Q in registers (32 columns each, over all of k; at np = 128 and 64
 // two and four groups of waves hold it), and the lines of X - rows of a tall matrix, columns of a wide one - go by in groups
 // of 8192 / np through two LDS buffers, converted once, the next group's loads in flight: one workgroup a CU.
-constexpr int PANEL_NP = OPERAND_NP, PANEL_LDS = 2 * 2 * 128 * (64 + 8) * 2;    // (np = 64 has the most padding)
+constexpr int PANEL_NP = 256, PANEL_LDS = 2 * 2 * 128 * (64 + 8) * 2;    // (np = 64 has the most padding)
 // a group's loads and LDS writes: 16 elements a thread, raw until they are stored
 template <typename E, bool TALL, int NP> struct PanelLines {
   static constexpr int GL = 8192 / NP, LD = NP + 8;    // (rows that start in 16 different bank groups)
@@ -1425,9 +1344,8 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
   };
   // matrices of np <= ROWS_PHASE take a launch a phase, of np = STEP_NP a launch a step, the others three a step
   auto by_products = [&](int i) { return jobs[i].np() > STEP_NP; };
-  bool small = true, any_phases = false, any_steps = false, any_products = false;
+  bool any_phases = false, any_steps = false, any_products = false;
   for (int i = 0; i < n; ++i) {
-    small = small && jobs[i].np() <= SMALL;
     any_phases = any_phases || jobs[i].np() <= ROWS_PHASE;
     any_steps = any_steps || jobs[i].np() == STEP_NP;
     any_products = any_products || by_products(i);
@@ -1539,12 +1457,11 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
           for (int w = 0; w < per && by_products(i); ++w) {
             ChainJob &g = ca.job[ca.n++];
             memset(&g, 0, sizeof(g));
-            g.n = jobs[i].n(); g.nt = jobs[i].np() / (small ? 32 : T); g.first = blocks; g.alpha = 1.f;
-            blocks += g.nt * (g.nt + 1) / 2;
+            g.n = jobs[i].n(); g.nt = jobs[i].np() / T; g.first = blocks; g.alpha = 1.f;
+            blocks += g.nt * (g.nt + 1);
             fill(g, i, w);
           }
-        if (small) hipLaunchKernelGGL(orth_chain_small_kernel, dim3(blocks), dim3(256), 0, st, ca);
-        else hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(512), CHAIN_LDS, st, ca);
+        hipLaunchKernelGGL(orth_chain_kernel, dim3(blocks), dim3(256), 0, st, ca);
         AGX_LAUNCH_CHECK();
         return AGX_OK;
       };
@@ -1650,8 +1567,6 @@ int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, co
 
 // (more LDS than the default limit of a launch)
 int agx::orth_prepare_device() {
-  AGX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&orth_chain_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              CHAIN_LDS));
   for (int k = 0; k <= ANY; ++k) {
     const void *f = nullptr;
     by_kind(k, [&](auto kind) { f = reinterpret_cast<const void *>(&orth_panel_kernel<decltype(kind)::value>); });
