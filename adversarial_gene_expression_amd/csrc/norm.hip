@@ -245,6 +245,20 @@ __device__ __forceinline__ uint32_t not_positive(const typename Vec<T>::type &m)
   return b;
 }
 
+// what the backward pass reads of a row
+template <typename T, int G, int C>
+struct Inputs {
+  Row<T, G, C> x, dy, m;
+  float mu, r;
+  __device__ __forceinline__ void load(const NormArgs &a, const Place<T, G, C> &w, int64_t row) {
+    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
+    w.load(dy, reinterpret_cast<const T *>(a.dy) + row * a.lddy);
+    if (a.ym) w.load(m, reinterpret_cast<const T *>(a.ym) + row * a.ldym);
+    mu = a.mean_in[row];
+    r = a.rstd_in[row];
+  }
+};
+
 template <typename T, int G, int C, bool PG>
 __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) {
   constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
@@ -256,19 +270,24 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) 
   const float inv_n = 1.f / (float)a.n;
   const Params<T, G, C> gamma(a.gamma, 1.f, w);
   float acc[2][C][V] = {}, aend[2] = {0.f, 0.f};
-  for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
-    Row<T, G, C> x, dy;
+  // (rows of one wave: the next one's loads are on their way while a row is worked on - 40000 x 1000 bf16 66 us instead of 68,
+  //  20000 x 600 35 instead of 37 - where its registers do not cost a workgroup: 20000 x 2000 bf16 79 us without, 88 with)
+  constexpr bool AHEAD = G <= 64 && C * V <= 16;
+  const int64_t step = (int64_t)gridDim.x * NG;
+  int64_t row = (int64_t)blockIdx.x * NG + grp;
+  Inputs<T, G, C> in;
+  if (AHEAD && row < a.rows) in.load(a, w, row);
+  for (; row < a.rows; row += step) {
+    if (!AHEAD) in.load(a, w, row);
+    const Row<T, G, C> x = in.x, dy = in.dy;
     uint32_t neg[C] = {}, nend = 0;
-    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
-    w.load(dy, reinterpret_cast<const T *>(a.dy) + row * a.lddy);
     if (a.ym) {
-      Row<T, G, C> m;
-      w.load(m, reinterpret_cast<const T *>(a.ym) + row * a.ldym);
 #pragma unroll
-      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(m.v[c]);
-      nend = (float)m.end > 0.f ? 0u : 1u;
+      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(in.m.v[c]);
+      nend = (float)in.m.end > 0.f ? 0u : 1u;
     }
-    const float mu = a.mean_in[row], r = a.rstd_in[row];
+    const float mu = in.mu, r = in.r;
+    if (AHEAD && row + step < a.rows) in.load(a, w, row + step);
     auto hat = [&](int c, int k) { return ((float)x.v[c][k] - mu) * r; };
     auto dn = [&](int c, int k) { return neg[c] >> k & 1 ? a.slope * (float)dy.v[c][k] : (float)dy.v[c][k]; };
     const float he = w.last >= 0 ? ((float)x.end - mu) * r : 0.f, de = nend ? a.slope * (float)dy.end : (float)dy.end;
@@ -545,16 +564,30 @@ __global__ __launch_bounds__(1024) void ln_param_kernel(const float *__restrict_
 enum { FWD, BWD, BWD2 };
 constexpr int PARAM_BLOCKS = 4;
 
+// One round of workgroups, as many as the kernel's registers let a CU hold: a second round would leave most of it idle, and a
+// workgroup more or less a CU is worth a lot (backward, a CU 2, 3, 4 and 6 of them: 40000 x 1000 bf16, of which 3 fit, 67, 67,
+// 78, 73 us; 6000 x 4297 bf16, 2 fit, 68, 88, 76, 90; second order of 8192 x 1077, 4 fit, 55, 45, 44, 49).
+template <auto KERNEL> int resident(int threads) {
+  static const int n = [&] {
+    int fit = 0;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, KERNEL, threads, 0) == hipSuccess ? std::max(1, fit) : 1;
+  }();
+  return n;
+}
+template <auto KERNEL> void launch_one(hipStream_t st, const NormArgs &a, int threads, int &blocks) {
+  blocks = std::min(blocks, agx::num_cus() * resident<KERNEL>(threads));
+  hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3(threads), 0, st, a);
+}
 template <int OP, typename T, int G, int C>
-void launch_cfg(hipStream_t st, const NormArgs &a, int blocks) {
-  const dim3 grid(blocks), thr(block_threads<G>());
-  if constexpr (OP == FWD) hipLaunchKernelGGL((ln_fwd_kernel<T, G, C>), grid, thr, 0, st, a);
+void launch_cfg(hipStream_t st, const NormArgs &a, int &blocks) {
+  constexpr int threads = block_threads<G>();
+  if constexpr (OP == FWD) launch_one<&ln_fwd_kernel<T, G, C>>(st, a, threads, blocks);
   else if constexpr (OP == BWD) {
-    if (a.part) hipLaunchKernelGGL((ln_bwd_kernel<T, G, C, true>), grid, thr, 0, st, a);
-    else hipLaunchKernelGGL((ln_bwd_kernel<T, G, C, false>), grid, thr, 0, st, a);
+    if (a.part) launch_one<&ln_bwd_kernel<T, G, C, true>>(st, a, threads, blocks);
+    else launch_one<&ln_bwd_kernel<T, G, C, false>>(st, a, threads, blocks);
   } else {
-    if (a.part) hipLaunchKernelGGL((ln_bwd2_kernel<T, G, C, true>), grid, thr, 0, st, a);
-    else hipLaunchKernelGGL((ln_bwd2_kernel<T, G, C, false>), grid, thr, 0, st, a);
+    if (a.part) launch_one<&ln_bwd2_kernel<T, G, C, true>>(st, a, threads, blocks);
+    else launch_one<&ln_bwd2_kernel<T, G, C, false>>(st, a, threads, blocks);
   }
 }
 
@@ -568,18 +601,17 @@ Cfg pick(int64_t width, int v) {
   if (nv <= 1024 * 4) return {1024, (int)agx::cdiv64(nv, 1024)};
   return {0, 0};
 }
-// workgroups of a launch: enough rows in flight to fill 256 CUs a few times over; with parameter gradients at most four
-// a CU, because each writes and the second launch reads a partial row
+// workgroups of a launch at most: a row each; with parameter gradients PARAM_BLOCKS a CU, because each writes and the second
+// launch reads a partial row (the workspace is made for these)
 int blocks_of(int64_t rows, const Cfg &c, bool params) {
   const int ng = c.g == 0 || c.g >= 256 ? 1 : 256 / c.g;
-  const int64_t need = agx::cdiv64(rows, ng);
-  return (int)std::min<int64_t>(need, (int64_t)agx::num_cus() * (params ? PARAM_BLOCKS : c.g == 64 || c.g == 16 ? 8 : 16));
+  return (int)std::min<int64_t>(agx::cdiv64(rows, ng), (int64_t)agx::num_cus() * (params ? PARAM_BLOCKS : 16));
 }
 
 template <int OP, typename T>
 int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int accumulate) {
   const Cfg c = pick(a.n, Vec<T>::V);
-  const int blocks = blocks_of(a.rows, c, a.part != nullptr);
+  int blocks = blocks_of(a.rows, c, a.part != nullptr);
   if (blocks > 0) {
     auto by_c = [&](auto g) {
       constexpr int G = decltype(g)::value;
@@ -592,9 +624,9 @@ int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int a
     else if (c.g == 64) by_c(std::integral_constant<int, 64>{});
     else if (c.g == 256) by_c(std::integral_constant<int, 256>{});
     else if (c.g == 1024) by_c(std::integral_constant<int, 1024>{});
-    else if constexpr (OP == FWD) hipLaunchKernelGGL(ln_fwd_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
-    else if constexpr (OP == BWD) hipLaunchKernelGGL(ln_bwd_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL(ln_bwd2_wide_kernel<T>, dim3(blocks), dim3(1024), 0, st, a);
+    else if constexpr (OP == FWD) launch_one<&ln_fwd_wide_kernel<T>>(st, a, 1024, blocks);
+    else if constexpr (OP == BWD) launch_one<&ln_bwd_wide_kernel<T>>(st, a, 1024, blocks);
+    else launch_one<&ln_bwd2_wide_kernel<T>>(st, a, 1024, blocks);
     AGX_LAUNCH_CHECK();
   }
   if (dgamma || dbeta) {
