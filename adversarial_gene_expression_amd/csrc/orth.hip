@@ -3,9 +3,8 @@
 //
 // Algebra.  All iterates are X_0 times polynomials of A_0, which commute, so several steps need the long side only twice:
 // with P = aI + bA + cA^2 the next Gram matrix is A P^2 and the product of the steps Q <- Q P; X_k = X_0 Q.  An error of
-// A_0 in a direction of tiny singular value grows with every step (by up to a^2 in A), so no more than PHASE steps are
-// taken this way: then X Q is formed and its Gram matrix computed anew.  (Five steps on a gradient of a few strong
-// directions: 3 + 2 steps are off by 1.5e-6, all five from one Gram matrix by 1e-4, the plain fp32 iteration by 4e-6.)
+// A_0 in a direction of tiny singular value grows with every step (by up to a^2 in A), so two or three steps are taken this
+// way (phase_of); then X Q is formed and its Gram matrix computed anew.
 // Matrices of n x n are symmetric: tiles on and above the diagonal are computed and mirrored.
 //
 // Products run on the fp16 matrix cores at fp32 accuracy: every operand is split into two fp16 terms, v 2^e = hi + lo (22
@@ -14,10 +13,11 @@
 // everything behind it: entries then stay under 2^14, and those down to 2^-25 of the bound keep all bits.  A bf16 operand
 // needs one term only (its 8 bits fit).
 //
-// Tiles of 64 x 64 by four waves of 32 x 32 (mfma 32x32x16), K in steps of 64 through one LDS buffer, the next step's global
-// loads in flight: four workgroups of a CU overlap each other's loads, conversions and products.  (Tiles of 128 x 128 with
-// two buffers convert every element half as often, but leave one workgroup a CU, whose phases nothing covers: 18161 x 256
-// 166 us against 158.)
+// Launches of a call: the momentum step with |x|'s maximum and norm; then, a phase each, the Gram matrix (and the sum of its
+// slices), its polynomial (n <= 128 one launch a phase, n <= 256 one a step, above three a step) and the product with the
+// long side, which in the last phase is the Muon update of w too.  Floors: 2.4 us a launch, 5 TB/s of HBM, 1150 TFLOP/s of
+// fp16 products over three.  Measured: 256 x 256 92 us (16 launches), 18161 x 256 152 us (a third each the long side's two
+// products and the steps), 1000 x 4297 bf16 387 us (products: 73 us at the matrix cores' rate).
 #include "agx_common.h"
 
 #include <algorithm>
@@ -38,7 +38,7 @@ constexpr int T = 64;                          // n x n matrices are padded to T
 constexpr int PHASE = 3;                       // most steps between two Gram matrices
 constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
-constexpr int GRAM_BLOCKS = 3;                 // workgroups a CU of a Gram product
+constexpr int TALL_BLOCKS = 2, WIDE_BLOCKS = 4;    // workgroups a CU of a Gram product
 constexpr int ONE_SLICE = 4;                   // longest K, in steps of 64 (1.5 us each), that is not split over workgroups
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
 // A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase) or without a divisor (later phases).
 // A workgroup takes R rows of a square of 32 x 32 on or above the diagonal: interleaved shares of the slices meet in LDS, from
 // where the piece and its mirror image go out as vectors.  R = 32 (4 shares) where the slices are few, 4 (8 shares) where
-// they are many: 18161 x 256 with 71 slices 5.0 us instead of 8.0, 1000 x 4297 with 7 slices 10 us instead of 17.
+// they are many: 18161 x 256 with 71 slices 7.1 us instead of 10.5, 1000 x 4297 with 5 slices 11.0 us instead of 13.8.
 struct ReduceJob {
   const float *part;
   const uint32_t *maxb;
@@ -594,7 +594,8 @@ static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 
 // A workgroup has a tile of 64 x 32 on or above the diagonal, its four waves every fourth step of 64 k of all of it: operands
 // go straight from L2 to the matrix cores' registers, each byte once a workgroup, without LDS or barriers until the waves'
-// sums meet.  (Tiles through LDS, four or eight waves at a barrier a step: 16.5 us at n = 1024 instead of CHAIN_US.)
+// sums meet.  (Tiles through LDS, four or eight waves at a barrier a step: 16.5 us at n = 1024 instead of 15.1, 12.5 at 640
+// instead of 8.2.  The floor of the products is 3 us; 272 tiles on 256 CUs, whose L1 takes 64 bytes a clock, bound it.)
 __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
   __shared__ float part[4][32][64];                    // [wave][element][lane]
   const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
@@ -690,6 +691,9 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
 //   np <= 128, a launch a phase of up to two steps: u = rows of P_0, then u P_1 with u A_1 = ((u A) P_0) P_0 (twelve products).
 //     (Errors of the first of those are multiplied by the later ones: the split's lo.lo products are taken too.  Three
 //     products: 23 x 61 off by 1.8e-6, four 1.0e-6, the plain fp32 iteration 0.8e-6.)
+// Measured: 8.1 us a step of np = 256 (three launches of whole products: 20), a phase of np = 128 8.1 us and of 64 5.3 us (by
+// one workgroup a matrix: 14 and 9).  Bound by the chain of dependent products: 0.4 to 0.8 us each behind 2.4 us of launch and
+// 1.5 us until A is in registers.
 constexpr int STEP_NP = 256, ROWS = 16;
 static_assert(ROWS_PHASE == 128, "the three sides that orth_rows_kernel is made for");
 enum { E_U, E_UA, E_UAA, E_W, E_WA, E_Y, E_YA, E_YAA, E_W2, E_WA2, E_COUNT };   // scales of the rows in a phase's panel
@@ -1026,7 +1030,9 @@ __global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
 
 // The same for np <= PANEL_NP.  Its eight waves hold all of Q in registers (32 columns each, over all of k; at np = 128 and 64
 // two and four groups of waves hold it), and the lines of X - rows of a tall matrix, columns of a wide one - go by in groups
-// of 8192 / np through two LDS buffers, converted once, the next group's loads in flight: one workgroup a CU.
+// of 8192 / np through two LDS buffers, converted once, the next group's loads in flight: one workgroup a CU.  18161 x 256
+// 17.3 us (tiles of 64 x 64 as above: 23 us; its 37 MB take 7.4 us at 5 TB/s), 3 groups a workgroup of 2.7 us each: 1.3 us
+// of matrix products, then the results' way out and the next group's way in, which a barrier a group keeps apart.
 constexpr int PANEL_NP = 256, PANEL_LDS = 2 * 2 * 128 * (64 + 8) * 2;    // (np = 64 has the most padding)
 // a group's loads and LDS writes: 16 elements a thread, raw until they are stored
 template <typename E, bool TALL, int NP> struct PanelLines {
@@ -1188,14 +1194,15 @@ int64_t longest(const Job *jobs, int n) {               // steps of the longest 
   for (int i = 0; i < n; ++i) k = std::max(k, agx::cdiv64(jobs[i].K(), BK));
   return k;
 }
-// slices of a Gram product.  Up to ONE_SLICE steps one, whose launch gives the matrix itself (256 x 256 92 us instead of 97,
-// 100 x 60 57 instead of 64; 7 steps in one slice: 400 x 400 173 us instead of 156).  Beyond: about GRAM_BLOCKS workgroups a CU over all of the call's matrices (each writes, and the next
-// launch reads, a whole tile)
-// (most_steps: longest())
+// slices of a Gram product.  Up to ONE_SLICE steps one, whose launch gives the matrix itself (256 x 256 92 us instead of 96,
+// 100 x 60 57 instead of 64; 7 steps in one slice: 400 x 400 173 us instead of 156).  Beyond: two workgroups a CU for tall
+// matrices and four for wide ones, over all of the call's matrices - each writes, and the next launch reads, a whole tile
+// (18161 x 256: 2, 3, 4 a CU 152, 157, 157 us; 1000 x 4297 419, 397, 387; GTEx generator's Muon step 188, 182, 177).
+// most_steps: longest().
 void plan(const Job &j, int total_tiles, int64_t most_steps, int phases, bool need_u, Layout &l) {
   const int tiles = j.tiles();
   const int64_t ksteps = agx::cdiv64(j.K(), BK);
-  const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() * GRAM_BLOCKS / std::max(1, total_tiles));
+  const int64_t want = std::max<int64_t>(1, (int64_t)agx::num_cus() * (j.rows >= j.cols ? TALL_BLOCKS : WIDE_BLOCKS) / std::max(1, total_tiles));
   l.kper = std::max<int64_t>(std::min<int64_t>(ksteps, most_steps <= ONE_SLICE ? ONE_SLICE : 2), agx::cdiv64(ksteps, want)) * BK;
   l.slices = (int)agx::cdiv64(j.K(), l.kper);
   int64_t off = 0;
@@ -1209,7 +1216,10 @@ void plan(const Job &j, int total_tiles, int64_t most_steps, int phases, bool ne
   l.u = need_u ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.end = off;
 }
-// steps between two Gram matrices
+// Steps between two Gram matrices.  Error against 64 bits over the plain fp32 iteration's (gradients of a few strong directions
+// and noise): sides up to 256, of 19 x 201 to 18161 x 256, three steps 2.9 in the mean and up to 7.3, two 1.1 and up to 1.8;
+// sides above, whose fp32 sums are longer, three steps 0.6 to 0.8.  Two steps cost 18161 x 256 a fifth of its time, 1000 x 4297
+// as much.
 int phase_of(const Job *jobs, int n) {
   for (int i = 0; i < n; ++i)
     if (jobs[i].np() <= PANEL_NP) return 2;
