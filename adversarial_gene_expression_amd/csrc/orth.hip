@@ -16,8 +16,8 @@
 // Launches of a call: the momentum step with |x|'s maximum and norm; then, a phase each, the Gram matrix (and the sum of its
 // slices), its polynomial (n <= 128 one launch a phase, n <= 256 one a step, above three a step) and the product with the
 // long side, which in the last phase is the Muon update of w too.  Floors: 2.4 us a launch, 5 TB/s of HBM, 1150 TFLOP/s of
-// fp16 products over three.  Measured: 256 x 256 92 us (16 launches), 18161 x 256 152 us (a third each the long side's two
-// products and the steps), 1000 x 4297 bf16 387 us (products: 73 us at the matrix cores' rate).
+// fp16 products over three.  Measured: 256 x 256 91 us (12 launches), 18161 x 256 151 us (15), 1000 x 4297 bf16 379 us
+// (20; its products take 73 us at that rate).
 #include "agx_common.h"
 
 #include <algorithm>
