@@ -1,9 +1,11 @@
 // Internal helpers shared by the libagx translation units (not part of the ABI).
 #pragma once
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdint>
+#include <utility>
 #include "../../include/agx.h"
 
 namespace agx {
@@ -108,6 +110,27 @@ int ff_hx(void *stream, const float *hrows, int ldh, int HL, float *X, int ldx, 
 // epilogue, without split-K (then fused and unfused runs sum in the same order: bit-identical)
 bool gemm_can_fuse_opt(int M, int N, int K, int64_t ws_floats);
 int fill_zero(void *stream, float *p, int64_t n);   // elementwise.hip
+// a matrix in memory (a NULL one is nowhere); leading dimension in elements of `bytes` bytes
+struct Region {
+  const void *p;
+  int64_t rows, cols, ld;
+  int bytes;
+};
+// true if two of them share an element.  Row starts of one stride (or a single row) are told apart by column, as blocks of
+// columns of one buffer are; with different strides any common range of addresses counts.
+inline bool overlap(Region a, Region b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+  if (reinterpret_cast<uintptr_t>(a.p) > reinterpret_cast<uintptr_t>(b.p)) std::swap(a, b);
+  const int64_t gap = reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p);   // bytes from a's start to b's
+  if (gap >= ((a.rows - 1) * a.ld + a.cols) * a.bytes) return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.rows == 1) a.ld = b.ld;
+  if (b.rows == 1) b.ld = a.ld;
+  if (a.ld != b.ld || a.bytes != b.bytes || gap % a.bytes || std::max(a.cols, b.cols) > a.ld) return true;
+  const int64_t row = gap / a.bytes / a.ld, col = gap / a.bytes % a.ld;                      // of a's grid, where b starts
+  if (row < a.rows && col < a.cols) return true;
+  return col + b.cols > a.ld && row + 1 < a.rows;                                            // b's rows reach a's next ones
+}
 // real += (1 - alpha[b]) d, fake += alpha[b] d over B rows of H values, all with leading dimension ld: the backward of
 // agx_gp_interp into gradients that are there already (elementwise.hip)
 int interp_back(void *stream, const float *d, float *real, float *fake, int ld, const float *alpha, int B, int H);

@@ -655,12 +655,26 @@ int check_mat(const agx_norm_t *p, const void *m, int64_t ld, const char *who, c
   AGX_CHECK_ARG((reinterpret_cast<uintptr_t>(m) & al) == 0, "%s: %s not aligned to its elements", who, name);
   return AGX_OK;
 }
+// an output may be the same matrix as an input, but not another one that shares elements with it
+int check_out(const agx_norm_t *p, const void *out, int64_t ldo, const char *who) {
+  const int bytes = p->dtype == AGX_F32 ? 4 : 2;
+  const void *in[4] = {p->x, p->dy, p->u, p->act ? p->y : nullptr};
+  const int64_t ld[4] = {p->ldx, p->lddy, p->ldu, p->ldy};
+  for (int i = 0; i < 4; ++i)
+    AGX_CHECK_ARG((in[i] == out && (ld[i] == ldo || p->rows == 1)) ||
+                      !agx::overlap({out, p->rows, p->width, ldo, bytes}, {in[i], p->rows, p->width, ld[i], bytes}),
+                  "%s: an output overlaps an input without being the same matrix", who);
+  return AGX_OK;
+}
 int check_back(const agx_norm_t *p, const char *who) {
   AGX_TRY(check_mat(p, p->x, p->ldx, who, "x"));
   AGX_TRY(check_mat(p, p->dy, p->lddy, who, "dy"));
   AGX_CHECK_ARG(p->mean && p->rstd, "%s: mean / rstd missing", who);
   if (p->act) AGX_TRY(check_mat(p, p->y, p->ldy, who, "y"));
-  if (p->dx) AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
+  if (p->dx) {
+    AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
+    AGX_TRY(check_out(p, p->dx, p->lddx, who));
+  }
   if (p->dgamma || p->dbeta) {
     const int64_t need = agx_layernorm_ws_floats(p->rows, p->width, p->dtype);
     if (need > 0 && (!p->ws || p->ws_floats < need)) {
@@ -693,6 +707,10 @@ extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
   if (p->rows == 0) return AGX_OK;
   AGX_TRY(check_mat(p, p->x, p->ldx, "agx_layernorm_fwd", "x"));
   AGX_TRY(check_mat(p, p->y, p->ldy, "agx_layernorm_fwd", "y"));
+  const int bytes = p->dtype == AGX_F32 ? 4 : 2;
+  AGX_CHECK_ARG((p->x == p->y && (p->ldx == p->ldy || p->rows == 1)) ||
+                    !agx::overlap({p->x, p->rows, p->width, p->ldx, bytes}, {p->y, p->rows, p->width, p->ldy, bytes}),
+                "agx_layernorm_fwd: y overlaps x without being the same matrix");
   NormArgs a = {};
   a.x = p->x; a.ldx = p->ldx; a.y = p->y; a.ldy = p->ldy;
   a.gamma = p->gamma; a.beta = p->beta; a.mean = p->mean; a.rstd = p->rstd;
@@ -718,7 +736,13 @@ extern "C" int agx_layernorm_bwd2(void *stream, const agx_norm_t *p) {
   if (p->rows > 0) {
     AGX_TRY(check_back(p, "agx_layernorm_bwd2"));
     AGX_TRY(check_mat(p, p->u, p->ldu, "agx_layernorm_bwd2", "u"));
-    if (p->ddy) AGX_TRY(check_mat(p, p->ddy, p->ldddy, "agx_layernorm_bwd2", "ddy"));
+    if (p->ddy) {
+      AGX_TRY(check_mat(p, p->ddy, p->ldddy, "agx_layernorm_bwd2", "ddy"));
+      AGX_TRY(check_out(p, p->ddy, p->ldddy, "agx_layernorm_bwd2"));
+      const int bytes = p->dtype == AGX_F32 ? 4 : 2;
+      AGX_CHECK_ARG(!agx::overlap({p->dx, p->rows, p->width, p->lddx, bytes}, {p->ddy, p->rows, p->width, p->ldddy, bytes}),
+                    "agx_layernorm_bwd2: dx and ddy overlap");
+    }
   }
   NormArgs a = back_args(p);
   a.u = p->u; a.ldu = p->ldu; a.ddy = p->ddy; a.ldddy = p->ldddy;

@@ -1604,6 +1604,14 @@ extern "C" int agx_orthogonalize(void *stream, const agx_orth_t *jobs, int32_t n
                   "%s: matrix %d not aligned to its elements", who, i);
     AGX_CHECK_ARG(j[i].x != j[i].out, "%s: matrix %d: the result cannot be written over the input", who, i);
   }
+  // (matrices of a call are worked on at once)
+  auto region = [&](const void *p, int i, int64_t ld) { return agx::Region{p, j[i].rows, j[i].cols, ld, j[i].dtype == AGX_F32 ? 4 : 2}; };
+  for (int i = 0; i < n; ++i)
+    for (int k = 0; k < n; ++k) {
+      const agx::Region out = region(j[i].out, i, j[i].ldo);
+      AGX_CHECK_ARG(!agx::overlap(out, region(j[k].x, k, j[k].ldx)) && (k <= i || !agx::overlap(out, region(j[k].out, k, j[k].ldo))),
+                    "%s: the result of matrix %d overlaps matrix %d or its result", who, i, k);
+    }
   return run(agx::as_stream(stream), j, n, o, 0.f, false, static_cast<char *>(ws), ws_size, who);
 }
 
@@ -1634,5 +1642,14 @@ extern "C" int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, con
                   "%s: matrix %d not aligned to its elements", who, i);
     AGX_CHECK_ARG(a.w != a.m && a.w != a.g && a.g != a.m, "%s: matrix %d: w, g and m must be different arrays", who, i);
   }
+  // (matrices of a call are worked on at once: what is written, w and m, must be nothing else's)
+  auto region = [&](const void *p, int i, int64_t ld) { return agx::Region{p, jobs[i].rows, jobs[i].cols, ld, 4}; };
+  for (int i = 0; i < n; ++i)
+    for (int k = 0; k < n; ++k) {
+      const agx::Region w = region(jobs[i].w, i, jobs[i].ldw), m = region(jobs[i].m, i, jobs[i].ldm), g = region(jobs[k].g, k, jobs[k].ldg);
+      const agx::Region wk = region(jobs[k].w, k, jobs[k].ldw), mk = region(jobs[k].m, k, jobs[k].ldm);
+      AGX_CHECK_ARG(!agx::overlap(w, g) && !agx::overlap(m, g) && !agx::overlap(w, mk) && (k <= i || (!agx::overlap(w, wk) && !agx::overlap(m, mk))),
+                    "%s: w, g and m of matrices %d and %d must be different arrays", who, i, k);
+    }
   return run(agx::as_stream(stream), j, n, &o->orth, o->momentum, o->nesterov != 0, static_cast<char *>(ws), ws_size, who);
 }

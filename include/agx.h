@@ -164,7 +164,7 @@ int agx_bn_moving_update(void *stream, float *moving_mean, float *moving_var, co
  *         q = rstd (u - mean(u) - h mean(u h)):  ddy = act'(y) gamma q,  dgamma = sum dn q,
  *         dx = rstd^2 (h (3 mean(gh) mean(uh) + mean(g) mean(u) - mean(gu)) - mean(uh) (g - mean(g)) - mean(gh) (u - mean(u)))
  * act: 1 = leaky ReLU of `slope` (its derivative is taken from the sign of y, which bwd / bwd2 then need), 0 = none.
- * Any output but mean / rstd may be NULL in bwd / bwd2; an output may be the same array as an input of its own shape.
+ * Any output but mean / rstd may be NULL in bwd / bwd2; an output may be the same matrix as an input, any other overlap is refused.
  * ws: needed where dgamma / dbeta are wanted (agx_layernorm_ws_floats).  Sums in a fixed order.                       */
 #define AGX_F32 0
 #define AGX_BF16 1
@@ -191,7 +191,8 @@ int agx_layernorm_bwd2(void *stream, const agx_norm_t *p);
 /* ---- orthogonalised updates (no reference counterpart: its optimizers are RMSprop / Adam, tf_utils.py:285-288) ----
  * X_0 = x / (|x|_F + eps); X <- X (a I + b A + c A^2), A = X^T X, `steps` times (A = X X^T from the left where
  * rows < cols): Newton-Schulz steps that bring the singular values of x towards 1.  n_coef: 1 (the same a, b, c for
- * every step) or `steps` triples.  min(rows, cols) <= AGX_ORTH_MAX_SIDE.  Products are fp32-accurate.                 */
+ * every step) or `steps` triples.  min(rows, cols) <= AGX_ORTH_MAX_SIDE.  Products are fp32-accurate.
+ * Matrices of a call are worked on at once: a result that shares memory with another one or with an x is refused.      */
 #define AGX_MAX_ORTH 16
 #define AGX_ORTH_MAX_SIDE 4096
 #define AGX_ORTH_MAX_STEPS 16
@@ -211,7 +212,8 @@ typedef struct agx_orth_opts {
 int64_t agx_orth_ws_bytes(const agx_orth_t *jobs, int32_t n, int32_t steps);
 int agx_orthogonalize(void *stream, const agx_orth_t *jobs, int32_t n, const agx_orth_opts_t *o, void *ws, int64_t ws_size);
 /* One Muon step over n fp32 matrices: m <- momentum m + g; u = g + momentum m (nesterov) or m;
- * w <- (1 - lr weight_decay) w - lr scale orth(u).  w, g, m: different arrays.                                         */
+ * w <- (1 - lr weight_decay) w - lr scale orth(u).  w, g, m: different arrays, within a matrix and
+ * between those of a call (a g may be read twice).                                                                     */
 typedef struct agx_muon {
   float *w;
   const float *g;

@@ -159,3 +159,27 @@ def test_side_stream(gpu):
         got = ops.layer_norm_backward(dy, x, m2, r2, ga)
     torch.cuda.current_stream().wait_stream(st)
     assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_without_an_eager_call_before(gpu):
+    """Kernels that no eager call has launched yet, straight into a graph; replays against eager calls behind it."""
+    from adversarial_gene_expression_amd import ops
+    g = torch.Generator().manual_seed(3)
+    x, dy, u = (torch.randn(9, 31000, generator=g).to(torch.bfloat16).to(gpu) for _ in range(3))
+    gamma, beta = torch.rand(31000, generator=g).to(gpu), torch.rand(31000, generator=g).to(gpu)
+    ops.layer_norm(x[:, :8])                             # (the library itself is initialised)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+
+    def run():
+        y, mean, rstd = ops.layer_norm(x, gamma, beta, act=1, slope=0.2)
+        a = ops.layer_norm_backward(dy, x, mean, rstd, gamma, y=y, act=1, slope=0.2)
+        return (y,) + a + ops.layer_norm_backward2(u, dy, x, mean, rstd, gamma, y=y, act=1, slope=0.2)
+    with torch.cuda.graph(graph):
+        kept = run()
+    for k in range(3):
+        x.mul_(0.5 + k)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(kept, run()):
+            assert torch.equal(a, b)

@@ -379,3 +379,41 @@ def test_two_ranks_take_the_one_process_step(gpu, tmp_path):
         else:
             assert diff <= 2 * 5e-4 * 10 ** 0.5     # (the first RMSprop step is lr sqrt(10) sign(g): a flipped sign of g ~ 0)
         np.testing.assert_allclose(r0['m%02d' % i], ref['m%02d' % i], rtol=0, atol=4 * t)
+
+
+def test_whatever_memory_held_before_stays_out(gpu):
+    """Odd widths leave padding behind the rows of intermediate results: memory full of NaN changes nothing."""
+    from adversarial_gene_expression_amd import tf_utils as T
+    p = case(61, (24, 17, 5), 9, 0.2, (True, True), 1)
+    gen, disc = nets(T, p, 0.2)
+
+    def run():
+        junk = [torch.full((n,), float('nan'), device=gpu) for n in [64, 192, 256, 512, 1024, 4096, 1 << 16, 1 << 20] * 8]
+        del junk
+        fake = T.predict(p['cc'], p['nc'], gen, z=p['z'])
+        return (fake, np.asarray(disc([p['x'], p['cc'], p['nc']])),
+                np.asarray(T.gradient_penalty(lambda x: disc([x, p['cc'], p['nc']], training=True), p['x'], fake, alpha=p['alpha'])))
+    first = run()
+    for a, b in zip(first, run()):
+        assert np.all(np.isfinite(a))
+        np.testing.assert_array_equal(a, b)
+
+
+def test_c_forward_entries(gpu):
+    """agx_cgan_gen_forward / disc_forward of normalised nets, the critic over up to three times the batch, against __call__."""
+    from adversarial_gene_expression_amd import _dev, _lib, tf_utils as T
+    p = case(61, (24, 17, 5), 33, 0.2, (True, True), 1)
+    gen, disc = nets(T, p, 0.2)
+    pair, lib = T._pair(gen, disc, 33), _lib.load()
+    x, z, nc = (_dev.to_dev(p[k]) for k in ('x', 'z', 'nc'))
+    cc = _dev.to_dev(p['cc'], torch.int32)
+    out = torch.empty(33, 61, device=gpu)
+    _lib.check(lib.agx_cgan_gen_forward(pair.handle, _dev.stream(), z.data_ptr(), cc.data_ptr(), nc.data_ptr(), 33, out.data_ptr(), 61))
+    want = torch.as_tensor(np.asarray(gen([z, cc, nc])), device=gpu)
+    assert float((out - want).abs().max()) <= 2.0 ** -18 * float(want.abs().max())
+    x3, cc3, nc3 = (t.repeat(3, 1).contiguous() for t in (x, cc, nc))
+    rows = 3 * pair.max_batch if 3 * pair.max_batch <= 99 else 99
+    s = torch.empty(rows, device=gpu)
+    _lib.check(lib.agx_cgan_disc_forward(pair.handle, _dev.stream(), x3.data_ptr(), 61, cc3.data_ptr(), nc3.data_ptr(), rows, s.data_ptr()))
+    want = torch.as_tensor(np.asarray(disc([x3[:rows], cc3[:rows], nc3[:rows]])), device=gpu).reshape(-1)
+    assert float((s - want).abs().max()) <= 2.0 ** -18 * float(want.abs().max())

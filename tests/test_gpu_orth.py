@@ -234,3 +234,26 @@ def test_muon_over_sides_of_every_size(gpu):
         step = 0.02 * max(1.0, w.shape[1] / w.shape[0]) ** 0.5
         err = torch.linalg.vector_norm(N.t64(w) - (w0 - step * o))
         assert float(err) <= step * tol * float(torch.linalg.vector_norm(o)) + 2.0 ** -23 * float(torch.linalg.vector_norm(w0))
+
+
+@pytest.mark.parametrize('rows,cols,dtype', [(1500, 1300, torch.float32), (2049, 4100, torch.bfloat16), (4096, 4096, torch.float32)])
+def test_large_sides(gpu, rows, cols, dtype):
+    """The same tolerance; the float64 iteration runs on the GPU here."""
+    from adversarial_gene_expression_amd import ops
+    x = torch.randn(rows, cols, generator=torch.Generator(device=gpu).manual_seed(rows), device=gpu).to(dtype)
+    got = ops.orthogonalize(x)
+    d = x.double()
+    sign = torch.randint(0, 2, d.shape, generator=torch.Generator(device=gpu).manual_seed(1), device=gpu).double() * 2 - 1
+    if rows < cols:                                      # (the oracle's transposed view, contiguous)
+        d, sign, got = d.t().contiguous(), sign.t().contiguous(), got.t().contiguous()
+
+    def oracle(v):
+        v = v / v.norm()
+        for _ in range(5):
+            A = v.t().contiguous() @ v
+            v = 3.4445 * v + v @ (-4.7750 * A + 2.0315 * (A @ A))
+        return v
+    err = lambda a, b: float((a - b).norm() / b.norm())  # noqa: E731
+    want = oracle(d)
+    tol = 16 * err(oracle(d * (1 + sign * 2.0 ** -21)), want) + 2.0 ** -20
+    assert err(got.double(), want) <= tol + half(dtype), (err(got.double(), want), tol)

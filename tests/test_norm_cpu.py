@@ -129,3 +129,26 @@ def test_formulas_against_autograd_and_differences(on, slope):
             args[0][at], args[1][at] = base + e, base - e
             fd = (dx_of(*args[0]) - dx_of(*args[1])) / (2 * h)
             assert abs(float(fd - grad.reshape(-1)[i])) < 1e-5
+
+
+def test_outputs_overlap_inputs_only_as_the_same_matrix():
+    """Refused before any launch; rows = 4, width = 6."""
+    lib = _lib.load()
+    err = lambda: lib.agx_last_error().decode()  # noqa: E731
+
+    def desc(**kw):
+        d = _lib.NormDesc()
+        d.rows, d.width, d.eps, d.act = 4, 6, 1e-3, 0
+        d.ldx = d.lddy = d.ldu = d.ldy = d.lddx = d.ldddy = 8
+        d.x, d.dy, d.u, d.y, d.mean, d.rstd = 4096, 8192, 12288, 16384, 20480, 24576
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+    assert lib.agx_layernorm_fwd(None, desc(y=4096 + 4)) == -1 and 'overlaps' in err()
+    assert lib.agx_layernorm_fwd(None, desc(y=4096, ldy=6)) == -1
+    for base in (4096, 8192):
+        assert lib.agx_layernorm_bwd(None, desc(dx=base + 32)) == -1 and 'overlaps' in err()
+    for base in (4096, 8192, 12288):
+        assert lib.agx_layernorm_bwd2(None, desc(ddy=base + 8)) == -1 and 'overlaps' in err()
+    assert lib.agx_layernorm_bwd2(None, desc(dx=28672, ddy=28672)) == -1 and 'dx and ddy' in err()
+    assert lib.agx_layernorm_bwd(None, desc(dx=16384 + 8, act=1)) == -1 and 'overlaps' in err()

@@ -111,3 +111,35 @@ def test_oracle_against_singular_values():
         for _ in range(5):
             s = 3.4445 * s - 4.7750 * s ** 3 + 2.0315 * s ** 5
         assert (N.orthogonalize(y) - u @ torch.diag(s) @ v).abs().max() < 1e-12
+
+
+def test_matrices_of_a_call_may_not_share_what_is_written():
+    """Refused before any launch: two jobs run at once."""
+    lib = _lib.load()
+    err = lambda: lib.agx_last_error().decode()  # noqa: E731
+    big = 1 << 40
+
+    def orth(*ptrs):                                                # (x, out) pairs of 4 x 6 matrices
+        j = (_lib.OrthDesc * len(ptrs))()
+        for q, (x, out, ld) in zip(j, ptrs):
+            q.x, q.out, q.ldx, q.ldo, q.rows, q.cols, q.dtype = x, out, ld, ld, 4, 6, 0
+        return lib.agx_orthogonalize(None, j, len(ptrs), _opts(), None, big)
+    for bad in ([(4096, 8192, 6), (12288, 8192, 6)], [(4096, 8192, 6), (8192, 12288, 6)], [(4096, 8192, 6), (16384, 8192 + 24 * 3, 6)],
+                [(4096, 4096 + 4, 6)], [(4096, 8192, 16), (16384, 8192 + 20, 16)]):
+        assert orth(*bad) == -1 and 'overlaps' in err(), bad
+    # blocks of columns of one buffer, neighbouring rows of a flat one and one input twice are told apart (workspace missing)
+    for good in ([(4096, 4096 + 24, 16)], [(4096, 8192, 6), (4096 + 96, 8192 + 96, 6)], [(4096, 8192, 6), (4096, 12288, 6)]):
+        assert orth(*good) == -3, (good, err())
+
+    o = _lib.MuonOpts()
+    o.orth, o.lr, o.momentum, o.nesterov = _opts(), 0.1, 0.9, 1
+
+    def muon(*ptrs):
+        j = (_lib.MuonDesc * len(ptrs))()
+        for q, (w, g, m) in zip(j, ptrs):
+            q.w, q.g, q.m, q.ldw, q.ldg, q.ldm, q.rows, q.cols, q.scale = w, g, m, 6, 6, 6, 4, 6, 1.0
+        return lib.agx_opt_muon(None, j, len(ptrs), o, None, big)
+    for bad in ([(4096, 8192, 12288), (4096, 16384, 20480)], [(4096, 8192, 12288), (20480, 16384, 12288)],
+                [(4096, 8192, 12288), (20480, 4096, 24576)], [(4096, 8192, 12288), (20480, 12288, 24576)], [(4096, 4096 + 8, 12288)]):
+        assert muon(*bad) == -1 and 'different arrays' in err(), bad
+    assert muon((4096, 8192, 12288), (16384, 8192, 20480)) == -3   # one gradient for two kernels is only read
