@@ -40,6 +40,7 @@ constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
 constexpr int TALL_BLOCKS = 2, WIDE_BLOCKS = 4;    // workgroups a CU of a Gram product
 constexpr int ONE_SLICE = 4;                   // longest K, in steps of 64 (1.5 us each), that is not split over workgroups
+constexpr int LINES_BLOCKS = 3, ONE_SLICE_LINES = 16;   // the same of the iterate's Gram product
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
@@ -64,6 +65,18 @@ __device__ __forceinline__ void placed(int np, int piece, int &row, int &k) {   
 __device__ __forceinline__ int exponent_of(uint32_t absbits) {   // e with |v| < 2^e for the float of these bits
   return absbits == 0 ? 0 : (int)(absbits >> 23) - 126;
 }
+// The iterate between two phases: its K lines (rows of a tall matrix, columns of a wide one) of n values as planes of np rows
+// by kp lines (K rounded up to 64; zeros behind n and K), in the same order: the operands of its Gram matrix.
+struct Lines {
+  _Float16 *hi;
+  int64_t kp;
+  int32_t e, np;
+  __device__ __forceinline__ _Float16 *lo() const { return hi + np * kp; }
+  __device__ __forceinline__ int64_t at(int i, int line) const {     // value i of a line (eight lines are neighbours)
+    return ((i >> 4) * (kp >> 6) + (line >> 6)) * 1024 + ((line >> 3) & 1) * 512 + (((line >> 4) & 3) * 16 + (i & 15)) * 8 + (line & 7);
+  }
+};
+
 // v = hi + lo, each rounded to nearest (two values an instruction)
 __device__ __forceinline__ void split4(f32x4 v, half4 &hi, half4 &lo) {
   hi = __builtin_convertvector(v, half4);
@@ -313,6 +326,32 @@ template <typename E> struct LoadT {
   }
 };
 
+// lines r0.. of the iterate, k the values of a line; blocks of 4 x 4 as above
+struct LoadLines {
+  static constexpr bool two = true;
+  const Lines *x;
+  int e;                                               // (not used: the planes are scaled)
+  half4 vh[4], vl[4];                                  // [k][line]
+  __device__ __forceinline__ int line() const { return (threadIdx.x >> 7) * 32 + (threadIdx.x & 7) * 4; }
+  __device__ __forceinline__ int kk() const { return (threadIdx.x >> 3 & 15) * 4; }
+  __device__ __forceinline__ void fetch(int64_t r0, int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t o = x->at((int)k0 + kk() + i, (int)r0 + line());
+      vh[i] = *reinterpret_cast<const half4 *>(x->hi + o);
+      vl[i] = *reinterpret_cast<const half4 *>(x->lo() + o);
+    }
+  }
+  __device__ __forceinline__ void store(_Float16 *t) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int o = (line() + i) * LDK + kk();
+      *reinterpret_cast<half4 *>(t + o) = half4{vh[0][i], vh[1][i], vh[2][i], vh[3][i]};
+      *reinterpret_cast<half4 *>(t + PL + o) = half4{vl[0][i], vl[1][i], vl[2][i], vl[3][i]};
+    }
+  }
+};
+
 // acc = A-tile (rows ra..) . B-tile (rows rb..)^T over k in [k0, k1), whole steps.  The matrix cores add a step's products,
 // the split's small terms first, and vector additions the steps: a long chain of additions to one fp32 sum would lose what
 // the split keeps.  same: both operands are the same rows, loaded once.
@@ -441,7 +480,7 @@ __device__ __forceinline__ void mirror(float *v, float *scratch) {
 
 // KIND: what all of a launch's matrices are (bit 0: wide, bit 1: bf16), or ANY: one loader's registers instead of the
 // largest of four let twice as many workgroups of a CU wait for memory at a time
-constexpr int ANY = 4;
+constexpr int ANY = 4, ITERATE = 5;            // (ITERATE: the planes between two phases)
 __device__ __host__ __forceinline__ bool is_kind(int kind, bool tall, int dtype) { return kind == (tall ? 0 : 1) + (dtype == AGX_F32 ? 0 : 2); }
 
 // ONE: the job is one slice, and its tiles (of all np x np) go out as A_0 itself, without a launch that adds slices
@@ -596,40 +635,39 @@ static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 // go straight from L2 to the matrix cores' registers, each byte once a workgroup, without LDS or barriers until the waves'
 // sums meet.  (Tiles through LDS, four or eight waves at a barrier a step: 16.5 us at n = 1024 instead of 15.1, 12.5 at 640
 // instead of 8.2.  The floor of the products is 3 us; 272 tiles on 256 CUs, whose L1 takes 64 bytes a clock, bound it.)
-__global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
-  __shared__ float part[4][32][64];                    // [wave][element][lane]
-  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
-  int q = 0;
-  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
-  const ChainJob &j = a.job[q];
-  int ti = 0, tj = id - j.first;                       // row ti of tiles starts at column 2 ti
-  while (tj >= 2 * (j.nt - ti)) tj -= 2 * (j.nt - ti++);
-  tj += 2 * ti;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), np = j.C.np, steps = np / BK;
+typedef float WaveSums[4][32][64];                    // [wave][element of two accumulators][lane]
+// tile of 64 x 32 of linear index t: row ti of tiles starts at column 2 ti
+__device__ __forceinline__ void half_tile(int t, int nt, int &ti, int &tj) {
+  ti = 0;
+  while (t >= 2 * (nt - ti)) t -= 2 * (nt - ti++);
+  tj = t + 2 * ti;
+}
+// the workgroup's product of 64 rows (x) and 32 rows (y) over steps s0.. < s1 of 64 k into `part`; rs: values of 16 rows
+__device__ __forceinline__ void wave_products(const _Float16 *xh, const _Float16 *xl, const _Float16 *yh, const _Float16 *yl, int64_t rs,
+                                              int s0, int s1, WaveSums &part) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (k runs in an order of its own, the same for both operands)
-  const int at = (lane & 31) / 16 * 16 * np + (lane >> 5) * 128 + (lane & 15) * 8;
-  const _Float16 *ah = j.L.hi + (int64_t)ti * 64 * np, *al = j.L.lo() + (int64_t)ti * 64 * np;
-  const _Float16 *bh = j.R.hi + (int64_t)tj * 32 * np, *bl = j.R.lo() + (int64_t)tj * 32 * np;
+  const int64_t at = (lane & 31) / 16 * rs + (lane >> 5) * 128 + (lane & 15) * 8;
   half8 x[2][2][2][2], y[2][2][2];                     // [half of a step][rows 32 ..][plane][vector], [half][plane][vector]
   auto fetch = [&](int s, int h) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int o = at + s * 1024 + h * 256 + i * 512;
+      const int64_t o = at + (int64_t)s * 1024 + h * 256 + i * 512;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        x[h][t][0][i] = *reinterpret_cast<const half8 *>(ah + t * 32 * np + o);
-        x[h][t][1][i] = *reinterpret_cast<const half8 *>(al + t * 32 * np + o);
+        x[h][t][0][i] = *reinterpret_cast<const half8 *>(xh + t * 2 * rs + o);
+        x[h][t][1][i] = *reinterpret_cast<const half8 *>(xl + t * 2 * rs + o);
       }
-      y[h][0][i] = *reinterpret_cast<const half8 *>(bh + o);
-      y[h][1][i] = *reinterpret_cast<const half8 *>(bl + o);
+      y[h][0][i] = *reinterpret_cast<const half8 *>(yh + o);
+      y[h][1][i] = *reinterpret_cast<const half8 *>(yl + o);
     }
   };
   f32x16 acc[2] = {};
-  if (wave < steps) {
-    fetch(wave, 0);
-    fetch(wave, 1);
+  if (s0 + wave < s1) {
+    fetch(s0 + wave, 0);
+    fetch(s0 + wave, 1);
   }
-  for (int s = wave; s < steps; s += 4) {
+  for (int s = s0 + wave; s < s1; s += 4) {
     f32x16 sum[2] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -644,7 +682,7 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int t = 0; t < 2; ++t) sum[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[h][t][0][i], y[h][0][i], sum[t], 0, 0, 0);
-      if (s + 4 < steps) fetch(s + 4, h);
+      if (s + 4 < s1) fetch(s + 4, h);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) acc[t] += sum[t];
@@ -654,20 +692,22 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) part[wave][t * 16 + i][lane] = acc[t][i];
   __syncthreads();
-  // a wave finishes half of a 32 x 32 tile: accumulator element f is row 8 (f / 4) + 4 (lane / 32) + f % 4
+}
+// A wave finishes half of a 32 x 32 tile: accumulator element f is row 8 (f / 4) + 4 (lane / 32) + f % 4.
+// C = fl * sums + fe * E + fd * I of a symmetric result
+__device__ __forceinline__ void finish_half(const WaveSums &part, int ti, int tj, const Planes &C, float fl, bool has_e, const Planes &E, float fe, float fd, int n) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, np = C.np;
   const int t = wave >> 1, fi = 2 * ti + t, c = tj * 32 + (lane & 31);
   if (fi > tj) return;
-  const float fl = __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e);
-  const float fe = __builtin_ldexpf(j.beta, j.C.e - j.E.e), fd = __builtin_ldexpf(j.gamma, j.C.e);
   auto total = [&](int f, int l) { return (part[0][t * 16 + f][l] + part[1][t * 16 + f][l]) + (part[2][t * 16 + f][l] + part[3][t * 16 + f][l]); };
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const int f0 = 8 * (wave & 1) + 4 * p, r = fi * 32 + 2 * f0 + 4 * (lane >> 5);
     half4 eh = {}, el = {};
-    if (j.beta != 0.f) {                               // (E is symmetric: its mirror image is one vector)
+    if (has_e) {                                       // (E is symmetric: its mirror image is one vector)
       const int o = place(np, c, r);
-      eh = *reinterpret_cast<const half4 *>(j.E.hi + o);
-      el = *reinterpret_cast<const half4 *>(j.E.lo() + o);
+      eh = *reinterpret_cast<const half4 *>(E.hi + o);
+      el = *reinterpret_cast<const half4 *>(E.lo() + o);
     }
     f32x4 v;
 #pragma unroll
@@ -677,9 +717,61 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
         const int cc = lane & 31;
         sum = total((cc & 3) + 4 * (cc >> 3), (r + i & 31) + 32 * (cc >> 2 & 1));
       }
-      v[i] = fmaf(fl, sum, fmaf(fe, (float)eh[i] + (float)el[i], r + i == c && c < j.n ? fd : 0.f));
+      v[i] = fmaf(fl, sum, fmaf(fe, (float)eh[i] + (float)el[i], r + i == c && c < n ? fd : 0.f));
     }
-    store_planes4(j.C, r, c, fi == tj, v);
+    store_planes4(C, r, c, fi == tj, v);
+  }
+}
+
+__global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
+  __shared__ WaveSums part;
+  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
+  int q = 0;
+  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
+  const ChainJob &j = a.job[q];
+  int ti, tj;
+  half_tile(id - j.first, j.nt, ti, tj);
+  const int64_t np = j.C.np, x = ti * 64 * np, y = tj * 32 * np;
+  wave_products(j.L.hi + x, j.L.lo() + x, j.R.hi + y, j.R.lo() + y, 16 * np, 0, (int)(np / BK), part);
+  finish_half(part, ti, tj, j.C, __builtin_ldexpf(j.alpha, j.C.e - j.L.e - j.R.e), j.beta != 0.f, j.E,
+              __builtin_ldexpf(j.beta, j.C.e - j.E.e), __builtin_ldexpf(j.gamma, j.C.e), j.n);
+}
+
+// Gram matrix of the iterate between two phases by the same means: partial tiles as orth_gram_kernel gives them, or (ONE
+// slice each) A itself
+struct LinesGramJob {
+  Lines x;
+  Planes A;
+  float *part;
+  int32_t nt, slices, per, first;                      // per: steps of 64 lines a slice
+};
+struct LinesGramArgs {
+  LinesGramJob job[AGX_MAX_ORTH];
+  int n;
+};
+template <bool ONE>
+__global__ __launch_bounds__(256, 2) void orth_gram_lines_kernel(LinesGramArgs a) {
+  __shared__ WaveSums part;
+  const int id = agx::xcd_logical_id(blockIdx.x, gridDim.x);
+  int q = 0;
+  while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
+  const LinesGramJob &j = a.job[q];
+  const int tiles = j.nt * (j.nt + 1), slice = ONE ? 0 : (id - j.first) / tiles;
+  int ti, tj;
+  half_tile((id - j.first) % tiles, j.nt, ti, tj);
+  const int64_t rs = 16 * j.x.kp, x = 4 * ti * rs, y = 2 * tj * rs;
+  const int s0 = slice * j.per, s1 = min(s0 + j.per, (int)(j.x.kp / BK));
+  wave_products(j.x.hi + x, j.x.lo() + x, j.x.hi + y, j.x.lo() + y, rs, s0, s1, part);
+  if constexpr (ONE) {
+    finish_half(part, ti, tj, j.A, __builtin_ldexpf(1.f, j.A.e - 2 * j.x.e), false, j.A, 0.f, 0.f, 0);
+  } else {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = ti * j.nt - ti * (ti - 1) / 2 + tj / 2 - ti;
+    float *p = j.part + ((int64_t)tile * j.slices + slice) * T * T + (tj & 1) * 32 + (lane & 31);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int f = wave * 8 + i, e = f & 15;
+      p[((f >> 4) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * T] = (part[0][f][lane] + part[1][f][lane]) + (part[2][f][lane] + part[3][f][lane]);
+    }
   }
 }
 
@@ -935,8 +1027,10 @@ struct ApplyJob {
   const uint32_t *maxb;
   const double *invd;           // NULL: no divisor
   float decay, step;            // a Muon step: out <- decay * out - step * Y
-  int32_t rows, cols, tall, dtype, otype, e, nb, muon, first;
+  int32_t rows, cols, tall, dtype, otype, e, nb, muon, lines, first;   // lines: of X, up to where they are wanted
+  Lines from, to;               // the iterate instead of x / out where they are there
 };
+static_assert(sizeof(ApplyJob) * AGX_MAX_ORTH <= 4000, "kernel argument size");
 struct ApplyArgs {
   ApplyJob job[AGX_MAX_ORTH];
   int n, per;                   // per: groups of lines a workgroup (orth_panel_kernel)
@@ -947,7 +1041,7 @@ struct Factor {
   double f;
   float ff;
   bool plain;
-  __device__ __forceinline__ Factor(const ApplyJob &j, int e) : f(ldexp(j.invd ? *j.invd : ldexp(1.0, -e), -j.Q.e)), ff((float)f) {
+  __device__ __forceinline__ Factor(const ApplyJob &j, int e) : f(ldexp(j.invd ? *j.invd : ldexp(1.0, -e), (j.to.hi ? j.to.e : 0) - j.Q.e)), ff((float)f) {
     plain = __builtin_amdgcn_readfirstlane((fabsf(ff) >= 1.2e-38f && fabsf(ff) <= 1e38f) || f == 0.0);
   }
 };
@@ -977,7 +1071,7 @@ __device__ __forceinline__ void write_tile(const ApplyJob &j, const f32x16 &acc,
   else if (j.otype == AGX_F32) write_tile<float, false, INSIDE>(reinterpret_cast<float *>(j.out), j, acc, r0, c0);
   else write_tile<__bf16, false, INSIDE>(reinterpret_cast<__bf16 *>(j.out), j, acc, r0, c0);
 }
-__device__ __forceinline__ void finish_tile(const ApplyJob &j, const Factor &f, f32x16 acc, int r0, int c0) {
+__device__ __forceinline__ void multiply(f32x16 &acc, const Factor &f) {
   if (f.plain) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) acc[k] *= f.ff;
@@ -985,24 +1079,46 @@ __device__ __forceinline__ void finish_tile(const ApplyJob &j, const Factor &f, 
 #pragma unroll
     for (int k = 0; k < 16; ++k) acc[k] = (float)((double)acc[k] * f.f);
   }
+}
+// the same of lines l0.. and values c0.. into the iterate: four lines of a value are neighbours
+__device__ __forceinline__ void finish_lines(const ApplyJob &j, const Factor &f, f32x16 acc, int l0, int c0) {
+  const int lane = threadIdx.x & 63;
+  multiply(acc, f);
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    half4 h, l;
+    split4(f32x4{acc[4 * p], acc[4 * p + 1], acc[4 * p + 2], acc[4 * p + 3]}, h, l);
+    const int64_t o = j.to.at(c0 + (lane & 31), l0 + 8 * p + 4 * (lane >> 5));
+    *reinterpret_cast<half4 *>(j.to.hi + o) = h;
+    *reinterpret_cast<half4 *>(j.to.lo() + o) = l;
+  }
+}
+__device__ __forceinline__ void finish_tile(const ApplyJob &j, const Factor &f, f32x16 acc, int r0, int c0) {
+  multiply(acc, f);
   // (tiles inside the matrix, nearly all, without a condition per element: each would wait for what is in flight)
   if (r0 + 32 <= j.rows && c0 + 32 <= j.cols) write_tile<true>(j, acc, r0, c0);
   else write_tile<false>(j, acc, r0, c0);
 }
 
-template <typename E, bool TALL>
-__device__ __forceinline__ f32x16 apply_tile(const ApplyJob &j, int tr, int tc, int &e, uint32_t *red, _Float16 *lds) {
+// lines tl * 64.. by values tn * 64..: XQ with the lines as the result's rows, as a tall matrix and the iterate want it
+template <bool XQ, class L>
+__device__ __forceinline__ f32x16 apply_tile(const ApplyJob &j, L &lx, int tl, int tn, int &e, uint32_t *red, _Float16 *lds) {
   LoadPlanes lq(j.Q);
-  if constexpr (TALL) {
-    LoadK<E> lx;
-    lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.rows; lx.kmax = j.cols;
-    return tile_product(lx, lq, (int64_t)tr * T, (int64_t)tc * T, 0, j.Q.np, lds, false,
-                        [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
+  auto late = [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; };
+  if constexpr (XQ) return tile_product(lx, lq, (int64_t)tl * T, (int64_t)tn * T, 0, j.Q.np, lds, false, late);
+  else return tile_product(lq, lx, (int64_t)tn * T, (int64_t)tl * T, 0, j.Q.np, lds, false, late);
+}
+template <class L>
+__device__ __forceinline__ void apply_job(const ApplyJob &j, L lx, int tl, int tn, uint32_t *red, _Float16 *lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a = (wave >> 1) * 32, b = (wave & 1) * 32;
+  int e;
+  if (j.tall || j.to.hi) {
+    const f32x16 acc = apply_tile<true>(j, lx, tl, tn, e, red, lds);
+    if (j.to.hi) finish_lines(j, Factor(j, e), acc, tl * T + a, tn * T + b);
+    else finish_tile(j, Factor(j, e), acc, tl * T + a, tn * T + b);
   } else {
-    LoadT<E> lx;
-    lx.p = reinterpret_cast<const E *>(j.x); lx.ld = j.ldx; lx.rows = j.cols; lx.kmax = j.rows;
-    return tile_product(lq, lx, (int64_t)tr * T, (int64_t)tc * T, 0, j.Q.np, lds, false,
-                        [&] { lx.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
+    const f32x16 acc = apply_tile<false>(j, lx, tl, tn, e, red, lds);
+    finish_tile(j, Factor(j, e), acc, tn * T + a, tl * T + b);
   }
 }
 
@@ -1015,17 +1131,23 @@ __global__ __launch_bounds__(256, 4) void orth_apply_kernel(ApplyArgs a) {
   int q = 0;
   while (q + 1 < a.n && id >= a.job[q + 1].first) ++q;
   const ApplyJob &j = a.job[q];
-  const int trs = (j.rows + T - 1) / T, tcs = (j.cols + T - 1) / T, local = id - j.first;
-  const int tr = j.tall ? local / tcs : local % trs, tc = j.tall ? local % tcs : local / trs;
-  int e;
-  f32x16 acc;
-  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
-  if (is(0)) acc = apply_tile<float, true>(j, tr, tc, e, red, lds);
-  else if (is(1)) acc = apply_tile<float, false>(j, tr, tc, e, red, lds);
-  else if (is(2)) acc = apply_tile<__bf16, true>(j, tr, tc, e, red, lds);
-  else acc = apply_tile<__bf16, false>(j, tr, tc, e, red, lds);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  finish_tile(j, Factor(j, e), acc, tr * T + (wave >> 1) * 32, tc * T + (wave & 1) * 32);
+  const int tns = j.to.hi ? j.Q.np / T : ((j.tall ? j.cols : j.rows) + T - 1) / T, tl = (id - j.first) / tns, tn = (id - j.first) % tns;
+  if constexpr (KIND == ITERATE) {
+    LoadLines lx;
+    lx.x = &j.from;
+    apply_job(j, lx, tl, tn, red, lds);
+  } else {
+    auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
+    auto user = [&](auto lx) {
+      lx.p = reinterpret_cast<decltype(lx.p)>(j.x);
+      lx.ld = j.ldx; lx.rows = j.tall ? j.rows : j.cols; lx.kmax = j.tall ? j.cols : j.rows;
+      apply_job(j, lx, tl, tn, red, lds);
+    };
+    if (is(0)) user(LoadK<float>{});
+    else if (is(1)) user(LoadT<float>{});
+    else if (is(2)) user(LoadK<__bf16>{});
+    else user(LoadT<__bf16>{});
+  }
 }
 
 // The same for np <= PANEL_NP.  Its eight waves hold all of Q in registers (32 columns each, over all of k; at np = 128 and 64
@@ -1037,6 +1159,7 @@ constexpr int PANEL_NP = 256, PANEL_LDS = 2 * 2 * 128 * (64 + 8) * 2;    // (np 
 // a group's loads and LDS writes: 16 elements a thread, raw until they are stored
 template <typename E, bool TALL, int NP> struct PanelLines {
   static constexpr int GL = 8192 / NP, LD = NP + 8;    // (rows that start in 16 different bank groups)
+  static constexpr bool two = sizeof(E) == 4;
   using V = typename Vec4<E>::type;
   V v[4];
   // tall: four vectors along k; wide: four k's of four lines
@@ -1070,11 +1193,40 @@ template <typename E, bool TALL, int NP> struct PanelLines {
     }
   }
 };
-template <typename E, bool TALL, int NP>
-__device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int g1, uint32_t *red, _Float16 *lds) {
-  typedef PanelLines<E, TALL, NP> X;
+// the same from the iterate: blocks of four values of four lines
+template <int NP> struct PanelIterate {
+  static constexpr int GL = 8192 / NP, LD = NP + 8;
+  static constexpr bool two = true;
+  half4 vh[4], vl[4];                                  // [value][line]
+  static __device__ __forceinline__ int line() { return threadIdx.x % (GL / 4) * 4; }
+  static __device__ __forceinline__ int k() { return threadIdx.x / (GL / 4) * 4; }
+  __device__ __forceinline__ void fetch(const ApplyJob &j, int l0) {
+    const int l = l0 + line();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      vh[q] = vl[q] = half4{};
+      if (l < j.from.kp) {
+        const int64_t o = j.from.at(k() + q, l);
+        vh[q] = *reinterpret_cast<const half4 *>(j.from.hi + o);
+        vl[q] = *reinterpret_cast<const half4 *>(j.from.lo() + o);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(_Float16 *hi, _Float16 *lo, int) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int o = (line() + q) * LD + k();
+      *reinterpret_cast<half4 *>(hi + o) = half4{vh[0][q], vh[1][q], vh[2][q], vh[3][q]};
+      *reinterpret_cast<half4 *>(lo + o) = half4{vl[0][q], vl[1][q], vl[2][q], vl[3][q]};
+    }
+  }
+};
+// XQ: as in apply_tile
+template <class X, int NP, bool XQ>
+__device__ __forceinline__ void panel_groups(const ApplyJob &j, int per, uint32_t *red, _Float16 *lds) {
   constexpr int CG = NP / 32, NB = NP / 32, PLANE = X::GL * X::LD;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cg = wave % CG, rg = wave / CG;
+  const int g0 = ((int)blockIdx.x - j.first) * per, g1 = min(g0 + per, (j.lines + X::GL - 1) / X::GL);
   X x;
   x.fetch(j, g0 * X::GL);
   // (k runs in an order of its own, the same for both operands: a lane's two vectors of a block are neighbours in memory)
@@ -1100,15 +1252,15 @@ __device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int g1, u
     for (int s = 0; s < NB; s += 2) {                  // (steps of 64 k, as in tile_product)
       f32x16 sum = {};
       auto mul = [&](half8 xv, half8 qv) {
-        sum = TALL ? __builtin_amdgcn_mfma_f32_32x32x16_f16(xv, qv, sum, 0, 0, 0)
-                   : __builtin_amdgcn_mfma_f32_32x32x16_f16(qv, xv, sum, 0, 0, 0);
+        sum = XQ ? __builtin_amdgcn_mfma_f32_32x32x16_f16(xv, qv, sum, 0, 0, 0)
+                 : __builtin_amdgcn_mfma_f32_32x32x16_f16(qv, xv, sum, 0, 0, 0);
       };
 #pragma unroll
       for (int b = s; b < s + 2; ++b) {
         const half8 x0 = at(b * 32), x1 = at(b * 32 + 8);
         mul(x0, ql[b][0]);
         mul(x1, ql[b][1]);
-        if (sizeof(E) == 4) {
+        if (X::two) {
           mul(at(PLANE + b * 32), qh[b][0]);
           mul(at(PLANE + b * 32 + 8), qh[b][1]);
         }
@@ -1118,31 +1270,49 @@ __device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int g1, u
       acc += sum;
       asm volatile("" : "+v"(acc));                    // (put off to the epilogue, the sums would not fit the registers)
     }
-    const int l = g * X::GL + rg * 32;
-    if (l < (TALL ? j.rows : j.cols) && cg * 32 < (TALL ? j.cols : j.rows)) finish_tile(j, f, acc, TALL ? l : cg * 32, TALL ? cg * 32 : l);
+    const int l = g * X::GL + rg * 32, c = cg * 32;
+    if (l < j.lines) {
+      if (XQ && j.to.hi) finish_lines(j, f, acc, l, c);
+      else if (c < (XQ ? j.cols : j.rows)) finish_tile(j, f, acc, XQ ? l : c, XQ ? c : l);
+    }
     if (g + 1 < g1) x.store(lds + (buf ^ 1) * 2 * PLANE, lds + (buf ^ 1) * 2 * PLANE + PLANE, e);
   }
 }
-template <typename E, bool TALL>
-__device__ __forceinline__ void panel_lines(const ApplyJob &j, int g0, int per, uint32_t *red, _Float16 *lds) {
-  const int lines = TALL ? j.rows : j.cols, g1 = min(g0 + per, (lines + 8192 / j.Q.np - 1) / (8192 / j.Q.np));
-  if (j.Q.np == 64) panel_lines<E, TALL, 64>(j, g0, g1, red, lds);
-  else if (j.Q.np == 128) panel_lines<E, TALL, 128>(j, g0, g1, red, lds);
-  else panel_lines<E, TALL, 256>(j, g0, g1, red, lds);
+template <class F, int NP>
+__device__ __forceinline__ void panel_order(const ApplyJob &j, int per, uint32_t *red, _Float16 *lds) {
+  if (F::tall || j.tall || j.to.hi) panel_groups<typename F::template X<NP>, NP, true>(j, per, red, lds);
+  else if constexpr (!F::tall) panel_groups<typename F::template X<NP>, NP, false>(j, per, red, lds);
 }
+template <class F>
+__device__ __forceinline__ void panel_job(const ApplyJob &j, int per, uint32_t *red, _Float16 *lds) {
+  if (j.Q.np == 64) panel_order<F, 64>(j, per, red, lds);
+  else if (j.Q.np == 128) panel_order<F, 128>(j, per, red, lds);
+  else panel_order<F, 256>(j, per, red, lds);
+}
+template <typename E, bool TALL> struct FromUser {
+  static constexpr bool tall = TALL;
+  template <int NP> using X = PanelLines<E, TALL, NP>;
+};
+struct FromIterate {
+  static constexpr bool tall = false;                  // (either, see panel_order)
+  template <int NP> using X = PanelIterate<NP>;
+};
 template <int KIND>
 __global__ __launch_bounds__(512, 2) void orth_panel_kernel(ApplyArgs a) {
   extern __shared__ _Float16 lds[];
   __shared__ uint32_t red[8];
   int q = 0;
   while (q + 1 < a.n && (int)blockIdx.x >= a.job[q + 1].first) ++q;
-  const ApplyJob &j = a.job[q];
-  const int g0 = ((int)blockIdx.x - j.first) * a.per;
-  auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
-  if (is(0)) panel_lines<float, true>(j, g0, a.per, red, lds);
-  else if (is(1)) panel_lines<float, false>(j, g0, a.per, red, lds);
-  else if (is(2)) panel_lines<__bf16, true>(j, g0, a.per, red, lds);
-  else panel_lines<__bf16, false>(j, g0, a.per, red, lds);
+  const ApplyJob j = a.job[q];                         // (by value: a reference into the arguments would go through scratch)
+  if constexpr (KIND == ITERATE) {
+    panel_job<FromIterate>(j, a.per, red, lds);
+  } else {
+    auto is = [&](int kind) { return KIND == ANY ? is_kind(kind, j.tall, j.dtype) : KIND == kind; };
+    if (is(0)) panel_job<FromUser<float, true>>(j, a.per, red, lds);
+    else if (is(1)) panel_job<FromUser<float, false>>(j, a.per, red, lds);
+    else if (is(2)) panel_job<FromUser<__bf16, true>>(j, a.per, red, lds);
+    else panel_job<FromUser<__bf16, false>>(j, a.per, red, lds);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1162,6 +1332,7 @@ struct Job {          // one matrix of a call
   bool tall() const { return rows > cols || (rows == cols && !square_wide); }
   int n() const { return std::min(rows, cols); }
   int64_t K() const { return std::max(rows, cols); }
+  int64_t kp() const { return (K() + BK - 1) / BK * BK; }
   int np() const { return n() <= T ? T : n() <= 2 * T ? 2 * T : n() <= STEP_NP ? STEP_NP : agx::cdiv(n(), T) * T; }
   int nt() const { return agx::cdiv(n(), T); }                   // tiles along the small side that hold anything
   int tiles() const { return nt() * (nt() + 1) / 2; }
@@ -1185,6 +1356,7 @@ template <class F> void by_kind(int kind, F f) {
     case 1: f(std::integral_constant<int, 1>{}); break;
     case 2: f(std::integral_constant<int, 2>{}); break;
     case 3: f(std::integral_constant<int, 3>{}); break;
+    case ITERATE: f(std::integral_constant<int, ITERATE>{}); break;
     default: f(std::integral_constant<int, ANY>{});
   }
 }
@@ -1212,7 +1384,7 @@ void plan(const Job &j, int total_tiles, int64_t most_steps, int phases, bool ne
   l.invd = take(8);
   for (int64_t &m : l.mat) m = take((int64_t)j.np() * j.np() * 4);
   l.part = take((int64_t)tiles * l.slices * T * T * 4);
-  for (int k = 0; k < 2; ++k) l.x[k] = phases > 1 + k ? take((int64_t)j.rows * j.cols * 4) : 0;
+  for (int k = 0; k < 2; ++k) l.x[k] = phases > 1 + k ? take(j.np() * j.kp() * 4) : 0;
   l.u = need_u ? take((int64_t)j.rows * j.cols * 4) : 0;
   l.end = off;
 }
@@ -1342,9 +1514,6 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     hipLaunchKernelGGL(orth_prep_kernel, dim3(gx, n), dim3(256), 0, st, pa);
     AGX_LAUNCH_CHECK();
   }
-  const void *x[AGX_MAX_ORTH];
-  int64_t ldx[AGX_MAX_ORTH];
-  for (int i = 0; i < n; ++i) { x[i] = jobs[i].x; ldx[i] = jobs[i].ldx; }
   auto planes = [&](int i, int k, int e) {
     Planes p;
     p.hi = reinterpret_cast<_Float16 *>(base[i] + lay[i].mat[k]);
@@ -1364,7 +1533,21 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
   for (int ph = 0, k = 0; ph < phases; ++ph) {
     const bool first = ph == 0, last = ph == phases - 1;
     const int ex = exponent_for(s);                 // scale of the iterate (later phases)
-    {
+    auto iterate = [&](int phase_number, int i, int e) {             // what that phase leaves
+      Lines l;
+      l.hi = reinterpret_cast<_Float16 *>(base[i] + lay[i].x[phase_number & 1]);
+      l.kp = jobs[i].kp();
+      l.e = e;
+      l.np = jobs[i].np();
+      return l;
+    };
+    auto add_slices = [&](ReduceArgs &ra, int blocks, int pieces) -> int {
+      if (pieces == 8) hipLaunchKernelGGL(orth_reduce_kernel<4>, dim3(blocks), dim3(reduce_threads<4>()), 0, st, ra);
+      else hipLaunchKernelGGL(orth_reduce_kernel<32>, dim3(blocks), dim3(reduce_threads<32>()), 0, st, ra);
+      AGX_LAUNCH_CHECK();
+      return AGX_OK;
+    };
+    if (first) {
       GramArgs ga;
       ReduceArgs ra;
       ga.n = ra.n = n;
@@ -1378,8 +1561,8 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         const Layout &l = lay[i];
         const int nt = one ? j.np() / T : j.nt();
         GramJob &g = ga.job[i];
-        g.x = x[i]; g.ld = ldx[i]; g.K = j.K(); g.kper = l.kper; g.n = j.n(); g.nt = nt; g.slices = l.slices; g.tall = j.tall();
-        g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
+        g.x = j.x; g.ld = j.ldx; g.K = j.K(); g.kper = l.kper; g.n = j.n(); g.nt = nt; g.slices = l.slices; g.tall = j.tall();
+        g.dtype = j.dtype; g.nb = nb[i];
         g.maxb = reinterpret_cast<const uint32_t *>(base[i] + l.maxb);
         g.part = reinterpret_cast<float *>(base[i] + l.part);
         g.squares = reinterpret_cast<const double *>(base[i] + l.squares);
@@ -1390,8 +1573,8 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         kind = joined_kind(kind, g.tall, g.dtype);
         ReduceJob &r = ra.job[i];
         r.part = g.part; r.squares = g.squares; r.maxb = g.maxb; r.invd = g.invd;
-        r.A = g.A; r.nt = nt; r.slices = l.slices; r.e = ex; r.nb = nb[i];
-        r.normalise = first; r.first = rb;
+        r.A = g.A; r.nt = nt; r.slices = l.slices; r.e = 0; r.nb = nb[i];
+        r.normalise = true; r.first = rb;
         rb += j.np() / 32 * (j.np() / 32 + 1) / 2 * pieces;
       }
       by_kind(kind, [&](auto k) {
@@ -1399,10 +1582,42 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         else hipLaunchKernelGGL((orth_gram_kernel<decltype(k)::value, false>), dim3(gb), dim3(256), 0, st, ga);
       });
       AGX_LAUNCH_CHECK();
-      if (one) {}
-      else if (pieces == 8) hipLaunchKernelGGL(orth_reduce_kernel<4>, dim3(rb), dim3(reduce_threads<4>()), 0, st, ra);
-      else hipLaunchKernelGGL(orth_reduce_kernel<32>, dim3(rb), dim3(reduce_threads<32>()), 0, st, ra);
+      if (!one) AGX_TRY(add_slices(ra, rb, pieces));
+    } else {
+      LinesGramArgs ga;
+      ReduceArgs ra;
+      memset(&ga, 0, sizeof(ga));
+      memset(&ra, 0, sizeof(ra));
+      ga.n = ra.n = n;
+      int gb = 0, rb = 0, most = 0;
+      for (int i = 0; i < n; ++i) {
+        const int steps_i = (int)(jobs[i].kp() / BK), want = std::max(1, agx::num_cus() * LINES_BLOCKS / std::max(1, 2 * tiles));
+        // (four steps at least, one a wave; no more slices than the first phase had room for)
+        const int per = longest(jobs, n) <= ONE_SLICE_LINES ? steps_i
+                                                           : std::max({std::min(steps_i, 4), agx::cdiv(steps_i, want), agx::cdiv(steps_i, lay[i].slices)});
+        ga.job[i].per = per;
+        ga.job[i].slices = agx::cdiv(steps_i, per);
+        most = std::max(most, ga.job[i].slices);
+      }
+      const bool one = most == 1;
+      const int pieces = most > FEW_SLICES ? 8 : 1;
+      for (int i = 0; i < n; ++i) {
+        const Job &j = jobs[i];
+        LinesGramJob &g = ga.job[i];
+        g.x = iterate(ph - 1, i, ex);
+        g.A = planes(i, 0, exponent_for(s * s));
+        g.part = reinterpret_cast<float *>(base[i] + lay[i].part);
+        g.nt = one ? j.np() / T : j.nt();
+        g.first = gb;
+        gb += g.nt * (g.nt + 1) * g.slices;
+        ReduceJob &r = ra.job[i];
+        r.part = g.part; r.A = g.A; r.nt = g.nt; r.slices = g.slices; r.e = ex; r.first = rb;
+        rb += j.np() / 32 * (j.np() / 32 + 1) / 2 * pieces;
+      }
+      if (one) hipLaunchKernelGGL(orth_gram_lines_kernel<true>, dim3(gb), dim3(256), 0, st, ga);
+      else hipLaunchKernelGGL(orth_gram_lines_kernel<false>, dim3(gb), dim3(256), 0, st, ga);
       AGX_LAUNCH_CHECK();
+      if (!one) AGX_TRY(add_slices(ra, rb, pieces));
     }
     // matrices: 0 A, 1 P, 2 A P, 3 / 4 Q (which of the two: 3 after an odd number of steps); a launch a step: 0 / 1 A
     const int steps = std::min(phase, o->steps - k);
@@ -1500,7 +1715,8 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       ApplyArgs aa;
       aa.n = 0;
       int blocks = 0, kind = -1, groups = 0;
-      auto groups_of = [](const Job &j) { return (int)agx::cdiv64(j.K(), 8192 / j.np()); };
+      auto lines_of = [&](const Job &j) { return (int)(last ? j.K() : j.kp()); };
+      auto groups_of = [&](const Job &j) { return agx::cdiv(lines_of(j), 8192 / j.np()); };
       for (int i = 0; i < n; ++i) groups += panel && jobs[i].np() <= PANEL_NP ? groups_of(jobs[i]) : 0;
       aa.per = agx::cdiv(groups, agx::num_cus());
       for (int i = 0; i < n; ++i) {
@@ -1508,21 +1724,20 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         if ((j.np() <= PANEL_NP) != panel) continue;
         ApplyJob &g = aa.job[aa.n++];
         memset(&g, 0, sizeof(g));
-        g.x = x[i]; g.ldx = ldx[i]; g.Q = planes(i, iq, eQ[steps - 1]);
+        g.x = j.x; g.ldx = j.ldx; g.Q = planes(i, iq, eQ[steps - 1]); g.lines = lines_of(j);
         g.maxb = reinterpret_cast<const uint32_t *>(base[i] + lay[i].maxb);
         g.invd = first ? reinterpret_cast<const double *>(base[i] + lay[i].invd) : nullptr;
         g.rows = j.rows; g.cols = j.cols; g.tall = j.tall();
-        g.dtype = first ? j.dtype : AGX_F32; g.e = ex; g.nb = first ? nb[i] : 0;
+        g.dtype = j.dtype; g.e = ex; g.nb = first ? nb[i] : 0;
+        if (!first) g.from = iterate(ph - 1, i, ex);
         if (last) {
           g.out = j.out; g.ldo = j.ldo; g.otype = j.dtype; g.muon = j.muon; g.decay = j.decay; g.step = j.step;
         } else {
-          g.out = base[i] + lay[i].x[ph & 1]; g.ldo = j.cols; g.otype = AGX_F32;
-          x[i] = g.out;
-          ldx[i] = g.ldo;
+          g.to = iterate(ph, i, exponent_for(s));
         }
-        kind = joined_kind(kind, g.tall, g.dtype);
+        kind = first ? joined_kind(kind, g.tall, g.dtype) : ITERATE;
         g.first = blocks;
-        blocks += panel ? agx::cdiv(groups_of(j), aa.per) : agx::cdiv(j.rows, T) * agx::cdiv(j.cols, T);
+        blocks += panel ? agx::cdiv(groups_of(j), aa.per) : agx::cdiv(g.lines, T) * (last ? j.nt() : j.np() / T);
       }
       if (!blocks) return AGX_OK;
       by_kind(kind, [&](auto k) {
@@ -1577,7 +1792,7 @@ int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, co
 
 // (more LDS than the default limit of a launch)
 int agx::orth_prepare_device() {
-  for (int k = 0; k <= ANY; ++k) {
+  for (int k = 0; k <= ITERATE; ++k) {
     const void *f = nullptr;
     by_kind(k, [&](auto kind) { f = reinterpret_cast<const void *>(&orth_panel_kernel<decltype(kind)::value>); });
     AGX_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, PANEL_LDS));
