@@ -16,7 +16,7 @@
 // Launches of a call: the momentum step with |x|'s maximum and norm; then, a phase each, the Gram matrix (and the sum of its
 // slices), its polynomial (n <= 128 one launch a phase, n <= 256 one a step, above three a step) and the product with the
 // long side, which in the last phase is the Muon update of w too.  Floors: 2.4 us a launch, 5 TB/s of HBM, 1150 TFLOP/s of
-// fp16 products over three.  Measured: 256 x 256 91 us (12 launches), 18161 x 256 151 us (15), 1000 x 4297 bf16 379 us
+// fp16 products over three.  Measured: 256 x 256 88 us (12 launches), 18161 x 256 147 us (15), 1000 x 4297 bf16 358 us
 // (20; its products take 73 us at that rate).
 #include "agx_common.h"
 
@@ -40,7 +40,7 @@ constexpr int MAXB = 1024;                     // partial maxima of one matrix
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
 constexpr int TALL_BLOCKS = 2, WIDE_BLOCKS = 4;    // workgroups a CU of a Gram product
 constexpr int ONE_SLICE = 4;                   // longest K, in steps of 64 (1.5 us each), that is not split over workgroups
-constexpr int LINES_BLOCKS = 3, ONE_SLICE_LINES = 16;   // the same of the iterate's Gram product
+constexpr int LINES_BLOCKS = 2, ONE_SLICE_LINES = 16;   // the same of the iterate's Gram product (see run)
 constexpr int FEW_SLICES = 16;                 // see orth_reduce_kernel
 constexpr int TARGET = 14;                     // scaled entries are below 2^TARGET
 
@@ -738,7 +738,8 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
 }
 
 // Gram matrix of the iterate between two phases by the same means: partial tiles as orth_gram_kernel gives them, or (ONE
-// slice each) A itself
+// slice each) A itself.  18161 x 256 11 us (through LDS, from fp32 lines that every tile splits anew: 15), 1000 x 4297 30 (44),
+// 256 x 256 5.2 (9).
 struct LinesGramJob {
   Lines x;
   Planes A;
@@ -1592,7 +1593,9 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
       int gb = 0, rb = 0, most = 0;
       for (int i = 0; i < n; ++i) {
         const int steps_i = (int)(jobs[i].kp() / BK), want = std::max(1, agx::num_cus() * LINES_BLOCKS / std::max(1, 2 * tiles));
-        // (four steps at least, one a wave; no more slices than the first phase had room for)
+        // (four steps at least, one a wave; no more slices than the first phase had room for.  Two workgroups a CU, as many as
+        //  fit it: 18161 x 256 1, 2, 3, 4 of them 146, 147, 150, 152 us, GTEx generator's Muon step 181, 168, 173, 169.  Up to
+        //  16 steps in one slice: 1024 x 1024 256 us, with slices 263; up to 32 makes no difference at 640 x 2000.)
         const int per = longest(jobs, n) <= ONE_SLICE_LINES ? steps_i
                                                            : std::max({std::min(steps_i, 4), agx::cdiv(steps_i, want), agx::cdiv(steps_i, lay[i].slices)});
         ga.job[i].per = per;
