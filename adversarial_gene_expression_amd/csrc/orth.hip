@@ -36,7 +36,7 @@ typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int T = 64;                          // n x n matrices are padded to T, 2 T, 4 T or a multiple of T above
 constexpr int PHASE = 3;                       // most steps between two Gram matrices
-constexpr int MAXB = 1024;                     // partial maxima of one matrix
+constexpr int MAXB = 1024;                     // workgroups of a matrix's first launch, each with its share of maximum and squares
 constexpr int ROWS_PHASE = 128;                // largest padded side for a phase in one launch
 constexpr int TALL_BLOCKS = 2, WIDE_BLOCKS = 4;    // workgroups a CU of a Gram product
 constexpr int ONE_SLICE = 4;                   // longest K, in steps of 64 (1.5 us each), that is not split over workgroups
@@ -211,7 +211,10 @@ __device__ __forceinline__ double normaliser(const double *squares, int nb, floa
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// tile product: operands in LDS as [64 rows][64 k] fp16 planes
+// tile product: operands in LDS as [64 rows][64 k] fp16 planes (the first Gram product, and for n > 256 the product with the
+// long side).  K in steps of 64 through one buffer, the next step's global loads in flight: four workgroups of a CU overlap
+// each other's loads, conversions and products.  (Two or four steps in flight: fewer workgroups, 18161 x 256 157 us became
+// 172; tiles of 128 x 128 with two buffers leave one workgroup a CU, whose phases nothing covers: 166 where this took 158.)
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int BK = 64, LDK = BK + 8, PL = T * LDK;   // k of a step; LDS rows of 144 bytes (16 of them start in 16 different bank
                                                      // groups); halves of a plane
@@ -404,16 +407,16 @@ __device__ __forceinline__ void each_element(const f32x16 &acc, Fn f) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Gram matrix of the long side, K split over workgroups: partial tiles [tile][slice][64][64] of the scaled matrix
+// Gram matrix of the caller's matrix, K split over workgroups: partial tiles [tile][slice][64][64] of the scaled matrix
 // ---------------------------------------------------------------------------------------------------------------------
 struct GramJob {
   const void *x;
   int64_t ld, K, kper;          // K: long side; kper: k of one slice (a multiple of BK)
   int32_t n, nt, slices, tall;  // n: small side, nt: tiles along it; tall: element (i, k) at x[k * ld + i]
-  int32_t dtype, e, nb;         // e: scale exponent where nb == 0, otherwise from the partial maxima
+  int32_t dtype, nb;            // nb: shares of the maximum (the scale's) and of the sum of squares
   const uint32_t *maxb;
   float *part;
-  const double *squares;        // (one slice) as in ReduceJob
+  const double *squares;        // this, invd and A: for one slice, as in ReduceJob
   double *invd;
   Planes A;
   int32_t first;                // first workgroup of the job
@@ -431,7 +434,7 @@ __device__ __forceinline__ f32x16 gram_tile(const GramJob &j, int ti, int tj, in
   la.ld = j.ld; la.rows = j.n; la.kmax = j.K;
   lb.p = la.p; lb.ld = la.ld; lb.rows = la.rows; lb.kmax = la.kmax;
   return tile_product(la, lb, (int64_t)ti * T, (int64_t)tj * T, k0, k1, lds, ti == tj,
-                      [&] { la.e = lb.e = e = j.nb ? scale_exponent(j.maxb, j.nb, red) : j.e; });
+                      [&] { la.e = lb.e = e = scale_exponent(j.maxb, j.nb, red); });
 }
 
 // Symmetric results are made symmetric to the last bit, from what is on and above the diagonal: products of matrices that are
@@ -508,12 +511,8 @@ __global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
     each_element(acc, [&](int r, int c, float v) { p[r * T + c] = v; });
   } else {
     __shared__ double sums[4];
-    double f = ldexp(1.0, j.A.e - 2 * e);
-    if (j.nb) {
-      const double inv = normaliser(j.squares, j.nb, a.eps, e, sums);
-      f = ldexp(inv * inv, j.A.e);
-      if (tile == 0 && threadIdx.x == 0) *j.invd = inv;
-    }
+    const double inv = normaliser(j.squares, j.nb, a.eps, e, sums), f = ldexp(inv * inv, j.A.e);
+    if (tile == 0 && threadIdx.x == 0) *j.invd = inv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fi = 2 * ti + (wave >> 1), fj = 2 * tj + (wave & 1);
     if (fi > fj) return;
     float v[16];
