@@ -245,6 +245,7 @@ SIGNATURES = {
     'agx_bn_backward': (C.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _f32, _i32, _i32, _vp, _vp]),
     'agx_bn_moving_update': (C.c_int, [_vp, _vp, _vp, _vp, _vp, _f32, _i32]),
     'agx_layernorm_ws_floats': (_i64, [_i64, _i64, _i32]),
+    'agx_layernorm_bwd_ws_floats': (_i64, [_i64, _i64, _i32]),
     'agx_layernorm_fwd': (C.c_int, [_vp, C.POINTER(NormDesc)]),
     'agx_layernorm_bwd': (C.c_int, [_vp, C.POINTER(NormDesc)]),
     'agx_layernorm_bwd2': (C.c_int, [_vp, C.POINTER(NormDesc)]),

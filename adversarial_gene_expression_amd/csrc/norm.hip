@@ -18,7 +18,8 @@
 // 16.6 us (4.2); backward with parameter gradients 40000 x 1000 bf16 66 us (4.8); second order 8192 x 1077 44 us (4.8).  Small
 // calls are the host's: 32 x 256 11 us, of which the GPU works 3.4.
 // Parameter gradients: every thread owns fixed columns, sums its rows in registers, the groups of a workgroup meet in
-// LDS, and a second launch adds the workgroups' partial rows in a fixed order (no atomics: bit-reproducible).
+// LDS, and a second launch adds the workgroups' partial rows in a fixed order (no atomics: bit-reproducible).  A backward pass
+// of few rows is one launch instead, with workgroups of columns beside those of rows: 1536 x 256 5.7 us of the GPU's instead of 7.6.
 #include "agx_common.h"
 
 #include <algorithm>
@@ -262,11 +263,11 @@ struct Inputs {
   }
 };
 
+// the rows of workgroup `block` of `blocks`; lds: lds_floats<T, G, C>() where PG
 template <typename T, int G, int C, bool PG>
-__global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) {
+__device__ __forceinline__ void back_rows(const NormArgs &a, int block, int blocks, float *lds) {
   constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
   __shared__ float red[G > 64 ? 2 * 2 * (G / 64) : 1];
-  __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
   int flip = 0;
   const Place<T, G, C> w(a.n);
   const int grp = threadIdx.x / G;
@@ -276,8 +277,8 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) 
   // (rows of one wave: the next one's loads are on their way while a row is worked on - 40000 x 1000 bf16 66 us instead of 68,
   //  20000 x 600 35 instead of 37 - where its registers do not cost a workgroup: 20000 x 2000 bf16 79 us without, 88 with)
   constexpr bool AHEAD = G <= 64 && C * V <= 16;
-  const int64_t step = (int64_t)gridDim.x * NG;
-  int64_t row = (int64_t)blockIdx.x * NG + grp;
+  const int64_t step = (int64_t)blocks * NG;
+  int64_t row = (int64_t)block * NG + grp;
   Inputs<T, G, C> in;
   if (AHEAD && row < a.rows) in.load(a, w, row);
   for (; row < a.rows; row += step) {
@@ -344,6 +345,83 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) 
     }
   }
   if constexpr (PG) write_partials<T, G, C, 2>(acc, aend, w, a, lds);
+}
+template <typename T, int G, int C, bool PG>
+__global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) {
+  __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
+  back_rows<T, G, C, PG>(a, blockIdx.x, gridDim.x, lds);
+}
+
+// Parameter gradients of V columns over all rows, by one workgroup of 256: with the statistics given they need no sum over a
+// row.  A thread has every 256th row, U of them in flight (6: 512 x 256 4.1 us instead of 3.7); the threads meet in LDS in a
+// fixed order.  Neighbouring strips are given to one XCD, which then fetches a line once for all of them: 1536 x 256 5.7 us, 12.8
+// without.
+template <typename T>
+__device__ __forceinline__ void column_sums(const NormArgs &a, int strip, float *dgamma, float *dbeta, int accumulate, float *lds) {
+  constexpr int V = Vec<T>::V, Q = 2 * V, LD = Q + 1, P = 256 / Q, U = 4;
+  using VT = typename Vec<T>::type;
+  const int64_t c0 = (int64_t)strip * V;
+  const int left = (int)min((int64_t)V, a.n - c0);
+  auto get = [&](const void *m, int64_t at) {
+    const T *p = reinterpret_cast<const T *>(m) + at + c0;
+    if (left == V) return *reinterpret_cast<const VT *>(p);
+    VT v = {};
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < left) v[k] = p[k];
+    return v;
+  };
+  float s[Q] = {};
+  for (int64_t row0 = threadIdx.x; row0 < a.rows; row0 += 256 * U) {
+    VT x[U], dy[U], m[U];
+    float mu[U], r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t row = min(row0 + 256 * i, a.rows - 1);
+      x[i] = get(a.x, row * a.ldx);
+      dy[i] = get(a.dy, row * a.lddy);
+      if (a.ym) m[i] = get(a.ym, row * a.ldym);
+      mu[i] = a.mean_in[row];
+      r[i] = a.rstd_in[row];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint32_t neg = a.ym ? not_positive<T>(m[i]) : 0u;
+      if (row0 + 256 * i < a.rows)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = neg >> k & 1 ? a.slope * (float)dy[i][k] : (float)dy[i][k];
+          s[k] += d * (((float)x[i][k] - mu[i]) * r[i]);
+          s[V + k] += d;
+        }
+    }
+  }
+  const int t = threadIdx.x, q = t % Q, part = t / Q;
+#pragma unroll
+  for (int k = 0; k < Q; ++k) lds[t * LD + k] = s[k];
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < Q; ++i) sum += lds[(part * Q + i) * LD + q];
+  __syncthreads();
+  lds[part * LD + q] = sum;
+  __syncthreads();
+  float *out = q < V ? dgamma : dbeta;
+  if (part == 0 && out && q % V < left) {
+    out += c0 + q % V;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) sum += lds[i * LD + q];
+    *out = accumulate ? *out + sum : sum;              // (what is there is added last: one rounding against it)
+  }
+}
+template <typename T> constexpr int strip_floats() { return 256 * (2 * Vec<T>::V + 1); }
+// the whole backward pass in one launch: the first `strips` workgroups are columns', the others rows'
+template <typename T, int G, int C>
+__global__ __launch_bounds__(256) void ln_bwd_small_kernel(NormArgs a, int strips, float *dgamma, float *dbeta, int accumulate) {
+  __shared__ float lds[strip_floats<T>()];
+  if ((int)blockIdx.x < strips) column_sums<T>(a, agx::xcd_logical_id(blockIdx.x, strips), dgamma, dbeta, accumulate, lds);
+  else back_rows<T, G, C, false>(a, blockIdx.x - strips, gridDim.x - strips, lds);
 }
 
 template <typename T, int G, int C, bool PG>
@@ -557,10 +635,10 @@ __global__ __launch_bounds__(1024) void ln_param_kernel(const float *__restrict_
   red[sh][col] = s;
   __syncthreads();
   if (sh == 0 && j < n) {
-    s = accumulate ? out[j] : 0.f;
+    s = 0.f;
 #pragma unroll
     for (int k = 0; k < 32; ++k) s += red[k][col];
-    out[j] = s;
+    out[j] = accumulate ? out[j] + s : s;
   }
 }
 
@@ -611,25 +689,57 @@ int blocks_of(int64_t rows, const Cfg &c, bool params) {
   return (int)std::min<int64_t>(agx::cdiv64(rows, ng), (int64_t)agx::num_cus() * (params ? PARAM_BLOCKS : 16));
 }
 
+// calls f with a configuration's G and C as constants; false: the wide kernels' rows
+template <class F> bool by_cfg(const Cfg &c, F f) {
+  auto by_c = [&](auto g) {
+    if (c.c == 1) f(g, std::integral_constant<int, 1>{});
+    else if (c.c == 2) f(g, std::integral_constant<int, 2>{});
+    else if (c.c == 3) f(g, std::integral_constant<int, 3>{});
+    else f(g, std::integral_constant<int, 4>{});
+  };
+  if (c.g == 16) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+  else if (c.g == 64) by_c(std::integral_constant<int, 64>{});
+  else if (c.g == 256) by_c(std::integral_constant<int, 256>{});
+  else if (c.g == 1024) by_c(std::integral_constant<int, 1024>{});
+  return c.g != 0;
+}
+
+// The backward pass with parameter gradients in one launch (ln_bwd_small_kernel) instead of two, up to SMALL_ROWS rows and
+// SMALL_VECTORS whole vectors a matrix.  GPU time of two launches and one, us: 16 x 256 5.1, 3.2; 512 x 256 6.4, 3.7; 1536 x 256 7.6,
+// 5.7; 2048 x 600 9.9, 11.7; 512 x 4000 16.0, 14.8; 1024 x 4000 21.4, 25.4; 512 x 4297 bf16 22.5, 13.1.  (The host's second
+// launch costs 3.4 us more.)
+constexpr int SMALL_ROWS = 1536, SMALL_VECTORS = 1 << 19;
+bool small_shape(int64_t rows, int64_t width, int v) {
+  const int g = pick(width, v).g;
+  return rows > 0 && rows <= SMALL_ROWS && rows * (width / v) <= SMALL_VECTORS && g != 0 && g <= 256;
+}
+bool small_back(const NormArgs &a, const float *dgamma, const float *dbeta, int v) {
+  // (not where dx is written over what the columns' workgroups still read)
+  const bool over = a.dx && (a.dx == a.x || a.dx == a.dy || a.dx == a.ym);
+  return (dgamma || dbeta) && !over && small_shape(a.rows, a.n, v);
+}
+
 template <int OP, typename T>
 int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int accumulate) {
   const Cfg c = pick(a.n, Vec<T>::V);
+  if constexpr (OP == BWD)
+    if (small_back(a, dgamma, dbeta, Vec<T>::V)) {
+      const int strips = (int)agx::cdiv64(a.n, Vec<T>::V), rows = a.dx ? blocks_of(a.rows, c, false) : 0;
+      by_cfg(c, [&](auto g, auto n) {
+        if constexpr (decltype(g)::value <= 256)
+          hipLaunchKernelGGL((ln_bwd_small_kernel<T, decltype(g)::value, decltype(n)::value>), dim3(strips + rows), dim3(256), 0, st, a,
+                             strips, dgamma, dbeta, accumulate);
+      });
+      AGX_LAUNCH_CHECK();
+      return AGX_OK;
+    }
   int blocks = blocks_of(a.rows, c, a.part != nullptr);
   if (blocks > 0) {
-    auto by_c = [&](auto g) {
-      constexpr int G = decltype(g)::value;
-      if (c.c == 1) launch_cfg<OP, T, G, 1>(st, a, blocks);
-      else if (c.c == 2) launch_cfg<OP, T, G, 2>(st, a, blocks);
-      else if (c.c == 3) launch_cfg<OP, T, G, 3>(st, a, blocks);
-      else launch_cfg<OP, T, G, 4>(st, a, blocks);
-    };
-    if (c.g == 16) launch_cfg<OP, T, 16, 1>(st, a, blocks);
-    else if (c.g == 64) by_c(std::integral_constant<int, 64>{});
-    else if (c.g == 256) by_c(std::integral_constant<int, 256>{});
-    else if (c.g == 1024) by_c(std::integral_constant<int, 1024>{});
-    else if constexpr (OP == FWD) launch_one<&ln_fwd_wide_kernel<T>>(st, a, 1024, blocks);
-    else if constexpr (OP == BWD) launch_one<&ln_bwd_wide_kernel<T>>(st, a, 1024, blocks);
-    else launch_one<&ln_bwd2_wide_kernel<T>>(st, a, 1024, blocks);
+    if (!by_cfg(c, [&](auto g, auto n) { launch_cfg<OP, T, decltype(g)::value, decltype(n)::value>(st, a, blocks); })) {
+      if constexpr (OP == FWD) launch_one<&ln_fwd_wide_kernel<T>>(st, a, 1024, blocks);
+      else if constexpr (OP == BWD) launch_one<&ln_bwd_wide_kernel<T>>(st, a, 1024, blocks);
+      else launch_one<&ln_bwd2_wide_kernel<T>>(st, a, 1024, blocks);
+    }
     AGX_LAUNCH_CHECK();
   }
   if (dgamma || dbeta) {
@@ -640,6 +750,7 @@ int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int a
   return AGX_OK;
 }
 
+int vector_of(int32_t dtype) { return dtype == AGX_BF16 ? 8 : 4; }
 int check_norm(const agx_norm_t *p, const char *who) {
   AGX_CHECK_ARG(p, "%s: null argument", who);
   AGX_CHECK_ARG(p->dtype == AGX_F32 || p->dtype == AGX_BF16, "%s: dtype %d", who, p->dtype);
@@ -666,24 +777,6 @@ int check_out(const agx_norm_t *p, const void *out, int64_t ldo, const char *who
                   "%s: an output overlaps an input without being the same matrix", who);
   return AGX_OK;
 }
-int check_back(const agx_norm_t *p, const char *who) {
-  AGX_TRY(check_mat(p, p->x, p->ldx, who, "x"));
-  AGX_TRY(check_mat(p, p->dy, p->lddy, who, "dy"));
-  AGX_CHECK_ARG(p->mean && p->rstd, "%s: mean / rstd missing", who);
-  if (p->act) AGX_TRY(check_mat(p, p->y, p->ldy, who, "y"));
-  if (p->dx) {
-    AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
-    AGX_TRY(check_out(p, p->dx, p->lddx, who));
-  }
-  if (p->dgamma || p->dbeta) {
-    const int64_t need = agx_layernorm_ws_floats(p->rows, p->width, p->dtype);
-    if (need > 0 && (!p->ws || p->ws_floats < need)) {
-      agx::set_error("%s: workspace of %lld floats, %lld needed", who, (long long)p->ws_floats, (long long)need);
-      return AGX_E_WORKSPACE;
-    }
-  }
-  return AGX_OK;
-}
 NormArgs back_args(const agx_norm_t *p) {
   NormArgs a = {};
   a.x = p->x; a.dy = p->dy; a.ym = p->act ? p->y : nullptr; a.dx = p->dx;
@@ -693,12 +786,42 @@ NormArgs back_args(const agx_norm_t *p) {
   a.rows = p->rows; a.n = p->width; a.slope = p->slope; a.act = p->act; a.add_dx = p->accumulate_dx ? 1 : 0;
   return a;
 }
+int check_back(const agx_norm_t *p, bool second, const char *who) {
+  AGX_TRY(check_mat(p, p->x, p->ldx, who, "x"));
+  AGX_TRY(check_mat(p, p->dy, p->lddy, who, "dy"));
+  AGX_CHECK_ARG(p->mean && p->rstd, "%s: mean / rstd missing", who);
+  if (p->act) AGX_TRY(check_mat(p, p->y, p->ldy, who, "y"));
+  if (p->dx) {
+    AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
+    AGX_TRY(check_out(p, p->dx, p->lddx, who));
+  }
+  if (p->dgamma || p->dbeta) {
+    const int64_t need = !second && small_back(back_args(p), p->dgamma, p->dbeta, vector_of(p->dtype))
+                             ? 0
+                             : agx_layernorm_ws_floats(p->rows, p->width, p->dtype);
+    if (need > 0 && (!p->ws || p->ws_floats < need)) {
+      agx::set_error("%s: workspace of %lld floats, %lld needed", who, (long long)p->ws_floats, (long long)need);
+      return AGX_E_WORKSPACE;
+    }
+    for (const float *out : {p->dgamma, p->dbeta}) {
+      const agx::Region o{out, 1, p->width, p->width, 4};
+      AGX_CHECK_ARG(!out || !((p->gamma && agx::overlap(o, {p->gamma, 1, p->width, p->width, 4})) ||
+                              agx::overlap(o, {p->mean, 1, p->rows, p->rows, 4}) || agx::overlap(o, {p->rstd, 1, p->rows, p->rows, 4})),
+                    "%s: a parameter gradient overlaps gamma or the statistics", who);
+    }
+  }
+  return AGX_OK;
+}
 
 }  // namespace
 
 extern "C" int64_t agx_layernorm_ws_floats(int64_t rows, int64_t width, int32_t dtype) {
   if (rows <= 0 || width <= 0) return 0;
-  return (int64_t)blocks_of(rows, pick(width, dtype == AGX_BF16 ? 8 : 4), true) * 2 * width;
+  return (int64_t)blocks_of(rows, pick(width, vector_of(dtype)), true) * 2 * width;
+}
+
+extern "C" int64_t agx_layernorm_bwd_ws_floats(int64_t rows, int64_t width, int32_t dtype) {
+  return rows > 0 && width > 0 && small_shape(rows, width, vector_of(dtype)) ? 0 : agx_layernorm_ws_floats(rows, width, dtype);
 }
 
 extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
@@ -721,7 +844,7 @@ extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
 
 extern "C" int agx_layernorm_bwd(void *stream, const agx_norm_t *p) {
   AGX_TRY(check_norm(p, "agx_layernorm_bwd"));
-  if (p->rows > 0) AGX_TRY(check_back(p, "agx_layernorm_bwd"));
+  if (p->rows > 0) AGX_TRY(check_back(p, false, "agx_layernorm_bwd"));
   AGX_CHECK_ARG(p->dx || p->dgamma || p->dbeta, "agx_layernorm_bwd: no output wanted");
   const NormArgs a = back_args(p);
   return p->dtype == AGX_F32
@@ -734,7 +857,7 @@ extern "C" int agx_layernorm_bwd2(void *stream, const agx_norm_t *p) {
   AGX_CHECK_ARG(!p->dbeta, "agx_layernorm_bwd2: the second-order pass has no term in beta");
   AGX_CHECK_ARG(p->dx || p->ddy || p->dgamma, "agx_layernorm_bwd2: no output wanted");
   if (p->rows > 0) {
-    AGX_TRY(check_back(p, "agx_layernorm_bwd2"));
+    AGX_TRY(check_back(p, true, "agx_layernorm_bwd2"));
     AGX_TRY(check_mat(p, p->u, p->ldu, "agx_layernorm_bwd2", "u"));
     if (p->ddy) {
       AGX_TRY(check_mat(p, p->ddy, p->ldddy, "agx_layernorm_bwd2", "ddy"));

@@ -89,7 +89,7 @@ def _matrix(t, name, like=None):
     rows, cols = shape
     if cols == 0:
         raise ValueError('%s has no columns' % name)
-    if like is not None and (shape != like.shape or dtype is not like.dtype or t.device != like.device):
+    if like is not None and (shape != like.shape or dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ValueError('%s must match the first operand: got %s %s on %s, expected %s %s on %s'
                          % (name, tuple(shape), dtype, t.device, tuple(like.shape), like.dtype, like.device))
     step, each = t.stride()
@@ -105,7 +105,7 @@ def _vector(t, name, n, like):
         return None
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise ValueError('%s must be a contiguous float32 vector of %d entries' % (name, n))
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError('%s is on %s, the rows on %s' % (name, t.device, like.device))
     return t.data_ptr()
 
@@ -177,8 +177,10 @@ def _norm_back(d, dy, x, mean, rstd, gamma, y, act):
     return _on_current(x)
 
 
-def _norm_ws(d, x, lib):
-    n = lib.agx_layernorm_ws_floats(d.rows, d.width, d.dtype)
+def _norm_ws(d, x, floats):
+    n = floats(d.rows, d.width, d.dtype)
+    if n == 0:
+        return None
     ws = _f32(n, x)
     d.ws, d.ws_floats = ws.data_ptr(), n
     return ws
@@ -195,7 +197,7 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, *, y=None, act=0, slope=0
     d.dx = dx.data_ptr()
     ws = dgamma = dbeta = None
     if param_grads:
-        ws = _norm_ws(d, x, lib)
+        ws = _norm_ws(d, x, lib.agx_layernorm_bwd_ws_floats)
         dgamma, dbeta = _f32(d.width, x), _f32(d.width, x)
         d.dgamma, d.dbeta = dgamma.data_ptr(), dbeta.data_ptr()
     _lib.check(lib.agx_layernorm_bwd(stream, d), 'agx_layernorm_bwd')
@@ -213,7 +215,7 @@ def layer_norm_backward2(u, dy, x, mean, rstd, gamma=None, *, y=None, act=0, slo
     d.dx, d.ddy = dx.data_ptr(), ddy.data_ptr()
     ws = dgamma = None
     if param_grads:
-        ws = _norm_ws(d, x, lib)
+        ws = _norm_ws(d, x, lib.agx_layernorm_ws_floats)
         dgamma = _f32(d.width, x)
         d.dgamma = dgamma.data_ptr()
     _lib.check(lib.agx_layernorm_bwd2(stream, d), 'agx_layernorm_bwd2')

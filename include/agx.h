@@ -165,7 +165,8 @@ int agx_bn_moving_update(void *stream, float *moving_mean, float *moving_var, co
  *         dx = rstd^2 (h (3 mean(gh) mean(uh) + mean(g) mean(u) - mean(gu)) - mean(uh) (g - mean(g)) - mean(gh) (u - mean(u)))
  * act: 1 = leaky ReLU of `slope` (its derivative is taken from the sign of y, which bwd / bwd2 then need), 0 = none.
  * Any output but mean / rstd may be NULL in bwd / bwd2; an output may be the same matrix as an input, any other overlap is refused.
- * ws: needed where dgamma / dbeta are wanted (agx_layernorm_ws_floats).  Sums in a fixed order.                       */
+ * ws: needed where dgamma / dbeta are wanted: agx_layernorm_ws_floats covers every call, agx_layernorm_bwd_ws_floats a bwd whose dx
+ * is none of its inputs (0 for few rows).  Sums in a fixed order.                                                     */
 #define AGX_F32 0
 #define AGX_BF16 1
 typedef struct agx_norm {
@@ -184,6 +185,7 @@ typedef struct agx_norm {
   int32_t accumulate_params;   /* dgamma / dbeta += instead of = (bwd, bwd2) */
 } agx_norm_t;
 int64_t agx_layernorm_ws_floats(int64_t rows, int64_t width, int32_t dtype);
+int64_t agx_layernorm_bwd_ws_floats(int64_t rows, int64_t width, int32_t dtype);
 int agx_layernorm_fwd(void *stream, const agx_norm_t *p);
 int agx_layernorm_bwd(void *stream, const agx_norm_t *p);
 int agx_layernorm_bwd2(void *stream, const agx_norm_t *p);

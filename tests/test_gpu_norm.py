@@ -183,3 +183,69 @@ def test_captured_without_an_eager_call_before(gpu):
         torch.cuda.synchronize()
         for a, b in zip(kept, run()):
             assert torch.equal(a, b)
+
+
+def check_backward(x, dy, ga, be, slope):
+    """The backward pass against the formula; returns its operands and results."""
+    from adversarial_gene_expression_amd import ops
+    y, mean, rstd = ops.layer_norm(x, ga, be, eps=EPS, act=1, slope=slope)
+    args = [N.t64(t) for t in (dy, x, mean, rstd, ga, y)]
+    got = ops.layer_norm_backward(dy, x, mean, rstd, ga, y=y, act=1, slope=slope)
+    want, size = N.backward(*args, slope, 1), N.backward_size(*args, slope, 1)
+    near(got[0], want[0], size[0], x.dtype)
+    for k in (1, 2):
+        near(got[k], want[k], size[k], torch.float32, 128 + x.shape[0])
+    return y, mean, rstd, got
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('width', [1, 7, 60, 257, 600, 1077, 2050, 4297])
+def test_backward_in_one_launch_and_in_two(gpu, width, dtype):
+    """Rows around those that the columns' workgroups take at once, and around the most that one launch takes."""
+    for rows in (1, 2, 255, 256, 257, 1023, 1024, 1025, 1535, 1536, 1537, 2100):
+        x, dy, _, ga, be = make(rows, width, dtype, rows + width, ld_extra=(rows + width) % 3)
+        check_backward(x, dy, ga, be, 0.2)
+
+
+@pytest.mark.parametrize('rows,width', [(300, 256), (40, 1077), (2000, 600)])
+def test_backward_through_the_c_entry(gpu, rows, width):
+    """dx over dy and over x, sums on top of what is there, single outputs: the same values as the plain call."""
+    from adversarial_gene_expression_amd import _dev, _lib
+    lib = _lib.load()
+    x, dy, _, ga, be = make(rows, width, torch.float32, rows)
+    x, dy = x.contiguous(), dy.contiguous()
+    y, mean, rstd, (dx, dg, db) = check_backward(x, dy, ga, be, 0.1)
+    ws = torch.empty(lib.agx_layernorm_ws_floats(rows, width, 0), device='cuda')
+
+    def call(x, dy, dx, dgamma, dbeta, add=0):
+        d = _lib.NormDesc()
+        d.rows, d.width, d.dtype, d.act, d.slope = rows, width, 0, 1, 0.1
+        d.x, d.dy, d.y, d.mean, d.rstd, d.gamma = (t.data_ptr() for t in (x, dy, y, mean, rstd, ga))
+        d.ldx, d.lddy, d.ldy, d.lddx = x.stride(0), dy.stride(0), y.stride(0), width if dx is None else dx.stride(0)
+        d.dx, d.dgamma, d.dbeta = (None if t is None else t.data_ptr() for t in (dx, dgamma, dbeta))
+        d.ws, d.ws_floats, d.accumulate_dx, d.accumulate_params = ws.data_ptr(), ws.numel(), add, add
+        _lib.check(lib.agx_layernorm_bwd(_dev.stream(), d), 'agx_layernorm_bwd')
+    new = lambda t: torch.full_like(t, 5.0)  # noqa: E731
+    # (over an input the sums of the parameter gradients run in another order: both are near the formula)
+    args = [N.t64(t) for t in (dy, x, mean, rstd, ga, y)]
+    want, size = N.backward(*args, 0.1, 1), N.backward_size(*args, 0.1, 1)
+    for over in ('x', 'dy'):
+        a, b, g, h = x.clone(), dy.clone(), new(dg), new(db)
+        o = a if over == 'x' else b
+        call(a, b, o, g, h)
+        assert torch.equal(o, dx)
+        near(g, want[1], size[1], torch.float32, 128 + rows)
+        near(h, want[2], size[2], torch.float32, 128 + rows)
+    o, g, h = new(dx), new(dg), new(db)
+    call(x, dy, o, g, h, add=1)
+    for got, plain in ((o, dx), (g, dg), (h, db)):      # (two roundings of the sum, one of the plain value)
+        assert bool(((got - 5.0 - plain).abs() <= 4 * E * (5.0 + plain.abs())).all())
+    g, h = new(dg), new(db)
+    call(x, dy, None, g, h)
+    assert torch.equal(g, dg) and torch.equal(h, db)
+    g, o = new(dg), new(dx)
+    call(x, dy, o, g, None)
+    assert torch.equal(g, dg) and torch.equal(o, dx)
+    h = new(db)
+    call(x, dy, None, None, h)
+    assert torch.equal(h, db)

@@ -96,6 +96,33 @@ def test_workspace_query():
             assert n % (2 * width) == 0 and 2 * width <= n <= 1024 * 2 * width
 
 
+def test_workspace_of_a_backward_pass():
+    """None for few rows, unless dx goes over an input; parameter gradients over an input vector are refused."""
+    lib = _lib.load()
+    most = lib.agx_layernorm_ws_floats
+    for dt in (0, 1):
+        assert lib.agx_layernorm_bwd_ws_floats(0, 8, dt) == 0
+        for rows, width in ((1, 1), (32, 256), (1536, 256)):
+            assert lib.agx_layernorm_bwd_ws_floats(rows, width, dt) == 0
+        # (537 vectors of bf16 a row; as float32 1074, which a group of 1024 threads takes, in two launches)
+        assert lib.agx_layernorm_bwd_ws_floats(16, 4297, dt) == (0 if dt else most(16, 4297, dt))
+        for rows, width in ((1537, 256), (3, 40000), (1500, 4297), (100000, 5)):
+            assert lib.agx_layernorm_bwd_ws_floats(rows, width, dt) == most(rows, width, dt) > 0
+    d = _lib.NormDesc()
+    d.rows, d.width, d.dtype, d.x, d.dy, d.ldx, d.lddy = 2000, 8, 0, 1 << 20, 1 << 21, 8, 8
+    d.mean, d.rstd, d.gamma, d.dx, d.lddx, d.dgamma = 4096, 65536, 32768, 1 << 22, 8, 1 << 23
+    assert lib.agx_layernorm_bwd(None, d) == -3
+    d.rows, d.dx = 32, 1 << 21                            # over dy
+    assert lib.agx_layernorm_bwd(None, d) == -3
+    d.dx = 1 << 22
+    for over in (32768, 32764, 4096, 65536 + 31 * 4):
+        d.dgamma = over
+        assert lib.agx_layernorm_bwd(None, d) == -1 and b'parameter gradient' in lib.agx_last_error()
+        d.dgamma, d.dbeta = None, over
+        assert lib.agx_layernorm_bwd(None, d) == -1 and b'parameter gradient' in lib.agx_last_error()
+        d.dbeta = None
+
+
 @pytest.mark.parametrize('on,slope', [(0, 0.0), (1, 0.0), (1, 0.2)])
 def test_formulas_against_autograd_and_differences(on, slope):
     """The oracle's closed forms of both backward passes against torch's autograd of the definition and against central
