@@ -13,7 +13,8 @@
 // was stored, by the G threads that own it (16, 64: part of or one wave, no barrier; 256, 1024: a workgroup), C vectors of
 // 16 bytes each, so that the two passes of a centred variance and the 2 to 5 row means cost no second read.  Vectors are
 // loaded at the element's alignment (the hardware needs no more), so odd widths and strides take the same path as padded
-// ones; the up to 7 elements behind the last whole vector are one more element of as many threads.
+// ones; the up to 7 elements behind the last whole vector are one more element of as many threads.  From 4096 fp32 values on the
+// backward passes read a row a second time where their registers do not suffice (back_holds), above 32768 all do.
 // Measured (a copy of 1 GiB: 5.1 TB/s): forward 100000 x 256 33 us (6.2 TB/s, in part from the last-level cache), 4096 x 4297 bf16
 // 16.6 us (4.2); backward with parameter gradients 40000 x 1000 bf16 66 us (4.8); second order 8192 x 1077 44 us (4.8).  Small
 // calls are the host's: 32 x 256 11 us, of which the GPU works 3.4.
@@ -57,13 +58,16 @@ struct Place {
   }
   __device__ __forceinline__ bool in(int c) const { return c * G + t < nv; }
   __device__ __forceinline__ int at(int c) const { return (c * G + t) * V; }
+  __device__ __forceinline__ typename Vec<T>::type vec(const T *p, int c) const {
+    typename Vec<T>::type v = {};
+    if (in(c)) v = *reinterpret_cast<const typename Vec<T>::type *>(p + at(c));
+    return v;
+  }
+  __device__ __forceinline__ T end(const T *p) const { return last >= 0 ? p[last] : (T)0.f; }
   __device__ __forceinline__ void load(Row<T, G, C> &r, const T *__restrict__ p) const {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      r.v[c] = typename Vec<T>::type{};
-      if (in(c)) r.v[c] = *reinterpret_cast<const typename Vec<T>::type *>(p + at(c));
-    }
-    r.end = last >= 0 ? p[last] : (T)0.f;
+    for (int c = 0; c < C; ++c) r.v[c] = vec(p, c);
+    r.end = end(p);
   }
 };
 // V parameters from p[i..]
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_fwd_kernel(NormArgs a) 
   __shared__ float red[G > 64 ? 2 * (G / 64) : 1];
   int flip = 0;
   const Place<T, G, C> w(a.n);
-  const int grp = threadIdx.x / G;
+  const int grp = G == block_threads<G>() ? 0 : threadIdx.x / G;
   const float inv_n = 1.f / (float)a.n;
   const Params<T, G, C> gamma(a.gamma, 1.f, w), beta(a.beta, 0.f, w);
   auto act = [&](float n) { return a.act ? (n > 0.f ? n : a.slope * n) : n; };
@@ -208,7 +212,7 @@ template <typename T, int G, int C, int NA>
 __device__ __forceinline__ void write_partials(float (&acc)[NA][C][Vec<T>::V], float (&end)[NA], const Place<T, G, C> &w,
                                                const NormArgs &a, float *lds) {
   constexpr int V = Vec<T>::V, NG = block_threads<G>() / G, W = G * C * V + V;   // (a group's columns, then its end elements)
-  const int grp = threadIdx.x / G;
+  const int grp = G == block_threads<G>() ? 0 : threadIdx.x / G;
 #pragma unroll
   for (int q = 0; q < NA; ++q) {
     float *p = a.part + ((int64_t)blockIdx.x * 2 + q) * a.n;
@@ -249,20 +253,44 @@ __device__ __forceinline__ uint32_t not_positive(const typename Vec<T>::type &m)
   return b;
 }
 
+// One operand of the backward passes at a row.  HOLD: kept in registers; else each use reads it.
+template <typename T, int G, int C, bool HOLD>
+struct Operand {
+  Row<T, G, C> held;
+  const T *p;
+  __device__ __forceinline__ void open(const Place<T, G, C> &w, const void *m, int64_t at) {
+    p = reinterpret_cast<const T *>(m) + at;
+    if constexpr (HOLD) w.load(held, p);
+    else held.end = w.end(p);
+  }
+  __device__ __forceinline__ typename Vec<T>::type vec(const Place<T, G, C> &w, int c) const {
+    if constexpr (HOLD) return held.v[c];
+    else return w.vec(p, c);
+  }
+  __device__ __forceinline__ float end() const { return (float)held.end; }
+};
 // what the backward pass reads of a row
-template <typename T, int G, int C>
+template <typename T, int G, int C, bool HOLD>
 struct Inputs {
-  Row<T, G, C> x, dy, m;
+  Operand<T, G, C, HOLD> x, dy, m;
   float mu, r;
   __device__ __forceinline__ void load(const NormArgs &a, const Place<T, G, C> &w, int64_t row) {
-    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
-    w.load(dy, reinterpret_cast<const T *>(a.dy) + row * a.lddy);
-    if (a.ym) w.load(m, reinterpret_cast<const T *>(a.ym) + row * a.ldym);
+    x.open(w, a.x, row * a.ldx);
+    dy.open(w, a.dy, row * a.lddy);
+    if (a.ym) m.open(w, a.ym, row * a.ldym);
     mu = a.mean_in[row];
     r = a.rstd_in[row];
   }
 };
+// (keeps a second reading of a row a reading, and how many vectors are in flight small)
+__device__ __forceinline__ void read_again() { asm volatile("" ::: "memory"); }
 
+// Rows of 1024 threads (8 to 32 values each, 128 registers a thread) are held where that leaves registers for the rest, else read
+// again, from L2 or the last-level cache, instead of spilled.  Held and read again, us: backward 2000 x 6000 (8 values) 38.1, 40.7;
+// without sums 1000 x 14000 (16) 70, 77; with them 1800 x 9000 (12) 77, 68; second order 1000 x 6000 51, 35; 900 x 16000 179,
+// 108; 1000 x 18154 bf16 206, 120.
+constexpr bool back_holds(int g, int values, bool pg) { return g < 1024 || values <= (pg ? 8 : 16); }
+constexpr bool back2_holds(int g) { return g < 1024; }
 // the rows of workgroup `block` of `blocks`; lds: lds_floats<T, G, C>() where PG
 template <typename T, int G, int C, bool PG>
 __device__ __forceinline__ void back_rows(const NormArgs &a, int block, int blocks, float *lds) {
@@ -270,7 +298,7 @@ __device__ __forceinline__ void back_rows(const NormArgs &a, int block, int bloc
   __shared__ float red[G > 64 ? 2 * 2 * (G / 64) : 1];
   int flip = 0;
   const Place<T, G, C> w(a.n);
-  const int grp = threadIdx.x / G;
+  const int grp = G == block_threads<G>() ? 0 : threadIdx.x / G;
   const float inv_n = 1.f / (float)a.n;
   const Params<T, G, C> gamma(a.gamma, 1.f, w);
   float acc[2][C][V] = {}, aend[2] = {0.f, 0.f};
@@ -279,22 +307,23 @@ __device__ __forceinline__ void back_rows(const NormArgs &a, int block, int bloc
   constexpr bool AHEAD = G <= 64 && C * V <= 16;
   const int64_t step = (int64_t)blocks * NG;
   int64_t row = (int64_t)block * NG + grp;
-  Inputs<T, G, C> in;
+  constexpr bool HOLD = back_holds(G, C * V, PG);
+  Inputs<T, G, C, HOLD> in;
   if (AHEAD && row < a.rows) in.load(a, w, row);
   for (; row < a.rows; row += step) {
     if (!AHEAD) in.load(a, w, row);
-    const Row<T, G, C> x = in.x, dy = in.dy;
+    const auto x = in.x, dy = in.dy;
     uint32_t neg[C] = {}, nend = 0;
     if (a.ym) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(in.m.v[c]);
-      nend = (float)in.m.end > 0.f ? 0u : 1u;
+      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(in.m.vec(w, c));
+      nend = in.m.end() > 0.f ? 0u : 1u;
     }
     const float mu = in.mu, r = in.r;
     if (AHEAD && row + step < a.rows) in.load(a, w, row + step);
-    auto hat = [&](int c, int k) { return ((float)x.v[c][k] - mu) * r; };
-    auto dn = [&](int c, int k) { return neg[c] >> k & 1 ? a.slope * (float)dy.v[c][k] : (float)dy.v[c][k]; };
-    const float he = w.last >= 0 ? ((float)x.end - mu) * r : 0.f, de = nend ? a.slope * (float)dy.end : (float)dy.end;
+    auto hat = [&](float v) { return (v - mu) * r; };
+    auto dn = [&](float v, int c, int k) { return neg[c] >> k & 1 ? a.slope * v : v; };
+    const float he = w.last >= 0 ? hat(x.end()) : 0.f, de = nend ? a.slope * dy.end() : dy.end();
     const float ge = de * gamma.end;
     if constexpr (PG) {
       aend[0] += de * he;
@@ -305,9 +334,11 @@ __device__ __forceinline__ void back_rows(const NormArgs &a, int block, int bloc
     for (int c = 0; c < C; ++c) {
       float ga[V], q[2] = {0.f, 0.f};
       gamma.get(w, c, ga);
+      if (!HOLD && c % 2 == 0) read_again();
+      const auto xv = x.vec(w, c), dv = dy.vec(w, c);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float h = hat(c, k), d = dn(c, k);
+        const float h = hat((float)xv[k]), d = dn((float)dv[k], c, k);
         if constexpr (PG) {
           acc[0][c][k] += d * h;
           acc[1][c][k] += d;
@@ -323,17 +354,19 @@ __device__ __forceinline__ void back_rows(const NormArgs &a, int block, int bloc
     }
     if (a.dx) {
       group_sum<G, 2>(s, red, flip);
-      const float mg = s[0] * inv_n, mgh = s[1] * inv_n;
+        const float mg = s[0] * inv_n, mgh = s[1] * inv_n;
       T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float ga[V];
         gamma.get(w, c, ga);
+        if (!HOLD && c % 2 == 0) read_again();
+      const auto xv = x.vec(w, c), dv = dy.vec(w, c);
         typename Vec<T>::type o = {};
         if (a.add_dx && w.in(c)) o = *reinterpret_cast<const typename Vec<T>::type *>(dx + w.at(c));
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float d = r * (dn(c, k) * ga[k] - mg - hat(c, k) * mgh);
+          const float d = r * (dn((float)dv[k], c, k) * ga[k] - mg - hat((float)xv[k]) * mgh);
           o[k] = (T)(a.add_dx ? (float)o[k] + d : d);
         }
         if (w.in(c)) *reinterpret_cast<typename Vec<T>::type *>(dx + w.at(c)) = o;
@@ -352,6 +385,28 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd_kernel(NormArgs a) 
   back_rows<T, G, C, PG>(a, blockIdx.x, gridDim.x, lds);
 }
 
+// `left` of V values of a row; a row's terms of both parameter gradients
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::type columns_at(const void *m, int64_t at, int left) {
+  const T *p = reinterpret_cast<const T *>(m) + at;
+  if (left == Vec<T>::V) return *reinterpret_cast<const typename Vec<T>::type *>(p);
+  typename Vec<T>::type v = {};
+#pragma unroll
+  for (int k = 0; k < Vec<T>::V; ++k)
+    if (k < left) v[k] = p[k];
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void add_columns(const NormArgs &a, const typename Vec<T>::type &x, const typename Vec<T>::type &dy, uint32_t neg,
+                                            float mu, float r, float *dgamma, float *dbeta) {
+#pragma unroll
+  for (int k = 0; k < Vec<T>::V; ++k) {
+    const float d = neg >> k & 1 ? a.slope * (float)dy[k] : (float)dy[k];
+    dgamma[k] += d * (((float)x[k] - mu) * r);
+    dbeta[k] += d;
+  }
+}
+
 // Parameter gradients of V columns over all rows, by one workgroup of 256: with the statistics given they need no sum over a
 // row.  A thread has every 256th row, U of them in flight (6: 512 x 256 4.1 us instead of 3.7); the threads meet in LDS in a
 // fixed order.  Neighbouring strips are given to one XCD, which then fetches a line once for all of them: 1536 x 256 5.7 us, 12.8
@@ -362,15 +417,7 @@ __device__ __forceinline__ void column_sums(const NormArgs &a, int strip, float 
   using VT = typename Vec<T>::type;
   const int64_t c0 = (int64_t)strip * V;
   const int left = (int)min((int64_t)V, a.n - c0);
-  auto get = [&](const void *m, int64_t at) {
-    const T *p = reinterpret_cast<const T *>(m) + at + c0;
-    if (left == V) return *reinterpret_cast<const VT *>(p);
-    VT v = {};
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (k < left) v[k] = p[k];
-    return v;
-  };
+  auto get = [&](const void *m, int64_t at) { return columns_at<T>(m, at + c0, left); };
   float s[Q] = {};
   for (int64_t row0 = threadIdx.x; row0 < a.rows; row0 += 256 * U) {
     VT x[U], dy[U], m[U];
@@ -385,16 +432,8 @@ __device__ __forceinline__ void column_sums(const NormArgs &a, int strip, float 
       r[i] = a.rstd_in[row];
     }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const uint32_t neg = a.ym ? not_positive<T>(m[i]) : 0u;
-      if (row0 + 256 * i < a.rows)
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = neg >> k & 1 ? a.slope * (float)dy[i][k] : (float)dy[i][k];
-          s[k] += d * (((float)x[i][k] - mu[i]) * r[i]);
-          s[V + k] += d;
-        }
-    }
+    for (int i = 0; i < U; ++i)
+      if (row0 + 256 * i < a.rows) add_columns<T>(a, x[i], dy[i], a.ym ? not_positive<T>(m[i]) : 0u, mu[i], r[i], s, s + V);
   }
   const int t = threadIdx.x, q = t % Q, part = t / Q;
 #pragma unroll
@@ -429,38 +468,41 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd2_kernel(NormArgs a)
   constexpr int V = Vec<T>::V, NG = block_threads<G>() / G;
   __shared__ float red[G > 64 ? 2 * 5 * (G / 64) : 1];
   __shared__ float lds[PG ? lds_floats<T, G, C>() : 1];
+  constexpr bool HOLD = back2_holds(G);
   int flip = 0;
   const Place<T, G, C> w(a.n);
-  const int grp = threadIdx.x / G;
+  const int grp = G == block_threads<G>() ? 0 : threadIdx.x / G;
   const float inv_n = 1.f / (float)a.n;
   const Params<T, G, C> gamma(a.gamma, 1.f, w);
   float acc[1][C][V] = {}, aend[1] = {0.f};
   for (int64_t row = (int64_t)blockIdx.x * NG + grp; row < a.rows; row += (int64_t)gridDim.x * NG) {
-    Row<T, G, C> x, dy, u;
+    Operand<T, G, C, HOLD> x, dy, u;
     uint32_t neg[C] = {}, nend = 0;
-    w.load(x, reinterpret_cast<const T *>(a.x) + row * a.ldx);
-    w.load(dy, reinterpret_cast<const T *>(a.dy) + row * a.lddy);
-    w.load(u, reinterpret_cast<const T *>(a.u) + row * a.ldu);
+    x.open(w, a.x, row * a.ldx);
+    dy.open(w, a.dy, row * a.lddy);
+    u.open(w, a.u, row * a.ldu);
     if (a.ym) {
-      Row<T, G, C> m;
-      w.load(m, reinterpret_cast<const T *>(a.ym) + row * a.ldym);
+      Operand<T, G, C, HOLD> m;
+      m.open(w, a.ym, row * a.ldym);
 #pragma unroll
-      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(m.v[c]);
-      nend = (float)m.end > 0.f ? 0u : 1u;
+      for (int c = 0; c < C; ++c) neg[c] = not_positive<T>(m.vec(w, c));
+      nend = m.end() > 0.f ? 0u : 1u;
     }
     const float mu = a.mean_in[row], r = a.rstd_in[row];
-    auto hat = [&](int c, int k) { return ((float)x.v[c][k] - mu) * r; };
-    auto dn = [&](int c, int k) { return neg[c] >> k & 1 ? a.slope * (float)dy.v[c][k] : (float)dy.v[c][k]; };
-    const float he = w.last >= 0 ? ((float)x.end - mu) * r : 0.f, de = nend ? a.slope * (float)dy.end : (float)dy.end;
-    const float ge = de * gamma.end, ue = (float)u.end;
+    auto hat = [&](float v) { return (v - mu) * r; };
+    auto dn = [&](float v, int c, int k) { return neg[c] >> k & 1 ? a.slope * v : v; };
+    const float he = w.last >= 0 ? hat(x.end()) : 0.f, de = nend ? a.slope * dy.end() : dy.end();
+    const float ge = de * gamma.end, ue = u.end();
     float s[5] = {ge, ge * he, ue, ue * he, ge * ue};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float ga[V], q[5] = {};
       gamma.get(w, c, ga);
+      if (!HOLD && c % 2 == 0) read_again();
+      const auto xv = x.vec(w, c), dv = dy.vec(w, c), uv = u.vec(w, c);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float h = hat(c, k), g = dn(c, k) * ga[k], uu = (float)u.v[c][k];
+        const float h = hat((float)xv[k]), g = dn((float)dv[k], c, k) * ga[k], uu = (float)uv[k];
         q[0] += g;
         q[1] += g * h;
         q[2] += uu;
@@ -481,11 +523,13 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd2_kernel(NormArgs a)
     for (int c = 0; c < C; ++c) {
       float ga[V];
       gamma.get(w, c, ga);
+      if (!HOLD && c % 2 == 0) read_again();
+      const auto xv = x.vec(w, c), dv = dy.vec(w, c), uv = u.vec(w, c);
       typename Vec<T>::type o = {}, e;
       if (a.dx && a.add_dx && w.in(c)) o = *reinterpret_cast<const typename Vec<T>::type *>(dx + w.at(c));
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float h = hat(c, k), d = dn(c, k), uu = (float)u.v[c][k];
+        const float h = hat((float)xv[k]), d = dn((float)dv[k], c, k), uu = (float)uv[k];
         const float q = r * (uu - mu_ - h * muh);
         if constexpr (PG) acc[0][c][k] += d * q;
         e[k] = (T)(neg[c] >> k & 1 ? ga[k] * q * a.slope : ga[k] * q);
@@ -505,8 +549,9 @@ __global__ __launch_bounds__(block_threads<G>()) void ln_bwd2_kernel(NormArgs a)
   if constexpr (PG) write_partials<T, G, C, 1>(acc, aend, w, a, lds);
 }
 
-// Rows wider than the registers of a workgroup hold: one workgroup a row, the row read again for each pass (it stays in
-// L2 between them).  Partial parameter gradients are added to the workgroup's own row of `part`, each column by one thread.
+// Rows of more than 32768 values: one workgroup a row, the row read again for each pass (it stays in L2 between them).  The second
+// order's partial parameter gradients are added to the workgroup's own row of `part`, each column by one thread; the backward
+// pass has them apart (ln_columns_kernel).
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(NormArgs a) {
   __shared__ float red[2 * 16];
@@ -540,8 +585,6 @@ template <typename T>
 __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(NormArgs a) {
   __shared__ float red[2 * 2 * 16];
   int flip = 0;
-  float *p0 = a.part ? a.part + (int64_t)blockIdx.x * 2 * a.n : nullptr, *p1 = a.part ? p0 + a.n : nullptr;
-  bool first = true;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *x = reinterpret_cast<const T *>(a.x) + row * a.ldx;
     const T *dy = reinterpret_cast<const T *>(a.dy) + row * a.lddy;
@@ -552,16 +595,10 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(NormArgs a) {
       float d = (float)dy[i];
       if (ym && !((float)ym[i] > 0.f)) d *= a.slope;
       const float h = ((float)x[i] - mu) * r;
-      if (p0) {
-        p0[i] = (first ? 0.f : p0[i]) + d * h;
-        p1[i] = (first ? 0.f : p1[i]) + d;
-      }
       const float g = d * (a.gamma ? a.gamma[i] : 1.f);
       s[0] += g;
       s[1] += g * h;
     }
-    first = false;
-    if (!a.dx) continue;
     group_sum<1024, 2>(s, red, flip);
     const float mg = s[0] / (float)a.n, mgh = s[1] / (float)a.n;
     T *dx = reinterpret_cast<T *>(a.dx) + row * a.lddx;
@@ -619,6 +656,41 @@ __global__ __launch_bounds__(1024) void ln_bwd2_wide_kernel(NormArgs a) {
   }
 }
 
+// Parameter gradients of the backward pass by itself, for rows whose workgroup has no registers for them: a thread has V columns
+// and every gridDim.y-th row; partial sums as above.
+template <typename T>
+__global__ __launch_bounds__(256) void ln_columns_kernel(NormArgs a) {
+  constexpr int V = Vec<T>::V, U = 4;
+  const int64_t c0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+  if (c0 >= a.n) return;
+  const int left = (int)min((int64_t)V, a.n - c0);
+  float s[2][V] = {};
+  const int64_t step = gridDim.y;
+  for (int64_t row0 = blockIdx.y; row0 < a.rows; row0 += U * step) {
+    typename Vec<T>::type x[U], dy[U], m[U];
+    float mu[U], r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t row = min(row0 + i * step, a.rows - 1);
+      x[i] = columns_at<T>(a.x, row * a.ldx + c0, left);
+      dy[i] = columns_at<T>(a.dy, row * a.lddy + c0, left);
+      if (a.ym) m[i] = columns_at<T>(a.ym, row * a.ldym + c0, left);
+      mu[i] = a.mean_in[row];
+      r[i] = a.rstd_in[row];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (row0 + i * step < a.rows) add_columns<T>(a, x[i], dy[i], a.ym ? not_positive<T>(m[i]) : 0u, mu[i], r[i], s[0], s[1]);
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    float *p = a.part + ((int64_t)blockIdx.y * 2 + q) * a.n + c0;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < left) p[k] = s[q][k];
+  }
+}
+
 // out_q[j] (+)= sum over workgroups b of part[b][q][j], b in a fixed order: 32 columns by 32 interleaved shares a workgroup
 __global__ __launch_bounds__(1024) void ln_param_kernel(const float *__restrict__ part, int nb, int64_t n, float *dgamma,
                                                         float *dbeta, int accumulate) {
@@ -659,13 +731,19 @@ template <auto KERNEL> void launch_one(hipStream_t st, const NormArgs &a, int th
   blocks = std::min(blocks, agx::num_cus() * resident<KERNEL>(threads));
   hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3(threads), 0, st, a);
 }
+// rows whose workgroup sums no parameter gradients in the backward pass (g: 0, or the threads of a row, values of each):
+// their sums take another launch (ln_columns_kernel), which reads x, dy and y once more.  Values, us in the rows' workgroups and
+// apart: 12 (1800 x 9000) 68, 80; 16 (1000 x 14000) 96, 70; 20 (800 x 18154) 119, 90; 24 (2000 x 18154 bf16) 246, 139.
+constexpr bool params_apart(int g, int values) { return g == 0 || (g == 1024 && values > 12); }
+
 template <int OP, typename T, int G, int C>
 void launch_cfg(hipStream_t st, const NormArgs &a, int &blocks) {
   constexpr int threads = block_threads<G>();
   if constexpr (OP == FWD) launch_one<&ln_fwd_kernel<T, G, C>>(st, a, threads, blocks);
   else if constexpr (OP == BWD) {
-    if (a.part) launch_one<&ln_bwd_kernel<T, G, C, true>>(st, a, threads, blocks);
-    else launch_one<&ln_bwd_kernel<T, G, C, false>>(st, a, threads, blocks);
+    if constexpr (!params_apart(G, C * Vec<T>::V))
+      if (a.part) return launch_one<&ln_bwd_kernel<T, G, C, true>>(st, a, threads, blocks);
+    launch_one<&ln_bwd_kernel<T, G, C, false>>(st, a, threads, blocks);
   } else {
     if (a.part) launch_one<&ln_bwd2_kernel<T, G, C, true>>(st, a, threads, blocks);
     else launch_one<&ln_bwd2_kernel<T, G, C, false>>(st, a, threads, blocks);
@@ -679,7 +757,7 @@ Cfg pick(int64_t width, int v) {
   if (nv <= 16) return {16, 1};
   if (nv <= 64 * 4) return {64, (int)agx::cdiv64(nv, 64)};
   if (nv <= 256 * 4) return {256, (int)agx::cdiv64(nv, 256)};
-  if (nv <= 1024 * 4) return {1024, (int)agx::cdiv64(nv, 1024)};
+  if (nv <= 1024 * (32 / v)) return {1024, (int)agx::cdiv64(nv, 1024)};
   return {0, 0};
 }
 // workgroups of a launch at most: a row each; with parameter gradients PARAM_BLOCKS a CU, because each writes and the second
@@ -690,12 +768,18 @@ int blocks_of(int64_t rows, const Cfg &c, bool params) {
 }
 
 // calls f with a configuration's G and C as constants; false: the wide kernels' rows
-template <class F> bool by_cfg(const Cfg &c, F f) {
+template <int V, class F> bool by_cfg(const Cfg &c, F f) {
   auto by_c = [&](auto g) {
-    if (c.c == 1) f(g, std::integral_constant<int, 1>{});
-    else if (c.c == 2) f(g, std::integral_constant<int, 2>{});
+    if constexpr (decltype(g)::value == 64)                             // (wider groups have more: see pick)
+      if (c.c == 1) return f(g, std::integral_constant<int, 1>{});
+    if (c.c == 2) f(g, std::integral_constant<int, 2>{});
     else if (c.c == 3) f(g, std::integral_constant<int, 3>{});
-    else f(g, std::integral_constant<int, 4>{});
+    else if (c.c == 4) f(g, std::integral_constant<int, 4>{});
+    else if constexpr (decltype(g)::value == 1024 && V == 4) {
+      if (c.c == 5) f(g, std::integral_constant<int, 5>{});
+      else if (c.c == 6) f(g, std::integral_constant<int, 6>{});
+      else f(g, std::integral_constant<int, 8>{});
+    }
   };
   if (c.g == 16) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
   else if (c.g == 64) by_c(std::integral_constant<int, 64>{});
@@ -725,7 +809,7 @@ int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int a
   if constexpr (OP == BWD)
     if (small_back(a, dgamma, dbeta, Vec<T>::V)) {
       const int strips = (int)agx::cdiv64(a.n, Vec<T>::V), rows = a.dx ? blocks_of(a.rows, c, false) : 0;
-      by_cfg(c, [&](auto g, auto n) {
+      by_cfg<Vec<T>::V>(c, [&](auto g, auto n) {
         if constexpr (decltype(g)::value <= 256)
           hipLaunchKernelGGL((ln_bwd_small_kernel<T, decltype(g)::value, decltype(n)::value>), dim3(strips + rows), dim3(256), 0, st, a,
                              strips, dgamma, dbeta, accumulate);
@@ -733,18 +817,28 @@ int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int a
       AGX_LAUNCH_CHECK();
       return AGX_OK;
     }
-  int blocks = blocks_of(a.rows, c, a.part != nullptr);
+  NormArgs rows = a;
+  int blocks = blocks_of(a.rows, c, a.part != nullptr), parts = 0;
+  if constexpr (OP == BWD)
+    if (a.part && a.rows > 0 && params_apart(c.g, c.c * Vec<T>::V)) {          // (before the rows: dx may be written over an input)
+      const int cols = (int)agx::cdiv64(a.n, 256 * Vec<T>::V);
+      parts = (int)std::min<int64_t>(a.rows, std::max(1, agx::num_cus() * PARAM_BLOCKS / cols));
+      hipLaunchKernelGGL(ln_columns_kernel<T>, dim3(cols, parts), dim3(256), 0, st, a);
+      AGX_LAUNCH_CHECK();
+      rows.part = nullptr;
+      blocks = a.dx ? blocks_of(a.rows, c, false) : 0;
+    }
   if (blocks > 0) {
-    if (!by_cfg(c, [&](auto g, auto n) { launch_cfg<OP, T, decltype(g)::value, decltype(n)::value>(st, a, blocks); })) {
-      if constexpr (OP == FWD) launch_one<&ln_fwd_wide_kernel<T>>(st, a, 1024, blocks);
-      else if constexpr (OP == BWD) launch_one<&ln_bwd_wide_kernel<T>>(st, a, 1024, blocks);
-      else launch_one<&ln_bwd2_wide_kernel<T>>(st, a, 1024, blocks);
+    if (!by_cfg<Vec<T>::V>(c, [&](auto g, auto n) { launch_cfg<OP, T, decltype(g)::value, decltype(n)::value>(st, rows, blocks); })) {
+      if constexpr (OP == FWD) launch_one<&ln_fwd_wide_kernel<T>>(st, rows, 1024, blocks);
+      else if constexpr (OP == BWD) launch_one<&ln_bwd_wide_kernel<T>>(st, rows, 1024, blocks);
+      else launch_one<&ln_bwd2_wide_kernel<T>>(st, rows, 1024, blocks);
     }
     AGX_LAUNCH_CHECK();
   }
   if (dgamma || dbeta) {
-    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)agx::cdiv64(a.n, 32), 2), dim3(1024), 0, st, a.part, blocks, a.n, dgamma,
-                       dbeta, accumulate);
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)agx::cdiv64(a.n, 32), 2), dim3(1024), 0, st, a.part, parts ? parts : blocks, a.n,
+                       dgamma, dbeta, accumulate);
     AGX_LAUNCH_CHECK();
   }
   return AGX_OK;

@@ -207,7 +207,7 @@ def test_backward_in_one_launch_and_in_two(gpu, width, dtype):
         check_backward(x, dy, ga, be, 0.2)
 
 
-@pytest.mark.parametrize('rows,width', [(300, 256), (40, 1077), (2000, 600)])
+@pytest.mark.parametrize('rows,width', [(300, 256), (40, 1077), (2000, 600), (300, 14000), (70, 18154), (20, 33001)])
 def test_backward_through_the_c_entry(gpu, rows, width):
     """dx over dy and over x, sums on top of what is there, single outputs: the same values as the plain call."""
     from adversarial_gene_expression_amd import _dev, _lib
@@ -249,3 +249,46 @@ def test_backward_through_the_c_entry(gpu, rows, width):
     h = new(db)
     call(x, dy, None, None, h)
     assert torch.equal(h, db)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('width', [4100, 8200, 12001, 14000, 16385, 18154, 20481, 24583, 32768, 32775, 33001, 65600])
+def test_wide_rows(gpu, width, dtype):
+    """Widths around every change of what a thread holds; one row, a few, more than the partial sums have."""
+    from adversarial_gene_expression_amd import ops
+    for rows in (1, 5, 300):
+        x, dy, u, ga, be = make(rows, width, dtype, rows + width, ld_extra=rows % 3)
+        y, mean, rstd, _ = check_backward(x, dy, ga, be, 0.2)
+        X, G, B = N.t64(x), N.t64(ga), N.t64(be)
+        wy, wm, wr = N.forward(X, G, B, EPS, 0.2, 1)
+        near(y, wy, N.forward_size(X, G, B, wr), dtype)
+        near(mean, wm, X.abs().mean(1), torch.float32)
+        args = [N.t64(t) for t in (u, dy, x, mean, rstd, ga, y)]
+        got = ops.layer_norm_backward2(u, dy, x, mean, rstd, ga, y=y, act=1, slope=0.2)
+        want, size = N.backward2(*args, 0.2, 1), N.backward2_size(*args, 0.2, 1)
+        near(got[0], want[0], size[0], dtype)
+        near(got[1], want[1], size[1], dtype)
+        near(got[2], want[2], size[2], torch.float32, 128 + rows)
+
+
+@pytest.mark.parametrize('width', [256, 1077, 6000, 18154, 33001])
+def test_second_order_over_its_inputs(gpu, width):
+    """ddy over dy and dx over x, or over u: the same values as into matrices of their own."""
+    from adversarial_gene_expression_amd import _dev, _lib, ops
+    lib = _lib.load()
+    rows = 37
+    x, dy, u, ga, be = (t.contiguous() for t in make(rows, width, torch.float32, width))
+    y, mean, rstd = ops.layer_norm(x, ga, be, eps=EPS, act=1, slope=0.2)
+    want = ops.layer_norm_backward2(u, dy, x, mean, rstd, ga, y=y, act=1, slope=0.2)
+    ws = torch.empty(lib.agx_layernorm_ws_floats(rows, width, 0), device='cuda')
+    for dx_over, ddy_over in (('x', 'dy'), ('u', 'x'), ('dy', 'u')):
+        m = {'x': x.clone(), 'dy': dy.clone(), 'u': u.clone()}
+        dg = torch.full_like(ga, 3.0)
+        d = _lib.NormDesc()
+        d.rows, d.width, d.dtype, d.act, d.slope = rows, width, 0, 1, 0.2
+        d.x, d.dy, d.u, d.y = m['x'].data_ptr(), m['dy'].data_ptr(), m['u'].data_ptr(), y.data_ptr()
+        d.ldx, d.lddy, d.ldu, d.ldy, d.lddx, d.ldddy = width, width, width, y.stride(0), width, width
+        d.mean, d.rstd, d.gamma, d.dgamma = mean.data_ptr(), rstd.data_ptr(), ga.data_ptr(), dg.data_ptr()
+        d.dx, d.ddy, d.ws, d.ws_floats = m[dx_over].data_ptr(), m[ddy_over].data_ptr(), ws.data_ptr(), ws.numel()
+        _lib.check(lib.agx_layernorm_bwd2(_dev.stream(), d), 'agx_layernorm_bwd2')
+        assert torch.equal(m[ddy_over], want[0]) and torch.equal(m[dx_over], want[1]) and torch.equal(dg, want[2])
