@@ -880,6 +880,17 @@ NormArgs back_args(const agx_norm_t *p) {
   a.rows = p->rows; a.n = p->width; a.slope = p->slope; a.act = p->act; a.add_dx = p->accumulate_dx ? 1 : 0;
   return a;
 }
+// nor share elements with a vector of the call
+int check_vectors(const agx_norm_t *p, const void *out, int64_t ldo, const char *who) {
+  const agx::Region o{out, p->rows, p->width, ldo, p->dtype == AGX_F32 ? 4 : 2};
+  const bool params = p->dgamma || p->dbeta;
+  const float *v[7] = {p->gamma, p->beta, p->mean, p->rstd, p->dgamma, p->dbeta, params ? p->ws : nullptr};
+  const int64_t n[7] = {p->width, p->width, p->rows, p->rows, p->width, p->width, params ? p->ws_floats : 0};
+  for (int i = 0; i < 7; ++i)
+    AGX_CHECK_ARG(!out || !v[i] || n[i] <= 0 || !agx::overlap(o, {v[i], 1, n[i], n[i], 4}),
+                  "%s: an output matrix overlaps a parameter, a statistic or the workspace", who);
+  return AGX_OK;
+}
 int check_back(const agx_norm_t *p, bool second, const char *who) {
   AGX_TRY(check_mat(p, p->x, p->ldx, who, "x"));
   AGX_TRY(check_mat(p, p->dy, p->lddy, who, "dy"));
@@ -904,7 +915,7 @@ int check_back(const agx_norm_t *p, bool second, const char *who) {
                     "%s: a parameter gradient overlaps gamma or the statistics", who);
     }
   }
-  return AGX_OK;
+  return check_vectors(p, p->dx, p->lddx, who);
 }
 
 }  // namespace
@@ -928,6 +939,7 @@ extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
   AGX_CHECK_ARG((p->x == p->y && (p->ldx == p->ldy || p->rows == 1)) ||
                     !agx::overlap({p->x, p->rows, p->width, p->ldx, bytes}, {p->y, p->rows, p->width, p->ldy, bytes}),
                 "agx_layernorm_fwd: y overlaps x without being the same matrix");
+  AGX_TRY(check_vectors(p, p->y, p->ldy, "agx_layernorm_fwd"));
   NormArgs a = {};
   a.x = p->x; a.ldx = p->ldx; a.y = p->y; a.ldy = p->ldy;
   a.gamma = p->gamma; a.beta = p->beta; a.mean = p->mean; a.rstd = p->rstd;
@@ -956,6 +968,7 @@ extern "C" int agx_layernorm_bwd2(void *stream, const agx_norm_t *p) {
     if (p->ddy) {
       AGX_TRY(check_mat(p, p->ddy, p->ldddy, "agx_layernorm_bwd2", "ddy"));
       AGX_TRY(check_out(p, p->ddy, p->ldddy, "agx_layernorm_bwd2"));
+      AGX_TRY(check_vectors(p, p->ddy, p->ldddy, "agx_layernorm_bwd2"));
       const int bytes = p->dtype == AGX_F32 ? 4 : 2;
       AGX_CHECK_ARG(!agx::overlap({p->dx, p->rows, p->width, p->lddx, bytes}, {p->ddy, p->rows, p->width, p->ldddy, bytes}),
                     "agx_layernorm_bwd2: dx and ddy overlap");

@@ -123,6 +123,21 @@ def test_workspace_of_a_backward_pass():
         d.dbeta = None
 
 
+def test_results_over_vectors_are_refused():
+    lib = _lib.load()
+    mb = 1 << 20
+    d = _lib.NormDesc()
+    d.rows, d.width, d.dtype, d.eps = 40, 8, 0, 1e-3
+    d.x, d.dy, d.u, d.ldx, d.lddy, d.ldu, d.ldy, d.lddx, d.ldddy = mb, 2 * mb, 3 * mb, 8, 8, 8, 8, 8, 8
+    d.gamma, d.beta, d.mean, d.rstd, d.dgamma, d.ws, d.ws_floats = 4 * mb, 5 * mb, 6 * mb, 7 * mb, 8 * mb, 9 * mb, 1 << 15
+    for over in (d.gamma, d.beta + 16, d.mean + 39 * 4, d.rstd, d.dgamma, d.ws + 64):
+        for entry, name in ((lib.agx_layernorm_fwd, 'y'), (lib.agx_layernorm_bwd, 'dx'), (lib.agx_layernorm_bwd2, 'dx'),
+                            (lib.agx_layernorm_bwd2, 'ddy')):
+            d.y = d.dx = d.ddy = None
+            setattr(d, name, over)
+            assert entry(None, d) == -1 and b'an output matrix overlaps' in lib.agx_last_error(), (hex(over), name)
+
+
 @pytest.mark.parametrize('on,slope', [(0, 0.0), (1, 0.0), (1, 0.2)])
 def test_formulas_against_autograd_and_differences(on, slope):
     """The oracle's closed forms of both backward passes against torch's autograd of the definition and against central
