@@ -860,17 +860,6 @@ int check_mat(const agx_norm_t *p, const void *m, int64_t ld, const char *who, c
   AGX_CHECK_ARG((reinterpret_cast<uintptr_t>(m) & al) == 0, "%s: %s not aligned to its elements", who, name);
   return AGX_OK;
 }
-// an output may be the same matrix as an input, but not another one that shares elements with it
-int check_out(const agx_norm_t *p, const void *out, int64_t ldo, const char *who) {
-  const int bytes = p->dtype == AGX_F32 ? 4 : 2;
-  const void *in[4] = {p->x, p->dy, p->u, p->act ? p->y : nullptr};
-  const int64_t ld[4] = {p->ldx, p->lddy, p->ldu, p->ldy};
-  for (int i = 0; i < 4; ++i)
-    AGX_CHECK_ARG((in[i] == out && (ld[i] == ldo || p->rows == 1)) ||
-                      !agx::overlap({out, p->rows, p->width, ldo, bytes}, {in[i], p->rows, p->width, ld[i], bytes}),
-                  "%s: an output overlaps an input without being the same matrix", who);
-  return AGX_OK;
-}
 NormArgs back_args(const agx_norm_t *p) {
   NormArgs a = {};
   a.x = p->x; a.dy = p->dy; a.ym = p->act ? p->y : nullptr; a.dx = p->dx;
@@ -880,15 +869,41 @@ NormArgs back_args(const agx_norm_t *p) {
   a.rows = p->rows; a.n = p->width; a.slope = p->slope; a.act = p->act; a.add_dx = p->accumulate_dx ? 1 : 0;
   return a;
 }
-// nor share elements with a vector of the call
-int check_vectors(const agx_norm_t *p, const void *out, int64_t ldo, const char *who) {
-  const agx::Region o{out, p->rows, p->width, ldo, p->dtype == AGX_F32 ? 4 : 2};
-  const bool params = p->dgamma || p->dbeta;
-  const float *v[7] = {p->gamma, p->beta, p->mean, p->rstd, p->dgamma, p->dbeta, params ? p->ws : nullptr};
-  const int64_t n[7] = {p->width, p->width, p->rows, p->rows, p->width, p->width, params ? p->ws_floats : 0};
+// What a call writes shares no element with anything else of its descriptor, but that an output may be the same matrix as an
+// input (a thread has read a place of it before it writes there).
+int check_overlaps(const agx_norm_t *p, int op, const char *who) {
+  const int bytes = p->dtype == AGX_F32 ? 4 : 2;
+  const bool back = op != FWD, params = p->dgamma || p->dbeta;
+  auto matrix = [&](const void *m, int64_t ld) { return agx::Region{m, p->rows, p->width, ld, bytes}; };
+  auto vec = [](const float *v, int64_t n) { return agx::Region{n > 0 ? v : nullptr, 1, n, n, 4}; };
+  struct Vector { agx::Region r; const char *name, *written; };                  // written: what it is where the call writes it
+  const char *stat = back ? nullptr : "a statistic", *grad = back ? "a parameter gradient" : nullptr;
+  const Vector vectors[7] = {
+      {vec(p->gamma, p->width), "gamma", nullptr}, {vec(p->beta, p->width), "beta", nullptr},
+      {vec(p->mean, p->rows), "mean", stat}, {vec(p->rstd, p->rows), "rstd", stat},
+      {vec(p->dgamma, p->width), "dgamma", grad}, {vec(p->dbeta, p->width), "dbeta", grad},
+      {vec(params ? p->ws : nullptr, std::min(p->ws_floats, agx_layernorm_ws_floats(p->rows, p->width, p->dtype))), "the workspace",
+       back ? "the workspace" : nullptr}};
+  struct Matrix { agx::Region r; const char *name; };
+  const Matrix in[4] = {{matrix(p->x, p->ldx), "x"},
+                        {matrix(back ? p->dy : nullptr, p->lddy), "dy"},
+                        {matrix(op == BWD2 ? p->u : nullptr, p->ldu), "u"},
+                        {matrix(back && p->act ? p->y : nullptr, p->ldy), "y"}};
+  const agx::Region out[2] = {back ? matrix(p->dx, p->lddx) : matrix(p->y, p->ldy), matrix(op == BWD2 ? p->ddy : nullptr, p->ldddy)};
   for (int i = 0; i < 7; ++i)
-    AGX_CHECK_ARG(!out || !v[i] || n[i] <= 0 || !agx::overlap(o, {v[i], 1, n[i], n[i], 4}),
-                  "%s: an output matrix overlaps a parameter, a statistic or the workspace", who);
+    for (int k = 0; k < 7; ++k)
+      AGX_CHECK_ARG(k == i || !vectors[i].written || !agx::overlap(vectors[i].r, vectors[k].r),
+                    "%s: %s overlaps %s", who, vectors[i].written, vectors[k].name);
+  for (const Vector &v : vectors) {
+    for (const Matrix &m : in)
+      AGX_CHECK_ARG(!v.written || !agx::overlap(v.r, m.r), "%s: %s overlaps %s", who, v.written, m.name);
+    for (const agx::Region &o : out) AGX_CHECK_ARG(!agx::overlap(o, v.r), "%s: an output matrix overlaps %s", who, v.name);
+  }
+  for (const agx::Region &o : out)
+    for (const Matrix &m : in)
+      AGX_CHECK_ARG((o.p == m.r.p && (o.ld == m.r.ld || p->rows == 1)) || !agx::overlap(o, m.r),
+                    "%s: an output matrix overlaps %s without being the same matrix", who, m.name);
+  AGX_CHECK_ARG(!agx::overlap(out[0], out[1]), "%s: dx and ddy overlap", who);
   return AGX_OK;
 }
 int check_back(const agx_norm_t *p, bool second, const char *who) {
@@ -896,9 +911,10 @@ int check_back(const agx_norm_t *p, bool second, const char *who) {
   AGX_TRY(check_mat(p, p->dy, p->lddy, who, "dy"));
   AGX_CHECK_ARG(p->mean && p->rstd, "%s: mean / rstd missing", who);
   if (p->act) AGX_TRY(check_mat(p, p->y, p->ldy, who, "y"));
-  if (p->dx) {
-    AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
-    AGX_TRY(check_out(p, p->dx, p->lddx, who));
+  if (p->dx) AGX_TRY(check_mat(p, p->dx, p->lddx, who, "dx"));
+  if (second) {
+    AGX_TRY(check_mat(p, p->u, p->ldu, who, "u"));
+    if (p->ddy) AGX_TRY(check_mat(p, p->ddy, p->ldddy, who, "ddy"));
   }
   if (p->dgamma || p->dbeta) {
     const int64_t need = !second && small_back(back_args(p), p->dgamma, p->dbeta, vector_of(p->dtype))
@@ -908,14 +924,8 @@ int check_back(const agx_norm_t *p, bool second, const char *who) {
       agx::set_error("%s: workspace of %lld floats, %lld needed", who, (long long)p->ws_floats, (long long)need);
       return AGX_E_WORKSPACE;
     }
-    for (const float *out : {p->dgamma, p->dbeta}) {
-      const agx::Region o{out, 1, p->width, p->width, 4};
-      AGX_CHECK_ARG(!out || !((p->gamma && agx::overlap(o, {p->gamma, 1, p->width, p->width, 4})) ||
-                              agx::overlap(o, {p->mean, 1, p->rows, p->rows, 4}) || agx::overlap(o, {p->rstd, 1, p->rows, p->rows, 4})),
-                    "%s: a parameter gradient overlaps gamma or the statistics", who);
-    }
   }
-  return check_vectors(p, p->dx, p->lddx, who);
+  return check_overlaps(p, second ? BWD2 : BWD, who);
 }
 
 }  // namespace
@@ -935,11 +945,7 @@ extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
   if (p->rows == 0) return AGX_OK;
   AGX_TRY(check_mat(p, p->x, p->ldx, "agx_layernorm_fwd", "x"));
   AGX_TRY(check_mat(p, p->y, p->ldy, "agx_layernorm_fwd", "y"));
-  const int bytes = p->dtype == AGX_F32 ? 4 : 2;
-  AGX_CHECK_ARG((p->x == p->y && (p->ldx == p->ldy || p->rows == 1)) ||
-                    !agx::overlap({p->x, p->rows, p->width, p->ldx, bytes}, {p->y, p->rows, p->width, p->ldy, bytes}),
-                "agx_layernorm_fwd: y overlaps x without being the same matrix");
-  AGX_TRY(check_vectors(p, p->y, p->ldy, "agx_layernorm_fwd"));
+  AGX_TRY(check_overlaps(p, FWD, "agx_layernorm_fwd"));
   NormArgs a = {};
   a.x = p->x; a.ldx = p->ldx; a.y = p->y; a.ldy = p->ldy;
   a.gamma = p->gamma; a.beta = p->beta; a.mean = p->mean; a.rstd = p->rstd;
@@ -962,18 +968,7 @@ extern "C" int agx_layernorm_bwd2(void *stream, const agx_norm_t *p) {
   AGX_TRY(check_norm(p, "agx_layernorm_bwd2"));
   AGX_CHECK_ARG(!p->dbeta, "agx_layernorm_bwd2: the second-order pass has no term in beta");
   AGX_CHECK_ARG(p->dx || p->ddy || p->dgamma, "agx_layernorm_bwd2: no output wanted");
-  if (p->rows > 0) {
-    AGX_TRY(check_back(p, true, "agx_layernorm_bwd2"));
-    AGX_TRY(check_mat(p, p->u, p->ldu, "agx_layernorm_bwd2", "u"));
-    if (p->ddy) {
-      AGX_TRY(check_mat(p, p->ddy, p->ldddy, "agx_layernorm_bwd2", "ddy"));
-      AGX_TRY(check_out(p, p->ddy, p->ldddy, "agx_layernorm_bwd2"));
-      AGX_TRY(check_vectors(p, p->ddy, p->ldddy, "agx_layernorm_bwd2"));
-      const int bytes = p->dtype == AGX_F32 ? 4 : 2;
-      AGX_CHECK_ARG(!agx::overlap({p->dx, p->rows, p->width, p->lddx, bytes}, {p->ddy, p->rows, p->width, p->ldddy, bytes}),
-                    "agx_layernorm_bwd2: dx and ddy overlap");
-    }
-  }
+  if (p->rows > 0) AGX_TRY(check_back(p, true, "agx_layernorm_bwd2"));
   NormArgs a = back_args(p);
   a.u = p->u; a.ldu = p->ldu; a.ddy = p->ddy; a.ldddy = p->ldddy;
   return p->dtype == AGX_F32

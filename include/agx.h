@@ -164,8 +164,8 @@ int agx_bn_moving_update(void *stream, float *moving_mean, float *moving_var, co
  *         q = rstd (u - mean(u) - h mean(u h)):  ddy = act'(y) gamma q,  dgamma = sum dn q,
  *         dx = rstd^2 (h (3 mean(gh) mean(uh) + mean(g) mean(u) - mean(gu)) - mean(uh) (g - mean(g)) - mean(gh) (u - mean(u)))
  * act: 1 = leaky ReLU of `slope` (its derivative is taken from the sign of y, which bwd / bwd2 then need), 0 = none.
- * Any output but mean / rstd may be NULL in bwd / bwd2; an output may be the same matrix as an input, any other overlap is refused
- * (with the vectors too; parameter gradients may not go over gamma or the statistics).
+ * Any output but mean / rstd may be NULL in bwd / bwd2.  A result matrix may be the same matrix as an input (x, dy, u, y); any other
+ * overlap of what a call writes (y, mean, rstd of fwd; dx, ddy, dgamma, dbeta, ws of bwd / bwd2) with another operand is refused.
  * ws: needed where dgamma / dbeta are wanted: agx_layernorm_ws_floats covers every call, agx_layernorm_bwd_ws_floats a bwd whose dx
  * is none of its inputs (0 for few rows).  Sums in a fixed order.                                                     */
 #define AGX_F32 0

@@ -194,3 +194,42 @@ def test_outputs_overlap_inputs_only_as_the_same_matrix():
         assert lib.agx_layernorm_bwd2(None, desc(ddy=base + 8)) == -1 and 'overlaps' in err()
     assert lib.agx_layernorm_bwd2(None, desc(dx=28672, ddy=28672)) == -1 and 'dx and ddy' in err()
     assert lib.agx_layernorm_bwd(None, desc(dx=16384 + 8, act=1)) == -1 and 'overlaps' in err()
+
+
+@pytest.mark.parametrize('rows,width', [(40, 8), (2000, 300)])
+def test_whatever_a_call_writes_is_its_own(rows, width):
+    """Refused before any launch: vectors that a pass writes over its matrices, over each other and inside the workspace, and
+    the workspace over what is read.  (The sizes take the backward pass in one launch and in two.)"""
+    lib = _lib.load()
+    mb = 1 << 26
+
+    def desc(**kw):
+        d = _lib.NormDesc()
+        d.rows, d.width, d.eps, d.act = rows, width, 1e-3, 1
+        d.ldx = d.lddy = d.ldu = d.ldy = d.lddx = d.ldddy = width + 3
+        d.x, d.dy, d.u, d.y, d.dx, d.ddy, d.gamma, d.beta, d.mean, d.rstd, d.dgamma, d.dbeta, d.ws = (mb * k for k in range(1, 14))
+        d.ws_floats = lib.agx_layernorm_ws_floats(rows, width, 0)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+    at = {k: getattr(desc(), k) for k in ('x', 'dy', 'u', 'y', 'dx', 'ddy', 'gamma', 'beta', 'mean', 'rstd', 'dgamma', 'dbeta', 'ws')}
+    last = 4 * ((rows - 1) * (width + 3) + width - 1)                  # bytes to a matrix's last element
+    fwd, bwd, bwd2 = lib.agx_layernorm_fwd, lib.agx_layernorm_bwd, lib.agx_layernorm_bwd2
+    bad = [(fwd, dict(mean=at['x'])), (fwd, dict(rstd=at['x'] + last)), (fwd, dict(mean=at['gamma'])), (fwd, dict(rstd=at['beta'])),
+           (fwd, dict(mean=at['rstd'] + 4 * rows - 4)), (fwd, dict(mean=at['y'] + last))]
+    for g in ('dgamma', 'dbeta'):
+        bad += [(bwd, {g: at[m]}) for m in ('x', 'dy', 'y', 'dx', 'mean', 'rstd', 'gamma', 'ws')]
+        bad += [(bwd, {g: at[m] + last}) for m in ('x', 'dy', 'y', 'dx')]
+    bad += [(bwd, dict(dbeta=at['dgamma'])), (bwd, dict(dbeta=at['dgamma'] + 4 * width - 4)), (bwd, dict(dgamma=at['ws'] + 8))]
+    bad += [(bwd, dict(ws=at[m])) for m in ('x', 'dy', 'y', 'dx', 'gamma', 'mean', 'rstd')]
+    bad += [(bwd2, dict(dbeta=None, dgamma=at[m])) for m in ('x', 'dy', 'u', 'y', 'dx', 'ddy', 'mean', 'rstd', 'gamma', 'ws')]
+    bad += [(bwd2, dict(dbeta=None, ws=at[m])) for m in ('x', 'dy', 'u', 'y', 'dx', 'ddy', 'mean', 'rstd', 'gamma')]
+    for entry, kw in bad:
+        assert entry(None, desc(**kw)) == -1 and b' overlaps ' in lib.agx_last_error(), (entry.__name__, kw, lib.agx_last_error())
+    if torch.cuda.is_available():
+        return                                                         # (made-up addresses: nothing that passes is launched)
+    # what is told apart: neighbours, vectors in the padding behind a matrix's columns, a matrix over an input (no device: -2)
+    for entry, kw in ((fwd, dict(mean=at['x'] + last + 4)), (fwd, dict(y=at['x'])), (bwd, dict(dbeta=at['dgamma'] + 4 * width)),
+                      (bwd, dict(dx=at['dy'])), (bwd, dict(act=0, dgamma=at['y'])), (bwd2, dict(dbeta=None, dx=at['u'], ddy=at['x'])),
+                      (bwd, dict(dgamma=None, dbeta=None, ws=at['x']))):
+        assert entry(None, desc(**kw)) == -2, (entry.__name__, kw, lib.agx_last_error())
