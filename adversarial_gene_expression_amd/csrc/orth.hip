@@ -1470,6 +1470,14 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
     return AGX_E_WORKSPACE;
   }
   AGX_CHECK_ARG(agx::aligned16(ws), "%s: workspace must be 16-byte aligned", who);
+  for (int i = 0; i < n; ++i) {
+    const Job &j = jobs[i];
+    const int size = j.dtype == AGX_F32 ? 4 : 2;
+    const agx::Region used{ws, 1, need, need, 1};
+    for (const agx::Region &r : {agx::Region{j.x, j.rows, j.cols, j.ldx, size}, agx::Region{j.out, j.rows, j.cols, j.ldo, size},
+                                 agx::Region{j.m, j.rows, j.cols, j.ldm, size}})
+      AGX_CHECK_ARG(!agx::overlap(used, r), "%s: the workspace overlaps matrix %d", who, i);
+  }
   int tiles = 0, wide = 0;
   for (int i = 0; i < n; ++i) {
     tiles += jobs[i].tiles();

@@ -195,7 +195,8 @@ int agx_layernorm_bwd2(void *stream, const agx_norm_t *p);
  * X_0 = x / (|x|_F + eps); X <- X (a I + b A + c A^2), A = X^T X, `steps` times (A = X X^T from the left where
  * rows < cols): Newton-Schulz steps that bring the singular values of x towards 1.  n_coef: 1 (the same a, b, c for
  * every step) or `steps` triples.  min(rows, cols) <= AGX_ORTH_MAX_SIDE.  Products are fp32-accurate.
- * Matrices of a call are worked on at once: a result that shares memory with another one or with an x is refused.      */
+ * Matrices of a call are worked on at once: a result that shares memory with another one or with an x is refused, and so
+ * is a workspace that shares memory with any of them.                                                                  */
 #define AGX_MAX_ORTH 16
 #define AGX_ORTH_MAX_SIDE 4096
 #define AGX_ORTH_MAX_STEPS 16

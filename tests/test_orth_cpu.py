@@ -143,3 +143,32 @@ def test_matrices_of_a_call_may_not_share_what_is_written():
                 [(4096, 8192, 12288), (20480, 4096, 24576)], [(4096, 8192, 12288), (20480, 12288, 24576)], [(4096, 4096 + 8, 12288)]):
         assert muon(*bad) == -1 and 'different arrays' in err(), bad
     assert muon((4096, 8192, 12288), (16384, 8192, 20480)) == -3   # one gradient for two kernels is only read
+
+
+@pytest.mark.parametrize('rows,cols,ld,dtype', [(4, 6, 6, 0), (300, 70, 75, 1)])
+def test_workspace_over_a_matrix_is_refused(rows, cols, ld, dtype):
+    """Refused before any launch: the call's own workspace over what it reads or writes, from either end."""
+    lib = _lib.load()
+    mb = 1 << 24
+    size = 2 if dtype else 4
+    last = ((rows - 1) * ld + cols - 1) * size // 16 * 16
+    jobs = lambda cls: (cls * 2)()  # noqa: E731
+    j = jobs(_lib.OrthDesc)
+    for k, q in enumerate(j):
+        q.x, q.out, q.ldx, q.ldo, q.rows, q.cols, q.dtype = (1 + 2 * k) * mb, (2 + 2 * k) * mb, ld, ld, rows, cols, dtype
+    n = lib.agx_orth_ws_bytes(j, 2, 5)
+    places = [a + d for q in j for a in (q.x, q.out) for d in (0, last, 16 - n)]
+    for ws in places:
+        assert lib.agx_orthogonalize(None, j, 2, _opts(), ws, n) == -1 and b'workspace overlaps' in lib.agx_last_error(), ws / mb
+    o = _lib.MuonOpts()
+    o.orth, o.lr, o.momentum, o.nesterov = _opts(), 0.1, 0.9, 1
+    m = jobs(_lib.MuonDesc)
+    last = ((rows - 1) * ld + cols - 1) * 4 // 16 * 16
+    for k, q in enumerate(m):
+        q.w, q.g, q.m, q.ldw, q.ldg, q.ldm, q.rows, q.cols, q.scale = *((1 + 3 * k + i) * mb for i in range(3)), ld, ld, ld, rows, cols, 1.0
+    n = lib.agx_opt_muon_ws_bytes(m, 2, o)
+    for ws in [a + d for q in m for a in (q.w, q.g, q.m) for d in (0, last, 16 - n)]:
+        assert lib.agx_opt_muon(None, m, 2, o, ws, n) == -1 and b'workspace overlaps' in lib.agx_last_error(), ws / mb
+    if not torch.cuda.is_available():                     # (made-up addresses: what passes would be launched)
+        assert lib.agx_orthogonalize(None, j, 2, _opts(), 20 * mb, n) == -2 and lib.agx_opt_muon(None, m, 2, o, 20 * mb, n) == -2
+        assert lib.agx_orthogonalize(None, j, 2, _opts(), mb + (last + 256) // 16 * 16, lib.agx_orth_ws_bytes(j, 2, 5)) == -2
