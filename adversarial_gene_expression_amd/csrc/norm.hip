@@ -957,7 +957,7 @@ extern "C" int agx_layernorm_fwd(void *stream, const agx_norm_t *p) {
 extern "C" int agx_layernorm_bwd(void *stream, const agx_norm_t *p) {
   AGX_TRY(check_norm(p, "agx_layernorm_bwd"));
   if (p->rows > 0) AGX_TRY(check_back(p, false, "agx_layernorm_bwd"));
-  AGX_CHECK_ARG(p->dx || p->dgamma || p->dbeta, "agx_layernorm_bwd: no output wanted");
+  AGX_CHECK_ARG(p->dx || p->dgamma || p->dbeta || p->rows == 0, "agx_layernorm_bwd: no output wanted");
   const NormArgs a = back_args(p);
   return p->dtype == AGX_F32
              ? launch<BWD, float>(agx::as_stream(stream), a, p->dgamma, p->dbeta, p->accumulate_params)
@@ -967,7 +967,7 @@ extern "C" int agx_layernorm_bwd(void *stream, const agx_norm_t *p) {
 extern "C" int agx_layernorm_bwd2(void *stream, const agx_norm_t *p) {
   AGX_TRY(check_norm(p, "agx_layernorm_bwd2"));
   AGX_CHECK_ARG(!p->dbeta, "agx_layernorm_bwd2: the second-order pass has no term in beta");
-  AGX_CHECK_ARG(p->dx || p->ddy || p->dgamma, "agx_layernorm_bwd2: no output wanted");
+  AGX_CHECK_ARG(p->dx || p->ddy || p->dgamma || p->rows == 0, "agx_layernorm_bwd2: no output wanted");
   if (p->rows > 0) AGX_TRY(check_back(p, true, "agx_layernorm_bwd2"));
   NormArgs a = back_args(p);
   a.u = p->u; a.ldu = p->ldu; a.ddy = p->ddy; a.ldddy = p->ldddy;

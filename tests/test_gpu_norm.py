@@ -292,3 +292,13 @@ def test_second_order_over_its_inputs(gpu, width):
         d.dx, d.ddy, d.ws, d.ws_floats = m[dx_over].data_ptr(), m[ddy_over].data_ptr(), ws.data_ptr(), ws.numel()
         _lib.check(lib.agx_layernorm_bwd2(_dev.stream(), d), 'agx_layernorm_bwd2')
         assert torch.equal(m[ddy_over], want[0]) and torch.equal(m[dx_over], want[1]) and torch.equal(dg, want[2])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_no_rows_without_parameter_gradients(gpu, dtype):
+    from adversarial_gene_expression_amd import ops
+    x, v = torch.zeros(0, 24, device='cuda', dtype=dtype), torch.zeros(0, device='cuda')
+    dx, dg, db = ops.layer_norm_backward(x, x, v, v, param_grads=False)
+    assert dx.shape == (0, 24) and dx.dtype == dtype and dg is None and db is None
+    ddy, dx, dg = ops.layer_norm_backward2(x, x, x, v, v, y=x, act=1, param_grads=False)
+    assert ddy.shape == dx.shape == (0, 24) and dg is None

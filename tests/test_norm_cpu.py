@@ -233,3 +233,15 @@ def test_whatever_a_call_writes_is_its_own(rows, width):
                       (bwd, dict(dx=at['dy'])), (bwd, dict(act=0, dgamma=at['y'])), (bwd2, dict(dbeta=None, dx=at['u'], ddy=at['x'])),
                       (bwd, dict(dgamma=None, dbeta=None, ws=at['x']))):
         assert entry(None, desc(**kw)) == -2, (entry.__name__, kw, lib.agx_last_error())
+
+
+def test_no_rows_ask_for_nothing():
+    """An empty matrix has no address: a backward pass without parameter gradients over it is no missing output."""
+    lib = _lib.load()
+    d = _lib.NormDesc()
+    d.rows, d.width, d.eps, d.ldx, d.lddy, d.ldu, d.ldy, d.lddx, d.ldddy = 0, 8, 1e-3, 8, 8, 8, 8, 8, 8
+    for entry in (lib.agx_layernorm_fwd, lib.agx_layernorm_bwd, lib.agx_layernorm_bwd2):
+        assert entry(None, d) == 0, entry.__name__
+    d.dtype = 7                                           # (what is malformed stays refused)
+    for entry in (lib.agx_layernorm_fwd, lib.agx_layernorm_bwd, lib.agx_layernorm_bwd2):
+        assert entry(None, d) == -1, entry.__name__
