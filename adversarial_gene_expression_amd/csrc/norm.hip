@@ -691,26 +691,31 @@ __global__ __launch_bounds__(256) void ln_columns_kernel(NormArgs a) {
   }
 }
 
-// out_q[j] (+)= sum over workgroups b of part[b][q][j], b in a fixed order: 32 columns by 32 interleaved shares a workgroup
+// out_q[j] (+)= sum over workgroups b of part[b][q][j], b in a fixed order: 32 columns by 32 interleaved shares a workgroup, which
+// takes every gridDim.x-th such piece (a launch has fewer than 2^32 threads along x: 2^27 columns at a piece a workgroup)
+constexpr int MAX_PIECES = 1 << 20;
 __global__ __launch_bounds__(1024) void ln_param_kernel(const float *__restrict__ part, int nb, int64_t n, float *dgamma,
                                                         float *dbeta, int accumulate) {
   __shared__ float red[32][33];
   float *out = blockIdx.y ? dbeta : dgamma;
   if (!out) return;
   const int col = threadIdx.x & 31, sh = threadIdx.x >> 5;
-  const int64_t j = (int64_t)blockIdx.x * 32 + col;
-  float s = 0.f;
-  if (j < n) {
+  for (int64_t j0 = (int64_t)blockIdx.x * 32; j0 < n; j0 += (int64_t)gridDim.x * 32) {
+    const int64_t j = j0 + col;
+    float s = 0.f;
+    if (j < n) {
 #pragma unroll 8
-    for (int b = sh; b < nb; b += 32) s += part[((int64_t)b * 2 + blockIdx.y) * n + j];
-  }
-  red[sh][col] = s;
-  __syncthreads();
-  if (sh == 0 && j < n) {
-    s = 0.f;
+      for (int b = sh; b < nb; b += 32) s += part[((int64_t)b * 2 + blockIdx.y) * n + j];
+    }
+    red[sh][col] = s;
+    __syncthreads();
+    if (sh == 0 && j < n) {
+      s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) s += red[k][col];
-    out[j] = accumulate ? out[j] + s : s;
+      for (int k = 0; k < 32; ++k) s += red[k][col];
+      out[j] = accumulate ? out[j] + s : s;
+    }
+    __syncthreads();
   }
 }
 
@@ -837,8 +842,8 @@ int launch(hipStream_t st, const NormArgs &a, float *dgamma, float *dbeta, int a
     AGX_LAUNCH_CHECK();
   }
   if (dgamma || dbeta) {
-    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)agx::cdiv64(a.n, 32), 2), dim3(1024), 0, st, a.part, parts ? parts : blocks, a.n,
-                       dgamma, dbeta, accumulate);
+    hipLaunchKernelGGL(ln_param_kernel, dim3((unsigned)std::min<int64_t>(agx::cdiv64(a.n, 32), MAX_PIECES), 2), dim3(1024), 0, st, a.part,
+                       parts ? parts : blocks, a.n, dgamma, dbeta, accumulate);
     AGX_LAUNCH_CHECK();
   }
   return AGX_OK;

@@ -156,7 +156,7 @@ int agx_bn_moving_update(void *stream, float *moving_mean, float *moving_var, co
                          float momentum, int32_t N);
 
 /* ---- layer normalisation of hidden layers (no reference counterpart: tf_utils.py:85-88 has no normalisation) ----
- * Rows [rows, width] of fp32 or bf16 values with a leading dimension in ELEMENTS; parameters, statistics and parameter
+ * Rows [rows, width <= 2^28] of fp32 or bf16 values with a leading dimension in ELEMENTS; parameters, statistics and parameter
  * gradients are fp32.  With h = (x - mean) * rstd, n = gamma * h + beta, y = act(n), mean(.) over a row:
  *   fwd   writes y and, where given, mean / rstd (rstd = 1 / sqrt(mean((x - mean)^2) + eps))
  *   bwd   dn = act'(y) dy, g = gamma dn:  dx = rstd (g - mean(g) - h mean(g h)), dgamma = sum dn h, dbeta = sum dn

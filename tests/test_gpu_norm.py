@@ -302,3 +302,46 @@ def test_no_rows_without_parameter_gradients(gpu, dtype):
     assert dx.shape == (0, 24) and dx.dtype == dtype and dg is None and db is None
     ddy, dx, dg = ops.layer_norm_backward2(x, x, x, v, v, y=x, act=1, param_grads=False)
     assert ddy.shape == dx.shape == (0, 24) and dg is None
+
+
+def test_rows_of_more_values_than_a_launch_has_threads(gpu):
+    """Two rows of 2^27 + 40 bf16 values, odd stride: 32 threads a column of the parameter gradients would be more than 2^32.
+    The values are -1, 0 and 1 and mean / rstd 0 / 1: a thread's sums over a row are integers of at most 2^17 + 1, a wave's
+    of 2^23 + 64, all exact, and with random signs so are the workgroup's (below 2^20, asserted of the whole).  What is left is
+    a rounding each of a mean, its product, two differences and dn q or the sum over the rows, of values up to 3: 8 * 3 e; and
+    half a bf16 step."""
+    from adversarial_gene_expression_amd import ops
+    n = (1 << 27) + 40
+    g = torch.Generator(device='cuda').manual_seed(5)
+    mk = lambda: torch.randint(-1, 2, (2, n + 1), generator=g, device='cuda', dtype=torch.int8).to(torch.bfloat16)[:, :n]  # noqa: E731
+    x, dy, u = mk(), mk(), mk()
+    mean, rstd = torch.zeros(2, device='cuda'), torch.ones(2, device='cuda')
+
+    def means(a, r):
+        out = float(a[r].double().mean()), float((a[r].double() * x[r].double()).mean())
+        assert max(abs(v) * n for v in out) < 2 ** 20
+        return out
+
+    def check(got, want):
+        assert float(((got.float() - want).abs() - 2.0 ** -8 * want.abs()).max()) <= 24 * E
+    dx, dg, db = ops.layer_norm_backward(dy, x, mean, rstd)
+    assert torch.equal(dg, (dy.float() * x.float()).sum(0)) and torch.equal(db, dy.float().sum(0))
+    for r in range(2):
+        mg, mgh = means(dy, r)
+        check(dx[r], dy[r].float() - mg - x[r].float() * mgh)
+    ddy, dx2, dg2 = ops.layer_norm_backward2(u, dy, x, mean, rstd)
+    total = torch.zeros(n, device='cuda')
+    for r in range(2):
+        mu, muh = means(u, r)
+        q = u[r].float() - mu - x[r].float() * muh
+        check(ddy[r], q)
+        total += dy[r].float() * q
+    assert float((dg2 - total).abs().max()) <= 48 * E
+    y, m, s = ops.layer_norm(x, eps=1.0)
+    for r in range(2):
+        mu = float(x[r].double().mean())
+        var = float(((x[r].double() - mu) ** 2).mean())
+        # (the mean: an exact sum over n as a float - 2^27 + 40 is none, off by 8 of 2^27, a rounding - and the quotient's own;
+        #  the variance: 2^17 + 5 additions of a thread's squares, halved by the root)
+        assert abs(float(m[r]) - mu) <= 2 * E * abs(mu) and abs(float(s[r]) - (var + 1) ** -0.5) <= 2.0 ** -7
+        check(y[r], (x[r].float() - float(m[r])) * float(s[r]))
