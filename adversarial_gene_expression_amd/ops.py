@@ -259,6 +259,16 @@ def _orth_opts(o, steps, coefficients, eps):
     return o
 
 
+def _kernel(t, name, like=None):
+    """_matrix of an operand that has rows, and sides that the descriptors' 32 bits hold."""
+    ld = _matrix(t, name, like)
+    if t.shape[0] == 0:
+        raise ValueError('%s has no rows' % name)
+    if max(t.shape) >= 1 << 31:
+        raise ValueError('%s is too large: %s' % (name, tuple(t.shape)))
+    return ld
+
+
 def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Newton-Schulz orthogonalisation of a matrix (float32 or bfloat16), or of each of a list of them (one call's launches
     are shared by up to 16): X_0 = x / (|x|_F + eps), then `steps` times X <- X (a I + b A + c A^2) with A = X^T X (from
@@ -267,7 +277,7 @@ def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     one = isinstance(x, torch.Tensor)
     xs = [x] if one else list(x)
     o = _orth_opts(_lib.OrthOpts(), steps, coefficients, eps)
-    lds = [_matrix(t, 'x') for t in xs]
+    lds = [_kernel(t, 'x') for t in xs]
     for t in xs:
         _on_current(t)
     lib, outs = _lib.load(), []
@@ -301,7 +311,7 @@ def muon(w, g, m, lr, *, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5
     for a, b, c in zip(ws_, gs, ms):
         if not isinstance(a, torch.Tensor) or a.dtype != torch.float32:
             raise ValueError('w must be float32')
-        lds.append((_matrix(a, 'w'), _matrix(b, 'g', a), _matrix(c, 'm', a)))
+        lds.append((_kernel(a, 'w'), _kernel(b, 'g', a), _kernel(c, 'm', a)))
     for a in ws_:
         _on_current(a)
     lib = _lib.load()

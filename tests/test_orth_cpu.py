@@ -172,3 +172,13 @@ def test_workspace_over_a_matrix_is_refused(rows, cols, ld, dtype):
     if not torch.cuda.is_available():                     # (made-up addresses: what passes would be launched)
         assert lib.agx_orthogonalize(None, j, 2, _opts(), 20 * mb, n) == -2 and lib.agx_opt_muon(None, m, 2, o, 20 * mb, n) == -2
         assert lib.agx_orthogonalize(None, j, 2, _opts(), mb + (last + 256) // 16 * 16, lib.agx_orth_ws_bytes(j, 2, 5)) == -2
+
+
+@pytest.mark.parametrize('shape,said', [((0, 6), 'no rows'), (((1 << 32) + 4, 2), 'too large'), ((2, (1 << 32) + 4), 'too large'),
+                                        ((1 << 31, 1), 'too large')])
+def test_refuses_empty_matrices_and_sides_beyond_32_bits(shape, said):
+    """Sides go to the library in 32 bits: 2^32 + 4 rows would have been taken for 4."""
+    x = torch.empty(*shape, device='meta')
+    for call in (lambda: ops.orthogonalize(x), lambda: ops.orthogonalize([torch.zeros(4, 6), x]), lambda: ops.muon(x, x, x, 0.1)):
+        with pytest.raises(ValueError, match=said):
+            call()
