@@ -253,6 +253,7 @@ SIGNATURES = {
     'agx_orthogonalize': (C.c_int, [_vp, C.POINTER(OrthDesc), _i32, C.POINTER(OrthOpts), _vp, _i64]),
     'agx_opt_muon_ws_bytes': (_i64, [C.POINTER(MuonDesc), _i32, C.POINTER(MuonOpts)]),
     'agx_opt_muon': (C.c_int, [_vp, C.POINTER(MuonDesc), _i32, C.POINTER(MuonOpts), _vp, _i64]),
+    'agx_opt_muon_check': (C.c_int, [C.POINTER(MuonDesc), _i32, C.POINTER(MuonOpts)]),
     'agx_op_sizeof': (_i64, [_i32]),
     'agx_embed_concat_fwd': (C.c_int, [_vp, C.POINTER(EmbedDesc), _vp, _vp, _i32, _i32, _vp, _i32, _i32,
                                        _vp, _i32, _i32, _i32, _vp, _i32]),

@@ -1851,14 +1851,15 @@ extern "C" int64_t agx_opt_muon_ws_bytes(const agx_muon_t *jobs, int32_t n, cons
   return ws_bytes(j, n, o->orth.steps, o->nesterov && o->momentum != 0.f);
 }
 
-extern "C" int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o, void *ws, int64_t ws_size) {
-  const char *who = "agx_opt_muon";
+// What is checked of a step's arguments apart from the workspace, over any number of matrices
+static int check_muon(const agx_muon_t *jobs, int n, const agx_muon_opts_t *o, const char *who) {
   AGX_CHECK_ARG(o, "%s: options missing", who);
   AGX_TRY(check_opts(&o->orth, who));
   AGX_CHECK_ARG(o->momentum >= 0.f && o->momentum < 1.f, "%s: momentum must be in [0, 1)", who);
   AGX_CHECK_ARG(std::isfinite(o->lr) && std::isfinite(o->weight_decay), "%s: learning rate / weight decay must be finite", who);
+  AGX_CHECK_ARG(jobs && n >= 1, "%s: no matrices", who);
   Job j[AGX_MAX_ORTH];
-  AGX_TRY(muon_jobs(jobs, n, o, j, who));
+  for (int lo = 0; lo < n; lo += AGX_MAX_ORTH) AGX_TRY(muon_jobs(jobs + lo, std::min(n - lo, AGX_MAX_ORTH), o, j, who));
   for (int i = 0; i < n; ++i) {
     const agx_muon_t &a = jobs[i];
     AGX_CHECK_ARG(a.w && a.g && a.m && a.ldw >= a.cols && a.ldg >= a.cols && a.ldm >= a.cols && a.ldm < (1 << 23) && std::isfinite(a.scale),
@@ -1874,7 +1875,20 @@ extern "C" int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, con
       const agx::Region w = region(jobs[i].w, i, jobs[i].ldw), m = region(jobs[i].m, i, jobs[i].ldm), g = region(jobs[k].g, k, jobs[k].ldg);
       const agx::Region wk = region(jobs[k].w, k, jobs[k].ldw), mk = region(jobs[k].m, k, jobs[k].ldm);
       AGX_CHECK_ARG(!agx::overlap(w, g) && !agx::overlap(m, g) && !agx::overlap(w, mk) && (k <= i || (!agx::overlap(w, wk) && !agx::overlap(m, mk))),
-                    "%s: w, g and m of matrices %d and %d must be different arrays", who, i, k);
+                    "%s: w, g and m of matrices %d and %d must be different arrays", who, std::min(i, k), std::max(i, k));
     }
+  return AGX_OK;
+}
+
+extern "C" int agx_opt_muon_check(const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o) {
+  return check_muon(jobs, n, o, "agx_opt_muon_check");
+}
+
+extern "C" int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o, void *ws, int64_t ws_size) {
+  const char *who = "agx_opt_muon";
+  AGX_CHECK_ARG(n <= AGX_MAX_ORTH, "%s: 1 to %d matrices a call", who, AGX_MAX_ORTH);
+  AGX_TRY(check_muon(jobs, n, o, who));
+  Job j[AGX_MAX_ORTH];
+  AGX_TRY(muon_jobs(jobs, n, o, j, who));
   return run(agx::as_stream(stream), j, n, &o->orth, o->momentum, o->nesterov != 0, static_cast<char *>(ws), ws_size, who);
 }

@@ -300,7 +300,7 @@ def muon(w, g, m, lr, *, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5
          scale=None):
     """One Muon step in place on float32 kernels w [in, out] (or lists of them) with gradients g and momentum buffers m:
     m <- momentum m + g; u = g + momentum m (nesterov) or m; w <- (1 - lr weight_decay) w - lr scale orthogonalize(u).
-    scale: default sqrt(max(1, out / in)) per kernel; a number applies to all."""
+    scale: default sqrt(max(1, out / in)) per kernel; a number applies to all.  A refused call changes nothing."""
     ws_, gs, ms = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (w, g, m))
     if not len(ws_) == len(gs) == len(ms):
         raise ValueError('w, g and m must be as many: got %d, %d, %d' % (len(ws_), len(gs), len(ms)))
@@ -314,19 +314,28 @@ def muon(w, g, m, lr, *, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5
         lds.append((_kernel(a, 'w'), _kernel(b, 'g', a), _kernel(c, 'm', a)))
     for a in ws_:
         _on_current(a)
-    lib = _lib.load()
-    for lo in range(0, len(ws_), _lib.AGX_MAX_ORTH):
-        part = list(zip(ws_, gs, ms, lds))[lo:lo + _lib.AGX_MAX_ORTH]
-        jobs = (_lib.MuonDesc * len(part))()
-        for j, (a, b, c, ld) in zip(jobs, part):
-            j.w, j.g, j.m = a.data_ptr(), b.data_ptr(), c.data_ptr()
-            j.ldw, j.ldg, j.ldm = ld
-            j.rows, j.cols = a.shape
-            j.scale = max(1.0, a.shape[1] / a.shape[0]) ** 0.5 if scale is None else scale
-        n = int(lib.agx_opt_muon_ws_bytes(jobs, len(part), o))
-        _lib.check(0 if n >= 0 else n, 'agx_opt_muon_ws_bytes')
-        ws = torch.empty(n, dtype=torch.uint8, device=part[0][0].device)
-        _lib.check(lib.agx_opt_muon(_dev.stream(), jobs, len(part), o, ws.data_ptr(), n), 'agx_opt_muon')
+    if not ws_:
+        return
+    # (all that can be refused or run out of memory before the first launch: a step is taken whole or not at all)
+    lib, most = _lib.load(), _lib.AGX_MAX_ORTH
+    jobs = (_lib.MuonDesc * len(ws_))()
+    for j, a, b, c, ld in zip(jobs, ws_, gs, ms, lds):
+        j.w, j.g, j.m = a.data_ptr(), b.data_ptr(), c.data_ptr()
+        j.ldw, j.ldg, j.ldm = ld
+        j.rows, j.cols = a.shape
+        j.scale = max(1.0, a.shape[1] / a.shape[0]) ** 0.5 if scale is None else scale
+    if len(ws_) > most:
+        _lib.check(lib.agx_opt_muon_check(jobs, len(ws_), o), 'agx_opt_muon_check')
+    calls = []
+    for lo in range(0, len(ws_), most):
+        n = min(most, len(ws_) - lo)
+        part = (_lib.MuonDesc * n).from_buffer(jobs, lo * _lib.C.sizeof(_lib.MuonDesc))
+        size = int(lib.agx_opt_muon_ws_bytes(part, n, o))
+        _lib.check(0 if size >= 0 else size, 'agx_opt_muon_ws_bytes')
+        calls.append((part, n, size))
+    ws = torch.empty(max(size for _, _, size in calls), dtype=torch.uint8, device=ws_[0].device)
+    for part, n, size in calls:
+        _lib.check(lib.agx_opt_muon(_dev.stream(), part, n, o, ws.data_ptr(), size), 'agx_opt_muon')
 
 
 def rng(n, seed, offset=0, normal=True):

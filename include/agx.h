@@ -234,6 +234,9 @@ typedef struct agx_muon_opts {
 } agx_muon_opts_t;
 int64_t agx_opt_muon_ws_bytes(const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o);
 int agx_opt_muon(void *stream, const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o, void *ws, int64_t ws_size);
+/* All that agx_opt_muon refuses, but of its workspace, over any n matrices; nothing is launched.  For a step of more matrices
+ * than a call takes: checked as a whole, before the first call.                                                        */
+int agx_opt_muon_check(const agx_muon_t *jobs, int32_t n, const agx_muon_opts_t *o);
 /* sizeof() of agx_norm_t (0), agx_orth_t (1), agx_orth_opts_t (2), agx_muon_t (3), agx_muon_opts_t (4), -1 otherwise */
 int64_t agx_op_sizeof(int32_t which);
 

@@ -257,3 +257,23 @@ def test_large_sides(gpu, rows, cols, dtype):
     want = oracle(d)
     tol = 16 * err(oracle(d * (1 + sign * 2.0 ** -21)), want) + 2.0 ** -20
     assert err(got.double(), want) <= tol + half(dtype), (err(got.double(), want), tol)
+
+
+def test_a_refused_step_of_many_kernels_changes_nothing(gpu):
+    """More kernels than one launch takes: a refusal of the last one, or one kernel twice, comes before any is stepped; without
+    it all of them are."""
+    from adversarial_gene_expression_amd import AgxError, ops
+    ks = _kernels(80, [(20 + k, 40 - k) for k in range(18)])
+    ws, gs, ms = (list(t) for t in zip(*ks))
+    big = [torch.zeros(4097, 4098, device=gpu) for _ in range(3)]
+    for last in (big, (ws[0], gs[17], torch.zeros_like(ws[0])), (ws[17], gs[17], ms[0][:1].expand(1, -1))):
+        before = [t.clone() for t in ws + ms]
+        with pytest.raises((AgxError, ValueError)):
+            ops.muon(ws[:17] + [last[0]], gs[:17] + [last[1]], ms[:17] + [last[2]], 0.02)
+        assert all(torch.equal(a, b) for a, b in zip(before, ws + ms))
+    apart = [[t.clone() for t in k] for k in ks]
+    ops.muon(ws, gs, ms, 0.02)
+    for lo, hi in ((0, 16), (16, 18)):
+        ops.muon(*zip(*apart[lo:hi]), 0.02)
+    for (w, _, m), (w2, _, m2) in zip(ks, apart):
+        assert torch.equal(w, w2) and torch.equal(m, m2)

@@ -182,3 +182,32 @@ def test_refuses_empty_matrices_and_sides_beyond_32_bits(shape, said):
     for call in (lambda: ops.orthogonalize(x), lambda: ops.orthogonalize([torch.zeros(4, 6), x]), lambda: ops.muon(x, x, x, 0.1)):
         with pytest.raises(ValueError, match=said):
             call()
+
+
+def test_muon_steps_of_any_number_of_kernels_are_checked_at_once():
+    """agx_opt_muon_check: the step's own refusals, over more kernels than a call takes, and nothing is launched."""
+    lib = _lib.load()
+    mb = 1 << 20
+    o = _lib.MuonOpts()
+    o.orth, o.lr, o.momentum, o.nesterov = _opts(), 0.1, 0.9, 1
+
+    def jobs(n, **kw):                                     # kw: of the last one
+        j = (_lib.MuonDesc * n)()
+        for k, q in enumerate(j):
+            q.w, q.g, q.m, q.ldw, q.ldg, q.ldm, q.rows, q.cols, q.scale = *((3 * k + i) * mb for i in (1, 2, 3)), 6, 6, 6, 4, 6, 1.0
+        for k, v in kw.items():
+            setattr(j[n - 1], k, v)
+        return j
+    check = lambda n, o=o, **kw: lib.agx_opt_muon_check(jobs(n, **kw), n, o)  # noqa: E731
+    for n in (1, 16, 17, 40):
+        assert check(n) == 0 and check(n, g=2 * mb) == 0   # (one gradient for two kernels is only read)
+    for kw in (dict(w=mb), dict(w=3 * mb), dict(w=2 * mb), dict(m=mb), dict(m=2 * mb), dict(m=3 * mb + 92), dict(g=mb), dict(g=3 * mb)):
+        assert check(18, **kw) == -1 and b'matrices 0 and 17' in lib.agx_last_error(), kw
+    for kw in (dict(rows=0), dict(rows=5000, cols=4097), dict(scale=float('inf')), dict(ldm=5), dict(w=None), dict(g=2 * mb + 1),
+               dict(ldg=1 << 23)):
+        assert check(18, **kw) == -1, kw
+    assert check(0) == -1 and lib.agx_opt_muon_check(None, 1, o) == -1 and lib.agx_opt_muon_check(jobs(1), 1, None) == -1
+    o.momentum = 1.0
+    assert check(18) == -1
+    o.momentum, o.orth.steps = 0.9, 0
+    assert check(18) == -1
