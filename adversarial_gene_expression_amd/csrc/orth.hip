@@ -7,11 +7,13 @@
 // way (phase_of); then X Q is formed and its Gram matrix computed anew.
 // Matrices of n x n are symmetric: tiles on and above the diagonal are computed and mirrored.
 //
-// Products run on the fp16 matrix cores at fp32 accuracy: every operand is split into two fp16 terms, v 2^e = hi + lo (22
-// bits), and hi.hi + hi.lo + lo.hi are accumulated in fp32 (lo.lo is below 2^-22 of the product).  e comes from the
-// largest |x| for the caller's matrix (first launch) and from a bound on the spectral norm, worked out on the host, for
-// everything behind it: entries then stay under 2^14, and those down to 2^-25 of the bound keep all bits.  A bf16 operand
-// needs one term only (its 8 bits fit).
+// Products run on the fp16 matrix cores: every operand is split into two fp16 terms, v 2^e = hi + lo (22 bits where fp32 has
+// 24), and hi.hi + hi.lo + lo.hi are accumulated in fp32 (lo.lo is below 2^-22 of the product).  e is one for a matrix: from the
+// largest |x| for the caller's (first launch), from a bound on the spectral norm, worked out on the host, for everything
+// behind it.  Entries then stay under 2^14, the largest (or the bound) at 2^13 or more; fp16's last bit is 2^-24, so that an
+// entry down to 2^-16 of the largest keeps its 22 bits and any is off by at most 2^-38 of the largest: rows or columns
+// that are far smaller than the others come out less exactly than in fp32 (a block at 1e-5 of the rest to 2e-6, at 1e-6 to 2e-5).  A bf16
+// operand needs one term only: its 8 bits fit, down to the same 2^-38.
 //
 // Launches of a call: the momentum step with |x|'s maximum and norm; then, a phase each, the Gram matrix (and the sum of its
 // slices), its polynomial (n <= 128 one launch a phase, n <= 256 one a step, above three a step) and the product with the

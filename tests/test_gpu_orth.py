@@ -277,3 +277,42 @@ def test_a_refused_step_of_many_kernels_changes_nothing(gpu):
         ops.muon(*zip(*apart[lo:hi]), 0.02)
     for (w, _, m), (w2, _, m2) in zip(ks, apart):
         assert torch.equal(w, w2) and torch.equal(m, m2)
+
+
+@pytest.mark.parametrize('rows,cols,split', [(400, 128, (200, 64)), (128, 400, (64, 200)), (400, 128, (200, 0)), (700, 300, (350, 150)),
+                                             (90, 60, (30, 20)), (300, 700, (0, 350))])
+@pytest.mark.parametrize('small', [1.0, 1e-4, 1e-5, 1e-6, 1e-7])
+def test_parts_far_smaller_than_the_rest(gpu, rows, cols, split, small):
+    """Rows behind split[0] and columns behind split[1] at `small` of the others, each part judged by itself: two blocks that
+    nothing couples, or (a 0) small rows or columns of one matrix.  Allowed, of a part's norm: 16 responses to 2^-21 as
+    above, and what the storage of X and of the iterates between phases (every two steps, three for sides above 256) leaves
+    out: an entry is off by at most 2^-25 where the largest, or the bound s on the singular values, is at 2^13 or more, so
+    by 2^-38 of it, which the steps behind it multiply as they do the entry; twice that, since a part's directions are
+    not multiplied alike."""
+    from adversarial_gene_expression_amd import ops
+    x = randn(rows + cols, rows, cols)
+    r, c = split
+    if r and c:
+        x[:r, c:] = 0
+        x[r:, :c] = 0
+    x[r:, c:] *= small
+    parts = [(slice(0, r), slice(0, c) if c else slice(None)), (slice(r, None), slice(c, None))] if r else \
+        [(slice(None), slice(0, c)), (slice(None), slice(c, None))]
+    got = N.t64(ops.orthogonalize(x.to(gpu)))
+    X = N.t64(x)
+    sign = torch.randint(0, 2, x.shape, generator=torch.Generator().manual_seed(1)).double() * 2 - 1
+    norm = float(torch.linalg.vector_norm(X))
+    a, b, d = 3.4445, -4.7750, 2.0315
+    every, s = 2 if min(rows, cols) <= 256 else 3, 1.0
+    stored = [(X / norm, float(X.abs().max()) / norm)]
+    for k in range(1, 5):
+        t = torch.linspace(0, s, 100001, dtype=torch.float64)
+        s = 1.001 * float((a * t + b * t ** 3 + d * t ** 5).abs().max())
+        if k % every == 0:
+            stored.append((N.orthogonalize(X, steps=k), s))
+    want, moved = N.orthogonalize(X), N.orthogonalize(X * (1 + sign * 2.0 ** -21))
+    for p in parts:
+        n = torch.linalg.vector_norm
+        tol = 16 * float(n((moved - want)[p]) / n(want[p])) + 16 * 2.0 ** -24
+        tol += sum(2 * 2.0 ** -38 * bound * v[p].numel() ** 0.5 / float(n(v[p])) for v, bound in stored)
+        assert float(n((got - want)[p]) / n(want[p])) <= tol, (p, float(n((got - want)[p]) / n(want[p])), tol)
