@@ -270,12 +270,12 @@ def _kernel(t, name, like=None):
 
 
 def orthogonalize(x, *, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
-    """Newton-Schulz orthogonalisation of a matrix (float32 or bfloat16), or of each of a list of them (one call's launches
-    are shared by up to 16): X_0 = x / (|x|_F + eps), then `steps` times X <- X (a I + b A + c A^2) with A = X^T X (from
-    the left with A = X X^T where rows < cols).  Products of operands of 22 bits, summed in float32, one rounding to x's type
-    at the end: errors are those of the float32 iteration relative to the matrix's largest entries; an entry below 2^-16 of the
-    largest is held to 2^-38 of that.  The smaller side may be at most 4096.  coefficients: (a, b, c), or one such triple per
-    step."""
+    """Newton-Schulz orthogonalisation of a matrix (float32 or bfloat16), or of each of a list of them: X_0 = x / (|x|_F + eps),
+    then `steps` times X <- X (a I + b A + c A^2) with A = X^T X (from the left with A = X X^T where rows < cols).  Products of
+    operands of 22 bits, summed in float32, one rounding to x's type at the end: errors are those of the float32 iteration
+    relative to the matrix's largest entries; an entry below 2^-16 of the largest is held to 2^-38 of that.  Launches are
+    shared by up to 16 matrices, whose sums are then split alike: a result's rounding depends on its companions.  The smaller
+    side may be at most 4096.  coefficients: (a, b, c), or one such triple per step."""
     one = isinstance(x, torch.Tensor)
     xs = [x] if one else list(x)
     o = _orth_opts(_lib.OrthOpts(), steps, coefficients, eps)

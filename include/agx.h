@@ -196,6 +196,8 @@ int agx_layernorm_bwd2(void *stream, const agx_norm_t *p);
  * rows < cols): Newton-Schulz steps that bring the singular values of x towards 1.  n_coef: 1 (the same a, b, c for
  * every step) or `steps` triples.  min(rows, cols) <= AGX_ORTH_MAX_SIDE.  Products take operands of 22 bits and are summed
  * in fp32; an entry below 2^-16 of its matrix's largest is held to 2^-38 of that, not to 22 bits of its own.
+ * How the sums of a product are split, and how many steps lie between two Gram matrices, is chosen for a call: the same call
+ * gives the same bits, a matrix among others the rounding of another order of sums than by itself.
  * Matrices of a call are worked on at once: a result that shares memory with another one or with an x is refused, and so
  * is a workspace that shares memory with any of them.                                                                  */
 #define AGX_MAX_ORTH 16

@@ -316,3 +316,19 @@ def test_parts_far_smaller_than_the_rest(gpu, rows, cols, split, small):
         tol = 16 * float(n((moved - want)[p]) / n(want[p])) + 16 * 2.0 ** -24
         tol += sum(2 * 2.0 ** -38 * bound * v[p].numel() ** 0.5 / float(n(v[p])) for v, bound in stored)
         assert float(n((got - want)[p]) / n(want[p])) <= tol, (p, float(n((got - want)[p]) / n(want[p])), tol)
+
+
+def test_companions_change_roundings_only(gpu):
+    """The same list gives the same bits; a matrix by itself or among others - one of a side up to 256 makes the larger ones
+    take two steps a phase instead of three - what the tolerance of each allows, taken twice."""
+    from adversarial_gene_expression_amd import ops
+    shapes = [(300, 700), (40, 64), (600, 530), (900, 260)] + [(30 + 9 * k, 200 - 5 * k) for k in range(14)]
+    xs = [even(r, c, 11 * k).to(gpu).to(torch.bfloat16 if k % 4 == 3 else torch.float32) for k, (r, c) in enumerate(shapes)]
+    together = ops.orthogonalize(xs)
+    assert all(torch.equal(a, b) for a, b in zip(together, ops.orthogonalize(xs)))
+    large = [xs[k] for k in (0, 2, 3)]
+    for lists, results in ((xs, together), (large, ops.orthogonalize(large))):
+        for x, y in zip(lists, results):
+            alone = ops.orthogonalize(x)
+            _, tol = allowed(x)
+            assert alone.dtype == y.dtype and rel(y, N.t64(alone)) <= 2 * (tol + half(x.dtype)), x.shape
