@@ -1352,15 +1352,19 @@ int joined_kind(int kind, bool tall, int dtype) {
   const int k = (tall ? 0 : 1) + (dtype != AGX_F32 ? 2 : 0);
   return kind < 0 || kind == k ? k : ANY;
 }
-template <class F> void by_kind(int kind, F f) {
+// calls f with the kind as a constant: what a caller's matrices are, or the iterate's planes too
+template <class F> void by_user_kind(int kind, F f) {
   switch (kind) {
     case 0: f(std::integral_constant<int, 0>{}); break;
     case 1: f(std::integral_constant<int, 1>{}); break;
     case 2: f(std::integral_constant<int, 2>{}); break;
     case 3: f(std::integral_constant<int, 3>{}); break;
-    case ITERATE: f(std::integral_constant<int, ITERATE>{}); break;
     default: f(std::integral_constant<int, ANY>{});
   }
+}
+template <class F> void by_kind(int kind, F f) {
+  if (kind == ITERATE) f(std::integral_constant<int, ITERATE>{});
+  else by_user_kind(kind, f);
 }
 
 int64_t longest(const Job *jobs, int n) {               // steps of the longest of a call's Gram products
@@ -1587,7 +1591,7 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
         r.normalise = true; r.first = rb;
         rb += j.np() / 32 * (j.np() / 32 + 1) / 2 * pieces;
       }
-      by_kind(kind, [&](auto k) {
+      by_user_kind(kind, [&](auto k) {
         if (one) hipLaunchKernelGGL((orth_gram_kernel<decltype(k)::value, true>), dim3(gb), dim3(256), 0, st, ga);
         else hipLaunchKernelGGL((orth_gram_kernel<decltype(k)::value, false>), dim3(gb), dim3(256), 0, st, ga);
       });
