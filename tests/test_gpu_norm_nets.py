@@ -417,3 +417,53 @@ def test_c_forward_entries(gpu):
     _lib.check(lib.agx_cgan_disc_forward(pair.handle, _dev.stream(), x3.data_ptr(), 61, cc3.data_ptr(), nc3.data_ptr(), rows, s.data_ptr()))
     want = torch.as_tensor(np.asarray(disc([x3[:rows], cc3[:rows], nc3[:rows]])), device=gpu).reshape(-1)
     assert float((s - want).abs().max()) <= 2.0 ** -18 * float(want.abs().max())
+
+
+@pytest.mark.parametrize('G,H,B,slope,which,seed', [CASES[2], CASES[3], CASES[4]])
+def test_augmented_steps_of_both_nets(gpu, G, H, B, slope, which, seed):
+    """Losses and gradients with noise on some of the rows (one row of it for all fake ones, tf_utils.py:209; a row each for
+    the generator's, :247), against the float64 oracle on the augmented rows; the noise is moved as the inputs are."""
+    from adversarial_gene_expression_amd import tf_utils as T
+    from oracle import cgan_norm_oracle as N, cgan_oracle as O
+    p = case(G, H, B, slope, which, seed)
+    rs = np.random.RandomState(seed + 40)
+    f = lambda *s: np.asarray(0.5 * rs.randn(*s), np.float32)  # noqa: E731
+    mask = np.asarray(np.arange(B) % 3 != 1, np.float32)
+    noise = dict(fake=f(G), real=f(B, G), gen=f(B, G))
+    m = torch.tensor(mask.astype(np.float64))[:, None]
+
+    def both(t, e, seen=None):
+        net = lambda key, x, **kw: N.forward(t[key], x, t['cc'], t['nc'], slope=slope, seen=seen, **kw)  # noqa: E731
+        ps = [a.detach().requires_grad_(True) for a in N.params(t['dp'])]
+        q = dict(t, dp=N.rebuild(t['dp'], ps))
+        with torch.no_grad():
+            fake = net('gp', t['z']) + m * e['fake']
+        real = t['x'] + m * e['real']
+        critic = lambda x: N.forward(q['dp'], x, t['cc'], t['nc'], slope=slope, seen=seen)  # noqa: E731
+        loss = O.discriminator_loss(critic(real), critic(fake)) + 10.0 * O.gradient_penalty(critic, real, fake, t['alpha'])
+        out = [loss.detach().reshape(1)] + N._grads(loss, ps)
+        ps = [a.detach().requires_grad_(True) for a in N.params(t['gp'])]
+        made = N.forward(N.rebuild(t['gp'], ps), t['z'], t['cc'], t['nc'], slope=slope, seen=seen) + m * e['gen']
+        loss = O.generator_loss(net('dp', made))
+        return out + [loss.detach().reshape(1)] + N._grads(loss, ps)
+
+    def moved(rel, s):
+        r = np.random.RandomState(s + 90)
+        return both(tensors(p, rel, s), {k: torch.tensor(v.astype(np.float64) * (1 + rel * r.choice([-1.0, 1.0], size=v.shape)))
+                                         for k, v in noise.items()}, seen)
+    seen = []
+    want = moved(0.0, 0)
+    assert min(float(v.abs().min()) for v in seen) > 4e-6
+    tol = [16 * 2.0 ** -24 * float(w.abs().max()) for w in want]
+    tol[len(params(p['dp']))] += 16 * 2.0 ** -24 * 2          # the critic's output bias, as in allowed()
+    others = [moved(2.0 ** -21, s) for s in (1, 2)]
+    tol = [t + 16 * max(float((o[i] - want[i]).abs().max()) for o in others) for i, t in enumerate(tol)]
+    gen, disc = nets(T, p, slope)
+    dl = T.train_disc(p['x'], p['z'], p['cc'], p['nc'], gen, disc, T.RMSprop(5e-4), alpha=p['alpha'], apply=False,
+                      aug=dict(mask=mask, noise_fake=noise['fake'], noise_real=noise['real']))
+    gl = T.train_gen(p['z'], p['cc'], p['nc'], gen, disc, T.RMSprop(5e-4), apply=False, aug=dict(mask=mask, noise=noise['gen']))
+    got = [np.float64(dl).reshape(1)] + disc.get_gradients() + [np.float64(gl).reshape(1)] + gen.get_gradients()
+    assert len(got) == len(want)
+    for i, (a, w, t) in enumerate(zip(got, want, tol)):
+        err = float(np.abs(np.asarray(a, np.float64) - w.numpy().reshape(np.shape(a))).max())
+        assert err <= t, (i, np.shape(a), err, t)
