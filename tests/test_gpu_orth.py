@@ -332,3 +332,36 @@ def test_companions_change_roundings_only(gpu):
             alone = ops.orthogonalize(x)
             _, tol = allowed(x)
             assert alone.dtype == y.dtype and rel(y, N.t64(alone)) <= 2 * (tol + half(x.dtype)), x.shape
+
+
+def test_muon_on_kernels_of_a_wide_net(gpu):
+    """The kernels of nets with hidden layers of 1024 over 20000 genes, in one step: m <- g, u = 1.95 g.  The tolerance of
+    test_muon_over_sides_of_every_size; the float64 iteration runs on the GPU, in the Gram form of the smaller side."""
+    from adversarial_gene_expression_amd import ops
+    g = torch.Generator(device=gpu).manual_seed(2)
+    mk = lambda r, c: torch.randn(r, c, generator=g, device=gpu)  # noqa: E731
+    shapes = [(20007, 1024), (1024, 1024), (1024, 20000)]
+    # gradients of 512 samples: low rank and noise
+    gs = [mk(r, 512) @ mk(512, c) / 512 + 0.01 * mk(r, c) for r, c in shapes]
+    ws = [0.05 * mk(r, c) for r, c in shapes]
+    ms = [torch.zeros_like(w) for w in ws]
+    before = [w.double() for w in ws]
+    ops.muon(ws, gs, ms, 0.02)
+
+    def oracle(v):
+        v = v / v.norm()
+        for _ in range(5):
+            A = v.t().contiguous() @ v
+            v = 3.4445 * v + v @ (-4.7750 * A + 2.0315 * (A @ A))
+        return v
+    for w0, w, gr, m in zip(before, ws, gs, ms):
+        assert torch.equal(m, gr)
+        x = 1.95 * gr.double()
+        sign = torch.randint(0, 2, x.shape, generator=g, device=gpu).double() * 2 - 1
+        wide = x.shape[0] < x.shape[1]
+        turn = lambda t: t.t().contiguous() if wide else t  # noqa: E731
+        o, moved = oracle(turn(x)), oracle(turn(x * (1 + sign * 2.0 ** -21)))
+        tol = 16 * float((moved - o).norm() / o.norm()) + 16 * 2.0 ** -24
+        step = 0.02 * max(1.0, w.shape[1] / w.shape[0]) ** 0.5
+        err = float((w.double() - (w0 - step * turn(o))).norm())
+        assert err <= step * tol * float(o.norm()) + 2.0 ** -23 * float(w0.norm()), (x.shape, err)
