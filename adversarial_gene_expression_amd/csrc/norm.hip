@@ -286,9 +286,11 @@ struct Inputs {
 __device__ __forceinline__ void read_again() { asm volatile("" ::: "memory"); }
 
 // Rows of 1024 threads (8 to 32 values each, 128 registers a thread) are held where that leaves registers for the rest, else read
-// again, from L2 or the last-level cache, instead of spilled.  Held and read again, us: backward 2000 x 6000 (8 values) 38.1, 40.7;
-// without sums 1000 x 14000 (16) 70, 77; with them 1800 x 9000 (12) 77, 68; second order 1000 x 6000 51, 35; 900 x 16000 179,
-// 108; 1000 x 18154 bf16 206, 120.
+// again, from L2 or the last-level cache, which takes fewer.  Held and read again, us (the same inputs every pass): backward
+// 2000 x 6000 (8 values) 38.1, 40.7; without sums 1000 x 14000 (16) 70, 77; with them 1800 x 9000 (12) 77, 68; second order
+// 1000 x 6000 51, 35; 900 x 16000 179, 108; 1000 x 18154 bf16 206, 129.  What still spills, by hipcc's report: the second order
+// with parameter gradients throughout (5 registers at 8 values to 69 at 32), without them up to 5, the backward pass with sums
+// at 12 values 7 and without at 32 values 17.
 constexpr bool back_holds(int g, int values, bool pg) { return g < 1024 || values <= (pg ? 8 : 16); }
 constexpr bool back2_holds(int g) { return g < 1024; }
 // the rows of workgroup `block` of `blocks`; lds: lds_floats<T, G, C>() where PG
@@ -793,10 +795,13 @@ template <int V, class F> bool by_cfg(const Cfg &c, F f) {
   return c.g != 0;
 }
 
-// The backward pass with parameter gradients in one launch (ln_bwd_small_kernel) instead of two, up to SMALL_ROWS rows and
-// SMALL_VECTORS whole vectors a matrix.  GPU time of two launches and one, us: 16 x 256 5.1, 3.2; 512 x 256 6.4, 3.7; 1536 x 256 7.6,
-// 5.7; 2048 x 600 9.9, 11.7; 512 x 4000 16.0, 14.8; 1024 x 4000 21.4, 25.4; 512 x 4297 bf16 22.5, 13.1.  (The host's second
-// launch costs 3.4 us more.)
+// The backward pass with parameter gradients in one launch (ln_bwd_small_kernel) instead of two, up to SMALL_ROWS rows - six a
+// thread of a columns' workgroup, up to which it is no slower at any width - and SMALL_VECTORS whole vectors a matrix.  GPU time of
+// two launches and one, us: 16 x 256 5.1, 3.2; widths 64, 256, 512, 1024 by 512 rows 5.4, 3.6; 6.5, 3.7; 7.3, 4.0; 8.9, 5.9;
+// by 1024 5.8, 4.0; 6.3, 4.4; 7.2, 5.6; 9.4, 8.0; by 1536 6.0, 5.3; 7.6, 5.7; 8.9, 6.8; 11.6, 11.4 (bf16 6.4, 5.9; 8.1, 6.3; 8.4,
+// 6.5; 10.9, 7.7); by 2048 6.4, 5.7; 7.5, 6.7; 9.0, 7.9; 12.7, 15.5 (bf16 6.7, 6.7; 7.8, 7.2; 8.3, 7.7; 11.1, 9.0); by 3000 6.9,
+// 7.5; 9.8, 8.6; 11.8, 16.4; 16.6, 20.3; by 4096 6.0, 9.2; 10.2, 10.5; 13.1, 22.0; 19.0, 25.2.  2048 x 600 9.9, 11.7; 512 x 4000
+// 16.0, 14.8; 1024 x 4000 21.4, 25.4; 512 x 4297 bf16 22.5, 13.1.  (The host's second launch costs 3.4 us more.)
 constexpr int SMALL_ROWS = 1536, SMALL_VECTORS = 1 << 19;
 bool small_shape(int64_t rows, int64_t width, int v) {
   const int g = pick(width, v).g;

@@ -18,8 +18,8 @@
 // Launches of a call: the momentum step with |x|'s maximum and norm; then, a phase each, the Gram matrix (and the sum of its
 // slices), its polynomial (n <= 128 one launch a phase, n <= 256 one a step, above three a step) and the product with the
 // long side, which in the last phase is the Muon update of w too.  Floors: 2.4 us a launch, 5 TB/s of HBM, 1150 TFLOP/s of
-// fp16 products over three.  Measured: 256 x 256 88 us (12 launches), 18161 x 256 147 us (15), 1000 x 4297 bf16 358 us
-// (20; its products take 73 us at that rate).
+// fp16 products over three.  Measured: 256 x 256 88 us (12 launches), 18161 x 256 147 us (15), 1000 x 4297 bf16 360 us
+// (19; its products take 73 us at that rate).
 #include "agx_common.h"
 
 #include <algorithm>
@@ -530,7 +530,8 @@ __global__ __launch_bounds__(256, 4) void orth_gram_kernel(GramArgs a) {
 // A_0 = (sum of the partial Gram tiles) / d^2 with d = |X|_F + eps (first phase) or without a divisor (later phases).
 // A workgroup takes R rows of a square of 32 x 32 on or above the diagonal: interleaved shares of the slices meet in LDS, from
 // where the piece and its mirror image go out as vectors.  R = 32 (4 shares) where the slices are few, 4 (8 shares) where
-// they are many: 18161 x 256 with 71 slices 7.1 us instead of 10.5, 1000 x 4297 with 5 slices 11.0 us instead of 13.8.
+// they are many: 18161 x 256 (48 slices) 5.6 us instead of 7.1, 4318 x 128 5.4 instead of 6.8; 1000 x 4297 (7 slices) 13.7 us
+// instead of 17.4, 640 x 2000 6.5 instead of 7.4.
 struct ReduceJob {
   const float *part;
   const uint32_t *maxb;
@@ -635,7 +636,9 @@ static_assert(sizeof(ChainArgs) <= 4096, "kernel argument size");
 // A workgroup has a tile of 64 x 32 on or above the diagonal, its four waves every fourth step of 64 k of all of it: operands
 // go straight from L2 to the matrix cores' registers, each byte once a workgroup, without LDS or barriers until the waves'
 // sums meet.  (Tiles through LDS, four or eight waves at a barrier a step: 16.5 us at n = 1024 instead of 15.1, 12.5 at 640
-// instead of 8.2.  The floor of the products is 3 us; 272 tiles on 256 CUs, whose L1 takes 64 bytes a clock, bound it.)
+// instead of 8.2.)  At n = 1024, 14 us a launch: the matrix cores work 1.5 us in the mean, a wave lives 8 us and waits for 30% of
+// it (186 registers and 272 tiles on 256 CUs: mostly one wave a SIMD), a CU with two tiles reads 786 KB or 5.1 us at 64 bytes a
+// clock, a quarter of the L2s' requests miss (13.6 MB from the last-level cache), the launch is 2.4.  No one of them bounds it.
 typedef float WaveSums[4][32][64];                    // [wave][element of two accumulators][lane]
 // tile of 64 x 32 of linear index t: row ti of tiles starts at column 2 ti
 __device__ __forceinline__ void half_tile(int t, int nt, int &ti, int &tj) {
@@ -739,8 +742,8 @@ __global__ __launch_bounds__(256, 2) void orth_chain_kernel(ChainArgs a) {
 }
 
 // Gram matrix of the iterate between two phases by the same means: partial tiles as orth_gram_kernel gives them, or (ONE
-// slice each) A itself.  18161 x 256 11 us (through LDS, from fp32 lines that every tile splits anew: 15), 1000 x 4297 30 (44),
-// 256 x 256 5.2 (9).
+// slice each) A itself.  18161 x 256 11 us (through LDS, from fp32 lines that every tile splits anew: 15), 256 x 256 5.2 (9),
+// 1000 x 4297 38 (44 and 14 for the sum of its slices): a wave lives 20 us and waits for 30% of it, the matrix cores work 6.
 struct LinesGramJob {
   Lines x;
   Planes A;
