@@ -146,9 +146,8 @@ def layer_norm(x, gamma=None, beta=None, *, eps=1e-3, act=0, slope=0.0, out=None
     """Layer normalisation of every row of x [rows, width] (float32 or bfloat16), with the (leaky-)ReLU of `slope` behind
     it when act=1: y = act(gamma * (x - mean) * rstd + beta), rstd = 1 / sqrt(var + eps), biased variance (Keras
     LayerNormalization).  gamma / beta: float32 vectors or None (1 / 0).  Returns (y, mean, rstd), the statistics in
-    float32 for the backward passes.  out: where to write y (x itself is allowed, another overlap
-    with it is not).  The reference has no normalisation
-    layer (tf_utils.py:85-88)."""
+    float32 for the backward passes, which read x too.  out: where to write y (x itself is allowed where no backward pass
+    follows, another overlap with it is not).  The reference has no normalisation layer (tf_utils.py:85-88)."""
     d = _norm_desc(x, act, slope)
     if not eps > 0.0:
         raise ValueError('eps must be positive, got %r' % (eps,))
