@@ -1772,23 +1772,24 @@ int run(hipStream_t st, Job *jobs, int n, const agx_orth_opts_t *o, float mu, bo
   return AGX_OK;
 }
 
-int to_jobs(const agx_orth_t *j, int n, Job *out, const char *who) {
+// (first: number of j[0] among the caller's matrices)
+int to_jobs(const agx_orth_t *j, int n, Job *out, const char *who, int first = 0) {
   AGX_CHECK_ARG(j && n >= 1 && n <= AGX_MAX_ORTH, "%s: 1 to %d matrices a call", who, AGX_MAX_ORTH);
   for (int i = 0; i < n; ++i) {
     const agx_orth_t &a = j[i];
-    AGX_CHECK_ARG(a.dtype == AGX_F32 || a.dtype == AGX_BF16, "%s: matrix %d: dtype %d", who, i, a.dtype);
+    AGX_CHECK_ARG(a.dtype == AGX_F32 || a.dtype == AGX_BF16, "%s: matrix %d: dtype %d", who, first + i, a.dtype);
     AGX_CHECK_ARG(a.rows > 0 && a.cols > 0 && std::min(a.rows, a.cols) <= AGX_ORTH_MAX_SIDE,
-                  "%s: matrix %d is %d x %d; the smaller side is at most %d", who, i, a.rows, a.cols, AGX_ORTH_MAX_SIDE);
+                  "%s: matrix %d is %d x %d; the smaller side is at most %d", who, first + i, a.rows, a.cols, AGX_ORTH_MAX_SIDE);
     AGX_CHECK_ARG((int64_t)a.rows * agx::cdiv64(a.cols, 4) < (1LL << 30) && agx::cdiv64(a.rows, T) * agx::cdiv64(a.cols, T) < (1 << 26),
-                  "%s: matrix %d is too large", who, i);
-    AGX_CHECK_ARG(a.ldx < (1 << 23) && a.ldo < (1 << 23), "%s: matrix %d: leading dimension above 2^23", who, i);
+                  "%s: matrix %d is too large", who, first + i);
+    AGX_CHECK_ARG(a.ldx < (1 << 23) && a.ldo < (1 << 23), "%s: matrix %d: leading dimension above 2^23", who, first + i);
     Job &b = out[i];
     b.x = a.x; b.out = a.out; b.ldx = a.ldx; b.ldo = a.ldo; b.rows = a.rows; b.cols = a.cols; b.dtype = a.dtype;
   }
   return AGX_OK;
 }
 
-int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, const char *who) {
+int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, const char *who, int first = 0) {
   AGX_CHECK_ARG(j && n >= 1 && n <= AGX_MAX_ORTH, "%s: 1 to %d matrices a call", who, AGX_MAX_ORTH);
   agx_orth_t m[AGX_MAX_ORTH];
   memset(m, 0, sizeof(m));
@@ -1796,7 +1797,7 @@ int muon_jobs(const agx_muon_t *j, int n, const agx_muon_opts_t *o, Job *out, co
     m[i].x = j[i].g; m[i].ldx = j[i].ldg; m[i].out = j[i].w; m[i].ldo = j[i].ldw;
     m[i].rows = j[i].rows; m[i].cols = j[i].cols; m[i].dtype = AGX_F32;
   }
-  AGX_TRY(to_jobs(m, n, out, who));
+  AGX_TRY(to_jobs(m, n, out, who, first));
   for (int i = 0; i < n; ++i) {
     out[i].muon = true;
     out[i].m = j[i].m;
@@ -1868,7 +1869,7 @@ static int check_muon(const agx_muon_t *jobs, int n, const agx_muon_opts_t *o, c
   AGX_CHECK_ARG(std::isfinite(o->lr) && std::isfinite(o->weight_decay), "%s: learning rate / weight decay must be finite", who);
   AGX_CHECK_ARG(jobs && n >= 1, "%s: no matrices", who);
   Job j[AGX_MAX_ORTH];
-  for (int lo = 0; lo < n; lo += AGX_MAX_ORTH) AGX_TRY(muon_jobs(jobs + lo, std::min(n - lo, AGX_MAX_ORTH), o, j, who));
+  for (int lo = 0; lo < n; lo += AGX_MAX_ORTH) AGX_TRY(muon_jobs(jobs + lo, std::min(n - lo, AGX_MAX_ORTH), o, j, who, lo));
   for (int i = 0; i < n; ++i) {
     const agx_muon_t &a = jobs[i];
     AGX_CHECK_ARG(a.w && a.g && a.m && a.ldw >= a.cols && a.ldg >= a.cols && a.ldm >= a.cols && a.ldm < (1 << 23) && std::isfinite(a.scale),

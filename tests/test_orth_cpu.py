@@ -211,3 +211,17 @@ def test_muon_steps_of_any_number_of_kernels_are_checked_at_once():
     assert check(18) == -1
     o.momentum, o.orth.steps = 0.9, 0
     assert check(18) == -1
+
+
+def test_refusals_of_long_lists_name_the_matrix():
+    lib = _lib.load()
+    o = _lib.MuonOpts()
+    o.orth, o.lr, o.momentum = _opts(), 0.1, 0.9
+    for n in (1, 16, 17, 33, 40):
+        for kw in (dict(rows=0), dict(rows=5000, cols=4097), dict(ldg=1 << 23), dict(scale=float('nan')), dict(w=1)):
+            j = (_lib.MuonDesc * n)()
+            for k, q in enumerate(j):
+                q.w, q.g, q.m, q.ldw, q.ldg, q.ldm, q.rows, q.cols, q.scale = *(((3 * k + i) << 20) for i in (1, 2, 3)), 6, 6, 6, 4, 6, 1.0
+            for k, v in kw.items():
+                setattr(j[n - 1], k, v)
+            assert lib.agx_opt_muon_check(j, n, o) == -1 and ('matrix %d' % (n - 1)) in lib.agx_last_error().decode(), (n, kw)
